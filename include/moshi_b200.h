@@ -555,6 +555,57 @@ int64_t b200_dlm_algorithmic_bytes(b200_dlm* h, int tokens, int context);
 int64_t b200_dlm_algorithmic_flops(b200_dlm* h, int tokens, int context);
 
 /* ------------------------------------------------------------------------------------------ */
+/* A paged 8-bit cache of keys and values (csrc/paged.cu)                                       */
+/* ------------------------------------------------------------------------------------------ */
+/* Memory goes to sequences page by page; the caller owns it, and every pointer below is on `device`.  No reference counterpart (its caches are rings).
+ * These calls hold no state and no workspace of their own, enqueue on the stream and do not synchronise; they may be captured into a graph.  They are launched early like
+ * b200_op_linear_sk, and read nothing before the kernel in front is done.  What the device's arrays say is checked on the device: what does not fit is left out, and
+ * recorded in the cache's flags. */
+typedef struct {
+  void *k_dev, *v_dev;                /* codes [pages][kv_heads][page_tokens][dim], int8 or e4m3 (B200_KV_*), 16-byte border */
+  float *k_scale_dev, *v_scale_dev;   /* [pages][kv_heads]: a code stands for code * scale */
+  int32_t* flags_dev;                 /* one word; B200_PAGED_* are ORed into it */
+  int32_t pages, page_tokens;         /* page_tokens 16, 32, 64 or 128 */
+  int32_t kv_heads, dim;              /* dim 64 or 128 */
+  int32_t kv_dtype, device;
+} b200_paged_cache;
+enum { B200_PAGED_BAD_BATCH = 1,      /* rows out of order or past total_rows / max_rows, negative lengths, or tokens past the table: the sequence was left out */
+       B200_PAGED_BAD_PAGE = 2,       /* a table names a page that the cache does not have: its tokens were left out */
+       B200_PAGED_NOT_FINITE = 4,     /* an appended value is NaN, infinite or above 2^64: stored as 0 */
+       B200_PAGED_WAIT = 8 };         /* a kernel waited ten seconds for its own copies in vain: the results are incomplete */
+
+/* A step: sequence s adds the rows rows[s] .. rows[s + 1] - 1 of the call's tensors (none, one or many) behind its before[s] tokens; token t of it lies in page
+ * table[s][t / page_tokens].  Rows from rows[sequences] on belong to nobody and are left as they are. */
+typedef struct {
+  const int32_t *table_dev;           /* [sequences][table_ld], table_width of them used */
+  const int32_t *before_dev;          /* [sequences] tokens in front of the step */
+  const int32_t *rows_dev;            /* [sequences + 1], rising from 0 on */
+  int64_t table_ld;
+  int32_t sequences, table_width;
+  int32_t total_rows;                 /* rows of the call's tensors */
+  int32_t max_rows;                   /* no sequence has more than this in the step */
+} b200_paged_batch;
+typedef struct {
+  const uint64_t* turns_dev;          /* [rot_dims / 2]: frequency / (2 pi), turns per position, as a fraction of 2^64 */
+  int32_t rot_dims, pairing;          /* a multiple of 16, <= dim; B200_ROT_HALVES / B200_ROT_ADJACENT */
+} b200_rotary;
+
+/* Appends k, v bf16 [total_rows][kv_heads * dim] (k_ld, v_ld elements from row to row, multiples of 8), keys rotated by their positions (rotary NULL: not), and rotates the queries q
+ * [total_rows][q_heads * dim] into q_out (q NULL: none; q_out may be q).  Scales: the rows that begin a page give it max|x| / 127 (e4m3: / 448), at least 2^-60; rows
+ * that come later double it until they fit, and the page's older codes are rounded to the new scale.  Appending the same rows again changes nothing.  A page
+ * that is written to must belong to one sequence of the batch only. */
+int b200_paged_append(const b200_paged_cache* cache, const b200_paged_batch* batch, const void* k_dev, int64_t k_ld, const void* v_dev, int64_t v_ld,
+                      const void* q_dev, int64_t q_ld, void* q_out_dev, int64_t q_out_ld, int q_heads, const b200_rotary* rotary, void* stream);
+/* Attention of the step's rows over the cache, behind b200_paged_append with the same batch: the row at position p sees the tokens j <= p of its sequence and, where
+ * window > 0, of these only p - j < window or j < sinks.  q, out bf16 [total_rows][q_heads * dim]; query head h reads cache head h / (q_heads / kv_heads).
+ * A row that sees nothing gets zeros.  work_dev: b200_paged_attention_bytes(...) bytes that this call alone uses (0: may be null). */
+int64_t b200_paged_attention_bytes(const b200_paged_cache* cache, const b200_paged_batch* batch, int q_heads, int window, int sinks);
+int b200_paged_attention(const b200_paged_cache* cache, const b200_paged_batch* batch, const void* q_dev, int64_t q_ld, void* out_dev, int64_t out_ld, int q_heads,
+                         float scale, int window, int sinks, void* work_dev, int64_t work_bytes, void* stream);
+/* What the cache holds of the batch's rows (positions before[s] + i): k, v bf16 [total_rows][kv_heads][dim]. */
+int b200_paged_read(const b200_paged_cache* cache, const b200_paged_batch* batch, void* k_out_dev, void* v_out_dev, void* stream);
+
+/* ------------------------------------------------------------------------------------------ */
 /* Kernel-level entry points (used by the parity tests; same kernels the handles launch)        */
 /* ------------------------------------------------------------------------------------------ */
 

@@ -14,6 +14,7 @@ LIB_PATH = Path(__file__).resolve().parent / "_C" / "libmoshi_b200.so"
 
 B200_OK, B200_ERR_INVALID, B200_ERR_SHAPE, B200_ERR_STATE, B200_ERR_CUDA, B200_ERR_MISSING = range(6)
 B200_F32, B200_BF16, B200_F16, B200_I64, B200_U8, B200_I8 = range(6)
+B200_KV_FP8_E4M3, B200_KV_INT8 = 1, 2
 ABI_VERSION = 8
 
 
@@ -66,8 +67,23 @@ class DLMConfigC(C.Structure):
                 ("side_dim", C.c_int), ("loop_start", C.c_int), ("loop_stop", C.c_int), ("loop_times", C.c_int)]
 
 
+class PagedCacheC(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("flags", C.c_void_p),
+                ("pages", C.c_int32), ("page_tokens", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32), ("kv_dtype", C.c_int32), ("device", C.c_int32)]
+
+
+class PagedBatchC(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("before", C.c_void_p), ("rows", C.c_void_p), ("table_ld", C.c_int64),
+                ("sequences", C.c_int32), ("table_width", C.c_int32), ("total_rows", C.c_int32), ("max_rows", C.c_int32)]
+
+
+class RotaryC(C.Structure):
+    _fields_ = [("turns", C.c_void_p), ("rot_dims", C.c_int32), ("pairing", C.c_int32)]
+
+
 _P = C.c_void_p
 _I = C.c_int
+_L = C.c_int64
 _PROTOTYPES: dict[str, tuple[tp.Any, list]] = {
     "b200_last_error": (C.c_char_p, []),
     "b200_abi_version": (_I, []),
@@ -158,6 +174,11 @@ _PROTOTYPES: dict[str, tuple[tp.Any, list]] = {
     "b200_frame_destroy": (_I, [_P]),
     "b200_frame_step": (_I, [_P, _P, _P, _P, _P, _P, _P, _P]),
     "b200_frame_read_buffer": (_I, [_P, C.c_char_p, _P, C.c_int64, C.POINTER(C.c_int64)]),
+    # paged 8-bit cache
+    "b200_paged_append": (_I, [_P, _P, _P, _L, _P, _L, _P, _L, _P, _L, _I, _P, _P]),
+    "b200_paged_attention_bytes": (_L, [_P, _P, _I, _I, _I]),
+    "b200_paged_attention": (_I, [_P, _P, _P, _L, _P, _L, _I, C.c_float, _I, _I, _P, _L, _P]),
+    "b200_paged_read": (_I, [_P, _P, _P, _P, _P]),
     # kernel-level
     "b200_op_linear_bf16": (_I, [_P, _P, _P, _I, _I, _I, _P]),
     "b200_op_packed_bytes": (C.c_int64, [_I, _I, _I, _I]),
