@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadP p) {
 // =========================================================================================================================
 // attention of few rows
 // =========================================================================================================================
-// Columns are (row of the sequence, query head of the group); a CTA has 8 * NT of them, one kv head and a range of the keys, in tiles of 16 tokens that its warps take in
+// Columns are (row of the sequence, query head of the group); a CTA has 8 * NT of them, one kv head and a run of the keys, in tiles of 32 tokens that its warps take in
 // turn.  Both products have the cache as the first operand of mma.m16n8k16: S^T = K Q^T (tokens x columns) and O^T += V^T P^T (dims x columns), so a single row of one head
 // wastes tensor-core columns and not cache bytes.  Codes go from memory into registers as fragments, 16 bytes at a time: which dimension of K is which
 // k of the product is free as long as Q has the same order, and so is which dimension of V is which row of O^T.  P^T comes out of S^T by movmatrix.
@@ -320,25 +320,17 @@ __global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadP p) {
 // values goes into the exponent, P = 2^(score + log2 s_v - M), with M the running maximum of the same, and the sum of the weights takes P / s_v: nothing is rounded on the way but P.
 // M follows only when a score passes it by 2^8, as then no column has to be compared across lanes for most tiles.
 constexpr int FEW_WARPS = 4, FEW_THREADS = FEW_WARPS * 32;
+constexpr int few_per_sm(int nt) { return nt <= 2 ? 3 : 2; }      // CTAs, by their registers
+constexpr int MIN_RUN = 8;                    // tiles of a CTA
 constexpr float SLACK = 8.f;
 
-__device__ __forceinline__ uint4 load_stream16(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
-}
-__device__ __forceinline__ uint2 load_stream8(const void* p) {
-  uint2 r;
-  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
-}
 __device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transposed8x8(uint32_t a) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
   return r;
 }
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
@@ -346,331 +338,10 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// a column's D / 16 sums from dimension d0 on, divided by the sum of the weights (0: nothing was seen)
 template <int D>
-struct Codes {                               // a warp's tile of 16 tokens, as its lanes hold it
-  uint32_t k[2][D / 16], v[4][D / 32];
-};
-
-template <int D, int FMT, int NT>
-__global__ void __launch_bounds__(FEW_THREADS, NT == 1 ? 4 : NT == 2 ? 3 : 2) few_rows_kernel(const AttnP p) {
-  pdl_trigger();
-  pdl_wait();
-  constexpr int KS = D / 16, MT = D / 16, COLS = 8 * NT;
-  __shared__ float o_s[FEW_WARPS][8][D + 4];
-  __shared__ float m_s[FEW_WARPS][8], l_s[FEW_WARPS][8];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-  int u = (int)blockIdx.x;
-  const int split = u % p.nsplit; u /= p.nsplit;
-  const int ct = u % p.ctiles; u /= p.ctiles;
-  const int h = u % p.H, s = u / p.H;
-  const Seq q = sequence(p.b, s, p.P);
-  if (!q.ok) {
-    if (threadIdx.x == 0) flag(p.flags, B200_PAGED_BAD_BATCH);
-    return;
-  }
-  const int n_cols = q.n * p.G, c0 = ct * COLS;
-  if (q.n >= p.from_rows || c0 >= n_cols) return;
-  const int pf = q.before + c0 / p.G, pl = q.before + (min(c0 + COLS, n_cols) - 1) / p.G;
-  const Tiles<4> tiles(pf, pl, p.window, p.sinks);
-  const int per = (tiles.n + p.nsplit - 1) / p.nsplit, t0 = split * per, t1 = min(t0 + per, tiles.n);
-  if (t0 >= t1) return;
-
-  // queries: lane (g, c) has of column 8 nt + g the dimensions 64 i + 16 c .. + 15
-  uint32_t qf[NT][KS][2];
-  float fac[NT][2];                          // of columns 8 nt + 2 c, + 1: what turns a product of codes into a score in base 2
-  int pos[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int col = c0 + nt * 8 + g;
-    const bool has = col < n_cols;
-    const int i = has ? col / p.G : 0;
-    const bf16* row = p.q + (long long)(q.r0 + i) * p.q_ld + (long long)(h * p.G + (has ? col - i * p.G : 0)) * D;
-    uint32_t raw[KS][2];
-    float top = 0.f;
-#pragma unroll
-    for (int b = 0; b < D / 64; ++b) {
-      const uint4 x = has ? *reinterpret_cast<const uint4*>(row + 64 * b + 16 * c) : make_uint4(0, 0, 0, 0);
-      const uint4 y = has ? *reinterpret_cast<const uint4*>(row + 64 * b + 16 * c + 8) : make_uint4(0, 0, 0, 0);
-      raw[4 * b][0] = x.x; raw[4 * b][1] = x.y; raw[4 * b + 1][0] = x.z; raw[4 * b + 1][1] = x.w;
-      raw[4 * b + 2][0] = y.x; raw[4 * b + 2][1] = y.y; raw[4 * b + 3][0] = y.z; raw[4 * b + 3][1] = y.w;
-    }
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float2 f = unpack_bf16(raw[k][e]);
-        const float a = fabsf(f.x), b = fabsf(f.y);
-        if (a < INFINITY) top = fmaxf(top, a);
-        if (b < INFINITY) top = fmaxf(top, b);
-      }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const float power = top > 0.f ? power_of_two_in(top) : 1.f;
-    const float up = 16384.f / power;        // the column's largest lands in [2^14, 2^15)
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float2 f = unpack_bf16(raw[k][e]);
-        qf[nt][k][e] = pack_f16(f.x * up, f.y * up);
-      }
-    const float back = power * (1.f / 16384.f);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      fac[nt][e] = __shfl_sync(0xffffffffu, back, (2 * c + e) * 4) * p.scale2;
-      const int cc = c0 + nt * 8 + 2 * c + e;
-      pos[nt][e] = cc < n_cols ? q.before + cc / p.G : -1;
-    }
-  }
-
-  float o[NT][MT][4], m[NT][2], l[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
-    m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.f;
-  }
-
-  const int32_t* table = p.b.table + s * p.b.table_ld;
-  const long long head = (long long)h * p.P, page_rows = (long long)p.H * p.P;
-  // lane i has the page and scales of the warp's i-th tile from here on
-  int my_page = -1;
-  float my_ks = 0.f, my_vs = 1.f;
-  auto look_up = [&](int t) {
-    const int mine = t + lane * FEW_WARPS;
-    my_page = -1; my_ks = 0.f; my_vs = 1.f;
-    if (mine < t1) {
-      const int page = table[(tiles[mine] << 4) >> p.page_shift];
-      if (page >= 0 && page < p.pages) {
-        my_page = page;
-        my_ks = p.k_scale[(long long)page * p.H + h];
-        const float v = p.v_scale[(long long)page * p.H + h];
-        my_vs = v > 0.f ? v : 1.f;           // all codes of a page of zeros are 0
-      } else flag(p.flags, B200_PAGED_BAD_PAGE);
-    }
-  };
-  auto load = [&](Codes<D>& x, int t, int page) {
-    if (page < 0) {
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int b = 0; b < D / 16; ++b) x.k[a][b] = 0;
-#pragma unroll
-      for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int b = 0; b < D / 32; ++b) x.v[a][b] = 0;
-      return;
-    }
-    const long long at = (page * page_rows + head + ((tiles[t] << 4) & (p.P - 1))) * D;
-    const uint8_t *k = p.k + at + 16 * c, *v = p.v + at + (D / 8) * g;
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-      for (int b = 0; b < D / 64; ++b) {
-        const uint4 w = load_stream16(k + (g + 8 * a) * D + 64 * b);
-        x.k[a][4 * b] = w.x; x.k[a][4 * b + 1] = w.y; x.k[a][4 * b + 2] = w.z; x.k[a][4 * b + 3] = w.w;
-      }
-#pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      const uint8_t* at_v = v + (2 * c + (a & 1) + 8 * (a >> 1)) * D;
-      if constexpr (D == 128) {
-        const uint4 w = load_stream16(at_v);
-        x.v[a][0] = w.x; x.v[a][1] = w.y; x.v[a][2] = w.z; x.v[a][3] = w.w;
-      } else {
-        const uint2 w = load_stream8(at_v);
-        x.v[a][0] = w.x; x.v[a][1] = w.y;
-      }
-    }
-  };
-  auto work = [&](Codes<D>& x, int t, int page, float ks, float vs) {
-    float sc[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const uint32_t w0 = ready<FMT>(x.k[0][k]), w1 = ready<FMT>(x.k[1][k]);
-      const uint32_t a0 = half2_of<FMT, 0>(w0), a1 = half2_of<FMT, 0>(w1), a2 = half2_of<FMT, 1>(w0), a3 = half2_of<FMT, 1>(w1);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma_f16(sc[nt], a0, a1, a2, a3, qf[nt][k][0], qf[nt][k][1]);
-    }
-    const float lv = __log2f(vs), inv = __frcp_rn(vs);
-    const int j0 = tiles[t] << 4;
-    const bool whole = page >= 0 && j0 + 15 <= pf && (p.window <= 0 || pl - j0 < p.window || j0 + 16 <= p.sinks);
-    if (!whole) {                            // codes of tokens that no column sees may be anything
-#pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const int j = j0 + 2 * c + (a & 1) + 8 * (a >> 1);
-        if (!(j <= pl && (p.window <= 0 || pf - j < p.window || j < p.sinks))) {
-#pragma unroll
-          for (int b = 0; b < D / 32; ++b) x.v[a][b] = 0;
-        }
-      }
-    }
-    bool grow = false;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float v = fmaf(sc[nt][e], ks * fac[nt][e & 1], lv);
-        if (!whole && !(page >= 0 && sees(pos[nt][e & 1], j0 + g + 8 * (e >> 1), p.window, p.sinks))) v = -INFINITY;
-        sc[nt][e] = v;
-        grow |= v > m[nt][e & 1] + SLACK;
-      }
-    if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float top = fmaxf(sc[nt][e], sc[nt][e + 2]);
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          const float now = fmaxf(m[nt][e], top), by = now == -INFINITY ? 1.f : exp2_fast(m[nt][e] - now);
-          m[nt][e] = now;
-          l[nt][e] *= by;
-#pragma unroll
-          for (int i = 0; i < MT; ++i) { o[nt][i][e] *= by; o[nt][i][e + 2] *= by; }
-        }
-    }
-    uint32_t b0[NT], b1[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = exp2_fast(sc[nt][e] - (m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1]));
-      l[nt][0] = fmaf(w[0] + w[2], inv, l[nt][0]);
-      l[nt][1] = fmaf(w[1] + w[3], inv, l[nt][1]);
-      b0[nt] = transposed8x8(pack_f16(w[0], w[1]));
-      b1[nt] = transposed8x8(pack_f16(w[2], w[3]));
-    }
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) {       // four dimensions of this lane's: words of tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9
-      const uint32_t v0 = ready<FMT>(x.v[0][j]), v1 = ready<FMT>(x.v[1][j]), v2 = ready<FMT>(x.v[2][j]), v3 = ready<FMT>(x.v[3][j]);
-      const uint32_t lo = prmt(v0, v1, 0x5140u), hi = prmt(v0, v1, 0x7362u), lo8 = prmt(v2, v3, 0x5140u), hi8 = prmt(v2, v3, 0x7362u);
-      const uint32_t a[8] = {half2_of<FMT, 0>(lo), half2_of<FMT, 1>(lo), half2_of<FMT, 0>(lo8), half2_of<FMT, 1>(lo8),
-                             half2_of<FMT, 0>(hi), half2_of<FMT, 1>(hi), half2_of<FMT, 0>(hi8), half2_of<FMT, 1>(hi8)};
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        mma_f16(o[nt][2 * j], a[0], a[1], a[2], a[3], b0[nt], b1[nt]);
-        mma_f16(o[nt][2 * j + 1], a[4], a[5], a[6], a[7], b0[nt], b1[nt]);
-      }
-    }
-  };
-
-  // the next tile's codes are on their way while a tile is worked on
-  Codes<D> x, y;
-  int at = 0;
-  const int first = t0 + warp;
-  if (first < t1) {
-    look_up(first);
-    int page = __shfl_sync(0xffffffffu, my_page, 0);
-    float ks = __shfl_sync(0xffffffffu, my_ks, 0), vs = __shfl_sync(0xffffffffu, my_vs, 0);
-    load(x, first, page);
-    for (int t = first; t < t1; t += FEW_WARPS) {
-      const int next = t + FEW_WARPS;
-      int page2 = -1;
-      float ks2 = 0.f, vs2 = 1.f;
-      if (next < t1) {
-        if (++at == 32) { look_up(next); at = 0; }
-        page2 = __shfl_sync(0xffffffffu, my_page, at);
-        ks2 = __shfl_sync(0xffffffffu, my_ks, at);
-        vs2 = __shfl_sync(0xffffffffu, my_vs, at);
-        load(y, next, page2);
-      }
-      work(x, t, page, ks, vs);
-      x = y; page = page2; ks = ks2; vs = vs2;
-    }
-  }
-
-  // join the warps, eight columns at a time
-  const int unit = (s * p.H + h) * p.ctiles + ct;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float sum = l[nt][e];
-      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-      if (g == 0) { m_s[warp][2 * c + e] = m[nt][e]; l_s[warp][2 * c + e] = sum; }
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) *reinterpret_cast<float2*>(&o_s[warp][2 * c + e][(D / 8) * g + 2 * i]) = make_float2(o[nt][i][e], o[nt][i][e + 2]);
-    __syncthreads();
-    constexpr int PER = D / 16;              // 16 threads a column
-    const int col = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * PER;
-    float top = -INFINITY, sum = 0.f, acc[PER];
-#pragma unroll
-    for (int w = 0; w < FEW_WARPS; ++w) top = fmaxf(top, m_s[w][col]);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-#pragma unroll
-    for (int w = 0; w < FEW_WARPS; ++w) {
-      const float by = m_s[w][col] == -INFINITY ? 0.f : exp2_fast(m_s[w][col] - top);
-      sum = fmaf(l_s[w][col], by, sum);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) acc[i] = fmaf(o_s[w][col][d0 + i], by, acc[i]);
-    }
-    const int cc = c0 + nt * 8 + col;
-    if (p.nsplit > 1) {
-      const long long at_part = ((long long)unit * p.nsplit + split) * COLS + nt * 8 + col;
-      if ((threadIdx.x & 15) == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at_part) = make_float2(top, sum);
-#pragma unroll
-      for (int i = 0; i < PER; i += 4) *reinterpret_cast<float4*>(p.part_o + at_part * D + d0 + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-    } else if (cc < n_cols) {
-      const float by = sum != 0.f ? 1.f / sum : 0.f;
-      const int i = cc / p.G;
-      bf16* out = p.out + (long long)(q.r0 + i) * p.out_ld + (long long)(h * p.G + cc - i * p.G) * D + d0;
-      uint32_t w[PER / 2];
-#pragma unroll
-      for (int e = 0; e < PER / 2; ++e) w[e] = pack_bf16(acc[2 * e] * by, acc[2 * e + 1] * by);
-      if constexpr (PER == 8) *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
-      else *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
-    }
-    __syncthreads();
-  }
-}
-
-// Joins the ranges of the keys: eight columns of a unit per CTA.
-template <int D, int NT>
-__global__ void __launch_bounds__(128) join_kernel(const AttnP p) {
-  pdl_trigger();
-  pdl_wait();
-  constexpr int COLS = 8 * NT, PER = D / 16;
-  int u = (int)blockIdx.x;
-  const int nt = u % NT; u /= NT;
-  const int unit = u, ct = u % p.ctiles; u /= p.ctiles;
-  const int h = u % p.H, s = u / p.H;
-  const Seq q = sequence(p.b, s, p.P);
-  const int n_cols = q.n * p.G, c0 = ct * COLS, col = threadIdx.x >> 4, cc = c0 + nt * 8 + col, d0 = (threadIdx.x & 15) * PER;
-  if (!q.ok || q.n >= p.from_rows || cc >= n_cols) return;
-  const Tiles<4> tiles(q.before + c0 / p.G, q.before + (min(c0 + COLS, n_cols) - 1) / p.G, p.window, p.sinks);
-  const int per = (tiles.n + p.nsplit - 1) / p.nsplit, parts = (tiles.n + per - 1) / per;
-  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
-  const long long first = (long long)unit * p.nsplit * COLS + nt * 8 + col;
-  float top = -INFINITY;
-  for (int i = 0; i < parts; ++i) top = fmaxf(top, ml[first + (long long)i * COLS].x);
-  float sum = 0.f, acc[PER];
-#pragma unroll
-  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const float2 x = ml[first + (long long)i * COLS];
-    const float by = x.x == -INFINITY ? 0.f : exp2_fast(x.x - top);
-    sum = fmaf(x.y, by, sum);
-    const float4* o = reinterpret_cast<const float4*>(p.part_o + (first + (long long)i * COLS) * D + d0);
-#pragma unroll
-    for (int e = 0; e < PER / 4; ++e) {
-      const float4 v = o[e];
-      acc[4 * e] = fmaf(v.x, by, acc[4 * e]); acc[4 * e + 1] = fmaf(v.y, by, acc[4 * e + 1]);
-      acc[4 * e + 2] = fmaf(v.z, by, acc[4 * e + 2]); acc[4 * e + 3] = fmaf(v.w, by, acc[4 * e + 3]);
-    }
-  }
+__device__ __forceinline__ void store_row(const AttnP& p, const Seq& q, int h, int cc, int d0, const float* acc, float sum) {
+  constexpr int PER = D / 16;
   const float by = sum != 0.f ? 1.f / sum : 0.f;
   const int i = cc / p.G;
   bf16* out = p.out + (long long)(q.r0 + i) * p.out_ld + (long long)(h * p.G + cc - i * p.G) * D + d0;
@@ -681,15 +352,589 @@ __global__ void __launch_bounds__(128) join_kernel(const AttnP p) {
   else *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
 }
 
+// ---- the flattened work ----
+// The tiles of all units (sequence, column tile, kv head) one behind the other are cut into equal runs, one per CTA: lengths of a batch may differ as they like.  A unit that lies in several runs
+// is joined by join_kernel; a run has at most two parts of such units, one that the run begins inside of and one that it ends inside of.
+__device__ __forceinline__ int units_of(const AttnP& p, const Seq& q) { return !q.ok || q.n == 0 || q.n >= p.from_rows ? 0 : p.H * ((q.n * p.G + p.cols - 1) / p.cols); }
+__device__ __forceinline__ int tiles_of(const AttnP& p, const Seq& q) { return Tiles<5>(q.before, q.before + q.n - 1, p.window, p.sinks).n; }
+__device__ __forceinline__ long long work_of(const AttnP& p, int s) {
+  const Seq q = sequence(p.b, s, p.P);
+  const int u = units_of(p, q);
+  return u ? (long long)u * tiles_of(p, q) : 0;
+}
+struct Run { long long from, to, base; int s; };      // this CTA's tiles; the sequence that it begins in and the tiles in front of that
+// by all threads of the block
+__device__ __forceinline__ Run run_of(const AttnP& p) {
+  __shared__ long long sums[FEW_WARPS];
+  __shared__ Run found;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long mine = 0, first = 0;
+  for (int s = threadIdx.x; s < p.b.S; s += FEW_THREADS) {
+    const long long w = work_of(p, s);
+    if (s == (int)threadIdx.x) first = w;
+    mine += w;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) sums[warp] = mine;
+  if (threadIdx.x == 0) found.s = -1;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < FEW_WARPS; ++w) total += sums[w];
+  long long run = (total + gridDim.x - 1) / gridDim.x;
+  run = max((run + FEW_WARPS - 1) / FEW_WARPS * FEW_WARPS, (long long)MIN_RUN);
+  Run r;
+  r.from = run * blockIdx.x; r.to = min(r.from + run, total); r.s = -1; r.base = 0;
+  if (r.from >= total) return r;
+  long long base = 0;
+  for (int s0 = 0; s0 < p.b.S; s0 += FEW_THREADS) {
+    const int s = s0 + (int)threadIdx.x;
+    const long long w = s0 == 0 ? first : s < p.b.S ? work_of(p, s) : 0;
+    long long in = w;                        // inclusive sums of the warp, then of the block
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, in, o);
+      if (lane >= o) in += x;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = in;
+    __syncthreads();
+    long long all = 0;
+#pragma unroll
+    for (int i = 0; i < FEW_WARPS; ++i) {
+      if (i < warp) in += sums[i];
+      all += sums[i];
+    }
+    if (base + in - w <= r.from && r.from < base + in) { found.s = s; found.base = base + in - w; }
+    __syncthreads();
+    if (found.s >= 0) break;
+    base += all;
+  }
+  r.s = found.s; r.base = found.base;
+  return r;
+}
+
+// int8 and eight columns: the codes of K go into the product as they are, and Q as three digits of 8 bits: 22 bits below the column's largest value, where f16 keeps 11 bits of each
+// value; sums are exact.  Three products of 32 dimensions are dearer than two of 16 by half, but the 160 instructions that make f16 of a tile's keys fall away.  More columns
+// share the conversion, and the digits' registers are not there.  (e4m3 by e4m3 is no instruction of its own: it takes as many products and conversions as f16.)
+constexpr bool few_digits(int fmt, int nt) { return fmt == INT8 && nt == 1; }
+constexpr int SEEN = 1, IN_PART = 0, HIDDEN = -1;      // a half of a tile: by all columns, by some, by none
+// four integers of up to 2^22 = 65536 x2 + 256 x1 + x0 with digits of -128 .. 127
+__device__ __forceinline__ void digits(float a, float b, float c, float d, uint32_t& d0, uint32_t& d1, uint32_t& d2) {
+  const int n[4] = {__float2int_rn(a), __float2int_rn(b), __float2int_rn(c), __float2int_rn(d)};
+  d0 = d1 = d2 = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int x0 = (int)(int8_t)n[i], n1 = (n[i] - x0) >> 8, x1 = (int)(int8_t)n1, x2 = (n1 - x1) >> 8;
+    d0 |= ((uint32_t)x0 & 255u) << (8 * i); d1 |= ((uint32_t)x1 & 255u) << (8 * i); d2 |= ((uint32_t)x2 & 255u) << (8 * i);
+  }
+}
+// sums n of up to 128 * 128 * 127 < 2^21 begin at the bits of 1.5 * 2^23, and so end as those of 1.5 * 2^23 + n
+constexpr uint32_t DIGIT_ZERO = 0x4b400000u;
+__device__ __forceinline__ float digit_sum(uint32_t a0, uint32_t a1, uint32_t a2) {
+  const float f0 = __uint_as_float(a0) - 12582912.f, f1 = __uint_as_float(a1) - 12582912.f, f2 = __uint_as_float(a2) - 12582912.f;
+  return fmaf(f2, 65536.f, fmaf(f1, 256.f, f0));
+}
+__device__ __forceinline__ void mma_s8(uint32_t* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Tiles lie in shared memory as the copies swizzle them: 16-byte piece n of row r.
+template <int D>
+__device__ __forceinline__ int piece(int r, int n) { return D == 128 ? r * 128 + ((n ^ (r & 7)) << 4) : r * 64 + ((n ^ ((r >> 1) & 3)) << 4); }
+// Which token is row i (and i + 8) of the fragments: an order in which neither the keys' nor the values' reads meet in a bank.  Eight lanes read keys of rows token_of(2 m), token_of(2 m + 1),
+// four pieces of each, and values of rows token_of(2 c) (or 2 c + 1), c = 0 .. 3, two pieces of each.
+template <int D>
+__device__ __forceinline__ int token_of(int i) { return (D == 128 ? 0x37156240u : 0x67542310u) >> (4 * i) & 7; }
+
+template <int D, int FMT, int NT>
+__global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnP p) {
+  constexpr int KS = D / 16, MT = D / 16, COLS = 8 * NT, SIDE = 32 * D;        // bytes of a tile's keys or values
+  constexpr bool DIGITS = few_digits(FMT, NT);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const ring = smem_raw + ((1024u - (tcp::smem_u32(smem_raw) & 1023u)) & 1023u);       // [warp]: two tiles of keys, two of values, as the copies swizzle them
+  __shared__ __align__(8) uint64_t bars[FEW_WARPS][4];                        // a ring's places
+  __shared__ volatile int quit;
+  __shared__ float4 meta[FEW_WARPS][64];                                      // per half of a tile: who sees it, keys' scale, log2 and reciprocal of the values'
+  __shared__ int rows_at[FEW_WARPS][64];                                      // and the row of codes that it begins at
+  __shared__ float m_s[FEW_WARPS][8], l_s[FEW_WARPS][8];
+  typedef float Sums[8][D + 4];
+  Sums* o_s = reinterpret_cast<Sums*>(ring);                                  // the warps' sums, when the ring is empty
+  const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, c = lane & 3;
+  const uint32_t bar = tcp::smem_u32(&bars[warp][0]);
+  if (lane < 4) tcp::mbar_init(bar + 8 * lane, 1);
+  if (threadIdx.x == 0) quit = 0;
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  const int key_row = token_of<D>(g), val_row[2] = {token_of<D>(2 * c), token_of<D>(2 * c + 1)};
+  int used = 0;                              // tiles that went through this warp's ring
+  pdl_trigger();
+  pdl_wait();
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < p.b.S; i += FEW_THREADS)
+      if (!sequence(p.b, i, p.P).ok) flag(p.flags, B200_PAGED_BAD_BATCH);
+  Run run = run_of(p);
+  if (run.s < 0) return;
+  int s = run.s, n_tiles = 1, n_units = 0;
+  long long base = run.base;
+  Seq q;
+  q = sequence(p.b, s, p.P);
+  n_units = units_of(p, q);
+  n_tiles = n_units ? tiles_of(p, q) : 1;
+  for (long long f = run.from; f < run.to;) {
+    while (f >= base + (long long)n_units * n_tiles && s + 1 < p.b.S) {        // the next sequence that has work
+      base += (long long)n_units * n_tiles;
+      ++s;
+      q = sequence(p.b, s, p.P);
+      n_units = units_of(p, q);
+      n_tiles = n_units ? tiles_of(p, q) : 1;
+    }
+    const int unit = (int)((f - base) / n_tiles), u0 = (int)((f - base) - (long long)unit * n_tiles), u1 = (int)min((long long)n_tiles, u0 + (run.to - f));
+    f += u1 - u0;
+    const int h = unit % p.H, ct = unit / p.H, c0 = ct * COLS, n_cols = q.n * p.G;
+    const int pf = q.before + c0 / p.G, pl = q.before + (min(c0 + COLS, n_cols) - 1) / p.G;
+    const Tiles<5> tiles(pf, pl, p.window, p.sinks);
+    const int t0 = min(u0, tiles.n), t1 = min(u1, tiles.n);                   // a column tile may see fewer keys than its sequence
+
+    // queries: lane (g, c) has of column 8 nt + g the dimensions 64 i + 16 c .. + 15, as f16 or as three digits of 8 bits
+    uint32_t qf[DIGITS ? 1 : NT][KS][2], qd[3][KS / 2][2];
+    float fac[NT][2];                        // of columns 8 nt + 2 c, + 1: what turns a product of codes into a score in base 2
+    int pos[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int col = c0 + nt * 8 + g;
+      const bool has = col < n_cols;
+      const int i = has ? col / p.G : 0;
+      const bf16* row = p.q + (long long)(q.r0 + i) * p.q_ld + (long long)(h * p.G + (has ? col - i * p.G : 0)) * D;
+      uint32_t raw[KS][2];
+#pragma unroll
+      for (int b = 0; b < D / 64; ++b) {
+        const uint4 x = has ? *reinterpret_cast<const uint4*>(row + 64 * b + 16 * c) : make_uint4(0, 0, 0, 0);
+        const uint4 y = has ? *reinterpret_cast<const uint4*>(row + 64 * b + 16 * c + 8) : make_uint4(0, 0, 0, 0);
+        raw[4 * b][0] = x.x; raw[4 * b][1] = x.y; raw[4 * b + 1][0] = x.z; raw[4 * b + 1][1] = x.w;
+        raw[4 * b + 2][0] = y.x; raw[4 * b + 2][1] = y.y; raw[4 * b + 3][0] = y.z; raw[4 * b + 3][1] = y.w;
+      }
+      float top = 0.f;                       // of the column's finite values; infinity if there are others
+      bool odd = false;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 v = unpack_bf16(raw[k][e]);
+          odd |= !(fabsf(v.x) < INFINITY) || !(fabsf(v.y) < INFINITY);
+          top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+        }
+      if (odd) top = INFINITY;
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float power = top > 0.f ? power_of_two_in(top) : 1.f;
+      constexpr float LAND = DIGITS ? 2097152.f : 16384.f;       // the column's largest lands in [LAND, 2 LAND)
+      const float up = LAND / power;
+      if constexpr (DIGITS) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const float2 u = unpack_bf16(raw[k][0]), v = unpack_bf16(raw[k][1]);
+          digits(u.x * up, u.y * up, v.x * up, v.y * up, qd[0][k >> 1][k & 1], qd[1][k >> 1][k & 1], qd[2][k >> 1][k & 1]);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 v = unpack_bf16(raw[k][e]);
+            qf[DIGITS ? 0 : nt][k][e] = pack_f16(v.x * up, v.y * up);
+          }
+      }
+      const float back = top < INFINITY ? power * (1.f / LAND) : NAN;         // such a column's results are NaN, and no other's
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        fac[nt][e] = __shfl_sync(0xffffffffu, back, (2 * c + e) * 4) * p.scale2;
+        const int cc = c0 + nt * 8 + 2 * c + e;
+        pos[nt][e] = cc < n_cols ? q.before + cc / p.G : -1;
+      }
+    }
+
+    float o[NT][MT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+
+    const int32_t* table = p.b.table + s * p.b.table_ld;
+    const int first = t0 + warp, count = first < t1 ? (t1 - first + FEW_WARPS - 1) / FEW_WARPS : 0;      // this warp's tiles
+    uint8_t* const my_ring = ring + warp * 4 * SIDE;
+    const uint32_t ring_at = tcp::smem_u32(my_ring);
+    // the warp's i-th tile on its way into the ring; every 16 tiles the lanes look up the pages of their halves
+    auto fetch = [&](int i, const CUtensorMap& map, int side) {
+      const int place = side + ((used + i) & 1);
+      const int r0 = rows_at[warp][(2 * i) & 63], r1 = rows_at[warp][(2 * i + 1) & 63];
+      if (tcp::elected()) {
+        const uint32_t to = ring_at + place * SIDE, b = bar + 8 * place;
+        tcp::mbar_expect_tx(b, (r0 >= 0 ? SIDE / 2 : 0) + (r1 >= 0 ? SIDE / 2 : 0));
+        if (r0 >= 0) tcp::tma_load_2d(to, &map, b, 0, r0);
+        if (r1 >= 0) tcp::tma_load_2d(to + SIDE / 2, &map, b, 0, r1);
+      }
+      __syncwarp();
+    };
+    auto arrived = [&](int i, int side) {
+      const uint32_t n = (uint32_t)(used + i);
+      if (!wait_or_quit(bar + 8 * (side + (n & 1)), (n >> 1) & 1u, &quit)) flag(p.flags, B200_PAGED_WAIT);
+      __syncwarp();
+    };
+    auto issue_keys = [&](int i) {
+      if (i >= count) return;
+      if ((i & 15) == 0) {
+        float4 x = make_float4(__int_as_float(HIDDEN), 0.f, -INFINITY, 0.f);
+        int off = -1;
+        const int mine = i + (lane >> 1), j = mine < count ? (tiles[first + mine * FEW_WARPS] << 5) + 16 * (lane & 1) : 0;
+        if (mine < count && j <= pl && (p.window <= 0 || pf - j - 15 < p.window || j < p.sinks)) {
+          const int page = table[j >> p.page_shift];
+          if (page >= 0 && page < p.pages) {
+            const bool all = j + 15 <= pf && (p.window <= 0 || pl - j < p.window || j + 16 <= p.sinks);
+            x.x = __int_as_float(all ? SEEN : IN_PART);
+            off = (page * p.H + h) * p.P + (j & (p.P - 1));
+            x.y = p.k_scale[(long long)page * p.H + h];
+            float vs = p.v_scale[(long long)page * p.H + h];
+            vs = vs > 0.f ? vs : 1.f;        // all codes of a page of zeros are 0
+            x.z = __log2f(vs); x.w = __frcp_rn(vs);
+          } else flag(p.flags, B200_PAGED_BAD_PAGE);
+        }
+        __syncwarp();
+        meta[warp][(2 * i + lane) & 63] = x;
+        rows_at[warp][(2 * i + lane) & 63] = off;
+        __syncwarp();
+      }
+      fetch(i, map_k, 0);
+    };
+    auto issue_values = [&](int i) {
+      if (i < count) fetch(i, map_v, 2);
+    };
+    struct Tile { float4 x[2]; bool whole; };
+    auto tile_at = [&](int i) {
+      Tile t;
+      t.x[0] = meta[warp][(2 * i) & 63];
+      t.x[1] = meta[warp][(2 * i + 1) & 63];
+      t.whole = __float_as_int(t.x[0].x) + __float_as_int(t.x[1].x) == 2 * SEEN;
+      return t;
+    };
+    // scores in base 2, log2 of the values' scale added
+    auto scores = [&](int i, const Tile& t, float (&sc)[2][NT][4]) {
+      const uint8_t* from = my_ring + ((used + i) & 1) * SIDE;
+      if constexpr (DIGITS) {
+        uint32_t acc[2][3][4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int d = 0; d < 3; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[half][d][e] = DIGIT_ZERO;
+#pragma unroll
+        for (int b = 0; b < D / 64; ++b)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint8_t* f_h = from + half * (SIDE / 2);
+            const uint4 r0 = *reinterpret_cast<const uint4*>(f_h + piece<D>(key_row, 4 * b + c)), r1 = *reinterpret_cast<const uint4*>(f_h + piece<D>(key_row + 8, 4 * b + c));
+#pragma unroll
+            for (int d = 0; d < 3; ++d) {
+              mma_s8(acc[half][d], r0.x, r1.x, r0.y, r1.y, qd[d][2 * b][0], qd[d][2 * b][1]);
+              mma_s8(acc[half][d], r0.z, r1.z, r0.w, r1.w, qd[d][2 * b + 1][0], qd[d][2 * b + 1][1]);
+            }
+          }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const float by[2] = {t.x[half].y * fac[0][0], t.x[half].y * fac[0][1]};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[half][0][e] = fmaf(digit_sum(acc[half][0][e], acc[half][1][e], acc[half][2][e]), by[e & 1], t.x[half].z);
+        }
+      } else {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) sc[half][nt][0] = sc[half][nt][1] = sc[half][nt][2] = sc[half][nt][3] = 0.f;
+#pragma unroll
+        for (int b = 0; b < D / 64; ++b)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint8_t* f_h = from + half * (SIDE / 2);
+            const uint4 r0 = *reinterpret_cast<const uint4*>(f_h + piece<D>(key_row, 4 * b + c)), r1 = *reinterpret_cast<const uint4*>(f_h + piece<D>(key_row + 8, 4 * b + c));
+            const uint32_t k0[4] = {r0.x, r0.y, r0.z, r0.w}, k1[4] = {r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t w0 = ready<FMT>(k0[k]), w1 = ready<FMT>(k1[k]);
+              const uint32_t a0 = half2_of<FMT, 0>(w0), a1 = half2_of<FMT, 0>(w1), a2 = half2_of<FMT, 1>(w0), a3 = half2_of<FMT, 1>(w1);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma_f16(sc[half][nt], a0, a1, a2, a3, qf[nt][4 * b + k][0], qf[nt][4 * b + k][1]);
+            }
+          }
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float by[2] = {t.x[half].y * fac[nt][0], t.x[half].y * fac[nt][1]};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[half][nt][e] = fmaf(sc[half][nt][e], by[e & 1], t.x[half].z);
+          }
+      }
+    };
+    uint32_t pb[2][NT][2];                   // weights of the tile whose values come next
+    // weights out of scores, and O and the sums brought to the maximum that they refer to
+    auto weigh = [&](int i, const Tile& t, float (&sc)[2][NT][4]) {
+      if (!t.whole) {
+        const int j0 = tiles[first + i * FEW_WARPS] << 5;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const bool has = __float_as_int(t.x[half].x) != HIDDEN;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!(has && sees(pos[nt][e & 1], j0 + 16 * half + key_row + 8 * (e >> 1), p.window, p.sinks))) sc[half][nt][e] = -INFINITY;
+        }
+      }
+      float top[NT][2];
+      bool grow = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          top[nt][e] = fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][e + 2]), fmaxf(sc[1][nt][e], sc[1][nt][e + 2]));
+          grow |= top[nt][e] > m[nt][e] + SLACK;
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float y = top[nt][e];
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
+            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+            const float now = fmaxf(m[nt][e], y), by = now == -INFINITY ? 1.f : exp2_fast(m[nt][e] - now);
+            m[nt][e] = now;
+            l[nt][e] *= by;
+#pragma unroll
+            for (int k = 0; k < MT; ++k) { o[nt][k][e] *= by; o[nt][k][e + 2] *= by; }
+          }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float off[2] = {m[nt][0] == -INFINITY ? 0.f : m[nt][0], m[nt][1] == -INFINITY ? 0.f : m[nt][1]};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = exp2_fast(sc[half][nt][e] - off[e & 1]);
+          l[nt][0] = fmaf(w[0] + w[2], t.x[half].w, l[nt][0]);
+          l[nt][1] = fmaf(w[1] + w[3], t.x[half].w, l[nt][1]);
+          pb[half][nt][0] = transposed8x8(pack_f16(w[0], w[1]));
+          pb[half][nt][1] = transposed8x8(pack_f16(w[2], w[3]));
+        }
+      }
+    };
+    // codes of tokens that no column sees may be anything: this lane's become 0
+    auto hide = [&](int i, const Tile& t) {
+      const int j0 = tiles[first + i * FEW_WARPS] << 5;
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const int r = val_row[a & 1] + 8 * (a >> 1), j = j0 + 16 * half + r;
+          if (__float_as_int(t.x[half].x) != HIDDEN && j <= pl && (p.window <= 0 || pf - j < p.window || j < p.sinks)) continue;
+          uint8_t* v = my_ring + (2 + ((used + i) & 1)) * SIDE + half * (SIDE / 2);
+          if constexpr (D == 128) *reinterpret_cast<uint4*>(v + piece<D>(r, g)) = make_uint4(0, 0, 0, 0);
+          else *reinterpret_cast<uint2*>(v + piece<D>(r, g >> 1) + 8 * (g & 1)) = make_uint2(0, 0);
+        }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");            // the next copy into this place comes behind these writes
+    };
+    auto add_values = [&](int i) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint8_t* f_h = my_ring + (2 + ((used + i) & 1)) * SIDE + half * (SIDE / 2);
+        uint32_t v[4][D / 32];
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const int r = val_row[a & 1] + 8 * (a >> 1);
+          if constexpr (D == 128) {
+            const uint4 w = *reinterpret_cast<const uint4*>(f_h + piece<D>(r, g));
+            v[a][0] = w.x; v[a][1] = w.y; v[a][2] = w.z; v[a][3] = w.w;
+          } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(f_h + piece<D>(r, g >> 1) + 8 * (g & 1));
+            v[a][0] = w.x; v[a][1] = w.y;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {   // four dimensions of this lane's
+          const uint32_t v0 = ready<FMT>(v[0][j]), v1 = ready<FMT>(v[1][j]), v2 = ready<FMT>(v[2][j]), v3 = ready<FMT>(v[3][j]);
+          const uint32_t lo = prmt(v0, v1, 0x5140u), hi = prmt(v0, v1, 0x7362u), lo8 = prmt(v2, v3, 0x5140u), hi8 = prmt(v2, v3, 0x7362u);
+          const uint32_t a[8] = {half2_of<FMT, 0>(lo), half2_of<FMT, 1>(lo), half2_of<FMT, 0>(lo8), half2_of<FMT, 1>(lo8),
+                                 half2_of<FMT, 0>(hi), half2_of<FMT, 1>(hi), half2_of<FMT, 0>(hi8), half2_of<FMT, 1>(hi8)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_f16(o[nt][2 * j], a[0], a[1], a[2], a[3], pb[half][nt][0], pb[half][nt][1]);
+            mma_f16(o[nt][2 * j + 1], a[4], a[5], a[6], a[7], pb[half][nt][0], pb[half][nt][1]);
+          }
+        }
+      }
+    };
+
+    // The scores of tile i + 1 and the values of tile i do not wait for one another, and lie in one stretch of code; behind them the weights of tile i + 1.
+    issue_keys(0);
+    issue_values(0);
+    issue_keys(1);
+    if (count) {
+      Tile t = tile_at(0);
+      float sc[2][NT][4];
+      arrived(0, 0);
+      scores(0, t, sc);
+      weigh(0, t, sc);
+      for (int i = 0; i + 1 < count; ++i) {
+        __syncwarp();                        // the places that these copies go to have been read
+        issue_values(i + 1);
+        issue_keys(i + 2);
+        arrived(i, 2);
+        if (!t.whole) hide(i, t);
+        t = tile_at(i + 1);
+        arrived(i + 1, 0);
+        scores(i + 1, t, sc);
+        add_values(i);
+        weigh(i + 1, t, sc);
+      }
+      arrived(count - 1, 2);
+      if (!t.whole) hide(count - 1, t);
+      add_values(count - 1);
+    }
+    used += count;
+
+    // join the warps, eight columns at a time
+    const bool alone = u0 == 0 && u1 == n_tiles;
+    const int slot = 2 * (int)blockIdx.x + (u0 == 0 ? 1 : 0);
+    if (u0 == 0 && threadIdx.x == 0) {       // where the unit's parts are: this run's and so many after it
+      const long long runs = run.to - run.from, left = n_tiles - u1;
+      p.parts[((long long)s * p.ctiles + ct) * p.H + h] = make_int2((int)blockIdx.x, alone ? 0 : (int)((left + runs - 1) / runs));
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if (c0 + nt * 8 >= n_cols) break;
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[nt][e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (g == 0) { m_s[warp][2 * c + e] = m[nt][e]; l_s[warp][2 * c + e] = sum; }
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) *reinterpret_cast<float2*>(&o_s[warp][2 * c + e][(D / 8) * g + 2 * i]) = make_float2(o[nt][i][e], o[nt][i][e + 2]);
+      __syncthreads();
+      constexpr int PER = D / 16;            // 16 threads a column
+      const int col = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * PER, cc = c0 + nt * 8 + col;
+      if (cc < n_cols) {
+        float top = -INFINITY, sum = 0.f, acc[PER];
+#pragma unroll
+        for (int w = 0; w < FEW_WARPS; ++w) top = fmaxf(top, m_s[w][col]);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < FEW_WARPS; ++w) {
+          const float by = m_s[w][col] == -INFINITY ? 0.f : exp2_fast(m_s[w][col] - top);
+          sum = fmaf(l_s[w][col], by, sum);
+#pragma unroll
+          for (int i = 0; i < PER; ++i) acc[i] = fmaf(o_s[w][col][d0 + i], by, acc[i]);
+        }
+        if (alone) store_row<D>(p, q, h, cc, d0, acc, sum);
+        else {
+          const long long at = (long long)slot * COLS + nt * 8 + col;
+          if ((threadIdx.x & 15) == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(top, sum);
+#pragma unroll
+          for (int i = 0; i < PER; i += 4) *reinterpret_cast<float4*>(p.part_o + at * D + d0 + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+        }
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();                         // the ring's next copies come behind these reads and writes
+  }
+  if (quit) {                                // let copies in flight land before the block ends
+    const uint64_t since = tcp::global_timer_ns();
+    while (tcp::global_timer_ns() - since < 2000000ull) {}
+  }
+}
+
+// Joins the parts of units that lie in several runs: a block a column, its eight teams of sixteen threads take the parts in turn.
+template <int D, int NT>
+__global__ void __launch_bounds__(128) join_kernel(const AttnP p) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int COLS = 8 * NT, PER = D / 16;
+  __shared__ float o_s[8][D + 4], m_s[8], l_s[8];
+  const int most = min(COLS, p.b.max_rows * p.G);       // columns of a unit
+  const int col = (int)(blockIdx.x % most), team = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * PER;
+  const long long unit = blockIdx.x / most;
+  const int h = (int)(unit % p.H), ct = (int)(unit / p.H % p.ctiles), s = (int)(unit / p.H / p.ctiles), cc = ct * COLS + col;
+  const Seq q = sequence(p.b, s, p.P);
+  if (units_of(p, q) == 0 || cc >= q.n * p.G) return;
+  const int2 parts = p.parts[unit];
+  if (parts.y == 0) return;
+  // the first part is its run's last, the others are their runs' first
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+  float top = -INFINITY, sum = 0.f, acc[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+#pragma unroll 2
+  for (int i = team; i <= parts.y; i += 8) {
+    const long long at = (long long)(2 * (parts.x + i) + (i == 0 ? 1 : 0)) * COLS + col;
+    const float2 y = ml[at];
+    const float now = fmaxf(top, y.x), keep = now == -INFINITY ? 0.f : exp2_fast(top - now), by = now == -INFINITY ? 0.f : exp2_fast(y.x - now);
+    const float4* o = reinterpret_cast<const float4*>(p.part_o + at * D + d0);
+    top = now;
+    sum = fmaf(sum, keep, y.y * by);
+#pragma unroll
+    for (int e = 0; e < PER / 4; ++e) {
+      const float4 v = o[e];
+      acc[4 * e] = fmaf(acc[4 * e], keep, v.x * by); acc[4 * e + 1] = fmaf(acc[4 * e + 1], keep, v.y * by);
+      acc[4 * e + 2] = fmaf(acc[4 * e + 2], keep, v.z * by); acc[4 * e + 3] = fmaf(acc[4 * e + 3], keep, v.w * by);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < PER; ++e) o_s[team][d0 + e] = acc[e];
+  if ((threadIdx.x & 15) == 0) { m_s[team] = top; l_s[team] = sum; }
+  __syncthreads();
+  if (team) return;
+  top = -INFINITY; sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, m_s[i]);
+#pragma unroll
+  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float by = m_s[i] == -INFINITY ? 0.f : exp2_fast(m_s[i] - top);
+    sum = fmaf(l_s[i], by, sum);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] = fmaf(o_s[i][d0 + e], by, acc[e]);
+  }
+  store_row<D>(p, q, h, cc, d0, acc, sum);
+}
+
 // =========================================================================================================================
 // host
 // =========================================================================================================================
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
 int check_cache(const b200_paged_cache* c, const char* what) {
   if (!c || !c->k_dev || !c->v_dev || !c->k_scale_dev || !c->v_scale_dev || !c->flags_dev) B200_FAIL(B200_ERR_INVALID, "%s: null pointer in the cache", what);
   if (c->kv_dtype != B200_KV_INT8 && c->kv_dtype != B200_KV_FP8_E4M3) B200_FAIL(B200_ERR_INVALID, "%s: kv_dtype %d", what, c->kv_dtype);
   if (c->dim != 64 && c->dim != 128) B200_FAIL(B200_ERR_SHAPE, "%s: head size %d (64 or 128)", what, c->dim);
   if (c->page_tokens != 16 && c->page_tokens != 32 && c->page_tokens != 64 && c->page_tokens != 128) B200_FAIL(B200_ERR_SHAPE, "%s: pages of %d tokens (16, 32, 64 or 128)", what, c->page_tokens);
-  if (c->pages < 1 || c->kv_heads < 1 || c->kv_heads > 1024) B200_FAIL(B200_ERR_SHAPE, "%s: %d pages, %d heads", what, c->pages, c->kv_heads);
+  if (c->pages < 1 || c->kv_heads < 1 || c->kv_heads > 1024 || (long long)c->pages * c->kv_heads * c->page_tokens > 0x7fffff00ll) B200_FAIL(B200_ERR_SHAPE, "%s: %d pages, %d heads", what, c->pages, c->kv_heads);
   if ((reinterpret_cast<uintptr_t>(c->k_dev) | reinterpret_cast<uintptr_t>(c->v_dev)) & 15) B200_FAIL(B200_ERR_INVALID, "%s: the cache's codes must begin on a 16-byte border", what);
   return B200_OK;
 }
@@ -709,9 +954,8 @@ Batch batch_of(const b200_paged_batch* b) {
 bool rows_fit(const void* p, long long ld, int heads, int dim) { return p && !(reinterpret_cast<uintptr_t>(p) & 15) && ld >= (long long)heads * dim && ld % 8 == 0; }
 int shift_of(int P) { return P == 16 ? 4 : P == 32 ? 5 : P == 64 ? 6 : 7; }
 
-// How the keys of a step are cut.  CTAs of 8 * nt columns; ranges so that the chip has about one wave of CTAs (four to an SM, 148 SMs), none shorter than 16 tiles
-// (two rounds of a CTA's warps, twice) by the longest that the tables allow.
-struct FewPlan { int nt, ctiles, nsplit; long long units; };
+// CTAs of 8 * nt columns, about one wave of them (four, three or two to an SM), fewer where the tables allow for less work than that.
+struct FewPlan { int nt, ctiles, ctas; long long units; };
 FewPlan few_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks, int few_rows) {
   FewPlan f;
   const long long rows = few_rows < b->max_rows ? few_rows : b->max_rows, cols = rows * G;
@@ -720,24 +964,50 @@ FewPlan few_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, in
   f.units = (long long)b->sequences * c->kv_heads * f.ctiles;
   long long keys = (long long)b->table_width * c->page_tokens;
   if (window > 0 && (long long)window + sinks + rows < keys) keys = (long long)window + sinks + rows;
-  const long long tiles = ceil_div64(keys, 16), slots = 148 * (f.nt == 1 ? 4 : f.nt == 2 ? 3 : 2);
-  long long n = f.units ? slots / f.units : 1;
-  if (n > tiles / 16) n = tiles / 16;
-  f.nsplit = n < 1 ? 1 : n > 256 ? 256 : (int)n;
+  const long long runs = ceil_div64(f.units * (ceil_div64(keys, 32) + 2), MIN_RUN), wave = 148 * few_per_sm(f.nt);
+  f.ctas = (int)(runs < wave ? runs : wave);
   return f;
 }
+// sums and (maximum, sum of the weights) of two parts per CTA, and where each unit's parts are
+int64_t few_bytes(const FewPlan& f, int D) { return (int64_t)f.ctas * 2 * 8 * f.nt * (D + 2) * 4 + f.units * 8; }
+
+}  // namespace
+
+int code_map(CUtensorMap* m, const void* codes, long long rows, int dim, int box_rows) {
+  static const EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  if (!fn) B200_FAIL(B200_ERR_CUDA, "cuTensorMapEncodeTiled not available");
+  cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)dim};
+  cuuint32_t box[2] = {(cuuint32_t)dim, (cuuint32_t)box_rows}, est[2] = {1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, est, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) B200_FAIL(B200_ERR_CUDA, "paged cache: tensor map of %lld rows of %d codes refused (%d)", rows, dim, (int)r);
+  return B200_OK;
+}
+
+namespace {
 
 template <int D, int FMT, int NT>
-int launch_few(const AttnP& p, long long units, cudaStream_t st) {
-  B200_TRY(launch_early(few_rows_kernel<D, FMT, NT>, dim3((unsigned)(units * p.nsplit)), dim3(FEW_THREADS), 0, st, p));
-  if (p.nsplit > 1) B200_TRY(launch_early(join_kernel<D, NT>, dim3((unsigned)(units * NT)), dim3(128), 0, st, p));
-  return B200_OK;
+int launch_few(const AttnP& p, const FewPlan& f, cudaStream_t st) {
+  constexpr int ring = FEW_WARPS * 4 * 32 * D, sums = FEW_WARPS * 8 * (D + 4) * 4, smem = (ring > sums ? ring : sums) + 1024;
+  static std::atomic<uint64_t> limits{0};
+  CUtensorMap map_k, map_v;
+  B200_TRY(code_map(&map_k, p.k, (long long)p.pages * p.H * p.P, D, 16));
+  B200_TRY(code_map(&map_v, p.v, (long long)p.pages * p.H * p.P, D, 16));
+  B200_TRY(allow_smem(limits, smem, few_rows_kernel<D, FMT, NT>));
+  B200_TRY(launch_early(few_rows_kernel<D, FMT, NT>, dim3((unsigned)f.ctas), dim3(FEW_THREADS), smem, st, map_k, map_v, p));
+  const long long most = (long long)p.b.max_rows * p.G < 8 * NT ? (long long)p.b.max_rows * p.G : 8 * NT;
+  return launch_early(join_kernel<D, NT>, dim3((unsigned)(f.units * most)), dim3(128), 0, st, p);
 }
 template <int D, int FMT>
 int launch_few_nt(const AttnP& p, const FewPlan& f, cudaStream_t st) {
-  if (f.nt == 1) return launch_few<D, FMT, 1>(p, f.units, st);
-  if (f.nt == 2) return launch_few<D, FMT, 2>(p, f.units, st);
-  return launch_few<D, FMT, 4>(p, f.units, st);
+  if (f.nt == 1) return launch_few<D, FMT, 1>(p, f, st);
+  if (f.nt == 2) return launch_few<D, FMT, 2>(p, f, st);
+  return launch_few<D, FMT, 4>(p, f, st);
 }
 
 template <int FMT, int D>
@@ -822,7 +1092,7 @@ int64_t b200_paged_attention_bytes(const b200_paged_cache* cache, const b200_pag
   if (!cache || !batch || cache->kv_heads < 1 || q_heads < cache->kv_heads || q_heads % cache->kv_heads || window < 0 || sinks < 0 || batch->sequences < 1 || batch->max_rows < 0) return 0;
   const int G = q_heads / cache->kv_heads;
   const FewPlan f = few_plan(cache, batch, G, window, sinks, 0x7fffffff);
-  return f.nsplit > 1 ? f.units * f.nsplit * 8 * f.nt * (cache->dim + 2) * (int64_t)sizeof(float) : 0;
+  return few_bytes(f, cache->dim);
 }
 
 int b200_paged_attention(const b200_paged_cache* cache, const b200_paged_batch* batch, const void* q_dev, int64_t q_ld, void* out_dev, int64_t out_ld, int q_heads,
@@ -844,15 +1114,13 @@ int b200_paged_attention(const b200_paged_cache* cache, const b200_paged_batch* 
   p.window = window; p.sinks = sinks; p.scale2 = scale * LOG2E;
   p.from_rows = 0x7fffffff; p.q_tiles = 0;
   const FewPlan f = few_plan(cache, batch, p.G, window, sinks, p.from_rows);
-  if (f.units * f.nsplit > 0x7fffffffll / 4) B200_FAIL(B200_ERR_SHAPE, "paged_attention: %d sequences of up to %d rows with %d heads in one call", batch->sequences, batch->max_rows, q_heads);
-  p.nsplit = f.nsplit; p.ctiles = f.ctiles; p.part_o = p.part_ml = nullptr;
-  if (f.nsplit > 1) {
-    const long long cols = f.units * f.nsplit * 8 * f.nt;
-    if (!work_dev || work_bytes < cols * (D + 2) * (long long)sizeof(float) || (reinterpret_cast<uintptr_t>(work_dev) & 15))
-      B200_FAIL(B200_ERR_INVALID, "paged_attention: a workspace of %lld bytes, b200_paged_attention_bytes asks for %lld on a 16-byte border", (long long)work_bytes, cols * (D + 2) * 4ll);
-    p.part_o = static_cast<float*>(work_dev);
-    p.part_ml = p.part_o + cols * D;
-  }
+  if (f.units > 0x7fffffffll / 64 || (long long)batch->max_rows * p.G > 0x3fffffffll) B200_FAIL(B200_ERR_SHAPE, "paged_attention: %d sequences of up to %d rows with %d heads in one call", batch->sequences, batch->max_rows, q_heads);
+  if (!work_dev || work_bytes < few_bytes(f, D) || (reinterpret_cast<uintptr_t>(work_dev) & 15))
+    B200_FAIL(B200_ERR_INVALID, "paged_attention: a workspace of %lld bytes; b200_paged_attention_bytes asks for %lld, on a 16-byte border", (long long)work_bytes, (long long)few_bytes(f, D));
+  p.cols = 8 * f.nt; p.ctiles = f.ctiles;
+  p.part_o = static_cast<float*>(work_dev);
+  p.part_ml = p.part_o + (long long)f.ctas * 2 * p.cols * D;
+  p.parts = reinterpret_cast<int2*>(p.part_ml + (long long)f.ctas * 2 * p.cols * 2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool i8 = cache->kv_dtype == B200_KV_INT8;
   if (D == 128) B200_TRY((i8 ? launch_few_nt<128, INT8>(p, f, st) : launch_few_nt<128, E4M3>(p, f, st)));

@@ -1,10 +1,12 @@
 // What the kernels of the paged 8-bit cache share (paged.cu: append, read, attention of few rows; paged_prompt.cu: attention of many rows of a sequence).
 #pragma once
 
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include "common.cuh"
+#include "tc_prims.cuh"
 
 namespace b200 {
 namespace paged {
@@ -99,8 +101,9 @@ struct AttnP {
   int window, sinks;
   float scale2;                              // score scale * log2(e)
   // few rows
-  int nsplit, ctiles;
-  float *part_o, *part_ml;
+  int cols, ctiles;                          // columns of a unit, units of a sequence and kv head
+  float *part_o, *part_ml;                   // [CTAs][2][cols][D], [CTAs][2][cols][2]
+  int2* parts;                               // [sequences][ctiles][H]: first CTA and number of further ones of a unit
   // many rows
   int from_rows, q_tiles;                    // sequences of fewer rows than this are the other kernel's
 };
@@ -118,6 +121,28 @@ struct Tiles {
   __device__ __forceinline__ int operator[](int i) const { return i < first ? i : from + i - first; }
 };
 __device__ __forceinline__ bool sees(int p, int j, int window, int sinks) { return j <= p && (window <= 0 || p - j < window || j < sinks); }
+
+// A wait of ten seconds at most; `quit`: somebody of the block has waited that long, and nobody waits any more.
+__device__ __forceinline__ bool wait_or_quit(uint32_t bar, uint32_t parity, volatile int* quit) {
+  uint32_t done, spins = 0;
+  uint64_t t0 = 0;
+  for (;;) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    if (done) return true;
+    if ((++spins & 1023u) == 0u) {
+      if (*quit) return false;
+      const uint64_t now = tcp::global_timer_ns();
+      if (t0 == 0) t0 = now;
+      else if (now - t0 > tcp::WAIT_LIMIT_NS) { *quit = 1; return false; }
+    }
+  }
+}
+// paged.cu: a tensor map over a cache's codes, [rows][dim], boxes of box_rows whole rows, swizzled by 128 bytes (dim 64: by 64)
+int code_map(CUtensorMap* m, const void* codes, long long rows, int dim, int box_rows);
 
 // paged_prompt.cu
 int prompt_rows(int dim, int G);                                             // from how many rows on a sequence is taken there

@@ -14,7 +14,6 @@ from __future__ import annotations
 
 import ctypes as C
 import typing as tp
-from fractions import Fraction
 
 import torch
 
@@ -23,7 +22,8 @@ from ..config import ROT_PAIRINGS
 
 _KV = {"int8": (torch.int8, _lib.B200_KV_INT8), "fp8_e4m3": (torch.float8_e4m3fn, _lib.B200_KV_FP8_E4M3)}
 _NAMES = {dtype: name for name, (dtype, _) in _KV.items()}
-_PI = Fraction(314159265358979323846264338327950288419716939937510, 10 ** 50)
+# floor(2^192 / (2 pi))
+_TURN = (1 << 192) * 10 ** 60 // (2 * 3141592653589793238462643383279502884197169399375105820974944)
 BAD_BATCH, BAD_PAGE, NOT_FINITE, WAIT = 1, 2, 4, 8
 
 
@@ -54,7 +54,7 @@ class RotaryTable:
         if len(freqs) != rot_dims // 2:
             raise ValueError(f"{len(freqs)} frequencies for {rot_dims} dimensions")
         # turns per position as a 64-bit fraction: its product with a position drops whole turns and nothing else
-        turns = [int(Fraction(f) / (2 * _PI) * (1 << 64) + Fraction(1, 2)) % (1 << 64) for f in freqs]
+        turns = [((num * _TURN // den + (1 << 127)) >> 128) % (1 << 64) for num, den in (f.as_integer_ratio() for f in freqs)]
         self.device = _cuda(device)
         self.rot_dims, self.pairing = rot_dims, pairing
         self.turns = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64, device=self.device)

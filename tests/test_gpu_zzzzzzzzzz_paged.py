@@ -120,32 +120,39 @@ def test_a_query_that_is_not_finite_spoils_its_own_results_only(new):
 def test_what_does_not_fit_is_left_out_and_recorded(new):
     c = Content([100 + new, 200 + new], 2, 64, 16, "int8")
     cache, q = c.cache(), torch.randn(2 * new, 2, 64).bfloat16().cuda()
-    want = cache.attend(batch_of(c.table, [100, 200], [new, new]), q)
+    exact = [oracle.attend(q[new * s:new * (s + 1)].double().cpu(), *c.kvt(s), (100, 200)[s], 0.125) for s in (0, 1)]
 
-    def run(table, before, rows, **kw):
+    def good(out, s):
+        want, tol = exact[s]
+        return bool(((out[new * s:new * (s + 1)].double().cpu() - want).abs() <= tol).all())
+
+    def untouched(out, s):
+        return bool((out[new * s:new * (s + 1)] == 7).all())
+
+    def run(table, before, rows, max_rows=None):
         out = torch.full_like(q, 7.0)
-        cache.attend(PagedBatch(*(torch.tensor(x, dtype=torch.int32).cuda() if not torch.is_tensor(x) else x.cuda() for x in (table, before, rows)), 2 * new, **kw), q, out=out)
+        cache.attend(PagedBatch(table.cuda(), *(torch.tensor(x, dtype=torch.int32).cuda() for x in (before, rows)), 2 * new, max_rows), q, out=out)
         flags = cache.error_flags()
         cache.clear_error_flags()
         return out, flags
     rows = [0, new, 2 * new]
-    for before, r, kw in (([-1, 200], rows, {}), ([2 ** 31 - 1, 200], rows, {}), ([100000, 200], rows, {}), ([100, 200], [-5, new, 2 * new], {})):
-        out, flags = run(c.table, before, r, max_rows=new, **kw)
-        assert flags == paged.BAD_BATCH and bool((out[:new] == 7).all()) and torch.equal(out[new:], want[new:])
-    out, flags = run(c.table, [100, 200], [0, new, 2 * new + 1], max_rows=2 * new)
-    assert flags == paged.BAD_BATCH and torch.equal(out[:new], want[:new]) and bool((out[new:] == 7).all())
+    for before, r in (([-1, 200], rows), ([2 ** 31 - 1, 200], rows), ([100000, 200], rows), ([100, 200], [-5, new, 2 * new])):
+        out, flags = run(c.table, before, r, new)
+        assert flags == paged.BAD_BATCH and untouched(out, 0) and good(out, 1), before
+    out, flags = run(c.table, [100, 200], [0, new, 2 * new + 1])
+    assert flags == paged.BAD_BATCH and good(out, 0) and untouched(out, 1)
     if new > 1:
-        out, flags = run(c.table, [100, 200], [0, new, 2 * new], max_rows=new - 1)
-        assert flags == paged.BAD_BATCH and bool((out == 7).all())
+        out, flags = run(c.table, [100, 200], rows, new - 1)
+        assert flags == paged.BAD_BATCH and untouched(out, 0) and untouched(out, 1)
     for bad in (-1, c.pages, 2 ** 31 - 1):
         table = c.table.clone()
         table[0, 2] = bad
         out, flags = run(table, [100, 200], rows)
-        assert flags == paged.BAD_PAGE and torch.equal(out[new:], want[new:])
+        assert flags == paged.BAD_PAGE and good(out, 1)
         k, v, top = (torch.cat((x[:32], x[48:])) for x in c.kvt(0))
         if new == 1:                                     # its tokens are left out
-            exact, tol = oracle.attend(q[:1].double().cpu(), k, v, top, len(k), 0.125)
-            assert bool(((out[:1].double().cpu() - exact).abs() <= tol).all())
+            want, tol = oracle.attend(q[:1].double().cpu(), k, v, top, len(k), 0.125)
+            assert bool(((out[:1].double().cpu() - want).abs() <= tol).all())
 
 
 # ------------------------------------------------------------------------------------------------------------------------
@@ -384,10 +391,16 @@ def test_shared_pages_of_a_prefix():
     k, v, q = (torch.randn(40, h, dim).bfloat16().cuda() for h in (2, 2, 4))
     batch = batch_of(table, [64, 64], [20, 20])
     cache.append(batch, k, v)
-    both = cache.attend(batch, q)
-    assert torch.equal(both[:20], cache.attend(batch_of(table[:1], [64], [20]), q[:20].clone()))
-    assert torch.equal(both[20:], cache.attend(batch_of(table[1:], [64], [20]), q[20:].clone()))
-    assert torch.equal(cache.k.cpu()[c.table[0].long()], c.codes[0].to(torch.int8)[c.table[0].long()])
+    out = cache.attend(batch, q)
+    codes = [x.float().double().cpu() for x in (cache.k, cache.v)]
+    scales = [x.double().cpu() for x in (cache.k_scale, cache.v_scale)]
+    assert torch.equal(codes[0][c.table[0].long()], c.codes[0][c.table[0].long()])
+    for s in range(2):
+        pg = table[s].long()
+        kk, vv, top = (x.transpose(1, 2).reshape(-1, 2, x.shape[3])[:84] for x in (codes[0][pg] * scales[0][pg][..., None, None], codes[1][pg] * scales[1][pg][..., None, None],
+                                                                                       (127 * scales[1][pg][..., None, None]).expand(-1, -1, page, 1)))
+        want, tol = oracle.attend(q[20 * s:20 * s + 20].double().cpu(), kk, vv, top[..., 0], 64, dim ** -0.5)
+        assert bool(((out[20 * s:20 * s + 20].double().cpu() - want).abs() <= tol).all())
 
 
 @pytest.mark.parametrize("new", [1, 6, 200])
