@@ -320,7 +320,8 @@ __global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadP p) {
 // values goes into the exponent, P = 2^(score + log2 s_v - M), with M the running maximum of the same, and the sum of the weights takes P / s_v: nothing is rounded on the way but P.
 // M follows only when a score passes it by 2^8, as then no column has to be compared across lanes for most tiles.
 constexpr int FEW_WARPS = 4, FEW_THREADS = FEW_WARPS * 32;
-constexpr int few_per_sm(int nt) { return nt <= 2 ? 3 : 2; }      // CTAs, by their registers
+constexpr int few_per_sm(int nt) { return 2; }      // CTAs, by their registers
+constexpr int DIRECT_TILES = 33;             // units of at most this many tiles are not cut where the chip holds all of them at once: no join
 constexpr int MIN_RUN = 8;                    // tiles of a CTA
 constexpr float SLACK = 8.f;
 
@@ -356,15 +357,26 @@ __device__ __forceinline__ void store_row(const AttnP& p, const Seq& q, int h, i
 // The tiles of all units (sequence, column tile, kv head) one behind the other are cut into equal runs, one per CTA: lengths of a batch may differ as they like.  A unit that lies in several runs
 // is joined by join_kernel; a run has at most two parts of such units, one that the run begins inside of and one that it ends inside of.
 __device__ __forceinline__ int units_of(const AttnP& p, const Seq& q) { return !q.ok || q.n == 0 || q.n >= p.from_rows ? 0 : p.H * ((q.n * p.G + p.cols - 1) / p.cols); }
+// What joining the warps, the first loads and the queries cost a unit, in tiles: a run of many short units is shorter.
+constexpr int UNIT_COST = 12;
 __device__ __forceinline__ int tiles_of(const AttnP& p, const Seq& q) { return Tiles<5>(q.before, q.before + q.n - 1, p.window, p.sinks).n; }
 __device__ __forceinline__ long long work_of(const AttnP& p, int s) {
   const Seq q = sequence(p.b, s, p.P);
   const int u = units_of(p, q);
-  return u ? (long long)u * tiles_of(p, q) : 0;
+  return u ? (long long)u * (tiles_of(p, q) + UNIT_COST) : 0;
 }
 struct Run { long long from, to, base; int s; };      // this CTA's tiles; the sequence that it begins in and the tiles in front of that
 // by all threads of the block
 __device__ __forceinline__ Run run_of(const AttnP& p) {
+  if (p.direct) {                            // a CTA a unit
+    const int per = p.H * p.ctiles, s = (int)blockIdx.x / per, u = (int)blockIdx.x - s * per;
+    const Seq q = sequence(p.b, s, p.P);
+    Run r;
+    r.s = u < units_of(p, q) ? s : -1; r.base = 0;
+    const int n = r.s >= 0 ? tiles_of(p, q) + UNIT_COST : 0;
+    r.from = (long long)u * n; r.to = r.from + n;
+    return r;
+  }
   __shared__ long long sums[FEW_WARPS];
   __shared__ Run found;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -461,41 +473,123 @@ __global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(c
   __shared__ int rows_at[FEW_WARPS][64];                                      // and the row of codes that it begins at
   __shared__ float m_s[FEW_WARPS][8], l_s[FEW_WARPS][8];
   typedef float Sums[8][D + 4];
-  Sums* o_s = reinterpret_cast<Sums*>(ring);                                  // the warps' sums, when the ring is empty
+  Sums* o_s = reinterpret_cast<Sums*>(ring + FEW_WARPS * 4 * SIDE);           // the warps' sums
   const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, c = lane & 3;
   const uint32_t bar = tcp::smem_u32(&bars[warp][0]);
   if (lane < 4) tcp::mbar_init(bar + 8 * lane, 1);
   if (threadIdx.x == 0) quit = 0;
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   const int key_row = token_of<D>(g), val_row[2] = {token_of<D>(2 * c), token_of<D>(2 * c + 1)};
-  int used = 0;                              // tiles that went through this warp's ring
   pdl_trigger();
   pdl_wait();
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i < p.b.S; i += FEW_THREADS)
       if (!sequence(p.b, i, p.P).ok) flag(p.flags, B200_PAGED_BAD_BATCH);
-  Run run = run_of(p);
+  const Run run = run_of(p);
   if (run.s < 0) return;
-  int s = run.s, n_tiles = 1, n_units = 0;
-  long long base = run.base;
-  Seq q;
-  q = sequence(p.b, s, p.P);
-  n_units = units_of(p, q);
-  n_tiles = n_units ? tiles_of(p, q) : 1;
-  for (long long f = run.from; f < run.to;) {
-    while (f >= base + (long long)n_units * n_tiles && s + 1 < p.b.S) {        // the next sequence that has work
-      base += (long long)n_units * n_tiles;
-      ++s;
-      q = sequence(p.b, s, p.P);
-      n_units = units_of(p, q);
-      n_tiles = n_units ? tiles_of(p, q) : 1;
+
+  // A part of a unit: its places of u0 .. u1 - 1 are the run's, of which the first UNIT_COST are no tiles.
+  struct Part {
+    Seq q;
+    int s, h, ct, u0, u1, n_pos, pf, pl, first, count, used;                  // this warp's tiles; used: how many went through its ring before
+    Tiles<5> tiles;
+  };
+  long long f = run.from, base = run.base;
+  int s_at = run.s;
+  Seq q_at = sequence(p.b, s_at, p.P);
+  int units_at = units_of(p, q_at), n_at = units_at ? tiles_of(p, q_at) + UNIT_COST : 1;
+  auto next_part = [&](int used) {
+    while (f >= base + (long long)units_at * n_at && s_at + 1 < p.b.S) {      // the next sequence that has work
+      base += (long long)units_at * n_at;
+      q_at = sequence(p.b, ++s_at, p.P);
+      units_at = units_of(p, q_at);
+      n_at = units_at ? tiles_of(p, q_at) + UNIT_COST : 1;
     }
-    const int unit = (int)((f - base) / n_tiles), u0 = (int)((f - base) - (long long)unit * n_tiles), u1 = (int)min((long long)n_tiles, u0 + (run.to - f));
+    const int unit = (int)((f - base) / n_at), u0 = (int)((f - base) - (long long)unit * n_at), u1 = (int)min((long long)n_at, u0 + (run.to - f));
     f += u1 - u0;
-    const int h = unit % p.H, ct = unit / p.H, c0 = ct * COLS, n_cols = q.n * p.G;
-    const int pf = q.before + c0 / p.G, pl = q.before + (min(c0 + COLS, n_cols) - 1) / p.G;
-    const Tiles<5> tiles(pf, pl, p.window, p.sinks);
-    const int t0 = min(u0, tiles.n), t1 = min(u1, tiles.n);                   // a column tile may see fewer keys than its sequence
+    const int h = unit % p.H, ct = unit / p.H, n_cols = q_at.n * p.G;
+    const int pf = q_at.before + ct * COLS / p.G, pl = q_at.before + (min(ct * COLS + COLS, n_cols) - 1) / p.G;
+    Part w{q_at, s_at, h, ct, u0, u1, n_at, pf, pl, 0, 0, used, Tiles<5>(pf, pl, p.window, p.sinks)};
+    const int t0 = min(max(u0 - UNIT_COST, 0), w.tiles.n), t1 = min(max(u1 - UNIT_COST, 0), w.tiles.n);       // a column tile may see fewer keys than its sequence
+    w.first = t0 + warp;
+    w.count = w.first < t1 ? (t1 - w.first + FEW_WARPS - 1) / FEW_WARPS : 0;
+    return w;
+  };
+  uint8_t* const my_ring = ring + warp * 4 * SIDE;
+  const uint32_t ring_at = tcp::smem_u32(my_ring);
+  auto fetch = [&](const Part& w, int i, const CUtensorMap& map, int side) {
+    const int place = side + ((w.used + i) & 1);
+    const int r0 = rows_at[warp][(2 * i) & 63], r1 = rows_at[warp][(2 * i + 1) & 63];
+    if (tcp::elected()) {
+      const uint32_t to = ring_at + place * SIDE, b = bar + 8 * place;
+      tcp::mbar_expect_tx(b, (r0 >= 0 ? SIDE / 2 : 0) + (r1 >= 0 ? SIDE / 2 : 0));
+      if (r0 >= 0) tcp::tma_load_2d(to, &map, b, 0, r0);
+      if (r1 >= 0) tcp::tma_load_2d(to + SIDE / 2, &map, b, 0, r1);
+    }
+    __syncwarp();
+  };
+  // The part's i-th tile on its way into the ring; every 16 tiles the lanes look up the pages of their halves, and their scales behind the copies' start.
+  auto issue_keys = [&](const Part& w, int i) {
+    if (i >= w.count) return;
+    if (i & 15) { fetch(w, i, map_k, 0); return; }
+    const int mine = i + (lane >> 1), j = mine < w.count ? (w.tiles[w.first + mine * FEW_WARPS] << 5) + 16 * (lane & 1) : 0;
+    int page = -1;
+    if (mine < w.count && j <= w.pl && (p.window <= 0 || w.pf - j - 15 < p.window || j < p.sinks)) {
+      page = p.b.table[w.s * p.b.table_ld + (j >> p.page_shift)];
+      if (page < 0 || page >= p.pages) { flag(p.flags, B200_PAGED_BAD_PAGE); page = -1; }
+    }
+    rows_at[warp][(2 * i + lane) & 63] = page < 0 ? -1 : (page * p.H + w.h) * p.P + (j & (p.P - 1));
+    __syncwarp();
+    fetch(w, i, map_k, 0);
+    float4 x = make_float4(__int_as_float(HIDDEN), 0.f, -INFINITY, 0.f);
+    if (page >= 0) {
+      const bool all = j + 15 <= w.pf && (p.window <= 0 || w.pl - j < p.window || j + 16 <= p.sinks);
+      x.x = __int_as_float(all ? SEEN : IN_PART);
+      x.y = p.k_scale[(long long)page * p.H + w.h];
+      float vs = p.v_scale[(long long)page * p.H + w.h];
+      vs = vs > 0.f ? vs : 1.f;              // all codes of a page of zeros are 0
+      x.z = __log2f(vs); x.w = __frcp_rn(vs);
+    }
+    meta[warp][(2 * i + lane) & 63] = x;
+    __syncwarp();
+  };
+  auto issue_values = [&](const Part& w, int i) {
+    if (i < w.count) fetch(w, i, map_v, 2);
+  };
+  // a part's first copies, which go out before the part in front of it is joined
+  auto start = [&](const Part& w) {
+    __syncwarp();
+    issue_keys(w, 0);
+    issue_values(w, 0);
+    issue_keys(w, 1);
+  };
+  auto arrived = [&](const Part& w, int i, int side) {
+    const uint32_t n = (uint32_t)(w.used + i);
+    if (!wait_or_quit(bar + 8 * (side + (n & 1)), (n >> 1) & 1u, &quit)) flag(p.flags, B200_PAGED_WAIT);
+    __syncwarp();
+  };
+
+  uint32_t raw[KS][2];                       // eight columns' queries of the part to come, as they are in memory
+  auto load_queries = [&](const Part& w, int nt) {
+    const int col = w.ct * COLS + nt * 8 + g;
+    const bool has = col < w.q.n * p.G;
+    const int i = has ? col / p.G : 0;
+    const bf16* row = p.q + (long long)(w.q.r0 + i) * p.q_ld + (long long)(w.h * p.G + (has ? col - i * p.G : 0)) * D;
+#pragma unroll
+    for (int b = 0; b < D / 64; ++b) {
+      const uint4 x = has ? *reinterpret_cast<const uint4*>(row + 64 * b + 16 * c) : make_uint4(0, 0, 0, 0);
+      const uint4 y = has ? *reinterpret_cast<const uint4*>(row + 64 * b + 16 * c + 8) : make_uint4(0, 0, 0, 0);
+      raw[4 * b][0] = x.x; raw[4 * b][1] = x.y; raw[4 * b + 1][0] = x.z; raw[4 * b + 1][1] = x.w;
+      raw[4 * b + 2][0] = y.x; raw[4 * b + 2][1] = y.y; raw[4 * b + 3][0] = y.z; raw[4 * b + 3][1] = y.w;
+    }
+  };
+  Part w = next_part(0);
+  start(w);
+  if constexpr (NT == 1) load_queries(w, 0);
+  for (;;) {
+    const Seq q = w.q;
+    const int h = w.h, c0 = w.ct * COLS, n_cols = q.n * p.G, pf = w.pf, pl = w.pl, first = w.first, count = w.count, used = w.used;
+    const Tiles<5> tiles = w.tiles;
 
     // queries: lane (g, c) has of column 8 nt + g the dimensions 64 i + 16 c .. + 15, as f16 or as three digits of 8 bits
     uint32_t qf[DIGITS ? 1 : NT][KS][2], qd[3][KS / 2][2];
@@ -503,18 +597,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(c
     int pos[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int col = c0 + nt * 8 + g;
-      const bool has = col < n_cols;
-      const int i = has ? col / p.G : 0;
-      const bf16* row = p.q + (long long)(q.r0 + i) * p.q_ld + (long long)(h * p.G + (has ? col - i * p.G : 0)) * D;
-      uint32_t raw[KS][2];
-#pragma unroll
-      for (int b = 0; b < D / 64; ++b) {
-        const uint4 x = has ? *reinterpret_cast<const uint4*>(row + 64 * b + 16 * c) : make_uint4(0, 0, 0, 0);
-        const uint4 y = has ? *reinterpret_cast<const uint4*>(row + 64 * b + 16 * c + 8) : make_uint4(0, 0, 0, 0);
-        raw[4 * b][0] = x.x; raw[4 * b][1] = x.y; raw[4 * b + 1][0] = x.z; raw[4 * b + 1][1] = x.w;
-        raw[4 * b + 2][0] = y.x; raw[4 * b + 2][1] = y.y; raw[4 * b + 3][0] = y.z; raw[4 * b + 3][1] = y.w;
-      }
+      if constexpr (NT > 1) load_queries(w, nt);
       float top = 0.f;                       // of the column's finite values; infinity if there are others
       bool odd = false;
 #pragma unroll
@@ -566,55 +649,6 @@ __global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(c
       l[nt][0] = l[nt][1] = 0.f;
     }
 
-    const int32_t* table = p.b.table + s * p.b.table_ld;
-    const int first = t0 + warp, count = first < t1 ? (t1 - first + FEW_WARPS - 1) / FEW_WARPS : 0;      // this warp's tiles
-    uint8_t* const my_ring = ring + warp * 4 * SIDE;
-    const uint32_t ring_at = tcp::smem_u32(my_ring);
-    // the warp's i-th tile on its way into the ring; every 16 tiles the lanes look up the pages of their halves
-    auto fetch = [&](int i, const CUtensorMap& map, int side) {
-      const int place = side + ((used + i) & 1);
-      const int r0 = rows_at[warp][(2 * i) & 63], r1 = rows_at[warp][(2 * i + 1) & 63];
-      if (tcp::elected()) {
-        const uint32_t to = ring_at + place * SIDE, b = bar + 8 * place;
-        tcp::mbar_expect_tx(b, (r0 >= 0 ? SIDE / 2 : 0) + (r1 >= 0 ? SIDE / 2 : 0));
-        if (r0 >= 0) tcp::tma_load_2d(to, &map, b, 0, r0);
-        if (r1 >= 0) tcp::tma_load_2d(to + SIDE / 2, &map, b, 0, r1);
-      }
-      __syncwarp();
-    };
-    auto arrived = [&](int i, int side) {
-      const uint32_t n = (uint32_t)(used + i);
-      if (!wait_or_quit(bar + 8 * (side + (n & 1)), (n >> 1) & 1u, &quit)) flag(p.flags, B200_PAGED_WAIT);
-      __syncwarp();
-    };
-    auto issue_keys = [&](int i) {
-      if (i >= count) return;
-      if ((i & 15) == 0) {
-        float4 x = make_float4(__int_as_float(HIDDEN), 0.f, -INFINITY, 0.f);
-        int off = -1;
-        const int mine = i + (lane >> 1), j = mine < count ? (tiles[first + mine * FEW_WARPS] << 5) + 16 * (lane & 1) : 0;
-        if (mine < count && j <= pl && (p.window <= 0 || pf - j - 15 < p.window || j < p.sinks)) {
-          const int page = table[j >> p.page_shift];
-          if (page >= 0 && page < p.pages) {
-            const bool all = j + 15 <= pf && (p.window <= 0 || pl - j < p.window || j + 16 <= p.sinks);
-            x.x = __int_as_float(all ? SEEN : IN_PART);
-            off = (page * p.H + h) * p.P + (j & (p.P - 1));
-            x.y = p.k_scale[(long long)page * p.H + h];
-            float vs = p.v_scale[(long long)page * p.H + h];
-            vs = vs > 0.f ? vs : 1.f;        // all codes of a page of zeros are 0
-            x.z = __log2f(vs); x.w = __frcp_rn(vs);
-          } else flag(p.flags, B200_PAGED_BAD_PAGE);
-        }
-        __syncwarp();
-        meta[warp][(2 * i + lane) & 63] = x;
-        rows_at[warp][(2 * i + lane) & 63] = off;
-        __syncwarp();
-      }
-      fetch(i, map_k, 0);
-    };
-    auto issue_values = [&](int i) {
-      if (i < count) fetch(i, map_v, 2);
-    };
     struct Tile { float4 x[2]; bool whole; };
     auto tile_at = [&](int i) {
       Tile t;
@@ -784,39 +818,42 @@ __global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(c
     };
 
     // The scores of tile i + 1 and the values of tile i do not wait for one another, and lie in one stretch of code; behind them the weights of tile i + 1.
-    issue_keys(0);
-    issue_values(0);
-    issue_keys(1);
     if (count) {
       Tile t = tile_at(0);
       float sc[2][NT][4];
-      arrived(0, 0);
+      arrived(w, 0, 0);
       scores(0, t, sc);
       weigh(0, t, sc);
       for (int i = 0; i + 1 < count; ++i) {
         __syncwarp();                        // the places that these copies go to have been read
-        issue_values(i + 1);
-        issue_keys(i + 2);
-        arrived(i, 2);
+        issue_values(w, i + 1);
+        issue_keys(w, i + 2);
+        arrived(w, i, 2);
         if (!t.whole) hide(i, t);
         t = tile_at(i + 1);
-        arrived(i + 1, 0);
+        arrived(w, i + 1, 0);
         scores(i + 1, t, sc);
         add_values(i);
         weigh(i + 1, t, sc);
       }
-      arrived(count - 1, 2);
+      arrived(w, count - 1, 2);
       if (!t.whole) hide(count - 1, t);
       add_values(count - 1);
     }
-    used += count;
+    const Part now = w;
+    const bool more = f < run.to;
+    if (more) {
+      w = next_part(used + count);
+      start(w);
+      if constexpr (NT == 1) load_queries(w, 0);
+    }
 
     // join the warps, eight columns at a time
-    const bool alone = u0 == 0 && u1 == n_tiles;
-    const int slot = 2 * (int)blockIdx.x + (u0 == 0 ? 1 : 0);
-    if (u0 == 0 && threadIdx.x == 0) {       // where the unit's parts are: this run's and so many after it
-      const long long runs = run.to - run.from, left = n_tiles - u1;
-      p.parts[((long long)s * p.ctiles + ct) * p.H + h] = make_int2((int)blockIdx.x, alone ? 0 : (int)((left + runs - 1) / runs));
+    const bool alone = now.u0 == 0 && now.u1 == now.n_pos;
+    const int slot = 2 * (int)blockIdx.x + (now.u0 == 0 ? 1 : 0);
+    if (!p.direct && now.u0 == 0 && threadIdx.x == 0) {                       // where the unit's parts are: this run's and so many after it
+      const long long runs = run.to - run.from, left = now.n_pos - now.u1;
+      p.parts[((long long)now.s * p.ctiles + now.ct) * p.H + now.h] = make_int2((int)blockIdx.x, alone ? 0 : (int)((left + runs - 1) / runs));
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -836,8 +873,11 @@ __global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(c
         for (int e = 0; e < 2; ++e) *reinterpret_cast<float2*>(&o_s[warp][2 * c + e][(D / 8) * g + 2 * i]) = make_float2(o[nt][i][e], o[nt][i][e + 2]);
       __syncthreads();
       constexpr int PER = D / 16;            // 16 threads a column
-      const int col = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * PER, cc = c0 + nt * 8 + col;
-      if (cc < n_cols) {
+      const int d0 = (threadIdx.x & 15) * PER;
+#pragma unroll
+      for (int col = threadIdx.x >> 4; col < 8; col += FEW_THREADS / 16) {
+        const int cc = c0 + nt * 8 + col;
+        if (cc >= n_cols) break;
         float top = -INFINITY, sum = 0.f, acc[PER];
 #pragma unroll
         for (int w = 0; w < FEW_WARPS; ++w) top = fmaxf(top, m_s[w][col]);
@@ -859,8 +899,7 @@ __global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(c
         }
       }
     }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();                         // the ring's next copies come behind these reads and writes
+    if (!more) break;
   }
   if (quit) {                                // let copies in flight land before the block ends
     const uint64_t since = tcp::global_timer_ns();
@@ -955,7 +994,7 @@ bool rows_fit(const void* p, long long ld, int heads, int dim) { return p && !(r
 int shift_of(int P) { return P == 16 ? 4 : P == 32 ? 5 : P == 64 ? 6 : 7; }
 
 // CTAs of 8 * nt columns, about one wave of them (four, three or two to an SM), fewer where the tables allow for less work than that.
-struct FewPlan { int nt, ctiles, ctas; long long units; };
+struct FewPlan { int nt, ctiles, ctas; long long units; bool direct; };
 FewPlan few_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks, int few_rows) {
   FewPlan f;
   const long long rows = few_rows < b->max_rows ? few_rows : b->max_rows, cols = rows * G;
@@ -964,12 +1003,13 @@ FewPlan few_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, in
   f.units = (long long)b->sequences * c->kv_heads * f.ctiles;
   long long keys = (long long)b->table_width * c->page_tokens;
   if (window > 0 && (long long)window + sinks + rows < keys) keys = (long long)window + sinks + rows;
-  const long long runs = ceil_div64(f.units * (ceil_div64(keys, 32) + 2), MIN_RUN), wave = 148 * few_per_sm(f.nt);
-  f.ctas = (int)(runs < wave ? runs : wave);
+  const long long tiles = ceil_div64(keys, 32) + 1, runs = ceil_div64(f.units * (tiles + 4), MIN_RUN), wave = 148 * few_per_sm(f.nt);
+  f.direct = f.units <= wave && tiles <= DIRECT_TILES;
+  f.ctas = (int)(f.direct ? f.units : runs < wave ? runs : wave);
   return f;
 }
 // sums and (maximum, sum of the weights) of two parts per CTA, and where each unit's parts are
-int64_t few_bytes(const FewPlan& f, int D) { return (int64_t)f.ctas * 2 * 8 * f.nt * (D + 2) * 4 + f.units * 8; }
+int64_t few_bytes(const FewPlan& f, int D) { return f.direct ? 0 : (int64_t)f.ctas * 2 * 8 * f.nt * (D + 2) * 4 + f.units * 8; }
 
 }  // namespace
 
@@ -993,13 +1033,14 @@ namespace {
 
 template <int D, int FMT, int NT>
 int launch_few(const AttnP& p, const FewPlan& f, cudaStream_t st) {
-  constexpr int ring = FEW_WARPS * 4 * 32 * D, sums = FEW_WARPS * 8 * (D + 4) * 4, smem = (ring > sums ? ring : sums) + 1024;
+  constexpr int ring = FEW_WARPS * 4 * 32 * D, sums = FEW_WARPS * 8 * (D + 4) * 4, smem = ring + sums + 1024;
   static std::atomic<uint64_t> limits{0};
   CUtensorMap map_k, map_v;
   B200_TRY(code_map(&map_k, p.k, (long long)p.pages * p.H * p.P, D, 16));
   B200_TRY(code_map(&map_v, p.v, (long long)p.pages * p.H * p.P, D, 16));
   B200_TRY(allow_smem(limits, smem, few_rows_kernel<D, FMT, NT>));
   B200_TRY(launch_early(few_rows_kernel<D, FMT, NT>, dim3((unsigned)f.ctas), dim3(FEW_THREADS), smem, st, map_k, map_v, p));
+  if (f.direct) return B200_OK;
   const long long most = (long long)p.b.max_rows * p.G < 8 * NT ? (long long)p.b.max_rows * p.G : 8 * NT;
   return launch_early(join_kernel<D, NT>, dim3((unsigned)(f.units * most)), dim3(128), 0, st, p);
 }
@@ -1115,9 +1156,9 @@ int b200_paged_attention(const b200_paged_cache* cache, const b200_paged_batch* 
   p.from_rows = 0x7fffffff; p.q_tiles = 0;
   const FewPlan f = few_plan(cache, batch, p.G, window, sinks, p.from_rows);
   if (f.units > 0x7fffffffll / 64 || (long long)batch->max_rows * p.G > 0x3fffffffll) B200_FAIL(B200_ERR_SHAPE, "paged_attention: %d sequences of up to %d rows with %d heads in one call", batch->sequences, batch->max_rows, q_heads);
-  if (!work_dev || work_bytes < few_bytes(f, D) || (reinterpret_cast<uintptr_t>(work_dev) & 15))
+  if ((!work_dev && !f.direct) || work_bytes < few_bytes(f, D) || (reinterpret_cast<uintptr_t>(work_dev) & 15))
     B200_FAIL(B200_ERR_INVALID, "paged_attention: a workspace of %lld bytes; b200_paged_attention_bytes asks for %lld, on a 16-byte border", (long long)work_bytes, (long long)few_bytes(f, D));
-  p.cols = 8 * f.nt; p.ctiles = f.ctiles;
+  p.cols = 8 * f.nt; p.ctiles = f.ctiles; p.direct = f.direct;
   p.part_o = static_cast<float*>(work_dev);
   p.part_ml = p.part_o + (long long)f.ctas * 2 * p.cols * D;
   p.parts = reinterpret_cast<int2*>(p.part_ml + (long long)f.ctas * 2 * p.cols * 2);

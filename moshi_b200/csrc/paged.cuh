@@ -102,6 +102,7 @@ struct AttnP {
   float scale2;                              // score scale * log2(e)
   // few rows
   int cols, ctiles;                          // columns of a unit, units of a sequence and kv head
+  int direct;                                // a CTA per unit
   float *part_o, *part_ml;                   // [CTAs][2][cols][D], [CTAs][2][cols][2]
   int2* parts;                               // [sequences][ctiles][H]: first CTA and number of further ones of a unit
   // many rows
