@@ -997,7 +997,7 @@ int shift_of(int P) { return P == 16 ? 4 : P == 32 ? 5 : P == 64 ? 6 : 7; }
 struct FewPlan { int nt, ctiles, ctas; long long units; bool direct; };
 FewPlan few_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks, int few_rows) {
   FewPlan f;
-  const long long rows = few_rows < b->max_rows ? few_rows : b->max_rows, cols = rows * G;
+  const long long rows = few_rows <= b->max_rows ? few_rows - 1 : b->max_rows, cols = rows * G;
   f.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
   f.ctiles = (int)ceil_div64(cols, 8 * f.nt);
   f.units = (long long)b->sequences * c->kv_heads * f.ctiles;
@@ -1030,6 +1030,19 @@ int code_map(CUtensorMap* m, const void* codes, long long rows, int dim, int box
 }
 
 namespace {
+
+// Sequences of more than 64 columns (rows times heads of a group) go to the tensor cores' kernel of whole tiles; the only sequence of a step goes there with all its rows if it may have that many.
+constexpr int FEW_COLS = 64;
+struct Route { int from_rows; FewPlan few; PromptPlan prompt; int64_t few_bytes, prompt_bytes; };
+Route route(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks) {
+  Route r;
+  memset(&r, 0, sizeof(r));
+  const bool many = (long long)b->max_rows * G > FEW_COLS;
+  r.from_rows = !many ? 0x7fffffff : b->sequences == 1 ? 1 : FEW_COLS / G + 1;
+  if (r.from_rows > 1) { r.few = few_plan(c, b, G, window, sinks, r.from_rows); r.few_bytes = (few_bytes(r.few, c->dim) + 15) / 16 * 16; }
+  if (many) { r.prompt = prompt_plan(c, b, G, window, sinks); r.prompt_bytes = prompt_bytes(r.prompt, c->dim); }
+  return r;
+}
 
 template <int D, int FMT, int NT>
 int launch_few(const AttnP& p, const FewPlan& f, cudaStream_t st) {
@@ -1132,8 +1145,9 @@ int64_t b200_paged_attention_bytes(const b200_paged_cache* cache, const b200_pag
   using namespace b200::paged;
   if (!cache || !batch || cache->kv_heads < 1 || q_heads < cache->kv_heads || q_heads % cache->kv_heads || window < 0 || sinks < 0 || batch->sequences < 1 || batch->max_rows < 0) return 0;
   const int G = q_heads / cache->kv_heads;
-  const FewPlan f = few_plan(cache, batch, G, window, sinks, 0x7fffffff);
-  return few_bytes(f, cache->dim);
+  if (batch->max_rows == 0) return 0;
+  const Route r = route(cache, batch, G, window, sinks);
+  return r.few_bytes + r.prompt_bytes;
 }
 
 int b200_paged_attention(const b200_paged_cache* cache, const b200_paged_batch* batch, const void* q_dev, int64_t q_ld, void* out_dev, int64_t out_ld, int q_heads,
@@ -1153,19 +1167,36 @@ int b200_paged_attention(const b200_paged_cache* cache, const b200_paged_batch* 
   p.flags = cache->flags_dev; p.b = batch_of(batch); p.q = static_cast<const __nv_bfloat16*>(q_dev); p.out = static_cast<__nv_bfloat16*>(out_dev);
   p.q_ld = q_ld; p.out_ld = out_ld; p.pages = cache->pages; p.P = cache->page_tokens; p.page_shift = shift_of(p.P); p.H = H; p.G = q_heads / H;
   p.window = window; p.sinks = sinks; p.scale2 = scale * LOG2E;
-  p.from_rows = 0x7fffffff; p.q_tiles = 0;
-  const FewPlan f = few_plan(cache, batch, p.G, window, sinks, p.from_rows);
-  if (f.units > 0x7fffffffll / 64 || (long long)batch->max_rows * p.G > 0x3fffffffll) B200_FAIL(B200_ERR_SHAPE, "paged_attention: %d sequences of up to %d rows with %d heads in one call", batch->sequences, batch->max_rows, q_heads);
-  if ((!work_dev && !f.direct) || work_bytes < few_bytes(f, D) || (reinterpret_cast<uintptr_t>(work_dev) & 15))
-    B200_FAIL(B200_ERR_INVALID, "paged_attention: a workspace of %lld bytes; b200_paged_attention_bytes asks for %lld, on a 16-byte border", (long long)work_bytes, (long long)few_bytes(f, D));
-  p.cols = 8 * f.nt; p.ctiles = f.ctiles; p.direct = f.direct;
-  p.part_o = static_cast<float*>(work_dev);
-  p.part_ml = p.part_o + (long long)f.ctas * 2 * p.cols * D;
-  p.parts = reinterpret_cast<int2*>(p.part_ml + (long long)f.ctas * 2 * p.cols * 2);
+  const Route r = route(cache, batch, p.G, window, sinks);
+  if (r.few.units > 0x7fffffffll / 64 || r.prompt.units * (r.prompt.nsplit ? r.prompt.nsplit : 1) > 0x7fffffffll / 64 || (long long)batch->max_rows * p.G > 0x3fffffffll)
+    B200_FAIL(B200_ERR_SHAPE, "paged_attention: %d sequences of up to %d rows with %d heads in one call", batch->sequences, batch->max_rows, q_heads);
+  const int64_t need = r.few_bytes + r.prompt_bytes;
+  if (need > 0 && (!work_dev || work_bytes < need || (reinterpret_cast<uintptr_t>(work_dev) & 15)))
+    B200_FAIL(B200_ERR_INVALID, "paged_attention: a workspace of %lld bytes; b200_paged_attention_bytes asks for %lld, on a 16-byte border", (long long)work_bytes, (long long)need);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool i8 = cache->kv_dtype == B200_KV_INT8;
-  if (D == 128) B200_TRY((i8 ? launch_few_nt<128, INT8>(p, f, st) : launch_few_nt<128, E4M3>(p, f, st)));
-  else B200_TRY((i8 ? launch_few_nt<64, INT8>(p, f, st) : launch_few_nt<64, E4M3>(p, f, st)));
+  const int fmt = cache->kv_dtype == B200_KV_INT8 ? INT8 : E4M3;
+  p.from_rows = r.from_rows;
+  p.cols = p.ctiles = p.direct = p.q_tiles = p.nsplit = 0; p.part_o = p.part_ml = nullptr; p.parts = nullptr;
+  if (r.prompt.units) {
+    AttnP x = p;
+    x.q_tiles = r.prompt.q_tiles; x.nsplit = r.prompt.nsplit;
+    if (r.prompt_bytes) {
+      x.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(work_dev) + r.few_bytes);
+      x.part_ml = x.part_o + r.prompt_bytes / 4 / (D + 2) * D;
+    }
+    B200_TRY(prompt_attention(x, r.prompt, fmt, D, st));
+  }
+  if (r.few.units) {
+    const FewPlan& f = r.few;
+    p.cols = 8 * f.nt; p.ctiles = f.ctiles; p.direct = f.direct;
+    if (!f.direct) {
+      p.part_o = static_cast<float*>(work_dev);
+      p.part_ml = p.part_o + (long long)f.ctas * 2 * p.cols * D;
+      p.parts = reinterpret_cast<int2*>(p.part_ml + (long long)f.ctas * 2 * p.cols * 2);
+    }
+    if (D == 128) B200_TRY((fmt == INT8 ? launch_few_nt<128, INT8>(p, f, st) : launch_few_nt<128, E4M3>(p, f, st)));
+    else B200_TRY((fmt == INT8 ? launch_few_nt<64, INT8>(p, f, st) : launch_few_nt<64, E4M3>(p, f, st)));
+  }
   return check_launch("paged_attention");
 }
 

@@ -106,7 +106,8 @@ struct AttnP {
   float *part_o, *part_ml;                   // [CTAs][2][cols][D], [CTAs][2][cols][2]
   int2* parts;                               // [sequences][ctiles][H]: first CTA and number of further ones of a unit
   // many rows
-  int from_rows, q_tiles;                    // sequences of fewer rows than this are the other kernel's
+  int from_rows;                             // sequences of at least this many rows
+  int q_tiles, nsplit;                       // units of a sequence and kv head; ranges of the keys
 };
 
 // Keys that the rows of positions pf .. pl see, in tiles of 1 << SHIFT tokens: `first` tiles from token 0 on (those of the sinks), then those from tile `from` on.
@@ -146,8 +147,10 @@ __device__ __forceinline__ bool wait_or_quit(uint32_t bar, uint32_t parity, vola
 int code_map(CUtensorMap* m, const void* codes, long long rows, int dim, int box_rows);
 
 // paged_prompt.cu
-int prompt_rows(int dim, int G);                                             // from how many rows on a sequence is taken there
-int prompt_attention(const AttnP& p, int fmt, int dim, cudaStream_t st);
+struct PromptPlan { int q_tiles, nsplit; long long units; };
+PromptPlan prompt_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks);
+int64_t prompt_bytes(const PromptPlan& f, int D);
+int prompt_attention(const AttnP& p, const PromptPlan& f, int fmt, int dim, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace b200

@@ -1,0 +1,491 @@
+// Attention of many rows of a sequence over the paged 8-bit cache, on the 5th-generation tensor cores.
+//
+// A CTA owns one kv head and up to 256 rows (row of the sequence, query head of the group) as two tiles of 128, and walks the keys in tiles of 128 tokens.  Warps 8..11 bring the codes from memory
+// through registers into f16 tiles (exact for both types) in SWIZZLE_128B, keys K-major and values as they lie, tokens by dims; warp 12 issues S_i = Q_i K^T and O_i += P_i V as
+// tcgen05.mma with fp32 accumulators in TMEM (S_0, S_1, O_0, O_1); warps 0..3 and 4..7 hold a row per thread, take their scores twice (maximum, then weights) and put P as f16 over the scores,
+// from where the second product reads it.  While one tile's weights are made, the other's products run.
+//
+// Scales as in paged.cu: that of a page's keys multiplies its 16 or more columns' scores, that of its values goes into the exponent.  O is rescaled only when a row's maximum grew by more than 2^8.
+#include "paged.cuh"
+
+namespace b200 {
+namespace paged {
+
+namespace {
+
+using namespace tcp;
+typedef __nv_bfloat16 bf16;
+
+constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 4, THREADS = (SOFT_WARPS + CONVERT_WARPS + 1) * 32, ROWS = 256, KEYS = 128, INFOS = 4;
+constexpr float SLACK = 8.f;
+
+template <int D>
+struct Smem {
+  static constexpr uint32_t TILE = 128 * D * 2, HALF = 128 * 128;             // 128 rows of f16, in halves of 64 dims
+  static constexpr uint32_t Q = 0, K = 2 * TILE, V = 4 * TILE, END = 6 * TILE, BYTES = END + 1024;
+};
+
+#define R32(r, o) "=r"((r)[o]), "=r"((r)[o + 1]), "=r"((r)[o + 2]), "=r"((r)[o + 3]), "=r"((r)[o + 4]), "=r"((r)[o + 5]), "=r"((r)[o + 6]), "=r"((r)[o + 7])
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : R32(r, 0), R32(r, 8), R32(r, 16), R32(r, 24) : "r"(taddr));
+}
+#undef R32
+#define R8(r, o) "r"((r)[o]), "r"((r)[o + 1]), "r"((r)[o + 2]), "r"((r)[o + 3]), "r"((r)[o + 4]), "r"((r)[o + 5]), "r"((r)[o + 6]), "r"((r)[o + 7])
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), R8(r, 0), R8(r, 8), R8(r, 16), R8(r, 24) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+               ::"r"(taddr), R8(r, 0), R8(r, 8) : "memory");
+}
+#undef R8
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* quit) { return __all_sync(0xffffffffu, wait_or_quit(bar, parity, quit)); }
+
+// kind::f16, f16 operands, fp32 accumulators, 128 rows by n columns; `tokens_first`: the second operand lies [k][n]
+constexpr uint32_t idesc_f16(int n, bool tokens_first) { return (1u << 4) | (tokens_first ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | (8u << 24); }
+// O += P V, 16 tokens: P in TMEM (8 columns of two f16), V [tokens][64 dims a half]: 8 tokens 1024 bytes on, the next 64 dims a half on
+__device__ __forceinline__ void product_pv(uint32_t d, uint32_t p, uint32_t v_smem, uint32_t half, uint32_t idesc, uint32_t accumulate) {
+  const uint64_t desc = (uint64_t)(((v_smem & 0x3FFFFu) >> 4) | ((half >> 4) << 16)) | (uint64_t)DESC_HIGH << 32;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(p), "l"(desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+struct Unit {
+  Seq q;
+  int s, h, split, r0, rows, n_rows;         // first row of the unit, rows in it, rows of the sequence
+  int pf, pl, t0, n;                         // first and last position; first tile and number of tiles of this range
+};
+__device__ __forceinline__ bool unit_of(const AttnP& p, Unit& u) {
+  int x = (int)blockIdx.x;
+  u.split = x % p.nsplit; x /= p.nsplit;
+  u.h = x % p.H; x /= p.H;
+  u.s = x % p.b.S;
+  const int ct = p.q_tiles - 1 - x / p.b.S;  // the longest first
+  u.q = sequence(p.b, u.s, p.P);
+  if (!u.q.ok || u.q.n < p.from_rows) return false;
+  u.n_rows = u.q.n * p.G;
+  u.r0 = ct * ROWS;
+  if (u.r0 >= u.n_rows) return false;
+  u.rows = min(ROWS, u.n_rows - u.r0);
+  u.pf = u.q.before + u.r0 / p.G;
+  u.pl = u.q.before + (u.r0 + u.rows - 1) / p.G;
+  const Tiles<7> tiles(u.pf, u.pl, p.window, p.sinks);
+  const int per = (tiles.n + p.nsplit - 1) / p.nsplit;
+  u.t0 = u.split * per;
+  u.n = min(per, tiles.n - u.t0);
+  return u.n > 0;
+}
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
+  typedef Smem<D> L;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bars[20 + INFOS];
+  __shared__ float4 info[INFOS][8];          // per 16 keys: keys' scale, log2 and reciprocal of the values', whether the page is there
+  __shared__ uint32_t tmem_at;
+  __shared__ volatile int quit;
+  __shared__ float tops[THREADS / 32];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t bar = smem_u32(bars), k_full = bar, k_empty = bar + 16, v_full = bar + 32, v_empty = bar + 48, s_full = bar + 64, p_full = bar + 80, o_done = bar + 96, i_full = bar + 112;
+  if (threadIdx.x == 0) {
+    quit = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(k_full + 8 * i, CONVERT_WARPS); mbar_init(k_empty + 8 * i, 1); mbar_init(v_full + 8 * i, CONVERT_WARPS); mbar_init(v_empty + 8 * i, 1);
+      mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, 4); mbar_init(o_done + 8 * i, 1);
+    }
+    for (int i = 0; i < INFOS; ++i) mbar_init(i_full + 8 * i, CONVERT_WARPS);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pdl_trigger();
+  pdl_wait();
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < p.b.S; i += THREADS)
+      if (!sequence(p.b, i, p.P).ok) atomicOr(p.flags, B200_PAGED_BAD_BATCH);
+  Unit u;
+  if (!unit_of(p, u)) return;
+  if (warp == SOFT_WARPS + CONVERT_WARPS) tmem_alloc(smem_u32(&tmem_at), 512);
+  const int tiles_q = u.rows > 128 ? 2 : 1;
+  const Tiles<7> tiles(u.pf, u.pl, p.window, p.sinks);
+
+  // ---- queries: f16 after one power of two for all of them ----
+  constexpr int PIECES = D / 8;              // 16-byte pieces of a row
+  auto query = [&](int x) {
+    const int r = x / PIECES, i = (u.r0 + r) / p.G, g = u.r0 + r - i * p.G;
+    return *reinterpret_cast<const uint4*>(p.q + (long long)(u.q.r0 + i) * p.q_ld + (long long)(u.h * p.G + g) * D + (x % PIECES) * 8);
+  };
+  float top = 0.f;
+  for (int x = threadIdx.x; x < u.rows * PIECES; x += THREADS) {
+    const uint4 w = query(x);
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = fabsf(__uint_as_float(v[i] << 16)), b = fabsf(__uint_as_float(v[i] & 0xffff0000u));
+      if (a < INFINITY) top = fmaxf(top, a);
+      if (b < INFINITY) top = fmaxf(top, b);
+    }
+  }
+  top = warp_max(top);
+  if (lane == 0) tops[warp] = top;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; ++i) top = fmaxf(top, tops[i]);
+  const float power = top > 0.f ? power_of_two_in(top) : 1.f, up = 16384.f / power;
+  for (int x = threadIdx.x; x < tiles_q * 128 * PIECES; x += THREADS) {
+    const int r = x / PIECES, c = x % PIECES;
+    const uint4 w = r < u.rows ? query(x) : make_uint4(0, 0, 0, 0);
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = pack_f16(__uint_as_float(v[i] << 16) * up, __uint_as_float(v[i] & 0xffff0000u) * up);
+    *reinterpret_cast<uint4*>(smem + L::Q + (r >> 7) * L::TILE + (c >> 3) * L::HALF + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+  const uint32_t tmem = tmem_at;
+  const int n = u.n;
+
+  if (warp >= SOFT_WARPS && warp < SOFT_WARPS + CONVERT_WARPS) {
+    // ---- codes into f16 tiles, 32 tokens a warp ----
+    const int w4 = warp & 3;
+    constexpr int LANES = D / 16, STEP = 32 / LANES, LOADS = 32 / STEP;       // lanes a row, rows a load, loads
+    const int row = lane / LANES, c = lane % LANES;
+    uint4 held[2][LOADS];                    // of the tile to come: keys, values
+    // lane l: page of the 16 keys that begin at token l * 16 of this warp's
+    auto look_up = [&](int i) {
+      const int j = (tiles[u.t0 + i] << 7) + 32 * w4 + 16 * (lane & 1);
+      int page = -1;
+      if (j <= u.pl && (p.window <= 0 || u.pf - j - 15 < p.window || j < p.sinks)) {
+        page = p.b.table[u.s * p.b.table_ld + (j >> p.page_shift)];
+        if (page < 0 || page >= p.pages) { page = -1; atomicOr(p.flags, B200_PAGED_BAD_PAGE); }
+      }
+      return page;
+    };
+    auto load = [&](int side, int i, int page) {
+      const int j0 = (tiles[u.t0 + i] << 7) + 32 * w4;
+#pragma unroll
+      for (int x = 0; x < LOADS; ++x) {
+        const int t = x * STEP + row, j = j0 + t, pg = __shfl_sync(0xffffffffu, page, t >> 4);
+        // values that no row sees may be anything; keys are masked
+        const bool seen = pg >= 0 && (side == 0 || (j <= u.pl && (p.window <= 0 || u.pf - j < p.window || j < p.sinks)));
+        held[side][x] = seen ? *reinterpret_cast<const uint4*>((side ? p.v : p.k) + (((long long)pg * p.H + u.h) * p.P + (j & (p.P - 1))) * D + 16 * c) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto convert = [&](int side, int st) {
+#pragma unroll
+      for (int x = 0; x < LOADS; ++x) {
+        const int t = 32 * w4 + x * STEP + row;
+        const uint4 h = held[side][x];
+        const uint32_t w[4] = {ready<FMT>(h.x), ready<FMT>(h.y), ready<FMT>(h.z), ready<FMT>(h.w)};
+        const uint4 lo = make_uint4(half2_of<FMT, 0>(w[0]), half2_of<FMT, 1>(w[0]), half2_of<FMT, 0>(w[1]), half2_of<FMT, 1>(w[1]));
+        const uint4 hi = make_uint4(half2_of<FMT, 0>(w[2]), half2_of<FMT, 1>(w[2]), half2_of<FMT, 0>(w[3]), half2_of<FMT, 1>(w[3]));
+        uint8_t* r = smem + (side ? L::V : L::K) + st * L::TILE + (c >> 2) * L::HALF + t * 128;
+        const int odd = (c >> 2) & 1, p0 = 2 * (c & 3) + odd, p1 = 2 * (c & 3) + 1 - odd;      // the second half's lanes begin with their second piece: no bank twice
+        *reinterpret_cast<uint4*>(r + ((p0 ^ (t & 7)) << 4)) = odd ? hi : lo;
+        *reinterpret_cast<uint4*>(r + ((p1 ^ (t & 7)) << 4)) = odd ? lo : hi;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive((side ? v_full : k_full) + 8 * st);
+    };
+    int page = look_up(0), page_next = n > 1 ? look_up(1) : -1;
+    load(0, 0, page);
+    load(1, 0, page);
+    for (int i = 0; i < n; ++i) {
+      const int st = i & 1;
+      const uint32_t parity = ((uint32_t)(i >> 1) & 1u) ^ 1u;
+      if (lane < 2) {                        // what the weights need to know of these keys' pages
+        float4 x = make_float4(0.f, 0.f, 0.f, -1.f);
+        if (page >= 0) {
+          const float vs = p.v_scale[(long long)page * p.H + u.h], v1 = vs > 0.f ? vs : 1.f;         // all codes of a page of zeros are 0
+          x = make_float4(p.k_scale[(long long)page * p.H + u.h], __log2f(v1), __frcp_rn(v1), 1.f);
+        }
+        info[i % INFOS][2 * w4 + lane] = x;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(i_full + 8 * (i % INFOS));
+      page = page_next;
+      if (!warp_wait(k_empty + 8 * st, parity, &quit)) break;
+      convert(0, st);
+      if (i + 1 < n) load(0, i + 1, page);
+      if (!warp_wait(v_empty + 8 * st, parity, &quit)) break;
+      convert(1, st);
+      if (i + 1 < n) load(1, i + 1, page);
+      page_next = i + 2 < n ? look_up(i + 2) : -1;
+    }
+  } else if (warp == SOFT_WARPS + CONVERT_WARPS) {
+    // ---- products ----
+    constexpr uint32_t id_s = idesc_f16(KEYS, false), id_o = idesc_f16(D, true);
+    auto scores = [&](int i, int x) {        // of tile x for queries i
+      const uint32_t a = desc_low(base + L::Q + i * L::TILE), b = desc_low(base + L::K + (x & 1) * L::TILE);
+#pragma unroll
+      for (int half = 0; half < D / 64; ++half) umma_block<1>(tmem + 128 * i, a + half * (L::HALF >> 4), b - a, id_s, half > 0 ? 1u : 0u);
+      commit_elected(s_full + 8 * i);
+    };
+    bool ok = warp_wait(k_full, 0, &quit);
+    if (ok) {
+      tc_fence_after();
+      for (int i = 0; i < tiles_q; ++i) scores(i, 0);
+      commit_elected(k_empty);
+    }
+    for (int x = 0; ok && x < n; ++x) {
+      const int st = x & 1;
+      for (int i = 0; ok && i < tiles_q; ++i) {
+        ok = (i > 0 || warp_wait(v_full + 8 * st, (uint32_t)(x >> 1) & 1u, &quit)) && warp_wait(p_full + 8 * i, (uint32_t)x & 1u, &quit);
+        if (!ok) break;
+        tc_fence_after();
+        if (elected()) {
+#pragma unroll
+          for (int k = 0; k < KEYS / 16; ++k)
+            product_pv(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k, base + L::V + st * L::TILE + k * 2048, L::HALF, id_o, x > 0 || k > 0 ? 1u : 0u);
+        }
+        __syncwarp();
+        commit_elected(o_done + 8 * i);
+        if (i == tiles_q - 1) commit_elected(v_empty + 8 * st);
+        if (x + 1 < n) {                     // the next scores lie over these weights
+          ok = (i > 0 || warp_wait(k_full + 8 * (st ^ 1), (uint32_t)((x + 1) >> 1) & 1u, &quit)) && warp_wait(o_done + 8 * i, (uint32_t)x & 1u, &quit);
+          if (!ok) break;
+          tc_fence_after();
+          scores(i, x + 1);
+          if (i == tiles_q - 1) commit_elected(k_empty + 8 * (st ^ 1));
+        }
+      }
+    }
+    __syncwarp();
+  } else if ((warp >> 2) < tiles_q) {
+    // ---- weights: a row per thread ----
+    const int i = warp >> 2, q4 = warp & 3, row = 128 * i + q4 * 32 + lane, rr = u.r0 + row;
+    const bool has = row < u.rows;
+    const int pos = has ? u.q.before + rr / p.G : -1, lo = p.window > 0 ? pos - p.window : -1;      // sees j <= pos, j > lo or j < sinks
+    const int pf = u.q.before + (u.r0 + 128 * i) / p.G, pl = u.q.before + (u.r0 + min(128 * i + 128, u.rows) - 1) / p.G;      // of this tile of queries
+    const uint32_t lanes = (uint32_t)(q4 * 32) << 16, ts = tmem + lanes + 128 * i, to = tmem + lanes + 256 + 128 * i;
+    const float fac = p.scale2 * power * (1.f / 16384.f);
+    float m = -INFINITY, sum = 0.f;
+    bool ok = true;
+    for (int x = 0; x < n; ++x) {
+      ok = wait_or_quit(i_full + 8 * (x % INFOS), (uint32_t)(x / INFOS) & 1u, &quit) && wait_or_quit(s_full + 8 * i, (uint32_t)x & 1u, &quit);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      tc_fence_after();
+      const int j0 = tiles[u.t0 + x] << 7;
+      const float4* ip = info[x % INFOS];
+      bool whole = j0 + KEYS - 1 <= pf && (p.window <= 0 || pl - j0 < p.window || j0 + KEYS <= p.sinks);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) whole = whole && ip[c].w > 0.f;
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t r[32];
+        tmem_ld32(ts + 32 * c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const float4 y = ip[2 * c + b];
+          const float by = y.x * fac;
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx[e & 1] = fmaxf(mx[e & 1], fmaf(__uint_as_float(r[16 * b + e]), by, y.y));
+          } else if (y.w > 0.f) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int j = j0 + 32 * c + 16 * b + e;
+              if (j <= pos && (j > lo || j < p.sinks)) mx[e & 1] = fmaxf(mx[e & 1], fmaf(__uint_as_float(r[16 * b + e]), by, y.y));
+            }
+          }
+        }
+      }
+      const float t = fmaxf(mx[0], mx[1]);
+      const bool grow = t > m + SLACK;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float factor = grow ? exp2_fast(m - t) : 1.f;
+        if (grow) { m = t; sum *= factor; }
+        if (x > 0) {
+          ok = wait_or_quit(o_done + 8 * i, (uint32_t)(x - 1) & 1u, &quit);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(to + 32 * c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+            tmem_st32(to + 32 * c, o);
+          }
+        }
+      }
+      const float off = m == -INFINITY ? 0.f : m;
+      // log2 s_v - M in one number is off by half a unit of M: only while that is no more than a quarter
+      const bool plain = whole && !__any_sync(0xffffffffu, fabsf(off) > 4194304.f);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t r[32], w[16];
+        tmem_ld32(ts + 32 * c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const float4 y = ip[2 * c + b];
+          const float by = y.x * fac, add = y.y - off;
+          float part[2] = {0.f, 0.f};
+          if (plain) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const float e0 = exp2_fast(fmaf(__uint_as_float(r[16 * b + e]), by, add)), e1 = exp2_fast(fmaf(__uint_as_float(r[16 * b + e + 1]), by, add));
+              part[0] += e0; part[1] += e1;
+              w[8 * b + (e >> 1)] = pack_f16(e0, e1);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const int j = j0 + 32 * c + 16 * b + e;
+              float e0 = exp2_fast(fmaf(__uint_as_float(r[16 * b + e]), by, y.y) - off), e1 = exp2_fast(fmaf(__uint_as_float(r[16 * b + e + 1]), by, y.y) - off);
+              if (!(y.w > 0.f && j <= pos && (j > lo || j < p.sinks))) e0 = 0.f;
+              if (!(y.w > 0.f && j + 1 <= pos && (j + 1 > lo || j + 1 < p.sinks))) e1 = 0.f;
+              part[0] += e0; part[1] += e1;
+              w[8 * b + (e >> 1)] = pack_f16(e0, e1);
+            }
+          }
+          sum = fmaf(part[0] + part[1], y.z, sum);
+        }
+        tmem_st16(ts + 16 * c, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full + 8 * i);
+    }
+    if (ok) {
+      ok = wait_or_quit(o_done + 8 * i, (uint32_t)(n - 1) & 1u, &quit);
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    if (ok) {
+      tc_fence_after();
+      const float inv = sum != 0.f ? 1.f / sum : 0.f;
+      const int token = rr / p.G, unit = (int)blockIdx.x;
+      bf16* out = p.out + (long long)(u.q.r0 + token) * p.out_ld + (long long)(u.h * p.G + rr - token * p.G) * D;
+      float* part = p.part_o + ((long long)unit * ROWS + row) * D;
+      if (p.nsplit > 1 && has) *reinterpret_cast<float2*>(p.part_ml + 2 * ((long long)unit * ROWS + row)) = make_float2(m, sum);
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        __syncwarp();
+        tmem_ld32(to + 32 * c, o);
+        tmem_ld_wait();
+        if (!has) continue;
+        if (p.nsplit > 1) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(part + 32 * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint4 v;
+            v.x = pack_bf16(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+            v.y = pack_bf16(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+            v.z = pack_bf16(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+            v.w = pack_bf16(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+            *reinterpret_cast<uint4*>(out + 32 * c + e) = v;
+          }
+        }
+      }
+      tc_fence_before();
+    }
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == SOFT_WARPS + CONVERT_WARPS) tmem_dealloc(tmem, 512);
+  if (threadIdx.x == 0 && quit) atomicOr(p.flags, B200_PAGED_WAIT);
+}
+
+// Joins the ranges of the keys: 16 threads a row.
+template <int D>
+__global__ void __launch_bounds__(128) prompt_join_kernel(const AttnP p) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int PER = D / 16;
+  const long long x = (long long)blockIdx.x * 8 + (threadIdx.x >> 4);
+  const int row = (int)(x % ROWS), d0 = (threadIdx.x & 15) * PER;
+  int unit = (int)(x / ROWS);
+  const long long first = (long long)unit * p.nsplit * ROWS + row;
+  const int h = unit % p.H; unit /= p.H;
+  const int s = unit % p.b.S, ct = p.q_tiles - 1 - unit / p.b.S, rr = ct * ROWS + row;
+  const Seq q = sequence(p.b, s, p.P);
+  if (!q.ok || q.n < p.from_rows || rr >= q.n * p.G) return;
+  const int rows = min(ROWS, q.n * p.G - ct * ROWS);
+  const Tiles<7> tiles(q.before + ct * ROWS / p.G, q.before + (ct * ROWS + rows - 1) / p.G, p.window, p.sinks);
+  const int per = (tiles.n + p.nsplit - 1) / p.nsplit, parts = (tiles.n + per - 1) / per;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+  float top = -INFINITY, sum = 0.f, acc[PER];
+  for (int i = 0; i < parts; ++i) top = fmaxf(top, ml[first + (long long)i * ROWS].x);
+#pragma unroll
+  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+  for (int i = 0; i < parts; ++i) {
+    const float2 y = ml[first + (long long)i * ROWS];
+    const float by = y.x == -INFINITY ? 0.f : exp2_fast(y.x - top);
+    sum = fmaf(y.y, by, sum);
+    const float4* o = reinterpret_cast<const float4*>(p.part_o + (first + (long long)i * ROWS) * D + d0);
+#pragma unroll
+    for (int e = 0; e < PER / 4; ++e) {
+      const float4 v = o[e];
+      acc[4 * e] = fmaf(v.x, by, acc[4 * e]); acc[4 * e + 1] = fmaf(v.y, by, acc[4 * e + 1]);
+      acc[4 * e + 2] = fmaf(v.z, by, acc[4 * e + 2]); acc[4 * e + 3] = fmaf(v.w, by, acc[4 * e + 3]);
+    }
+  }
+  const float by = sum != 0.f ? 1.f / sum : 0.f;
+  const int token = rr / p.G;
+  bf16* out = p.out + (long long)(q.r0 + token) * p.out_ld + (long long)(h * p.G + rr - token * p.G) * D + d0;
+#pragma unroll
+  for (int e = 0; e < PER; e += 4) *reinterpret_cast<uint2*>(out + e) = make_uint2(pack_bf16(acc[e] * by, acc[e + 1] * by), pack_bf16(acc[e + 2] * by, acc[e + 3] * by));
+}
+
+template <int D, int FMT>
+int launch(const AttnP& p, long long units, cudaStream_t st) {
+  static std::atomic<uint64_t> limits{0};
+  B200_TRY(allow_smem(limits, (int)Smem<D>::BYTES, prompt_kernel<D, FMT>));
+  B200_TRY(launch_early(prompt_kernel<D, FMT>, dim3((unsigned)(units * p.nsplit)), dim3(THREADS), Smem<D>::BYTES, st, p));
+  if (p.nsplit > 1) B200_TRY(launch_early(prompt_join_kernel<D>, dim3((unsigned)(units * (ROWS / 8))), dim3(128), 0, st, p));
+  return B200_OK;
+}
+
+}  // namespace
+
+PromptPlan prompt_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks) {
+  PromptPlan f;
+  f.q_tiles = (int)ceil_div64((long long)b->max_rows * G, ROWS);
+  f.units = (long long)b->sequences * c->kv_heads * f.q_tiles;
+  long long keys = (long long)b->table_width * c->page_tokens;
+  if (window > 0 && (long long)window + sinks + ROWS / G < keys) keys = (long long)window + sinks + ROWS / G;
+  const long long tiles = ceil_div64(keys, KEYS);
+  long long n = f.units ? 148 / f.units : 1;
+  if (n > tiles / 4) n = tiles / 4;          // ranges of four tiles at least
+  f.nsplit = n < 1 ? 1 : (int)n;
+  return f;
+}
+int64_t prompt_bytes(const PromptPlan& f, int D) { return f.nsplit > 1 ? f.units * f.nsplit * ROWS * (D + 2) * 4 : 0; }
+
+int prompt_attention(const AttnP& p, const PromptPlan& f, int fmt, int dim, cudaStream_t st) {
+  if (dim == 128) return fmt == INT8 ? launch<128, INT8>(p, f.units, st) : launch<128, E4M3>(p, f.units, st);
+  return fmt == INT8 ? launch<64, INT8>(p, f.units, st) : launch<64, E4M3>(p, f.units, st);
+}
+
+}  // namespace paged
+}  // namespace b200
