@@ -1,7 +1,7 @@
 // Attention of many rows of a sequence over the paged 8-bit cache, on the 5th-generation tensor cores.
 //
-// A CTA owns one kv head and up to 256 rows (row of the sequence, query head of the group) as two tiles of 128, and walks the keys in tiles of 128 tokens.  Warps 8..11 bring the codes from memory
-// through registers into f16 tiles (exact for both types) in SWIZZLE_128B, keys K-major and values as they lie, tokens by dims; warp 12 issues S_i = Q_i K^T and O_i += P_i V as
+// A CTA owns one kv head and up to 256 rows (row of the sequence, query head of the group) as two tiles of 128, and walks the keys in tiles of 128 tokens.  Warps 8..15 bring the codes from memory
+// through registers into f16 tiles (exact for both types) in SWIZZLE_128B, keys K-major and values as they lie, tokens by dims; warp 16 issues S_i = Q_i K^T and O_i += P_i V as
 // tcgen05.mma with fp32 accumulators in TMEM (S_0, S_1, O_0, O_1); warps 0..3 and 4..7 hold a row per thread, take their scores twice (maximum, then weights) and put P as f16 over the scores,
 // from where the second product reads it.  While one tile's weights are made, the other's products run.
 //
@@ -16,7 +16,7 @@ namespace {
 using namespace tcp;
 typedef __nv_bfloat16 bf16;
 
-constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 4, THREADS = (SOFT_WARPS + CONVERT_WARPS + 1) * 32, ROWS = 256, KEYS = 128, INFOS = 4;
+constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 8, THREADS = (SOFT_WARPS + CONVERT_WARPS + 1) * 32, ROWS = 256, KEYS = 128, INFOS = 4;
 constexpr float SLACK = 8.f;
 
 template <int D>
@@ -53,6 +53,24 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t together(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t two(float a) { return together(a, a); }
+__device__ __forceinline__ void apart(uint64_t x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* quit) { return __all_sync(0xffffffffu, wait_or_quit(bar, parity, quit)); }
 
@@ -110,10 +128,10 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
   if (threadIdx.x == 0) {
     quit = 0;
     for (int i = 0; i < 2; ++i) {
-      mbar_init(k_full + 8 * i, CONVERT_WARPS); mbar_init(k_empty + 8 * i, 1); mbar_init(v_full + 8 * i, CONVERT_WARPS); mbar_init(v_empty + 8 * i, 1);
+      mbar_init(k_full + 8 * i, CONVERT_WARPS / 2); mbar_init(k_empty + 8 * i, 1); mbar_init(v_full + 8 * i, CONVERT_WARPS / 2); mbar_init(v_empty + 8 * i, 1);
       mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, 4); mbar_init(o_done + 8 * i, 1);
     }
-    for (int i = 0; i < INFOS; ++i) mbar_init(i_full + 8 * i, CONVERT_WARPS);
+    for (int i = 0; i < INFOS; ++i) mbar_init(i_full + 8 * i, CONVERT_WARPS / 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   pdl_trigger();
@@ -167,12 +185,14 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
   const int n = u.n;
 
   if (warp >= SOFT_WARPS && warp < SOFT_WARPS + CONVERT_WARPS) {
-    // ---- codes into f16 tiles, 32 tokens a warp ----
-    const int w4 = warp & 3;
+    // ---- codes into f16 tiles: four warps the keys, four the values, 32 tokens each ----
+    const int side = (warp - SOFT_WARPS) >> 2, w4 = warp & 3;
+    const uint8_t* codes = side ? p.v : p.k;
+    const uint32_t full = side ? v_full : k_full, empty = side ? v_empty : k_empty;
     constexpr int LANES = D / 16, STEP = 32 / LANES, LOADS = 32 / STEP;       // lanes a row, rows a load, loads
     const int row = lane / LANES, c = lane % LANES;
-    uint4 held[2][LOADS];                    // of the tile to come: keys, values
-    // lane l: page of the 16 keys that begin at token l * 16 of this warp's
+    uint4 held[LOADS];                       // of the tile to come
+    // lane l: page of the 16 keys that begin at token (l & 1) * 16 of this warp's
     auto look_up = [&](int i) {
       const int j = (tiles[u.t0 + i] << 7) + 32 * w4 + 16 * (lane & 1);
       int page = -1;
@@ -182,56 +202,53 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       }
       return page;
     };
-    auto load = [&](int side, int i, int page) {
+    float2 scales = make_float2(0.f, 1.f);   // of that page, for the tile whose codes are held
+    // lanes of a row's second 64 dims take the neighbouring row, so that eight lanes' pieces of the f16 tile lie in different banks
+    const int r_in = row ^ (D == 128 ? c >> 2 : 0);
+    auto load = [&](int i, int page) {
       const int j0 = (tiles[u.t0 + i] << 7) + 32 * w4;
+      if (side == 0 && page >= 0) scales = make_float2(p.k_scale[(long long)page * p.H + u.h], p.v_scale[(long long)page * p.H + u.h]);
 #pragma unroll
-      for (int x = 0; x < LOADS; ++x) {
-        const int t = x * STEP + row, j = j0 + t, pg = __shfl_sync(0xffffffffu, page, t >> 4);
+      for (int half = 0; half < 2; ++half) {
+        const int pg = __shfl_sync(0xffffffffu, page, half), j1 = j0 + 16 * half;
+        const uint8_t* from = codes + (((long long)pg * p.H + u.h) * p.P + (j1 & (p.P - 1)) + r_in) * D + 16 * c;
         // values that no row sees may be anything; keys are masked
-        const bool seen = pg >= 0 && (side == 0 || (j <= u.pl && (p.window <= 0 || u.pf - j < p.window || j < p.sinks)));
-        held[side][x] = seen ? *reinterpret_cast<const uint4*>((side ? p.v : p.k) + (((long long)pg * p.H + u.h) * p.P + (j & (p.P - 1))) * D + 16 * c) : make_uint4(0, 0, 0, 0);
+        const bool all = side == 0 || (j1 + 15 <= u.pl && (p.window <= 0 || u.pf - j1 < p.window || j1 + 16 <= p.sinks));
+#pragma unroll
+        for (int x = 0; x < LOADS / 2; ++x) {
+          const int j = j1 + x * STEP + r_in;
+          const bool seen = pg >= 0 && (all || (j <= u.pl && (p.window <= 0 || u.pf - j < p.window || j < p.sinks)));
+          held[half * (LOADS / 2) + x] = seen ? *reinterpret_cast<const uint4*>(from + x * STEP * D) : make_uint4(0, 0, 0, 0);
+        }
       }
     };
-    auto convert = [&](int side, int st) {
+    int page = look_up(0), page_next = n > 1 ? look_up(1) : -1;
+    load(0, page);
+    for (int i = 0; i < n; ++i) {
+      const int st = i & 1;
+      if (side == 0) {                       // what the weights need to know of these keys' pages
+        if (lane < 2) {
+          const float vs = scales.y > 0.f ? scales.y : 1.f;                   // all codes of a page of zeros are 0
+          info[i % INFOS][2 * w4 + lane] = page >= 0 ? make_float4(scales.x, __log2f(vs), __frcp_rn(vs), 1.f) : make_float4(0.f, 0.f, 0.f, -1.f);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(i_full + 8 * (i % INFOS));
+      }
+      if (!warp_wait(empty + 8 * st, ((uint32_t)(i >> 1) & 1u) ^ 1u, &quit)) break;
+      uint8_t* const dst = smem + (side ? L::V : L::K) + st * L::TILE + (c >> 2) * L::HALF;
 #pragma unroll
       for (int x = 0; x < LOADS; ++x) {
-        const int t = 32 * w4 + x * STEP + row;
-        const uint4 h = held[side][x];
-        const uint32_t w[4] = {ready<FMT>(h.x), ready<FMT>(h.y), ready<FMT>(h.z), ready<FMT>(h.w)};
-        const uint4 lo = make_uint4(half2_of<FMT, 0>(w[0]), half2_of<FMT, 1>(w[0]), half2_of<FMT, 0>(w[1]), half2_of<FMT, 1>(w[1]));
-        const uint4 hi = make_uint4(half2_of<FMT, 0>(w[2]), half2_of<FMT, 1>(w[2]), half2_of<FMT, 0>(w[3]), half2_of<FMT, 1>(w[3]));
-        uint8_t* r = smem + (side ? L::V : L::K) + st * L::TILE + (c >> 2) * L::HALF + t * 128;
-        const int odd = (c >> 2) & 1, p0 = 2 * (c & 3) + odd, p1 = 2 * (c & 3) + 1 - odd;      // the second half's lanes begin with their second piece: no bank twice
-        *reinterpret_cast<uint4*>(r + ((p0 ^ (t & 7)) << 4)) = odd ? hi : lo;
-        *reinterpret_cast<uint4*>(r + ((p1 ^ (t & 7)) << 4)) = odd ? lo : hi;
+        const int t = 32 * w4 + x * STEP + r_in;
+        const uint32_t w[4] = {ready<FMT>(held[x].x), ready<FMT>(held[x].y), ready<FMT>(held[x].z), ready<FMT>(held[x].w)};
+        uint8_t* r = dst + t * 128;
+        *reinterpret_cast<uint4*>(r + (((2 * (c & 3)) ^ (t & 7)) << 4)) = make_uint4(half2_of<FMT, 0>(w[0]), half2_of<FMT, 1>(w[0]), half2_of<FMT, 0>(w[1]), half2_of<FMT, 1>(w[1]));
+        *reinterpret_cast<uint4*>(r + (((2 * (c & 3) + 1) ^ (t & 7)) << 4)) = make_uint4(half2_of<FMT, 0>(w[2]), half2_of<FMT, 1>(w[2]), half2_of<FMT, 0>(w[3]), half2_of<FMT, 1>(w[3]));
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive((side ? v_full : k_full) + 8 * st);
-    };
-    int page = look_up(0), page_next = n > 1 ? look_up(1) : -1;
-    load(0, 0, page);
-    load(1, 0, page);
-    for (int i = 0; i < n; ++i) {
-      const int st = i & 1;
-      const uint32_t parity = ((uint32_t)(i >> 1) & 1u) ^ 1u;
-      if (lane < 2) {                        // what the weights need to know of these keys' pages
-        float4 x = make_float4(0.f, 0.f, 0.f, -1.f);
-        if (page >= 0) {
-          const float vs = p.v_scale[(long long)page * p.H + u.h], v1 = vs > 0.f ? vs : 1.f;         // all codes of a page of zeros are 0
-          x = make_float4(p.k_scale[(long long)page * p.H + u.h], __log2f(v1), __frcp_rn(v1), 1.f);
-        }
-        info[i % INFOS][2 * w4 + lane] = x;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(i_full + 8 * (i % INFOS));
+      if (lane == 0) mbar_arrive(full + 8 * st);
       page = page_next;
-      if (!warp_wait(k_empty + 8 * st, parity, &quit)) break;
-      convert(0, st);
-      if (i + 1 < n) load(0, i + 1, page);
-      if (!warp_wait(v_empty + 8 * st, parity, &quit)) break;
-      convert(1, st);
-      if (i + 1 < n) load(1, i + 1, page);
+      if (i + 1 < n) load(i + 1, page);
       page_next = i + 2 < n ? look_up(i + 2) : -1;
     }
   } else if (warp == SOFT_WARPS + CONVERT_WARPS) {
@@ -292,29 +309,39 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       bool whole = j0 + KEYS - 1 <= pf && (p.window <= 0 || pl - j0 < p.window || j0 + KEYS <= p.sinks);
 #pragma unroll
       for (int c = 0; c < 8; ++c) whole = whole && ip[c].w > 0.f;
-      float mx[2] = {-INFINITY, -INFINITY};
+      float t = -INFINITY;
+      if (whole) {                           // a page's scale is not negative: the largest score of its keys is that of their largest product
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t r[32];
-        tmem_ld32(ts + 32 * c, r);
-        tmem_ld_wait();
+        for (int c = 0; c < 4; ++c) {
+          uint32_t r[32];
+          tmem_ld32(ts + 32 * c, r);
+          tmem_ld_wait();
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const float4 y = ip[2 * c + b];
-          const float by = y.x * fac;
-          if (whole) {
+          for (int b = 0; b < 2; ++b) {
+            float mx[2] = {__uint_as_float(r[16 * b]), __uint_as_float(r[16 * b + 1])};
 #pragma unroll
-            for (int e = 0; e < 16; ++e) mx[e & 1] = fmaxf(mx[e & 1], fmaf(__uint_as_float(r[16 * b + e]), by, y.y));
-          } else if (y.w > 0.f) {
+            for (int e = 2; e < 16; ++e) mx[e & 1] = fmaxf(mx[e & 1], __uint_as_float(r[16 * b + e]));
+            t = fmaxf(t, fmaf(fmaxf(mx[0], mx[1]), ip[2 * c + b].x * fac, ip[2 * c + b].y));
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t r[32];
+          tmem_ld32(ts + 32 * c, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const float4 y = ip[2 * c + b];
+            const float by = y.x * fac;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               const int j = j0 + 32 * c + 16 * b + e;
-              if (j <= pos && (j > lo || j < p.sinks)) mx[e & 1] = fmaxf(mx[e & 1], fmaf(__uint_as_float(r[16 * b + e]), by, y.y));
+              if (y.w > 0.f && j <= pos && (j > lo || j < p.sinks)) t = fmaxf(t, fmaf(__uint_as_float(r[16 * b + e]), by, y.y));
             }
           }
         }
       }
-      const float t = fmaxf(mx[0], mx[1]);
       const bool grow = t > m + SLACK;
       if (__any_sync(0xffffffffu, grow)) {
         const float factor = grow ? exp2_fast(m - t) : 1.f;
@@ -337,24 +364,42 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       const float off = m == -INFINITY ? 0.f : m;
       // log2 s_v - M in one number is off by half a unit of M: only while that is no more than a quarter
       const bool plain = whole && !__any_sync(0xffffffffu, fabsf(off) > 4194304.f);
+      if (plain) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t r[32], w[16];
-        tmem_ld32(ts + 32 * c, r);
-        tmem_ld_wait();
+        for (int c = 0; c < 4; ++c) {
+          uint32_t r[32], w[16];
+          tmem_ld32(ts + 32 * c, r);
+          tmem_ld_wait();
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const float4 y = ip[2 * c + b];
-          const float by = y.x * fac, add = y.y - off;
-          float part[2] = {0.f, 0.f};
-          if (plain) {
+          for (int b = 0; b < 2; ++b) {
+            const float4 y = ip[2 * c + b];
+            const uint64_t by = two(y.x * fac), add = two(y.y - off);
+            uint64_t part = 0;
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-              const float e0 = exp2_fast(fmaf(__uint_as_float(r[16 * b + e]), by, add)), e1 = exp2_fast(fmaf(__uint_as_float(r[16 * b + e + 1]), by, add));
-              part[0] += e0; part[1] += e1;
+              float e0, e1;
+              apart(fma2(together(__uint_as_float(r[16 * b + e]), __uint_as_float(r[16 * b + e + 1])), by, add), e0, e1);
+              e0 = exp2_fast(e0); e1 = exp2_fast(e1);
+              part = add2(part, together(e0, e1));
               w[8 * b + (e >> 1)] = pack_f16(e0, e1);
             }
-          } else {
+            float s0, s1;
+            apart(part, s0, s1);
+            sum = fmaf(s0 + s1, y.z, sum);
+          }
+          tmem_st16(ts + 16 * c, w);
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t r[32], w[16];
+          tmem_ld32(ts + 32 * c, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const float4 y = ip[2 * c + b];
+            const float by = y.x * fac;
+            float part[2] = {0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
               const int j = j0 + 32 * c + 16 * b + e;
@@ -364,10 +409,10 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
               part[0] += e0; part[1] += e1;
               w[8 * b + (e >> 1)] = pack_f16(e0, e1);
             }
+            sum = fmaf(part[0] + part[1], y.z, sum);
           }
-          sum = fmaf(part[0] + part[1], y.z, sum);
+          tmem_st16(ts + 16 * c, w);
         }
-        tmem_st16(ts + 16 * c, w);
       }
       tmem_st_wait();
       tc_fence_before();
