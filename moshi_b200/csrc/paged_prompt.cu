@@ -1,8 +1,8 @@
 // Attention of many rows of a sequence over the paged 8-bit cache, on the 5th-generation tensor cores.
 //
-// A CTA owns one kv head and up to 256 rows (row of the sequence, query head of the group) as two tiles of 128, and walks the keys in tiles of 128 tokens.  Warps 8..15 bring the codes from memory
-// through registers into f16 tiles (exact for both types) in SWIZZLE_128B, keys K-major and values as they lie, tokens by dims; warp 16 issues S_i = Q_i K^T and O_i += P_i V as
-// tcgen05.mma with fp32 accumulators in TMEM (S_0, S_1, O_0, O_1); warps 0..3 and 4..7 hold a row per thread, take their scores twice (maximum, then weights) and put P as f16 over the scores,
+// A CTA owns one kv head and up to 256 rows (row of the sequence, query head of the group) as two tiles of 128, and walks the keys in tiles of 128 tokens.  Warps 8..14 bring the codes from memory
+// through registers into f16 tiles (exact for both types) in SWIZZLE_128B, keys K-major and values as they lie, tokens by dims; warp 15 issues S_i = Q_i K^T and O_i += P_i V as
+// tcgen05.mma with fp32 accumulators in TMEM (S_0, S_1, O_0, O_1); warps 0..3 and 4..7 hold a row per thread, with all its 128 scores, and put P as f16 over the scores,
 // from where the second product reads it.  While one tile's weights are made, the other's products run.
 //
 // Scales as in paged.cu: that of a page's keys multiplies its 16 or more columns' scores, that of its values goes into the exponent.  O is rescaled only when a row's maximum grew by more than 2^8.
@@ -16,7 +16,7 @@ namespace {
 using namespace tcp;
 typedef __nv_bfloat16 bf16;
 
-constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 8, THREADS = (SOFT_WARPS + CONVERT_WARPS + 1) * 32, ROWS = 256, KEYS = 128, INFOS = 4;
+constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 7, THREADS = (SOFT_WARPS + CONVERT_WARPS + 1) * 32, ROWS = 256, KEYS = 128, INFOS = 4;
 constexpr float SLACK = 8.f;
 
 template <int D>
@@ -116,7 +116,7 @@ template <int D, int FMT>
 __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
   typedef Smem<D> L;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[20 + INFOS];
+  __shared__ __align__(8) uint64_t bars[24 + INFOS];
   __shared__ float4 info[INFOS][8];          // per 16 keys: keys' scale, log2 and reciprocal of the values', whether the page is there
   __shared__ uint32_t tmem_at;
   __shared__ volatile int quit;
@@ -124,14 +124,15 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t bar = smem_u32(bars), k_full = bar, k_empty = bar + 16, v_full = bar + 32, v_empty = bar + 48, s_full = bar + 64, p_full = bar + 80, o_done = bar + 96, i_full = bar + 112;
+  const uint32_t bar = smem_u32(bars), k_full = bar, k_empty = bar + 16, v_full = bar + 32, v_empty = bar + 48, s_full = bar + 64, p_full = bar + 80, o_done = bar + 96, p_half = bar + 112, turns = bar + 128, i_full = bar + 192;
   if (threadIdx.x == 0) {
     quit = 0;
     for (int i = 0; i < 2; ++i) {
-      mbar_init(k_full + 8 * i, CONVERT_WARPS / 2); mbar_init(k_empty + 8 * i, 1); mbar_init(v_full + 8 * i, CONVERT_WARPS / 2); mbar_init(v_empty + 8 * i, 1);
-      mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, 4); mbar_init(o_done + 8 * i, 1);
+      mbar_init(k_full + 8 * i, 4); mbar_init(k_empty + 8 * i, 1); mbar_init(v_full + 8 * i, 4); mbar_init(v_empty + 8 * i, 1);
+      mbar_init(s_full + 8 * i, 1); mbar_init(p_half + 8 * i, 4); mbar_init(p_full + 8 * i, 4); mbar_init(o_done + 8 * i, 1);
     }
-    for (int i = 0; i < INFOS; ++i) mbar_init(i_full + 8 * i, CONVERT_WARPS / 2);
+    for (int i = 0; i < 8; ++i) mbar_init(turns + 8 * i, 1);
+    for (int i = 0; i < INFOS; ++i) mbar_init(i_full + 8 * i, 4);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   pdl_trigger();
@@ -184,17 +185,21 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
   const uint32_t tmem = tmem_at;
   const int n = u.n;
 
-  if (warp >= SOFT_WARPS && warp < SOFT_WARPS + CONVERT_WARPS) {
-    // ---- codes into f16 tiles: four warps the keys, four the values, 32 tokens each ----
-    const int side = (warp - SOFT_WARPS) >> 2, w4 = warp & 3;
-    const uint8_t* codes = side ? p.v : p.k;
-    const uint32_t full = side ? v_full : k_full, empty = side ? v_empty : k_empty;
+  // registers go to the warps that hold a row's scores: 8 x 184 + 8 x 72 = 16 x 128
+  if (warp >= SOFT_WARPS) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  if (warp < SOFT_WARPS + CONVERT_WARPS) {
+    // ---- codes into f16 tiles: 32 tokens of a tile's keys or values at a time, eight such tasks a tile, which the warps take in turn ----
     constexpr int LANES = D / 16, STEP = 32 / LANES, LOADS = 32 / STEP;       // lanes a row, rows a load, loads
     const int row = lane / LANES, c = lane % LANES;
-    uint4 held[LOADS];                       // of the tile to come
-    // lane l: page of the 16 keys that begin at token (l & 1) * 16 of this warp's
-    auto look_up = [&](int i) {
-      const int j = (tiles[u.t0 + i] << 7) + 32 * w4 + 16 * (lane & 1);
+    // lanes of a row's second 64 dims take the neighbouring row, so that eight lanes' pieces of the f16 tile lie in different banks
+    const int r_in = row ^ (D == 128 ? c >> 2 : 0);
+    const int tasks = 8 * n;
+    uint4 held[LOADS];                       // of the task to come
+    float2 scales = make_float2(0.f, 1.f);   // of its pages: lane l has the one of token (l & 1) * 16
+    auto look_up = [&](int task) {
+      if (task >= tasks) return -1;
+      const int j = (tiles[u.t0 + (task >> 3)] << 7) + 32 * (task & 3) + 16 * (lane & 1);
       int page = -1;
       if (j <= u.pl && (p.window <= 0 || u.pf - j - 15 < p.window || j < p.sinks)) {
         page = p.b.table[u.s * p.b.table_ld + (j >> p.page_shift)];
@@ -202,18 +207,18 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       }
       return page;
     };
-    float2 scales = make_float2(0.f, 1.f);   // of that page, for the tile whose codes are held
-    // lanes of a row's second 64 dims take the neighbouring row, so that eight lanes' pieces of the f16 tile lie in different banks
-    const int r_in = row ^ (D == 128 ? c >> 2 : 0);
-    auto load = [&](int i, int page) {
-      const int j0 = (tiles[u.t0 + i] << 7) + 32 * w4;
-      if (side == 0 && page >= 0) scales = make_float2(p.k_scale[(long long)page * p.H + u.h], p.v_scale[(long long)page * p.H + u.h]);
+    auto load = [&](int task, int page) {
+      if (task >= tasks) return;
+      const bool keys = !(task & 4);
+      const uint8_t* codes = keys ? p.k : p.v;
+      const int j0 = (tiles[u.t0 + (task >> 3)] << 7) + 32 * (task & 3);
+      if (keys && page >= 0) scales = make_float2(p.k_scale[(long long)page * p.H + u.h], p.v_scale[(long long)page * p.H + u.h]);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int pg = __shfl_sync(0xffffffffu, page, half), j1 = j0 + 16 * half;
         const uint8_t* from = codes + (((long long)pg * p.H + u.h) * p.P + (j1 & (p.P - 1)) + r_in) * D + 16 * c;
         // values that no row sees may be anything; keys are masked
-        const bool all = side == 0 || (j1 + 15 <= u.pl && (p.window <= 0 || u.pf - j1 < p.window || j1 + 16 <= p.sinks));
+        const bool all = keys || (j1 + 15 <= u.pl && (p.window <= 0 || u.pf - j1 < p.window || j1 + 16 <= p.sinks));
 #pragma unroll
         for (int x = 0; x < LOADS / 2; ++x) {
           const int j = j1 + x * STEP + r_in;
@@ -222,20 +227,21 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
         }
       }
     };
-    int page = look_up(0), page_next = n > 1 ? look_up(1) : -1;
-    load(0, page);
-    for (int i = 0; i < n; ++i) {
-      const int st = i & 1;
-      if (side == 0) {                       // what the weights need to know of these keys' pages
+    int task = warp - SOFT_WARPS, page = look_up(task), page_next = look_up(task + CONVERT_WARPS);
+    load(task, page);
+    for (; task < tasks; task += CONVERT_WARPS) {
+      const int i = task >> 3, st = i & 1, w4 = task & 3;
+      const bool keys = !(task & 4);
+      if (keys) {                            // what the weights need to know of these keys' pages
         if (lane < 2) {
           const float vs = scales.y > 0.f ? scales.y : 1.f;                   // all codes of a page of zeros are 0
           info[i % INFOS][2 * w4 + lane] = page >= 0 ? make_float4(scales.x, __log2f(vs), __frcp_rn(vs), 1.f) : make_float4(0.f, 0.f, 0.f, -1.f);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(i_full + 8 * (i % INFOS));
       }
-      if (!warp_wait(empty + 8 * st, ((uint32_t)(i >> 1) & 1u) ^ 1u, &quit)) break;
-      uint8_t* const dst = smem + (side ? L::V : L::K) + st * L::TILE + (c >> 2) * L::HALF;
+      if (!warp_wait((keys ? k_empty : v_empty) + 8 * st, ((uint32_t)(i >> 1) & 1u) ^ 1u, &quit)) break;
+      if (keys && lane == 0) mbar_arrive(i_full + 8 * (i % INFOS));
+      uint8_t* const dst = smem + (keys ? L::K : L::V) + st * L::TILE + (c >> 2) * L::HALF;
 #pragma unroll
       for (int x = 0; x < LOADS; ++x) {
         const int t = 32 * w4 + x * STEP + r_in;
@@ -246,12 +252,12 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(full + 8 * st);
+      if (lane == 0) mbar_arrive((keys ? k_full : v_full) + 8 * st);
       page = page_next;
-      if (i + 1 < n) load(i + 1, page);
-      page_next = i + 2 < n ? look_up(i + 2) : -1;
+      load(task + CONVERT_WARPS, page);
+      page_next = look_up(task + 2 * CONVERT_WARPS);
     }
-  } else if (warp == SOFT_WARPS + CONVERT_WARPS) {
+  } else {
     // ---- products ----
     constexpr uint32_t id_s = idesc_f16(KEYS, false), id_o = idesc_f16(D, true);
     auto scores = [&](int i, int x) {        // of tile x for queries i
@@ -269,15 +275,20 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
     for (int x = 0; ok && x < n; ++x) {
       const int st = x & 1;
       for (int i = 0; ok && i < tiles_q; ++i) {
-        ok = (i > 0 || warp_wait(v_full + 8 * st, (uint32_t)(x >> 1) & 1u, &quit)) && warp_wait(p_full + 8 * i, (uint32_t)x & 1u, &quit);
-        if (!ok) break;
-        tc_fence_after();
-        if (elected()) {
+        ok = i > 0 || warp_wait(v_full + 8 * st, (uint32_t)(x >> 1) & 1u, &quit);
 #pragma unroll
-          for (int k = 0; k < KEYS / 16; ++k)
-            product_pv(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k, base + L::V + st * L::TILE + k * 2048, L::HALF, id_o, x > 0 || k > 0 ? 1u : 0u);
+        for (int half = 0; half < 2; ++half) {                                // of the keys: the second half's weights are made beside the first's product
+          ok = ok && warp_wait((half ? p_full : p_half) + 8 * i, (uint32_t)x & 1u, &quit);
+          if (!ok) break;
+          tc_fence_after();
+          if (elected()) {
+#pragma unroll
+            for (int k = half * KEYS / 32; k < (half + 1) * KEYS / 32; ++k)
+              product_pv(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k, base + L::V + st * L::TILE + k * 2048, L::HALF, id_o, x > 0 || k > 0 ? 1u : 0u);
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (!ok) break;
         commit_elected(o_done + 8 * i);
         if (i == tiles_q - 1) commit_elected(v_empty + 8 * st);
         if (x + 1 < n) {                     // the next scores lie over these weights
@@ -290,7 +301,10 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       }
     }
     __syncwarp();
-  } else if ((warp >> 2) < tiles_q) {
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    if ((warp >> 2) < tiles_q) {
     // ---- weights: a row per thread ----
     const int i = warp >> 2, q4 = warp & 3, row = 128 * i + q4 * 32 + lane, rr = u.r0 + row;
     const bool has = row < u.rows;
@@ -306,41 +320,49 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       tc_fence_after();
       const int j0 = tiles[u.t0 + x] << 7;
       const float4* ip = info[x % INFOS];
-      bool whole = j0 + KEYS - 1 <= pf && (p.window <= 0 || pl - j0 < p.window || j0 + KEYS <= p.sinks);
+      bool there = true;                     // all pages
 #pragma unroll
-      for (int c = 0; c < 8; ++c) whole = whole && ip[c].w > 0.f;
-      float t = -INFINITY;
-      if (whole) {                           // a page's scale is not negative: the largest score of its keys is that of their largest product
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t r[32];
-          tmem_ld32(ts + 32 * c, r);
-          tmem_ld_wait();
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            float mx[2] = {__uint_as_float(r[16 * b]), __uint_as_float(r[16 * b + 1])};
-#pragma unroll
-            for (int e = 2; e < 16; ++e) mx[e & 1] = fmaxf(mx[e & 1], __uint_as_float(r[16 * b + e]));
-            t = fmaxf(t, fmaf(fmaxf(mx[0], mx[1]), ip[2 * c + b].x * fac, ip[2 * c + b].y));
-          }
-        }
-      } else {
+      for (int c = 0; c < 8; ++c) there &= ip[c].w > 0.f;
+      const bool whole = there & (j0 + KEYS - 1 <= pf) & ((p.window <= 0) | (pl - j0 < p.window) | (j0 + KEYS <= p.sinks));
+      bool made = false;                     // scores, no longer products, in TMEM
+      // Rare, and so kept short: a loop over TMEM, that the usual way's instructions stay together.
+      auto make = [&] {
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
-          uint32_t r[32];
-          tmem_ld32(ts + 32 * c, r);
+          uint32_t y[32];
+          tmem_ld32(ts + 32 * c, y);
           tmem_ld_wait();
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            const float4 y = ip[2 * c + b];
-            const float by = y.x * fac;
+            const float4 z = ip[2 * c + b];
+            const float by = z.x * fac;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int j = j0 + 32 * c + 16 * b + e;
-              if (y.w > 0.f && j <= pos && (j > lo || j < p.sinks)) t = fmaxf(t, fmaf(__uint_as_float(r[16 * b + e]), by, y.y));
+            for (int e = 16 * b; e < 16 * b + 16; ++e) {
+              const int j = j0 + 32 * c + e;
+              y[e] = z.w > 0.f && j <= pos && (j > lo || j < p.sinks) ? __float_as_uint(fmaf(__uint_as_float(y[e]), by, z.y)) : 0xff800000u;
             }
           }
+          tmem_st32(ts + 32 * c, y);
         }
+        tmem_st_wait();
+        made = true;
+      };
+      if (!whole) make();
+      uint32_t r[KEYS];                      // the row's scores: read once, as the registers have room for them
+      float t = -INFINITY;
+      tmem_ld32(ts, r);
+      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (c < 3) tmem_ld32(ts + 32 * c + 32, r + 32 * c + 32);
+#pragma unroll
+        for (int b = 2 * c; b < 2 * c + 2; ++b) {                             // a page's scale is not negative: the largest score of its keys is that of their largest product
+          float mx[2] = {__uint_as_float(r[16 * b]), __uint_as_float(r[16 * b + 1])};
+#pragma unroll
+          for (int e = 2; e < 16; ++e) mx[e & 1] = fmaxf(mx[e & 1], __uint_as_float(r[16 * b + e]));
+          t = fmaxf(t, fmaf(fmaxf(mx[0], mx[1]), made ? 1.f : ip[b].x * fac, made ? 0.f : ip[b].y));
+        }
+        if (c < 3) tmem_ld_wait();
       }
       const bool grow = t > m + SLACK;
       if (__any_sync(0xffffffffu, grow)) {
@@ -351,73 +373,58 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
           if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
           tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(to + 32 * c, o);
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(to + 16 * c, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-            tmem_st32(to + 32 * c, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+            tmem_st16(to + 16 * c, o);
           }
         }
       }
       const float off = m == -INFINITY ? 0.f : m;
       // log2 s_v - M in one number is off by half a unit of M: only while that is no more than a quarter
-      const bool plain = whole && !__any_sync(0xffffffffu, fabsf(off) > 4194304.f);
-      if (plain) {
+      // The two warps of a quarter of the SM, one of each tile, make their weights in turn: side by side both would wait for the exponentials' unit and then, together, for the products.
+      if (tiles_q > 1 && (i > 0 || x > 0)) {
+        ok = warp_wait(turns + 8 * (4 * i + q4), (uint32_t)(i > 0 ? x : x - 1) & 1u, &quit);
+        if (!ok) break;
+      }
+      if (!made && __any_sync(0xffffffffu, fabsf(off) > 4194304.f && off < INFINITY)) {
+        make();
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t r[32], w[16];
-          tmem_ld32(ts + 32 * c, r);
-          tmem_ld_wait();
+        for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r + 32 * c);
+        tmem_ld_wait();
+      }
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const float4 y = ip[2 * c + b];
-            const uint64_t by = two(y.x * fac), add = two(y.y - off);
-            uint64_t part = 0;
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[16];
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              float e0, e1;
-              apart(fma2(together(__uint_as_float(r[16 * b + e]), __uint_as_float(r[16 * b + e + 1])), by, add), e0, e1);
-              e0 = exp2_fast(e0); e1 = exp2_fast(e1);
-              part = add2(part, together(e0, e1));
-              w[8 * b + (e >> 1)] = pack_f16(e0, e1);
-            }
-            float s0, s1;
-            apart(part, s0, s1);
-            sum = fmaf(s0 + s1, y.z, sum);
+        for (int b = 2 * c; b < 2 * c + 2; ++b) {
+          const float4 y = ip[b];
+          const uint64_t by = two(made ? 1.f : y.x * fac), add = two(made ? -off : y.y - off);
+          uint64_t part = 0;
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            float e0, e1;
+            apart(fma2(together(__uint_as_float(r[16 * b + e]), __uint_as_float(r[16 * b + e + 1])), by, add), e0, e1);
+            e0 = exp2_fast(e0); e1 = exp2_fast(e1);
+            part = add2(part, together(e0, e1));
+            w[8 * (b & 1) + (e >> 1)] = pack_f16(e0, e1);
           }
-          tmem_st16(ts + 16 * c, w);
+          float s0, s1;
+          apart(part, s0, s1);
+          sum = fmaf(s0 + s1, y.z, sum);
         }
-      } else {
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t r[32], w[16];
-          tmem_ld32(ts + 32 * c, r);
-          tmem_ld_wait();
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const float4 y = ip[2 * c + b];
-            const float by = y.x * fac;
-            float part[2] = {0.f, 0.f};
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              const int j = j0 + 32 * c + 16 * b + e;
-              float e0 = exp2_fast(fmaf(__uint_as_float(r[16 * b + e]), by, y.y) - off), e1 = exp2_fast(fmaf(__uint_as_float(r[16 * b + e + 1]), by, y.y) - off);
-              if (!(y.w > 0.f && j <= pos && (j > lo || j < p.sinks))) e0 = 0.f;
-              if (!(y.w > 0.f && j + 1 <= pos && (j + 1 > lo || j + 1 < p.sinks))) e1 = 0.f;
-              part[0] += e0; part[1] += e1;
-              w[8 * b + (e >> 1)] = pack_f16(e0, e1);
-            }
-            sum = fmaf(part[0] + part[1], y.z, sum);
-          }
-          tmem_st16(ts + 16 * c, w);
+        tmem_st16(ts + 16 * c, w);
+        if (c == 3 && tiles_q > 1 && lane == 0) mbar_arrive(turns + 8 * (4 * (i ^ 1) + q4));
+        if (c & 1) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive((c == 1 ? p_half : p_full) + 8 * i);
         }
       }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + 8 * i);
     }
     if (ok) {
       ok = wait_or_quit(o_done + 8 * i, (uint32_t)(n - 1) & 1u, &quit);
@@ -453,6 +460,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
         }
       }
       tc_fence_before();
+    }
     }
   }
   __syncthreads();
