@@ -8,6 +8,8 @@
 // Scales as in paged.cu: that of a page's keys multiplies its 16 or more columns' scores, that of its values goes into the exponent.  O is rescaled only when a row's maximum grew by more than 2^8.
 #include "paged.cuh"
 
+#include <cfloat>
+
 namespace b200 {
 namespace paged {
 
@@ -34,12 +36,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
 }
 #undef R32
 #define R8(r, o) "r"((r)[o]), "r"((r)[o + 1]), "r"((r)[o + 2]), "r"((r)[o + 3]), "r"((r)[o + 4]), "r"((r)[o + 5]), "r"((r)[o + 6]), "r"((r)[o + 7])
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-      ::"r"(taddr), R8(r, 0), R8(r, 8), R8(r, 16), R8(r, 24) : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
                ::"r"(taddr), R8(r, 0), R8(r, 8) : "memory");
@@ -72,6 +68,8 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// bits 0 .. x of 32
+__device__ __forceinline__ uint32_t upto(int x) { return x < 0 ? 0u : x > 31 ? 0xffffffffu : 0xffffffffu >> (31 - x); }
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* quit) { return __all_sync(0xffffffffu, wait_or_quit(bar, parity, quit)); }
 
 // kind::f16, f16 operands, fp32 accumulators, 128 rows by n columns; `tokens_first`: the second operand lies [k][n]
@@ -116,22 +114,22 @@ template <int D, int FMT>
 __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
   typedef Smem<D> L;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[24 + INFOS];
+  __shared__ __align__(8) uint64_t bars[17 + INFOS];
   __shared__ float4 info[INFOS][8];          // per 16 keys: keys' scale, log2 and reciprocal of the values', whether the page is there
   __shared__ uint32_t tmem_at;
   __shared__ volatile int quit;
-  __shared__ float tops[THREADS / 32];
+  __shared__ float tops[SOFT_WARPS];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t bar = smem_u32(bars), k_full = bar, k_empty = bar + 16, v_full = bar + 32, v_empty = bar + 48, s_full = bar + 64, p_full = bar + 80, o_done = bar + 96, p_half = bar + 112, turns = bar + 128, i_full = bar + 192;
+  const uint32_t bar = smem_u32(bars), k_full = bar, k_empty = bar + 16, v_full = bar + 32, v_empty = bar + 48, s_full = bar + 64, p_full = bar + 80, o_done = bar + 96, p_half = bar + 112, q_full = bar + 128, i_full = bar + 136;
   if (threadIdx.x == 0) {
     quit = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(k_full + 8 * i, 4); mbar_init(k_empty + 8 * i, 1); mbar_init(v_full + 8 * i, 4); mbar_init(v_empty + 8 * i, 1);
       mbar_init(s_full + 8 * i, 1); mbar_init(p_half + 8 * i, 4); mbar_init(p_full + 8 * i, 4); mbar_init(o_done + 8 * i, 1);
     }
-    for (int i = 0; i < 8; ++i) mbar_init(turns + 8 * i, 1);
+    mbar_init(q_full, SOFT_WARPS);
     for (int i = 0; i < INFOS; ++i) mbar_init(i_full + 8 * i, 4);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -146,42 +144,9 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
   const int tiles_q = u.rows > 128 ? 2 : 1;
   const Tiles<7> tiles(u.pf, u.pl, p.window, p.sinks);
 
-  // ---- queries: f16 after one power of two for all of them ----
-  constexpr int PIECES = D / 8;              // 16-byte pieces of a row
-  auto query = [&](int x) {
-    const int r = x / PIECES, i = (u.r0 + r) / p.G, g = u.r0 + r - i * p.G;
-    return *reinterpret_cast<const uint4*>(p.q + (long long)(u.q.r0 + i) * p.q_ld + (long long)(u.h * p.G + g) * D + (x % PIECES) * 8);
-  };
-  float top = 0.f;
-  for (int x = threadIdx.x; x < u.rows * PIECES; x += THREADS) {
-    const uint4 w = query(x);
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = fabsf(__uint_as_float(v[i] << 16)), b = fabsf(__uint_as_float(v[i] & 0xffff0000u));
-      if (a < INFINITY) top = fmaxf(top, a);
-      if (b < INFINITY) top = fmaxf(top, b);
-    }
-  }
-  top = warp_max(top);
-  if (lane == 0) tops[warp] = top;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-#pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) top = fmaxf(top, tops[i]);
-  const float power = top > 0.f ? power_of_two_in(top) : 1.f, up = 16384.f / power;
-  for (int x = threadIdx.x; x < tiles_q * 128 * PIECES; x += THREADS) {
-    const int r = x / PIECES, c = x % PIECES;
-    const uint4 w = r < u.rows ? query(x) : make_uint4(0, 0, 0, 0);
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-    uint32_t o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = pack_f16(__uint_as_float(v[i] << 16) * up, __uint_as_float(v[i] & 0xffff0000u) * up);
-    *reinterpret_cast<uint4*>(smem + L::Q + (r >> 7) * L::TILE + (c >> 3) * L::HALF + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-  }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  __syncthreads();
   const uint32_t tmem = tmem_at;
   const int n = u.n;
 
@@ -235,7 +200,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       if (keys) {                            // what the weights need to know of these keys' pages
         if (lane < 2) {
           const float vs = scales.y > 0.f ? scales.y : 1.f;                   // all codes of a page of zeros are 0
-          info[i % INFOS][2 * w4 + lane] = page >= 0 ? make_float4(scales.x, __log2f(vs), __frcp_rn(vs), 1.f) : make_float4(0.f, 0.f, 0.f, -1.f);
+          info[i % INFOS][2 * w4 + lane] = page >= 0 ? make_float4(scales.x > 0.f ? scales.x : 1.f, __log2f(vs), __frcp_rn(vs), 1.f) : make_float4(0.f, 0.f, 0.f, -1.f);
         }
         __syncwarp();
       }
@@ -266,7 +231,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       for (int half = 0; half < D / 64; ++half) umma_block<1>(tmem + 128 * i, a + half * (L::HALF >> 4), b - a, id_s, half > 0 ? 1u : 0u);
       commit_elected(s_full + 8 * i);
     };
-    bool ok = warp_wait(k_full, 0, &quit);
+    bool ok = warp_wait(q_full, 0, &quit) && warp_wait(k_full, 0, &quit);
     if (ok) {
       tc_fence_after();
       for (int i = 0; i < tiles_q; ++i) scores(i, 0);
@@ -304,6 +269,47 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    // ---- queries: f16 after one power of two for all of them ----
+    constexpr int PIECES = D / 8, MINE = 2 * 128 * PIECES / (SOFT_WARPS * 32);          // 16-byte pieces of a row, and of this thread
+    float power;
+    {
+      uint4 raw[MINE];
+      float top = 0.f;
+#pragma unroll
+      for (int k = 0; k < MINE; ++k) {
+        const int x = k * SOFT_WARPS * 32 + threadIdx.x, r = x / PIECES, i = (u.r0 + r) / p.G, g = u.r0 + r - i * p.G;
+        raw[k] = r < u.rows ? *reinterpret_cast<const uint4*>(p.q + (long long)(u.q.r0 + i) * p.q_ld + (long long)(u.h * p.G + g) * D + (x % PIECES) * 8) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < MINE; ++k) {
+        const uint32_t v[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float a = fabsf(__uint_as_float(v[i] << 16)), b = fabsf(__uint_as_float(v[i] & 0xffff0000u));
+          if (a < INFINITY) top = fmaxf(top, a);
+          if (b < INFINITY) top = fmaxf(top, b);
+        }
+      }
+      top = warp_max(top);
+      if (lane == 0) tops[warp] = top;
+      asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
+#pragma unroll
+      for (int i = 0; i < SOFT_WARPS; ++i) top = fmaxf(top, tops[i]);
+      power = top > 0.f ? power_of_two_in(top) : 1.f;
+      const float up = 16384.f / power;
+#pragma unroll
+      for (int k = 0; k < MINE; ++k) {
+        const int x = k * SOFT_WARPS * 32 + threadIdx.x, r = x / PIECES, c = x % PIECES;
+        const uint32_t v[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = pack_f16(__uint_as_float(v[i] << 16) * up, __uint_as_float(v[i] & 0xffff0000u) * up);
+        *reinterpret_cast<uint4*>(smem + L::Q + (r >> 7) * L::TILE + (c >> 3) * L::HALF + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
     if ((warp >> 2) < tiles_q) {
     // ---- weights: a row per thread ----
     const int i = warp >> 2, q4 = warp & 3, row = 128 * i + q4 * 32 + lane, rr = u.r0 + row;
@@ -324,30 +330,6 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
 #pragma unroll
       for (int c = 0; c < 8; ++c) there &= ip[c].w > 0.f;
       const bool whole = there & (j0 + KEYS - 1 <= pf) & ((p.window <= 0) | (pl - j0 < p.window) | (j0 + KEYS <= p.sinks));
-      bool made = false;                     // scores, no longer products, in TMEM
-      // Rare, and so kept short: a loop over TMEM, that the usual way's instructions stay together.
-      auto make = [&] {
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t y[32];
-          tmem_ld32(ts + 32 * c, y);
-          tmem_ld_wait();
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const float4 z = ip[2 * c + b];
-            const float by = z.x * fac;
-#pragma unroll
-            for (int e = 16 * b; e < 16 * b + 16; ++e) {
-              const int j = j0 + 32 * c + e;
-              y[e] = z.w > 0.f && j <= pos && (j > lo || j < p.sinks) ? __float_as_uint(fmaf(__uint_as_float(y[e]), by, z.y)) : 0xff800000u;
-            }
-          }
-          tmem_st32(ts + 32 * c, y);
-        }
-        tmem_st_wait();
-        made = true;
-      };
-      if (!whole) make();
       uint32_t r[KEYS];                      // the row's scores: read once, as the registers have room for them
       float t = -INFINITY;
       tmem_ld32(ts, r);
@@ -355,12 +337,21 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         if (c < 3) tmem_ld32(ts + 32 * c + 32, r + 32 * c + 32);
+        if (!whole) {                        // keys that the row does not see: a bit for each of 32
+          const int at = j0 + 32 * c;
+          uint32_t seen = upto(pos - at) & (~upto(lo - at) | upto(p.sinks - 1 - at));
+          if (!(ip[2 * c].w > 0.f)) seen &= 0xffff0000u;
+          if (!(ip[2 * c + 1].w > 0.f)) seen &= 0xffffu;
 #pragma unroll
-        for (int b = 2 * c; b < 2 * c + 2; ++b) {                             // a page's scale is not negative: the largest score of its keys is that of their largest product
+          for (int e = 0; e < 32; ++e)
+            if (!(seen >> e & 1u)) r[32 * c + e] = 0xff800000u;
+        }
+#pragma unroll
+        for (int b = 2 * c; b < 2 * c + 2; ++b) {                             // `by` is positive: the largest score of a page's keys is that of their largest product
           float mx[2] = {__uint_as_float(r[16 * b]), __uint_as_float(r[16 * b + 1])};
 #pragma unroll
           for (int e = 2; e < 16; ++e) mx[e & 1] = fmaxf(mx[e & 1], __uint_as_float(r[16 * b + e]));
-          t = fmaxf(t, fmaf(fmaxf(mx[0], mx[1]), made ? 1.f : ip[b].x * fac, made ? 0.f : ip[b].y));
+          t = fmaxf(t, fmaf(fmaxf(mx[0], mx[1]), fmaxf(ip[b].x * fac, FLT_MIN), ip[b].y));
         }
         if (c < 3) tmem_ld_wait();
       }
@@ -385,16 +376,10 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       }
       const float off = m == -INFINITY ? 0.f : m;
       // log2 s_v - M in one number is off by half a unit of M: only while that is no more than a quarter
-      // The two warps of a quarter of the SM, one of each tile, make their weights in turn: side by side both would wait for the exponentials' unit and then, together, for the products.
-      if (tiles_q > 1 && (i > 0 || x > 0)) {
-        ok = warp_wait(turns + 8 * (4 * i + q4), (uint32_t)(i > 0 ? x : x - 1) & 1u, &quit);
-        if (!ok) break;
-      }
-      if (!made && __any_sync(0xffffffffu, fabsf(off) > 4194304.f && off < INFINITY)) {
-        make();
+      const bool far = __any_sync(0xffffffffu, fabsf(off) > 4194304.f && off < INFINITY);
+      if (far) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r + 32 * c);
-        tmem_ld_wait();
+        for (int e = 0; e < KEYS; ++e) r[e] = __float_as_uint(fmaf(__uint_as_float(r[e]), fmaxf(ip[e / 16].x * fac, FLT_MIN), ip[e / 16].y));
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -402,7 +387,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
 #pragma unroll
         for (int b = 2 * c; b < 2 * c + 2; ++b) {
           const float4 y = ip[b];
-          const uint64_t by = two(made ? 1.f : y.x * fac), add = two(made ? -off : y.y - off);
+          const uint64_t by = two(far ? 1.f : fmaxf(y.x * fac, FLT_MIN)), add = two(far ? -off : y.y - off);
           uint64_t part = 0;
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
@@ -417,7 +402,6 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
           sum = fmaf(s0 + s1, y.z, sum);
         }
         tmem_st16(ts + 16 * c, w);
-        if (c == 3 && tiles_q > 1 && lane == 0) mbar_arrive(turns + 8 * (4 * (i ^ 1) + q4));
         if (c & 1) {
           tmem_st_wait();
           tc_fence_before();
