@@ -35,6 +35,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
       : R32(r, 0), R32(r, 8), R32(r, 16), R32(r, 24) : "r"(taddr));
 }
 #undef R32
+// Waits for loads, these 32 among them: nothing that uses them may come in front.
+#define R32(r, o) "+r"((r)[o]), "+r"((r)[o + 1]), "+r"((r)[o + 2]), "+r"((r)[o + 3]), "+r"((r)[o + 4]), "+r"((r)[o + 5]), "+r"((r)[o + 6]), "+r"((r)[o + 7])
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : R32(r, 0), R32(r, 8), R32(r, 16), R32(r, 24) :: "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait16(uint32_t* r) { asm volatile("tcgen05.wait::ld.sync.aligned;" : R32(r, 0), R32(r, 8) :: "memory"); }
+#undef R32
 #define R8(r, o) "r"((r)[o]), "r"((r)[o + 1]), "r"((r)[o + 2]), "r"((r)[o + 3]), "r"((r)[o + 4]), "r"((r)[o + 5]), "r"((r)[o + 6]), "r"((r)[o + 7])
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
@@ -275,10 +282,16 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
     {
       uint4 raw[MINE];
       float top = 0.f;
+      // the thread has piece c of every APART-th row from `at` on; token and head of a row by counting, not by division
+      constexpr int APART = SOFT_WARPS * 32 / PIECES;
+      const int c = threadIdx.x % PIECES, at = threadIdx.x / PIECES, step_i = APART / p.G, step_g = APART - step_i * p.G;
+      int i = (u.r0 + at) / p.G, g = u.r0 + at - i * p.G;
+      const bf16* const q0 = p.q + (long long)u.q.r0 * p.q_ld + (long long)u.h * p.G * D + c * 8;
 #pragma unroll
       for (int k = 0; k < MINE; ++k) {
-        const int x = k * SOFT_WARPS * 32 + threadIdx.x, r = x / PIECES, i = (u.r0 + r) / p.G, g = u.r0 + r - i * p.G;
-        raw[k] = r < u.rows ? *reinterpret_cast<const uint4*>(p.q + (long long)(u.q.r0 + i) * p.q_ld + (long long)(u.h * p.G + g) * D + (x % PIECES) * 8) : make_uint4(0, 0, 0, 0);
+        raw[k] = at + k * APART < u.rows ? *reinterpret_cast<const uint4*>(q0 + i * p.q_ld + g * D) : make_uint4(0, 0, 0, 0);
+        i += step_i; g += step_g;
+        if (g >= p.G) { g -= p.G; ++i; }
       }
 #pragma unroll
       for (int k = 0; k < MINE; ++k) {
@@ -299,7 +312,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       const float up = 16384.f / power;
 #pragma unroll
       for (int k = 0; k < MINE; ++k) {
-        const int x = k * SOFT_WARPS * 32 + threadIdx.x, r = x / PIECES, c = x % PIECES;
+        const int r = at + k * APART;
         const uint32_t v[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
         uint32_t o[4];
 #pragma unroll
@@ -333,7 +346,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       uint32_t r[KEYS];                      // the row's scores: read once, as the registers have room for them
       float t = -INFINITY;
       tmem_ld32(ts, r);
-      tmem_ld_wait();
+      tmem_ld_wait32(r);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         if (c < 3) tmem_ld32(ts + 32 * c + 32, r + 32 * c + 32);
@@ -353,7 +366,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
           for (int e = 2; e < 16; ++e) mx[e & 1] = fmaxf(mx[e & 1], __uint_as_float(r[16 * b + e]));
           t = fmaxf(t, fmaf(fmaxf(mx[0], mx[1]), fmaxf(ip[b].x * fac, FLT_MIN), ip[b].y));
         }
-        if (c < 3) tmem_ld_wait();
+        if (c < 3) tmem_ld_wait32(r + 32 * c + 32);
       }
       const bool grow = t > m + SLACK;
       if (__any_sync(0xffffffffu, grow)) {
@@ -367,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
           for (int c = 0; c < D / 16; ++c) {
             uint32_t o[16];
             tmem_ld16(to + 16 * c, o);
-            tmem_ld_wait();
+            tmem_ld_wait16(o);
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
             tmem_st16(to + 16 * c, o);
@@ -417,21 +430,28 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
     if (ok) {
       tc_fence_after();
       const float inv = sum != 0.f ? 1.f / sum : 0.f;
-      const int token = rr / p.G, unit = (int)blockIdx.x;
-      bf16* out = p.out + (long long)(u.q.r0 + token) * p.out_ld + (long long)(u.h * p.G + rr - token * p.G) * D;
-      float* part = p.part_o + ((long long)unit * ROWS + row) * D;
-      if (p.nsplit > 1 && has) *reinterpret_cast<float2*>(p.part_ml + 2 * ((long long)unit * ROWS + row)) = make_float2(m, sum);
+      if (p.nsplit > 1) {
+        const long long at = (long long)blockIdx.x * ROWS + row;
+        if (has) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m, sum);
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        __syncwarp();
-        tmem_ld32(to + 32 * c, o);
-        tmem_ld_wait();
-        if (!has) continue;
-        if (p.nsplit > 1) {
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_ld32(to + 32 * c, o);
+          tmem_ld_wait32(o);
+          if (has) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(part + 32 * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-        } else {
+            for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(p.part_o + at * D + 32 * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+      } else {
+        // through the queries' place, which nobody reads any more: whole rows go out, and not 16 bytes of 32 rows at a time
+        uint8_t* const mine = smem + L::Q + (i * 4 + q4) * (32 * D * 2);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(to + 32 * c, o);
+          tmem_ld_wait32(o);
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             uint4 v;
@@ -439,8 +459,19 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
             v.y = pack_bf16(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
             v.z = pack_bf16(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
             v.w = pack_bf16(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-            *reinterpret_cast<uint4*>(out + 32 * c + e) = v;
+            const int piece = 4 * c + e / 8;
+            *reinterpret_cast<uint4*>(mine + lane * D * 2 + ((piece ^ (lane & 7)) << 4)) = v;
           }
+        }
+        __syncwarp();
+        constexpr int AT_ONCE = 32 / PIECES;
+        const int c = lane % PIECES;
+        bf16* const out0 = p.out + (long long)u.q.r0 * p.out_ld + (long long)u.h * p.G * D + c * 8;
+#pragma unroll 4
+        for (int k = 0; k < 32; k += AT_ONCE) {
+          const int r = k + lane / PIECES, x = u.r0 + 128 * i + 32 * q4 + r, token = x / p.G;
+          if (128 * i + 32 * q4 + r < u.rows)
+            *reinterpret_cast<uint4*>(out0 + token * p.out_ld + (x - token * p.G) * D) = *reinterpret_cast<const uint4*>(mine + r * D * 2 + ((c ^ (r & 7)) << 4));
         }
       }
       tc_fence_before();
