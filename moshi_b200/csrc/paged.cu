@@ -39,7 +39,7 @@ struct AppendP {
   long long k_ld, v_ld, q_ld, q_out_ld;
   const uint64_t* turns;                     // per pair of dimensions: turns per position as a 64-bit fraction; null: no rotation
   int rot, halves;                           // rotated dimensions; pairs are (j, j + rot / 2), else (2j, 2j + 1)
-  int pages, P, H, Hq, page_tasks, page_ctas, q_rows;
+  int pages, P, H, Hq, items, heads_per_block, page_ctas, q_rows;            // items: numbers of touched pages
 };
 
 // Sixteen dimensions of a row: eight from `lo` on and eight from `hi` on, so that a rotated pair is always in one thread's hands.
@@ -63,14 +63,17 @@ __device__ __forceinline__ void turn_of(Turn& t, const uint64_t* turns, int j, i
     sincospif((float)part * 4.656612873077393e-10f, &t.sn[i], &t.cs[i]);      // 2^-31: half turns
   }
 }
-__device__ __forceinline__ void load16(float* x, const bf16* row, const Chunk& c) {
-  const uint4 a = *reinterpret_cast<const uint4*>(row + c.lo), b = *reinterpret_cast<const uint4*>(row + c.hi);
-  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+__device__ __forceinline__ void unpack16(float* x, const uint4* raw) {
+  const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float2 f = unpack_bf16(w[i]);
     x[2 * i] = f.x; x[2 * i + 1] = f.y;
   }
+}
+__device__ __forceinline__ void load16(float* x, const bf16* row, const Chunk& c) {
+  const uint4 raw[2] = {*reinterpret_cast<const uint4*>(row + c.lo), *reinterpret_cast<const uint4*>(row + c.hi)};
+  unpack16(x, raw);
 }
 __device__ __forceinline__ void rotate16(float* x, const Turn& t, int halves) {
 #pragma unroll
@@ -82,170 +85,261 @@ __device__ __forceinline__ void rotate16(float* x, const Turn& t, int halves) {
   }
 }
 
-constexpr int APPEND_THREADS = 256;
-
-// A team of threads per (page that the step touches, kv head, side).  What the step adds to a page is read once and held in registers (KEEP sweeps of the team over the
-// rows; further ones are read again), because the page's scale has to be known before its first code.  The queries' blocks come behind the pages'.
-//
-// The step's touched pages are numbered without a pass over the sequences: sequence s has the numbers from rows[s] / P + 2 s on, and n rows from any place in a page on
-// touch at most n / P + 2 pages.
-// Bounds: bytes for prompts, the launch and a chain of four dependent reads for a frame.
-template <int FMT, int D, int TEAM, int KEEP>
-__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendP p) {
-  pdl_trigger();
-  pdl_wait();
-  constexpr int CHUNKS = D / 16, RPS = TEAM / CHUNKS, TEAMS = APPEND_THREADS / TEAM;
-  const int tid = threadIdx.x, lane = tid & 31;
-  if ((int)blockIdx.x >= p.page_ctas) {                 // ---- queries: rotate, round, store ----
-    __shared__ int row_pos[APPEND_THREADS / CHUNKS];
-    const int slots = (APPEND_THREADS / CHUNKS) / p.q_rows;      // heads side by side
-    const int r_first = ((int)blockIdx.x - p.page_ctas) * p.q_rows;
-    for (int i = tid >> 5; i < p.q_rows; i += APPEND_THREADS / 32) {
-      const int r = r_first + i;
-      int pos = -1;
-      if (r < p.b.T) {
-        const int s = sequence_of_row(p.b, r);
-        if (s < p.b.S) {
-          const Seq q = sequence(p.b, s, p.P);
-          if (q.ok && r >= q.r0) pos = q.before + r - q.r0;
-        }
-      }
-      if (lane == 0) row_pos[i] = pos;
-    }
-    __syncthreads();
-    const int slot = tid / CHUNKS, j = tid % CHUNKS, i = slot / slots, r = r_first + i, pos = row_pos[i];
-    if (pos < 0) return;
-    const Chunk c(j, p.rot, p.halves);
-    Turn t;
-    if (c.turned) turn_of(t, p.turns, j, pos);
-    for (int h = slot % slots; h < p.Hq; h += slots) {
-      float x[16];
-      load16(x, p.q + r * p.q_ld + (long long)h * D, c);
-      if (c.turned) { if (p.halves) rotate16(x, t, 1); else rotate16(x, t, 0); }
-      bf16* out = p.q_out + r * p.q_out_ld + (long long)h * D;
-      *reinterpret_cast<uint4*>(out + c.lo) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
-      *reinterpret_cast<uint4*>(out + c.hi) = make_uint4(pack_bf16(x[8], x[9]), pack_bf16(x[10], x[11]), pack_bf16(x[12], x[13]), pack_bf16(x[14], x[15]));
-    }
-    return;
-  }
-
-  // ---- pages ----
-  const int task = (int)blockIdx.x * TEAMS + tid / TEAM, me = tid % TEAM;
-  if (task >= p.page_tasks) return;                     // whole teams
-  const int side = task & 1, h = (task >> 1) % p.H, item = (task >> 1) / p.H;
+// Which sequence and page the step's touched page number `item` is.  They are numbered without a pass over the sequences: sequence s has the numbers from rows[s] / P + 2 s on, and n rows
+// from any place in a page on touch at most n / P + 2 pages.  The whole warp asks together.
+struct Page { int seq, first, page, o, e, r; bool ok; };      // position of its first slot; slots o .. e - 1 are the step's, from batch row r on
+__device__ __forceinline__ Page page_of(const AppendP& p, int item, bool tell) {
+  const int lane = threadIdx.x & 31;
   int s = 0;                                            // the last sequence whose numbers begin at or in front of `item`
   for (int i = lane + 1; i - lane - 1 < p.b.S - 1; i += 32) s += __popc(__ballot_sync(0xffffffffu, i < p.b.S && (long long)p.b.rows[i] / p.P + 2ll * i <= item));
   const Seq q = sequence(p.b, s, p.P);
-  const int block = (q.ok ? q.before : 0) / p.P + item - (q.ok ? q.r0 / p.P + 2 * s : 0);
+  Page g;
+  g.ok = false; g.seq = s;
   if (!q.ok) {
-    if (me == 0) flag(p.flags, B200_PAGED_BAD_BATCH);
-    return;
+    if (tell) flag(p.flags, B200_PAGED_BAD_BATCH);
+    return g;
   }
-  const long long page_first = (long long)block * p.P;
-  if (q.n == 0 || page_first >= (long long)q.before + q.n) return;
-  const int page = p.b.table[s * p.b.table_ld + block];
-  if (page < 0 || page >= p.pages) {
-    if (me == 0) flag(p.flags, B200_PAGED_BAD_PAGE);
-    return;
+  const int block = q.before / p.P + item - (q.r0 / p.P + 2 * s);
+  const long long first = (long long)block * p.P;
+  if (q.n == 0 || first >= (long long)q.before + q.n) return g;
+  g.page = p.b.table[s * p.b.table_ld + block];
+  if (g.page < 0 || g.page >= p.pages) {
+    if (tell) flag(p.flags, B200_PAGED_BAD_PAGE);
+    return g;
   }
-  const int o = max(q.before - (int)page_first, 0), e = (int)min((long long)q.before + q.n - page_first, (long long)p.P);
-  const int r = q.r0 + (int)(page_first + o - q.before);            // batch row of slot o
-  const bool keys = side == 0;
-  const int rot = keys ? p.rot : 0;
+  g.first = (int)first;
+  g.o = max(q.before - g.first, 0);
+  g.e = (int)min((long long)q.before + q.n - first, (long long)p.P);
+  g.r = q.r0 + (g.first + g.o - q.before);
+  g.ok = true;
+  return g;
+}
+// A page's scale for new rows whose largest magnitude is `top`; doublings: how often the older rows' codes are halved, -1: they become 0.
+template <int FMT>
+__device__ __forceinline__ float scale_for(float top, int older, float s_old, int* doublings) {
+  const float need = top > 0.f ? fmaxf(top / code_max<FMT>(), SCALE_MIN) : 0.f;
+  *doublings = 0;
+  if (older == 0) return need;
+  if (!(s_old > 0.f)) { *doublings = -1; return need; }
+  if (!(need > s_old)) return s_old;
+  const float ratio = need / s_old;                     // the least power of two with s_old * 2^k >= need
+  int power;
+  const float part = frexpf(ratio, &power);
+  *doublings = part == 0.5f ? power - 1 : power;
+  return ldexpf(s_old, *doublings);
+}
+template <int FMT>
+__device__ __forceinline__ void store16(uint8_t* row, const Chunk& c, const float* x, float scale) {
+  // x / scale, rounded like a division: a product with the reciprocal, and what it left over once more.  (Scales lie between 2^-60 and 2^58 and |x| <= 2^64: nothing over- or underflows.)
+  const float div = scale > 0.f ? scale : 1.f, inv = 1.f / div;
+  float y[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float q = x[i] * inv;
+    y[i] = fmaf(fmaf(-q, div, x[i]), inv, q);
+  }
+  *reinterpret_cast<uint2*>(row + c.lo) = make_uint2(codes4<FMT>(y[0], y[1], y[2], y[3]), codes4<FMT>(y[4], y[5], y[6], y[7]));
+  *reinterpret_cast<uint2*>(row + c.hi) = make_uint2(codes4<FMT>(y[8], y[9], y[10], y[11]), codes4<FMT>(y[12], y[13], y[14], y[15]));
+}
+template <int FMT>
+__device__ __forceinline__ void halve16(uint8_t* at, int doublings) {
+  const float by = doublings >= 0 ? ldexpf(1.f, -doublings) : 0.f;
+  const uint4 was = *reinterpret_cast<const uint4*>(at);
+  const uint32_t w[4] = {was.x, was.y, was.z, was.w};
+  uint32_t now[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 a = float2_of<FMT, 0>(ready<FMT>(w[i])), b = float2_of<FMT, 1>(ready<FMT>(w[i]));
+    now[i] = doublings >= 0 ? codes4<FMT>(a.x * by, a.y * by, b.x * by, b.y * by) : 0u;
+  }
+  *reinterpret_cast<uint4*>(at) = make_uint4(now[0], now[1], now[2], now[3]);
+}
+// what is not finite, or larger than 2^64, becomes 0
+__device__ __forceinline__ bool only_finite(float* x) {
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (!(fabsf(x[i]) <= MAGNITUDE)) { x[i] = 0.f; odd = true; }
+  return odd;
+}
+__device__ __forceinline__ float largest16(const float* x) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[i]));
+  return top;
+}
+
+// Queries: rotate, round, store.  `slots` rows of a head side by side in the block; q_rows rows of the batch, whose angles serve all heads.
+template <int D>
+__device__ void append_queries(const AppendP& p, int block) {
+  constexpr int CHUNKS = D / 16;
+  __shared__ int row_pos[8];
+  const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x >> 5;
+  const int slots = blockDim.x / CHUNKS / p.q_rows, r_first = block * p.q_rows;
+  for (int i = tid >> 5; i < p.q_rows; i += warps) {
+    const int r = r_first + i;
+    int pos = -1;
+    if (r < p.b.T) {
+      const int s = sequence_of_row(p.b, r);
+      if (s < p.b.S) {
+        const Seq q = sequence(p.b, s, p.P);
+        if (q.ok && r >= q.r0) pos = q.before + r - q.r0;
+      }
+    }
+    if (lane == 0) row_pos[i] = pos;
+  }
+  __syncthreads();
+  const int slot = tid / CHUNKS, j = tid % CHUNKS, i = slot / slots, r = r_first + i, pos = row_pos[i];
+  if (pos < 0) return;
+  const Chunk c(j, p.rot, p.halves);
+  Turn t;
+  if (c.turned) turn_of(t, p.turns, j, pos);
+  constexpr int ROUND = 4;                   // heads asked for together: results may lie over the queries, so the compiler keeps loads behind stores
+  for (int h0 = slot % slots; h0 < p.Hq; h0 += ROUND * slots) {
+    uint4 raw[ROUND][2];
+#pragma unroll
+    for (int k = 0; k < ROUND; ++k) {
+      const bf16* row = p.q + r * p.q_ld + (long long)(h0 + k * slots) * D;
+      if (h0 + k * slots < p.Hq) { raw[k][0] = *reinterpret_cast<const uint4*>(row + c.lo); raw[k][1] = *reinterpret_cast<const uint4*>(row + c.hi); }
+    }
+#pragma unroll
+    for (int k = 0; k < ROUND; ++k) {
+      if (h0 + k * slots >= p.Hq) break;
+      float x[16];
+      unpack16(x, raw[k]);
+      if (c.turned) { if (p.halves) rotate16(x, t, 1); else rotate16(x, t, 0); }
+      bf16* out = p.q_out + r * p.q_out_ld + (long long)(h0 + k * slots) * D;
+      *reinterpret_cast<uint4*>(out + c.lo) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+      *reinterpret_cast<uint4*>(out + c.hi) = make_uint4(pack_bf16(x[8], x[9]), pack_bf16(x[10], x[11]), pack_bf16(x[12], x[13]), pack_bf16(x[14], x[15]));
+    }
+  }
+}
+
+// Few rows a sequence: a warp per (page that the step touches, kv head, side); rows past the first sweep of the warp are read twice, for the scale and for the codes.
+// Bounds: the launch and a chain of four dependent reads (rows, table, scale, codes).
+constexpr int APPEND_THREADS = 256;
+template <int FMT, int D>
+__global__ void __launch_bounds__(APPEND_THREADS) append_few_kernel(const AppendP p) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int CHUNKS = D / 16, RPS = 32 / CHUNKS;
+  if ((int)blockIdx.x >= p.page_ctas) { append_queries<D>(p, (int)blockIdx.x - p.page_ctas); return; }
+  const int lane = threadIdx.x & 31, task = (int)blockIdx.x * (APPEND_THREADS / 32) + (threadIdx.x >> 5);
+  if (task >= p.items * p.H * 2) return;
+  const bool keys = !(task & 1);
+  const int h = (task >> 1) % p.H;
+  const Page g = page_of(p, (task >> 1) / p.H, lane == 0);
+  if (!g.ok) return;
   const bf16* src = (keys ? p.k : p.v) + (long long)h * D;
   const long long ld = keys ? p.k_ld : p.v_ld;
-  uint8_t* codes = (keys ? p.k_codes : p.v_codes) + ((long long)page * p.H + h) * p.P * D;
-  float* scale_at = (keys ? p.k_scale : p.v_scale) + (long long)page * p.H + h;
-  const float s_old = o > 0 ? *scale_at : 0.f;
-  const int j = me % CHUNKS, row0 = me / CHUNKS;
-  const Chunk c(j, rot, p.halves);
-  float top = 0.f;
-  bool odd = false;                                     // a value that is not finite, or too large
+  uint8_t* codes = (keys ? p.k_codes : p.v_codes) + ((long long)g.page * p.H + h) * p.P * D;
+  float* scale_at = (keys ? p.k_scale : p.v_scale) + (long long)g.page * p.H + h;
+  const float s_old = g.o > 0 ? *scale_at : 0.f;
+  const int j = lane % CHUNKS, row0 = lane / CHUNKS;
+  const Chunk c(j, keys ? p.rot : 0, p.halves);
+  bool odd = false;
   auto fetch = [&](float* x, int slot) {
-    load16(x, src + (r + slot - o) * ld, c);
+    load16(x, src + (g.r + slot - g.o) * ld, c);
     if (c.turned) {
       Turn t;
-      turn_of(t, p.turns, j, (int)page_first + slot);
+      turn_of(t, p.turns, j, g.first + slot);
       if (p.halves) rotate16(x, t, 1); else rotate16(x, t, 0);
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (!(fabsf(x[i]) <= MAGNITUDE)) { x[i] = 0.f; odd = true; }
+    odd |= only_finite(x);
   };
-  float kept[KEEP][16];
-#pragma unroll
-  for (int k = 0; k < KEEP; ++k) {
-    const int slot = o + row0 + k * RPS;
-    if (slot < e) fetch(kept[k], slot);
-    else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) kept[k][i] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(kept[k][i]));
-  }
-  for (int slot = o + row0 + KEEP * RPS; slot < e; slot += RPS) {
+  float kept[16], top = 0.f;
+  if (g.o + row0 < g.e) { fetch(kept, g.o + row0); top = largest16(kept); }
+  for (int slot = g.o + row0 + RPS; slot < g.e; slot += RPS) {
     float x[16];
     fetch(x, slot);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[i]));
+    top = fmaxf(top, largest16(x));
   }
   top = warp_max(top);
-  if constexpr (TEAM > 32) {
-    __shared__ float tops[TEAM / 32];
-    if (lane == 0) tops[tid >> 5] = top;
-    __syncthreads();                                    // one team: all threads of the block are here
-#pragma unroll
-    for (int i = 0; i < TEAM / 32; ++i) top = fmaxf(top, tops[i]);
-  }
   if (__any_sync(0xffffffffu, odd) && lane == 0) flag(p.flags, B200_PAGED_NOT_FINITE);
-  const float need = top > 0.f ? fmaxf(top / code_max<FMT>(), SCALE_MIN) : 0.f;
-  float sc = need;
-  int doublings = 0;
-  if (s_old > 0.f) {
-    sc = s_old;
-    if (need > s_old) {                                 // the least power of two with s_old * 2^k >= need
-      const float ratio = need / s_old;
-      int power;
-      const float part = frexpf(ratio, &power);
-      doublings = part == 0.5f ? power - 1 : power;
-      sc = ldexpf(s_old, doublings);
-    }
-  }
+  int doublings;
+  const float sc = scale_for<FMT>(top, g.o, s_old, &doublings);
   __syncwarp();
-  if (me == 0) *scale_at = sc;
-  const float div = sc > 0.f ? sc : 1.f;
-  auto store = [&](const float* x, int slot) {
-    uint8_t* row = codes + (long long)slot * D;
-    float y[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) y[i] = x[i] / div;
-    *reinterpret_cast<uint2*>(row + c.lo) = make_uint2(codes4<FMT>(y[0], y[1], y[2], y[3]), codes4<FMT>(y[4], y[5], y[6], y[7]));
-    *reinterpret_cast<uint2*>(row + c.hi) = make_uint2(codes4<FMT>(y[8], y[9], y[10], y[11]), codes4<FMT>(y[12], y[13], y[14], y[15]));
-  };
-#pragma unroll
-  for (int k = 0; k < KEEP; ++k)
-    if (o + row0 + k * RPS < e) store(kept[k], o + row0 + k * RPS);
-  for (int slot = o + row0 + KEEP * RPS; slot < e; slot += RPS) {
+  if (lane == 0) *scale_at = sc;
+  if (g.o + row0 < g.e) store16<FMT>(codes + (long long)(g.o + row0) * D, c, kept, sc);
+  for (int slot = g.o + row0 + RPS; slot < g.e; slot += RPS) {
     float x[16];
     fetch(x, slot);
-    store(x, slot);
+    store16<FMT>(codes + (long long)slot * D, c, x, sc);
   }
-  if (o > 0 && (doublings > 0 || !(s_old > 0.f))) {     // the older rows' codes in the new scale
-    const float by = s_old > 0.f ? ldexpf(1.f, -doublings) : 0.f;
-    for (int slot = row0; slot < o; slot += RPS) {
-      uint4* at = reinterpret_cast<uint4*>(codes + (long long)slot * D + 16 * j);
-      const uint4 was = *at;
-      const uint32_t w[4] = {was.x, was.y, was.z, was.w};
-      uint32_t now[4];
+  if (doublings != 0)
+    for (int slot = row0; slot < g.o; slot += RPS) halve16<FMT>(codes + (long long)slot * D + 16 * j, doublings);
+}
+
+// Many rows: a block of P * D / 32 threads, two chunks each, has a page and goes through some of its heads, keys and values; the next head's rows are on their way while one is worked on, and
+// the angles of the page's positions serve all heads.  Everything is read once, as the scale has to be known before the first code.
+// Bounds: bytes, once the chain of reads in front is shared by several heads.
+template <int FMT, int D>
+__global__ void __launch_bounds__(512) append_many_kernel(const AppendP p) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int CHUNKS = D / 16;
+  if ((int)blockIdx.x >= p.page_ctas) { append_queries<D>(p, (int)blockIdx.x - p.page_ctas); return; }
+  __shared__ float tops[2][16];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  const int groups = (p.H + p.heads_per_block - 1) / p.heads_per_block, item = (int)blockIdx.x / groups, h0 = ((int)blockIdx.x - item * groups) * p.heads_per_block;
+  const Page g = page_of(p, item, tid == 0);
+  if (!g.ok) return;                                    // the whole block
+  const int j = tid % CHUNKS, row0 = tid / CHUNKS, half = p.P / 2, works = 2 * (min(h0 + p.heads_per_block, p.H) - h0);
+  const int slot[2] = {row0, row0 + half};
+  const bool mine[2] = {slot[0] >= g.o && slot[0] < g.e, slot[1] >= g.o && slot[1] < g.e};
+  const Chunk ck(j, p.rot, p.halves), cv(j, 0, 0);
+  Turn t[2];
+  if (ck.turned) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 a = float2_of<FMT, 0>(ready<FMT>(w[i])), b = float2_of<FMT, 1>(ready<FMT>(w[i]));
-        now[i] = s_old > 0.f ? codes4<FMT>(a.x * by, a.y * by, b.x * by, b.y * by) : 0u;
-      }
-      *at = make_uint4(now[0], now[1], now[2], now[3]);
+    for (int k = 0; k < 2; ++k) turn_of(t[k], p.turns, j, g.first + slot[k]);
+  }
+  uint4 raw[2][2];
+  float s_next;
+  auto ask = [&](int w) {
+    if (w >= works) return;
+    const int h = h0 + (w >> 1);
+    const bool keys = !(w & 1);
+    const bf16* src = (keys ? p.k : p.v) + (long long)h * D;
+    const long long ld = keys ? p.k_ld : p.v_ld;
+    const int lo = keys ? ck.lo : cv.lo, hi = keys ? ck.hi : cv.hi;
+    s_next = g.o > 0 ? (keys ? p.k_scale : p.v_scale)[(long long)g.page * p.H + h] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const bf16* row = src + (g.r + slot[k] - g.o) * ld;
+      raw[k][0] = mine[k] ? *reinterpret_cast<const uint4*>(row + lo) : make_uint4(0, 0, 0, 0);
+      raw[k][1] = mine[k] ? *reinterpret_cast<const uint4*>(row + hi) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  ask(0);
+  bool odd = false;
+  for (int w = 0; w < works; ++w) {
+    const int h = h0 + (w >> 1);
+    const bool keys = !(w & 1);
+    float x[2][16], top = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      unpack16(x[k], raw[k]);
+      if (keys && ck.turned) { if (p.halves) rotate16(x[k], t[k], 1); else rotate16(x[k], t[k], 0); }
+      odd |= only_finite(x[k]);
+      top = fmaxf(top, largest16(x[k]));
+    }
+    const float s_old = s_next;
+    ask(w + 1);
+    top = warp_max(top);
+    if (lane == 0) tops[w & 1][warp] = top;             // two places: the next round's maxima may come before the last thread has read these
+    __syncthreads();
+    for (int i = 0; i < warps; ++i) top = fmaxf(top, tops[w & 1][i]);
+    int doublings;
+    const float sc = scale_for<FMT>(top, g.o, s_old, &doublings);
+    uint8_t* codes = (keys ? p.k_codes : p.v_codes) + ((long long)g.page * p.H + h) * p.P * D;
+    if (tid == 0) (keys ? p.k_scale : p.v_scale)[(long long)g.page * p.H + h] = sc;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (mine[k]) { if (keys) store16<FMT>(codes + slot[k] * D, ck, x[k], sc); else store16<FMT>(codes + slot[k] * D, cv, x[k], sc); }
+      if (doublings != 0 && slot[k] < g.o) halve16<FMT>(codes + slot[k] * D + 16 * j, doublings);
     }
   }
+  if (__any_sync(0xffffffffu, odd) && lane == 0) flag(p.flags, B200_PAGED_NOT_FINITE);
 }
 
 // =========================================================================================================================
@@ -1064,15 +1158,23 @@ int launch_few_nt(const AttnP& p, const FewPlan& f, cudaStream_t st) {
   return launch_few<D, FMT, 4>(p, f, st);
 }
 
+constexpr int WAVE = 148 * 3 / 2;
 template <int FMT, int D>
-int launch_append(AppendP& p, int max_rows, int q_ctas_rows, cudaStream_t st) {
-  // few rows to a page: a warp each; else a block, which holds whole pages in registers
-  const bool few = max_rows <= 4;
-  const long long ctas = ceil_div64(p.page_tasks, few ? APPEND_THREADS / 32 : 1);
-  p.page_ctas = (int)ctas;
-  const dim3 grid((unsigned)(ctas + q_ctas_rows));
-  if (few) return launch_early(append_kernel<FMT, D, 32, 1>, grid, dim3(APPEND_THREADS), 0, st, p);
-  return launch_early(append_kernel<FMT, D, 256, D / 32>, grid, dim3(APPEND_THREADS), 0, st, p);
+int launch_append(AppendP& p, cudaStream_t st) {
+  // A page gets at most four rows of a sequence: a warp each, and all of its heads side by side (48 rows of 32 heads: 6.9 us as blocks of whole pages, 5.x as warps).
+  const bool few = p.b.max_rows <= 4;
+  const int threads = few ? APPEND_THREADS : p.P * D / 32;
+  // as many heads to a block as leave the chip a wave of blocks, two to an SM
+  p.heads_per_block = 1;
+  while (!few && p.heads_per_block < p.H && (long long)p.items * ceil_div(p.H, 2 * p.heads_per_block) >= WAVE) p.heads_per_block *= 2;
+  p.page_ctas = few ? (int)ceil_div64((long long)p.items * p.H * 2, APPEND_THREADS / 32) : p.items * ceil_div(p.H, p.heads_per_block);
+  // a block's queries: one row where there are few, else up to eight rows, whose angles then serve more heads
+  const int slots = threads / (D / 16);
+  p.q_rows = 1;
+  while (p.q_rows < 8 && 2 * p.q_rows <= slots && (long long)p.b.T * p.Hq >= 148ll * 8 * slots * p.q_rows) p.q_rows *= 2;
+  const dim3 grid((unsigned)(p.page_ctas + (p.Hq ? ceil_div(p.b.T, p.q_rows) : 0)));
+  if (few) return launch_early(append_few_kernel<FMT, D>, grid, dim3(threads), 0, st, p);
+  return launch_early(append_many_kernel<FMT, D>, grid, dim3(threads), 0, st, p);
 }
 
 }  // namespace
@@ -1104,18 +1206,14 @@ int b200_paged_append(const b200_paged_cache* cache, const b200_paged_batch* bat
   p.q_out = static_cast<__nv_bfloat16*>(q_out_dev); p.k_ld = k_ld; p.v_ld = v_ld; p.q_ld = q_ld; p.q_out_ld = q_out_ld;
   p.turns = rotary ? rotary->turns_dev : nullptr; p.rot = rotary ? rotary->rot_dims : 0; p.halves = rotary ? rotary->pairing == B200_ROT_HALVES : 0;
   p.pages = cache->pages; p.P = cache->page_tokens; p.H = cache->kv_heads; p.Hq = q_dev ? q_heads : 0;
-  const long long tasks = ((long long)batch->total_rows / p.P + 2ll * batch->sequences) * p.H * 2;
-  if (tasks > (1ll << 30)) B200_FAIL(B200_ERR_SHAPE, "paged_append: %d rows of %d sequences with %d heads in one call", batch->total_rows, batch->sequences, p.H);
-  p.page_tasks = (int)tasks;
-  // a block's queries: one row where there are few (all heads at once), else eight rows, whose angles then serve several heads
-  const int slots = APPEND_THREADS / (D / 16);
-  p.q_rows = (long long)batch->total_rows * q_heads >= 148ll * 8 * slots ? 8 : 1;
-  const int q_ctas = q_dev ? ceil_div(batch->total_rows, p.q_rows) : 0;
+  const long long items = (long long)batch->total_rows / p.P + 2ll * batch->sequences;
+  if (items * p.H * 2 > (1ll << 30)) B200_FAIL(B200_ERR_SHAPE, "paged_append: %d rows of %d sequences with %d heads in one call", batch->total_rows, batch->sequences, p.H);
+  p.items = (int)items;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool i8 = cache->kv_dtype == B200_KV_INT8;
   int rc;
-  if (D == 128) rc = i8 ? launch_append<INT8, 128>(p, batch->max_rows, q_ctas, st) : launch_append<E4M3, 128>(p, batch->max_rows, q_ctas, st);
-  else rc = i8 ? launch_append<INT8, 64>(p, batch->max_rows, q_ctas, st) : launch_append<E4M3, 64>(p, batch->max_rows, q_ctas, st);
+  if (D == 128) rc = i8 ? launch_append<INT8, 128>(p, st) : launch_append<E4M3, 128>(p, st);
+  else rc = i8 ? launch_append<INT8, 64>(p, st) : launch_append<E4M3, 64>(p, st);
   B200_TRY(rc);
   return check_launch("paged_append");
 }

@@ -73,8 +73,9 @@ __device__ constexpr float code_max() { return FMT == INT8 ? 127.f : 448.f; }
 template <int FMT>
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
   if constexpr (FMT == INT8) {
-    auto one = [](float x) { return (uint32_t)(int)fminf(fmaxf(rintf(x), -127.f), 127.f) & 0xffu; };
-    return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+    // to the nearest whole number, ties to the even one: the sum with 1.5 * 2^23 has it in its last bits
+    auto one = [](float x) { return __float_as_uint(fminf(fmaxf(x, -127.f), 127.f) + 12582912.f); };
+    return prmt(prmt(one(a), one(b), 0x0040u), prmt(one(c), one(d), 0x0040u), 0x5410u);
   } else {
     return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) | (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3) << 16;
   }

@@ -34,6 +34,10 @@ def _cuda(device: torch.device | str) -> torch.device:
     return torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
 
 
+def _stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
 def _entry(name: str):
     fn = getattr(_lib.lib(), name, None)
     if fn is None:
@@ -82,6 +86,7 @@ class PagedBatch:
             raise ValueError(f"total_rows {total_rows}, max_rows {max_rows}")
         self.table, self.before, self.rows, self.total_rows, self.max_rows = table, before, rows, total_rows, min(max_rows, total_rows)
         self.device, self.sequences = table.device, S
+        self._index, self._work = table.device.index, {}
         self._c = _lib.PagedBatchC(table.data_ptr(), before.data_ptr(), rows.data_ptr(), max(table.stride(0), table.shape[1]), S, table.shape[1], total_rows, self.max_rows)
         self._ref = C.addressof(self._c)
 
@@ -119,23 +124,30 @@ class PagedKVCache:
         self.k, self.v, self.k_scale, self.v_scale, self.device = k, v, k_scale, v_scale, k.device
         self.pages, self.kv_heads, self.page_tokens, self.head_dim = k.shape
         self.dtype = _NAMES[k.dtype]
+        self._index, self._shape = self.device.index, (self.page_tokens, self.kv_heads, self.head_dim)
         self.flags = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._c = _lib.PagedCacheC(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.flags.data_ptr(), self.pages, self.page_tokens, self.kv_heads, self.head_dim, _KV[self.dtype][1], self.device.index)
         self._ref = C.addressof(self._c)
         self._append, self._attend, self._bytes, self._read = (_entry(f"b200_paged_{n}") for n in ("append", "attention", "attention_bytes", "read"))
 
-    def _rows(self, name: str, t: torch.Tensor, batch: PagedBatch, heads: int | None) -> int:
+    def _rows(self, name: str, t: torch.Tensor, batch: PagedBatch, heads: int) -> int:
         """Checks a step's tensor [total_rows, heads, head_dim]; its elements from row to row."""
-        if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[0] != batch.total_rows or t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
-            raise ValueError(f"{name}: bf16 [{batch.total_rows}, {'heads' if heads is None else heads}, {self.head_dim}]; got {t.dtype} {tuple(t.shape)}")
-        if t.device != self.device or batch.device != self.device:
+        T, D = batch.total_rows, self.head_dim
+        if t.dtype is not torch.bfloat16 or t.shape != (T, heads, D):
+            raise ValueError(f"{name}: bf16 {[T, heads, D]}; got {t.dtype} {list(t.shape)}")
+        if t.get_device() != self._index or batch._index != self._index:
             raise ValueError(f"{name} on {t.device}, the batch on {batch.device}, the cache on {self.device}")
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} asks for a gradient: the paged cache has none")
         ld, head, one = t.stride()
-        if (one != 1 and t.shape[2] > 1) or (head != self.head_dim and t.shape[1] > 1):
+        if one != 1 or (head != D and heads > 1):
             raise ValueError(f"{name}: a row's heads have to lie side by side; strides {t.stride()}")
-        return ld if t.shape[0] > 1 else t.shape[1] * self.head_dim
+        return ld if T > 1 else heads * D
+
+    def _heads(self, name: str, t: torch.Tensor) -> int:
+        if t.dim() != 3:
+            raise ValueError(f"{name}: [total_rows, heads, head_dim]; got {list(t.shape)}")
+        return t.shape[1]
 
     def append(self, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None, rotary: RotaryTable | None = None,
                q_out: torch.Tensor | None = None) -> torch.Tensor | None:
@@ -146,15 +158,17 @@ class PagedKVCache:
             raise ValueError(f"{rotary.rot_dims} rotated dimensions on {rotary.device} for heads of {self.head_dim} on {self.device}")
         q_ptr = q_ld = o_ptr = o_ld = heads = 0
         if q is not None:
-            q_ld, heads = self._rows("q", q, batch, None), q.shape[1]
+            heads = self._heads("q", q)
+            q_ld = self._rows("q", q, batch, heads)
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
-            o_ld = self._rows("q_out", q_out, batch, heads)
+                q_out, o_ld = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device), heads * self.head_dim
+            else:
+                o_ld = self._rows("q_out", q_out, batch, heads)
             q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")
         rc = self._append(self._ref, batch._ref, k.data_ptr(), k_ld, v.data_ptr(), v_ld, q_ptr, q_ld, o_ptr, o_ld, heads, rotary._ref if rotary is not None else None,
-                          torch.cuda.current_stream(self.device).cuda_stream)
+                          _stream(self._index))
         if rc:
             _lib.check(rc)
         return q_out
@@ -163,26 +177,31 @@ class PagedKVCache:
         """Attention of the step's rows over what their sequences have cached, the step's own rows included (``append`` comes first): the row at position p sees tokens j <= p
         and, with a ``window``, of these only p - j < window and the first ``sinks`` tokens.  q bf16 [total_rows, q_heads, head_dim], q_heads a multiple of kv_heads; scores are
         multiplied by ``scale`` (default head_dim ** -0.5).  Rows that belong to no sequence are left as they are in ``out``."""
-        q_ld, heads = self._rows("q", q, batch, None), q.shape[1]
+        heads = self._heads("q", q)
+        q_ld = self._rows("q", q, batch, heads)
         if out is None:
-            out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
-        o_ld = self._rows("out", out, batch, heads)
+            out, o_ld = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device), heads * self.head_dim
+        else:
+            o_ld = self._rows("out", out, batch, heads)
         if not 0 <= window < 1 << 31 or not 0 <= sinks < 1 << 31:
             raise ValueError(f"window {window}, {sinks} first tokens")
-        n = self._bytes(self._ref, batch._ref, heads, window, sinks)
+        of = (self._shape, heads, window, sinks)
+        n = batch._work.get(of)                       # a size, by sizes alone; the layers of a step ask for the same
+        if n is None:
+            n = batch._work[of] = self._bytes(self._ref, batch._ref, heads, window, sinks)
         work = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
         rc = self._attend(self._ref, batch._ref, q.data_ptr(), q_ld, out.data_ptr(), o_ld, heads, self.head_dim ** -0.5 if scale is None else scale, window, sinks,
-                          work.data_ptr() if n else None, n, torch.cuda.current_stream(self.device).cuda_stream)
+                          work.data_ptr() if n else None, n, _stream(self._index))
         if rc:
             _lib.check(rc)
         return out
 
     def read(self, batch: PagedBatch) -> tuple[torch.Tensor, torch.Tensor]:
         """What the cache holds at the batch's positions ``before[s] + i``: keys and values bf16 [total_rows, kv_heads, head_dim]."""
-        if batch.device != self.device:
+        if batch._index != self._index:
             raise ValueError(f"the batch on {batch.device}, the cache on {self.device}")
         k, v = (torch.empty(batch.total_rows, self.kv_heads, self.head_dim, dtype=torch.bfloat16, device=self.device) for _ in range(2))
-        rc = self._read(self._ref, batch._ref, k.data_ptr(), v.data_ptr(), torch.cuda.current_stream(self.device).cuda_stream)
+        rc = self._read(self._ref, batch._ref, k.data_ptr(), v.data_ptr(), _stream(self._index))
         if rc:
             _lib.check(rc)
         return k, v
