@@ -353,52 +353,57 @@ struct ReadP {
   bf16 *k, *v;                               // [T][H][D]
   int pages, P, H;
 };
-constexpr int READ_THREADS = 256, READ_ROWS = 4;
+constexpr int READ_THREADS = 256;
 
+// A warp per row and side; four 16-byte pieces of codes in flight a lane.  Bounds: bytes, and for few rows the same chain of reads as append's.
 template <int FMT, int D>
 __global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadP p) {
   pdl_trigger();
   pdl_wait();
-  __shared__ int at[READ_ROWS][2];           // page and slot of the rows
-  const int warp = threadIdx.x >> 5, r_first = (int)blockIdx.x * READ_ROWS;
-  if (warp < READ_ROWS) {
-    const int r = r_first + warp;
-    int page = -1, slot = 0;
-    if (r < p.b.T) {
-      const int s = sequence_of_row(p.b, r);
-      if (s < p.b.S) {
-        const Seq q = sequence(p.b, s, p.P);
-        if (q.ok && r >= q.r0) {
-          const int pos = q.before + r - q.r0;
-          page = p.b.table[s * p.b.table_ld + pos / p.P];
-          slot = pos % p.P;
-          if (page < 0 || page >= p.pages) { page = -1; if ((threadIdx.x & 31) == 0) flag(p.flags, B200_PAGED_BAD_PAGE); }
-        } else if (!q.ok && (threadIdx.x & 31) == 0) flag(p.flags, B200_PAGED_BAD_BATCH);
+  const int lane = threadIdx.x & 31, task = (int)blockIdx.x * (READ_THREADS / 32) + (threadIdx.x >> 5), r = task >> 1, side = task & 1;
+  if (r >= p.b.T) return;
+  const int s = sequence_of_row(p.b, r);
+  if (s >= p.b.S) return;
+  const Seq q = sequence(p.b, s, p.P);
+  if (!q.ok || r < q.r0) {
+    if (!q.ok && lane == 0) flag(p.flags, B200_PAGED_BAD_BATCH);
+    return;
+  }
+  const int pos = q.before + r - q.r0, page = p.b.table[s * p.b.table_ld + pos / p.P], slot = pos % p.P;
+  if (page < 0 || page >= p.pages) {
+    if (lane == 0) flag(p.flags, B200_PAGED_BAD_PAGE);
+    return;
+  }
+  constexpr int CHUNKS = D / 16, ROUND = 4;
+  const int n = p.H * CHUNKS;
+  const uint8_t* codes = (side ? p.v_codes : p.k_codes) + ((long long)page * p.H * p.P + slot) * D;
+  const float* scales = (side ? p.v_scale : p.k_scale) + (long long)page * p.H;
+  bf16* out = (side ? p.v : p.k) + (long long)r * p.H * D;
+  for (int x0 = lane; x0 < n; x0 += 32 * ROUND) {
+    uint4 c[ROUND];
+    float sc[ROUND];
+#pragma unroll
+    for (int k = 0; k < ROUND; ++k) {
+      const int x = x0 + 32 * k;
+      if (x < n) {
+        c[k] = *reinterpret_cast<const uint4*>(codes + (long long)(x / CHUNKS) * p.P * D + 16 * (x % CHUNKS));
+        sc[k] = scales[x / CHUNKS];
       }
     }
-    if ((threadIdx.x & 31) == 0) { at[warp][0] = page; at[warp][1] = slot; }
-  }
-  __syncthreads();
-  constexpr int CHUNKS = D / 16;
-  const int per_row = p.H * CHUNKS * 2;
-  for (int i = threadIdx.x; i < per_row * READ_ROWS; i += READ_THREADS) {
-    const int row = i / per_row, x = i - row * per_row, side = x >= per_row / 2, y = x - side * (per_row / 2), h = y / CHUNKS, j = y % CHUNKS;
-    const int page = at[row][0];
-    if (page < 0) continue;
-    const long long ph = (long long)page * p.H + h;
-    const float sc = (side ? p.v_scale : p.k_scale)[ph];
-    const uint4 c = *reinterpret_cast<const uint4*>((side ? p.v_codes : p.k_codes) + (ph * p.P + at[row][1]) * D + 16 * j);
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    uint32_t o[8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 a = float2_of<FMT, 0>(ready<FMT>(w[k])), b = float2_of<FMT, 1>(ready<FMT>(w[k]));
-      o[2 * k] = pack_bf16(a.x * sc, a.y * sc);
-      o[2 * k + 1] = pack_bf16(b.x * sc, b.y * sc);
+    for (int k = 0; k < ROUND; ++k) {
+      if (x0 + 32 * k >= n) break;
+      const uint32_t w[4] = {c[k].x, c[k].y, c[k].z, c[k].w};
+      uint32_t o[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 a = float2_of<FMT, 0>(ready<FMT>(w[i])), b = float2_of<FMT, 1>(ready<FMT>(w[i]));
+        o[2 * i] = pack_bf16(a.x * sc[k], a.y * sc[k]);
+        o[2 * i + 1] = pack_bf16(b.x * sc[k], b.y * sc[k]);
+      }
+      *reinterpret_cast<uint4*>(out + 16 * (x0 + 32 * k)) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4*>(out + 16 * (x0 + 32 * k) + 8) = make_uint4(o[4], o[5], o[6], o[7]);
     }
-    bf16* out = (side ? p.v : p.k) + ((long long)(r_first + row) * p.H + h) * D + 16 * j;
-    *reinterpret_cast<uint4*>(out) = make_uint4(o[0], o[1], o[2], o[3]);
-    *reinterpret_cast<uint4*>(out + 8) = make_uint4(o[4], o[5], o[6], o[7]);
   }
 }
 
@@ -1231,7 +1236,7 @@ int b200_paged_read(const b200_paged_cache* cache, const b200_paged_batch* batch
   p.k_codes = static_cast<const uint8_t*>(cache->k_dev); p.v_codes = static_cast<const uint8_t*>(cache->v_dev); p.k_scale = cache->k_scale_dev; p.v_scale = cache->v_scale_dev;
   p.flags = cache->flags_dev; p.b = batch_of(batch); p.k = static_cast<__nv_bfloat16*>(k_out_dev); p.v = static_cast<__nv_bfloat16*>(v_out_dev);
   p.pages = cache->pages; p.P = cache->page_tokens; p.H = cache->kv_heads;
-  const dim3 grid((unsigned)ceil_div(batch->total_rows, READ_ROWS));
+  const dim3 grid((unsigned)ceil_div(batch->total_rows, READ_THREADS / 64));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool i8 = cache->kv_dtype == B200_KV_INT8;
   if (D == 128) { if (i8) EARLY_LAUNCH((read_kernel<INT8, 128>), grid, READ_THREADS, 0, st, p); else EARLY_LAUNCH((read_kernel<E4M3, 128>), grid, READ_THREADS, 0, st, p); }
