@@ -533,7 +533,8 @@ constexpr bool few_digits(int fmt, int nt) { return fmt == INT8 && nt == 1; }
 constexpr int SEEN = 1, IN_PART = 0, HIDDEN = -1;      // a half of a tile: by all columns, by some, by none
 // four integers of up to 2^22 = 65536 x2 + 256 x1 + x0 with digits of -128 .. 127
 __device__ __forceinline__ void digits(float a, float b, float c, float d, uint32_t& d0, uint32_t& d1, uint32_t& d2) {
-  const int n[4] = {__float2int_rn(a), __float2int_rn(b), __float2int_rn(c), __float2int_rn(d)};
+  auto whole = [](float x) { return __float_as_int(x + 12582912.f) - 0x4b400000; };        // the last bits of a sum with 1.5 * 2^23
+  const int n[4] = {whole(a), whole(b), whole(c), whole(d)};
   d0 = d1 = d2 = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -604,7 +605,9 @@ __global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(c
       units_at = units_of(p, q_at);
       n_at = units_at ? tiles_of(p, q_at) + UNIT_COST : 1;
     }
-    const int unit = (int)((f - base) / n_at), u0 = (int)((f - base) - (long long)unit * n_at), u1 = (int)min((long long)n_at, u0 + (run.to - f));
+    const long long at = f - base;
+    const int unit = at < 0x7fffffffll ? (int)((uint32_t)at / (uint32_t)n_at) : (int)(at / n_at);
+    const int u0 = (int)(at - (long long)unit * n_at), u1 = (int)min((long long)n_at, u0 + (run.to - f));
     f += u1 - u0;
     const int h = unit % p.H, ct = unit / p.H, n_cols = q_at.n * p.G;
     const int pf = q_at.before + ct * COLS / p.G, pl = q_at.before + (min(ct * COLS + COLS, n_cols) - 1) / p.G;
@@ -627,10 +630,8 @@ __global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(c
     }
     __syncwarp();
   };
-  // The part's i-th tile on its way into the ring; every 16 tiles the lanes look up the pages of their halves, and their scales behind the copies' start.
-  auto issue_keys = [&](const Part& w, int i) {
-    if (i >= w.count) return;
-    if (i & 15) { fetch(w, i, map_k, 0); return; }
+  // Every 16 tiles the lanes look up the pages of their halves; what the scores need of them comes behind the copies' start.
+  auto look_up = [&](const Part& w, int i) {
     const int mine = i + (lane >> 1), j = mine < w.count ? (w.tiles[w.first + mine * FEW_WARPS] << 5) + 16 * (lane & 1) : 0;
     int page = -1;
     if (mine < w.count && j <= w.pl && (p.window <= 0 || w.pf - j - 15 < p.window || j < p.sinks)) {
@@ -639,7 +640,10 @@ __global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(c
     }
     rows_at[warp][(2 * i + lane) & 63] = page < 0 ? -1 : (page * p.H + w.h) * p.P + (j & (p.P - 1));
     __syncwarp();
-    fetch(w, i, map_k, 0);
+    return page;
+  };
+  auto tell = [&](const Part& w, int i, int page) {
+    const int mine = i + (lane >> 1), j = mine < w.count ? (w.tiles[w.first + mine * FEW_WARPS] << 5) + 16 * (lane & 1) : 0;
     float4 x = make_float4(__int_as_float(HIDDEN), 0.f, -INFINITY, 0.f);
     if (page >= 0) {
       const bool all = j + 15 <= w.pf && (p.window <= 0 || w.pl - j < p.window || j + 16 <= p.sinks);
@@ -652,22 +656,17 @@ __global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(c
     meta[warp][(2 * i + lane) & 63] = x;
     __syncwarp();
   };
+  // the part's i-th tile on its way into the ring
+  auto issue_keys = [&](const Part& w, int i) {
+    if (i >= w.count) return;
+    if (i & 15) { fetch(w, i, map_k, 0); return; }
+    const int page = look_up(w, i);
+    fetch(w, i, map_k, 0);
+    tell(w, i, page);
+  };
   auto issue_values = [&](const Part& w, int i) {
     if (i < w.count) fetch(w, i, map_v, 2);
   };
-  // a part's first copies, which go out before the part in front of it is joined
-  auto start = [&](const Part& w) {
-    __syncwarp();
-    issue_keys(w, 0);
-    issue_values(w, 0);
-    issue_keys(w, 1);
-  };
-  auto arrived = [&](const Part& w, int i, int side) {
-    const uint32_t n = (uint32_t)(w.used + i);
-    if (!wait_or_quit(bar + 8 * (side + (n & 1)), (n >> 1) & 1u, &quit)) flag(p.flags, B200_PAGED_WAIT);
-    __syncwarp();
-  };
-
   uint32_t raw[KS][2];                       // eight columns' queries of the part to come, as they are in memory
   auto load_queries = [&](const Part& w, int nt) {
     const int col = w.ct * COLS + nt * 8 + g;
@@ -682,9 +681,28 @@ __global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(c
       raw[4 * b + 2][0] = y.x; raw[4 * b + 2][1] = y.y; raw[4 * b + 3][0] = y.z; raw[4 * b + 3][1] = y.w;
     }
   };
+  // a part's first copies, which go out before the part in front of it is joined
+  auto start = [&](const Part& w) {
+    __syncwarp();
+    if (w.count == 0) {
+      if constexpr (NT == 1) load_queries(w, 0);
+      return;
+    }
+    const int page = look_up(w, 0);
+    fetch(w, 0, map_k, 0);
+    fetch(w, 0, map_v, 2);
+    if (w.count > 1) fetch(w, 1, map_k, 0);
+    if constexpr (NT == 1) load_queries(w, 0);                                // their way is as long as the scales'
+    tell(w, 0, page);
+  };
+  auto arrived = [&](const Part& w, int i, int side) {
+    const uint32_t n = (uint32_t)(w.used + i);
+    if (!wait_or_quit(bar + 8 * (side + (n & 1)), (n >> 1) & 1u, &quit)) flag(p.flags, B200_PAGED_WAIT);
+    __syncwarp();
+  };
+
   Part w = next_part(0);
   start(w);
-  if constexpr (NT == 1) load_queries(w, 0);
   for (;;) {
     const Seq q = w.q;
     const int h = w.h, c0 = w.ct * COLS, n_cols = q.n * p.G, pf = w.pf, pl = w.pl, first = w.first, count = w.count, used = w.used;
@@ -944,7 +962,6 @@ __global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(c
     if (more) {
       w = next_part(used + count);
       start(w);
-      if constexpr (NT == 1) load_queries(w, 0);
     }
 
     // join the warps, eight columns at a time
@@ -1151,6 +1168,9 @@ int launch_few(const AttnP& p, const FewPlan& f, cudaStream_t st) {
   B200_TRY(code_map(&map_k, p.k, (long long)p.pages * p.H * p.P, D, 16));
   B200_TRY(code_map(&map_v, p.v, (long long)p.pages * p.H * p.P, D, 16));
   B200_TRY(allow_smem(limits, smem, few_rows_kernel<D, FMT, NT>));
+  // all of an SM's L1 as shared memory, also for what runs in between: left to the driver an SM keeps what the kernel in front left, and then holds one CTA and not two
+  static std::atomic<uint64_t> shares{0};
+  B200_TRY(prefer_smem(shares, 100, few_rows_kernel<D, FMT, NT>, join_kernel<D, NT>));
   B200_TRY(launch_early(few_rows_kernel<D, FMT, NT>, dim3((unsigned)f.ctas), dim3(FEW_THREADS), smem, st, map_k, map_v, p));
   if (f.direct) return B200_OK;
   const long long most = (long long)p.b.max_rows * p.G < 8 * NT ? (long long)p.b.max_rows * p.G : 8 * NT;
@@ -1178,6 +1198,8 @@ int launch_append(AppendP& p, cudaStream_t st) {
   p.q_rows = 1;
   while (p.q_rows < 8 && 2 * p.q_rows <= slots && (long long)p.b.T * p.Hq >= 148ll * 8 * slots * p.q_rows) p.q_rows *= 2;
   const dim3 grid((unsigned)(p.page_ctas + (p.Hq ? ceil_div(p.b.T, p.q_rows) : 0)));
+  static std::atomic<uint64_t> shares{0};
+  B200_TRY(prefer_smem(shares, 100, append_few_kernel<FMT, D>, append_many_kernel<FMT, D>, read_kernel<FMT, D>));
   if (few) return launch_early(append_few_kernel<FMT, D>, grid, dim3(threads), 0, st, p);
   return launch_early(append_many_kernel<FMT, D>, grid, dim3(threads), 0, st, p);
 }

@@ -528,7 +528,9 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(const AttnP p) {
 template <int D, int FMT>
 int launch(const AttnP& p, long long units, cudaStream_t st) {
   static std::atomic<uint64_t> limits{0};
+  static std::atomic<uint64_t> shares{0};
   B200_TRY(allow_smem(limits, (int)Smem<D>::BYTES, prompt_kernel<D, FMT>));
+  B200_TRY(prefer_smem(shares, 100, prompt_kernel<D, FMT>, prompt_join_kernel<D>));
   B200_TRY(launch_early(prompt_kernel<D, FMT>, dim3((unsigned)(units * p.nsplit)), dim3(THREADS), Smem<D>::BYTES, st, p));
   if (p.nsplit > 1) B200_TRY(launch_early(prompt_join_kernel<D>, dim3((unsigned)(units * (ROWS / 8))), dim3(128), 0, st, p));
   return B200_OK;
