@@ -99,7 +99,12 @@ __device__ __forceinline__ Page page_of(const AppendP& p, int item, bool tell) {
     if (tell) flag(p.flags, B200_PAGED_BAD_BATCH);
     return g;
   }
-  const int block = q.before / p.P + item - (q.r0 / p.P + 2 * s);
+  const int nth = item - (q.r0 / p.P + 2 * s);          // of the sequence's pages; rows out of order could make it negative
+  if (nth < 0) {
+    if (tell) flag(p.flags, B200_PAGED_BAD_BATCH);
+    return g;
+  }
+  const int block = q.before / p.P + nth;
   const long long first = (long long)block * p.P;
   if (q.n == 0 || first >= (long long)q.before + q.n) return g;
   g.page = p.b.table[s * p.b.table_ld + block];
@@ -1198,8 +1203,6 @@ int launch_append(AppendP& p, cudaStream_t st) {
   p.q_rows = 1;
   while (p.q_rows < 8 && 2 * p.q_rows <= slots && (long long)p.b.T * p.Hq >= 148ll * 8 * slots * p.q_rows) p.q_rows *= 2;
   const dim3 grid((unsigned)(p.page_ctas + (p.Hq ? ceil_div(p.b.T, p.q_rows) : 0)));
-  static std::atomic<uint64_t> shares{0};
-  B200_TRY(prefer_smem(shares, 100, append_few_kernel<FMT, D>, append_many_kernel<FMT, D>, read_kernel<FMT, D>));
   if (few) return launch_early(append_few_kernel<FMT, D>, grid, dim3(threads), 0, st, p);
   return launch_early(append_many_kernel<FMT, D>, grid, dim3(threads), 0, st, p);
 }
@@ -1270,7 +1273,7 @@ int64_t b200_paged_attention_bytes(const b200_paged_cache* cache, const b200_pag
   using namespace b200::paged;
   if (!cache || !batch || cache->kv_heads < 1 || q_heads < cache->kv_heads || q_heads % cache->kv_heads || window < 0 || sinks < 0 || batch->sequences < 1 || batch->max_rows < 0) return 0;
   const int G = q_heads / cache->kv_heads;
-  if (batch->max_rows == 0) return 0;
+  if (batch->total_rows <= 0 || batch->max_rows == 0) return 0;
   const Route r = route(cache, batch, G, window, sinks);
   return r.few_bytes + r.prompt_bytes;
 }

@@ -122,7 +122,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
   typedef Smem<D> L;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[17 + INFOS];
-  __shared__ float4 info[INFOS][8];          // per 16 keys: keys' scale, log2 and reciprocal of the values', whether the page is there
+  __shared__ float4 info[INFOS][8];          // per 16 keys: keys' scale, log2 and reciprocal of the values'; there: whether the page is
+  __shared__ __align__(16) uint32_t there[INFOS][8];
   __shared__ uint32_t tmem_at;
   __shared__ volatile int quit;
   __shared__ float tops[SOFT_WARPS];
@@ -207,7 +208,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       if (keys) {                            // what the weights need to know of these keys' pages
         if (lane < 2) {
           const float vs = scales.y > 0.f ? scales.y : 1.f;                   // all codes of a page of zeros are 0
-          info[i % INFOS][2 * w4 + lane] = page >= 0 ? make_float4(scales.x > 0.f ? scales.x : 1.f, __log2f(vs), __frcp_rn(vs), 1.f) : make_float4(0.f, 0.f, 0.f, -1.f);
+          there[i % INFOS][2 * w4 + lane] = page >= 0 ? 1u : 0u;
+          info[i % INFOS][2 * w4 + lane] = page >= 0 ? make_float4(scales.x > 0.f ? scales.x : 1.f, __log2f(vs), __frcp_rn(vs), 0.f) : make_float4(1.f, 0.f, 0.f, 0.f);
         }
         __syncwarp();
       }
@@ -339,12 +341,10 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       tc_fence_after();
       const int j0 = tiles[u.t0 + x] << 7;
       const float4* ip = info[x % INFOS];
-      bool there = true;                     // all pages
-#pragma unroll
-      for (int c = 0; c < 8; ++c) there &= ip[c].w > 0.f;
-      const bool whole = there & (j0 + KEYS - 1 <= pf) & ((p.window <= 0) | (pl - j0 < p.window) | (j0 + KEYS <= p.sinks));
+      const uint4 t0 = *reinterpret_cast<const uint4*>(there[x % INFOS]), t1 = *reinterpret_cast<const uint4*>(there[x % INFOS] + 4);
+      const bool whole = ((t0.x & t0.y & t0.z & t0.w & t1.x & t1.y & t1.z & t1.w) != 0u) & (j0 + KEYS - 1 <= pf) & ((p.window <= 0) | (pl - j0 < p.window) | (j0 + KEYS <= p.sinks));
       uint32_t r[KEYS];                      // the row's scores: read once, as the registers have room for them
-      float t = -INFINITY;
+      float t = -INFINITY, by[8], lv[8];     // score in base 2 = product * by + lv; by > 0, so that the largest score of a page's keys is that of their largest product
       tmem_ld32(ts, r);
       tmem_ld_wait32(r);
 #pragma unroll
@@ -353,18 +353,20 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
         if (!whole) {                        // keys that the row does not see: a bit for each of 32
           const int at = j0 + 32 * c;
           uint32_t seen = upto(pos - at) & (~upto(lo - at) | upto(p.sinks - 1 - at));
-          if (!(ip[2 * c].w > 0.f)) seen &= 0xffff0000u;
-          if (!(ip[2 * c + 1].w > 0.f)) seen &= 0xffffu;
+          if (!there[x % INFOS][2 * c]) seen &= 0xffff0000u;
+          if (!there[x % INFOS][2 * c + 1]) seen &= 0xffffu;
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (!(seen >> e & 1u)) r[32 * c + e] = 0xff800000u;
         }
 #pragma unroll
-        for (int b = 2 * c; b < 2 * c + 2; ++b) {                             // `by` is positive: the largest score of a page's keys is that of their largest product
+        for (int b = 2 * c; b < 2 * c + 2; ++b) {
+          by[b] = fmaxf(ip[b].x * fac, FLT_MIN);
+          lv[b] = ip[b].y;
           float mx[2] = {__uint_as_float(r[16 * b]), __uint_as_float(r[16 * b + 1])};
 #pragma unroll
           for (int e = 2; e < 16; ++e) mx[e & 1] = fmaxf(mx[e & 1], __uint_as_float(r[16 * b + e]));
-          t = fmaxf(t, fmaf(fmaxf(mx[0], mx[1]), fmaxf(ip[b].x * fac, FLT_MIN), ip[b].y));
+          t = fmaxf(t, fmaf(fmaxf(mx[0], mx[1]), by[b], lv[b]));
         }
         if (c < 3) tmem_ld_wait32(r + 32 * c + 32);
       }
@@ -389,30 +391,30 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       }
       const float off = m == -INFINITY ? 0.f : m;
       // log2 s_v - M in one number is off by half a unit of M: only while that is no more than a quarter
-      const bool far = __any_sync(0xffffffffu, fabsf(off) > 4194304.f && off < INFINITY);
-      if (far) {
+      if (__any_sync(0xffffffffu, fabsf(off) > 4194304.f && off < INFINITY)) {
 #pragma unroll
-        for (int e = 0; e < KEYS; ++e) r[e] = __float_as_uint(fmaf(__uint_as_float(r[e]), fmaxf(ip[e / 16].x * fac, FLT_MIN), ip[e / 16].y));
+        for (int e = 0; e < KEYS; ++e) r[e] = __float_as_uint(fmaf(__uint_as_float(r[e]), by[e / 16], lv[e / 16]));
+#pragma unroll
+        for (int b = 0; b < 8; ++b) { by[b] = 1.f; lv[b] = 0.f; }
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t w[16];
 #pragma unroll
         for (int b = 2 * c; b < 2 * c + 2; ++b) {
-          const float4 y = ip[b];
-          const uint64_t by = two(far ? 1.f : fmaxf(y.x * fac, FLT_MIN)), add = two(far ? -off : y.y - off);
+          const uint64_t by2 = two(by[b]), add = two(lv[b] - off);
           uint64_t part = 0;
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
             float e0, e1;
-            apart(fma2(together(__uint_as_float(r[16 * b + e]), __uint_as_float(r[16 * b + e + 1])), by, add), e0, e1);
+            apart(fma2(together(__uint_as_float(r[16 * b + e]), __uint_as_float(r[16 * b + e + 1])), by2, add), e0, e1);
             e0 = exp2_fast(e0); e1 = exp2_fast(e1);
             part = add2(part, together(e0, e1));
             w[8 * (b & 1) + (e >> 1)] = pack_f16(e0, e1);
           }
           float s0, s1;
           apart(part, s0, s1);
-          sum = fmaf(s0 + s1, y.z, sum);
+          sum = fmaf(s0 + s1, ip[b].z, sum);
         }
         tmem_st16(ts + 16 * c, w);
         if (c & 1) {

@@ -45,6 +45,11 @@ def _entry(name: str):
     return fn
 
 
+def turns_of(freqs: tp.Iterable[float]) -> list[int]:
+    """Turns per position, of frequencies in radians, as fractions of 2^64: the product with a position drops whole turns and nothing else."""
+    return [((num * _TURN // den + (1 << 127)) >> 128) % (1 << 64) for num, den in (f.as_integer_ratio() for f in freqs)]
+
+
 class RotaryTable:
     """Frequencies of a position rotation: ``base ** (-2 j / rot_dims)`` radians per position for the pair j, or ``freqs`` (rot_dims / 2 numbers).  ``pairing``: "adjacent" turns
     dimensions (2j, 2j + 1), "halves" (j, j + rot_dims / 2); dimensions from ``rot_dims`` on stay as they are."""
@@ -57,8 +62,7 @@ class RotaryTable:
         freqs = [base ** (-2.0 * j / rot_dims) for j in range(rot_dims // 2)] if freqs is None else [float(f) for f in freqs]
         if len(freqs) != rot_dims // 2:
             raise ValueError(f"{len(freqs)} frequencies for {rot_dims} dimensions")
-        # turns per position as a 64-bit fraction: its product with a position drops whole turns and nothing else
-        turns = [((num * _TURN // den + (1 << 127)) >> 128) % (1 << 64) for num, den in (f.as_integer_ratio() for f in freqs)]
+        turns = turns_of(freqs)
         self.device = _cuda(device)
         self.rot_dims, self.pairing = rot_dims, pairing
         self.turns = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64, device=self.device)

@@ -338,6 +338,80 @@ def test_append_leaves_out_what_does_not_fit():
             assert torch.equal(q[:rows[1]], x[:rows[1]])
 
 
+@pytest.mark.parametrize("rows", [[0, 10, 5, 12], [12, 4, 2, 0], [3, 3, 1, 9], [0, 2 ** 31 - 1, -2 ** 31, 4]])
+def test_rows_out_of_order_stay_within_the_tensors(rows):
+    """Recorded, and nothing else than the batch's own pages and rows is touched."""
+    c = Content([40, 40, 40], 2, 64, 16, "int8", capacity=[60, 60, 60], spare=5)
+    cache = c.cache()
+    was = [x.clone() for x in (cache.k.view(torch.int8), cache.v.view(torch.int8))]
+    x = torch.randn(14, 2, 64).bfloat16().cuda()
+    wide = torch.full((34, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    q = wide[10:24]
+    batch = PagedBatch(c.table.cuda(), torch.tensor([40] * 3, dtype=torch.int32).cuda(), torch.tensor(rows, dtype=torch.int32).cuda(), 14)
+    for new in (x, x.repeat(1, 1, 1)):
+        cache.append(batch, new, new, q=q, q_out=q, rotary=RotaryTable(64))
+    cache.attend(batch, q.clone(), out=q)
+    cache.read(batch)
+    assert cache.error_flags() & paged.BAD_BATCH
+    assert bool((wide[:10] == 7).all()) and bool((wide[24:] == 7).all())
+    mine = c.table[c.table >= 0].long()
+    others = torch.ones(c.pages, dtype=torch.bool)
+    others[mine] = False
+    for a, b in zip((cache.k.view(torch.int8), cache.v.view(torch.int8)), was):
+        assert torch.equal(a.cpu()[others], b.cpu()[others])
+        assert torch.equal(a.cpu()[c.table[:, :2].long()], b.cpu()[c.table[:, :2].long()])      # pages that are full already
+
+
+def test_rows_in_front_of_the_first_sequence():
+    c = Content([41, 52], 2, 128, 16, "int8", capacity=[45, 60])
+    cache = c.cache()
+    x, q = torch.randn(9, 2, 128).bfloat16().cuda(), torch.randn(9, 4, 128).bfloat16().cuda()
+    args = [torch.tensor(t, dtype=torch.int32).cuda() for t in ([41, 52], [3, 4, 6])]
+    batch = PagedBatch(c.table.cuda(), *args, 9, 2)
+    turned = cache.append(batch, x, x, q=q, rotary=RotaryTable(128), q_out=torch.full_like(q, 7.0))
+    out = cache.attend(batch, turned, out=torch.full_like(q, 7.0))
+    for t in (turned, out):
+        assert bool((t[:3] == 7).all()) and bool((t[6:] == 7).all()) and not bool((t[3:6] == 7).all())
+    other = c.cache()
+    batch = batch_of(c.table, [41, 52], [1, 2])
+    turned = other.append(batch, x[3:6].clone(), x[3:6].clone(), q=q[3:6].clone(), rotary=RotaryTable(128))
+    assert torch.equal(other.attend(batch, turned), out[3:6]) and torch.equal(other.k, cache.k) and cache.error_flags() == 0
+
+
+def test_tensors_that_do_not_fit_are_refused():
+    cache = PagedKVCache(8, 2, 128, 16, "int8")
+    batch = batch_of(torch.zeros(2, 4, dtype=torch.int32), [0, 0], [1, 2])
+    good, q = torch.zeros(3, 2, 128, dtype=torch.bfloat16, device="cuda"), torch.zeros(3, 4, 128, dtype=torch.bfloat16, device="cuda")
+    for k in (good.float(), good[:2], good[..., :64], good[:, :1], good.transpose(0, 1), good.cpu(), good[..., None], torch.zeros(3, 128, 2, dtype=torch.bfloat16, device="cuda").transpose(1, 2),
+              torch.zeros(3, 2, 128, dtype=torch.bfloat16, device="cuda", requires_grad=True), torch.zeros(1, 2, 128, dtype=torch.bfloat16, device="cuda").expand(3, 2, 128),
+              torch.zeros(3 * 260 + 4, dtype=torch.bfloat16, device="cuda")[4:784].view(3, 260)[:, :256].unflatten(1, (2, 128))):
+        with pytest.raises((ValueError, AssertionError)):
+            cache.append(batch, k, good)
+        with pytest.raises((ValueError, AssertionError)):
+            cache.append(batch, good, k)
+    for bad in (q[..., :64], q.float(), q[:2], q.flatten(1), torch.zeros(3, 3, 128, dtype=torch.bfloat16, device="cuda"), q.clone().requires_grad_()):
+        with pytest.raises((ValueError, AssertionError)):
+            cache.attend(batch, bad)
+        with pytest.raises((ValueError, AssertionError)):
+            cache.attend(batch, q, out=bad)
+    for kw in (dict(window=-1), dict(sinks=-1), dict(window=2 ** 31), dict(window=2 ** 32 + 5), dict(scale=0.0), dict(scale=float("nan"))):
+        with pytest.raises(ValueError):
+            cache.attend(batch, q, **kw)
+    with pytest.raises(ValueError):
+        cache.append(batch, good, good, q_out=q)
+    with pytest.raises(ValueError):
+        cache.append(batch, good, good, q=q, rotary=RotaryTable(256))
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for args in ((torch.zeros(2, 4, **i32), torch.zeros(3, **i32), torch.zeros(3, **i32), 3), (torch.zeros(2, 4, **i32).long(), torch.zeros(2, **i32), torch.zeros(3, **i32), 3),
+                 (torch.zeros(4, 2, **i32).t(), torch.zeros(2, **i32), torch.zeros(3, **i32), 3), (torch.zeros(2, 4, **i32), torch.zeros(2, **i32), torch.zeros(3, **i32), -1),
+                 (torch.zeros(1, 4, **i32).expand(2, 4), torch.zeros(2, **i32), torch.zeros(3, **i32), 3), (torch.zeros(2, 4, **i32), torch.zeros(2, **i32).cpu(), torch.zeros(3, **i32), 3)):
+        with pytest.raises(ValueError):
+            PagedBatch(*args)
+    with torch.no_grad():                                # a tensor that could have a gradient, where none is asked for
+        cache.append(batch, good.clone().requires_grad_(), good)
+    assert cache.error_flags() == 0
+
+
 # ------------------------------------------------------------------------------------------------------------------------
 # a run of them together
 # ------------------------------------------------------------------------------------------------------------------------
