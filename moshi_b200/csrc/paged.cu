@@ -415,14 +415,23 @@ __global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadP p) {
 // =========================================================================================================================
 // attention of few rows
 // =========================================================================================================================
-// Columns are (row of the sequence, query head of the group); a CTA has 8 * NT of them, one kv head and a run of the keys, in tiles of 32 tokens that its warps take in
-// turn.  Both products have the cache as the first operand of mma.m16n8k16: S^T = K Q^T (tokens x columns) and O^T += V^T P^T (dims x columns), so a single row of one head
-// wastes tensor-core columns and not cache bytes.  Codes go from memory into registers as fragments, 16 bytes at a time: which dimension of K is which
-// k of the product is free as long as Q has the same order, and so is which dimension of V is which row of O^T.  P^T comes out of S^T by movmatrix.
+// Columns are (row of the sequence, query head of the group); a unit is 8 * NT of them with one kv head, over tiles of 32 tokens that a CTA's warps take in turn.  Both products have the cache as
+// the first operand of mma.sync: S^T = K Q^T (tokens x columns) and O^T += V^T P^T (dims x columns), so that a single row of one head wastes tensor-core columns and not
+// cache bytes.  Which dimension of K is which k of the product is free as long as Q has the same order, and so is which dimension of V is which row of O^T, and which token is which row of S^T and
+// k of the other product: a lane reads its fragments as 16 neighbouring codes.  P^T comes out of S^T by movmatrix.
 //
-// Codes of both types are exact in f16, and so are bf16 queries after a power of two per column; P is f16 in (0, 2^8].  The scale of a page's keys multiplies the scores; that of its
-// values goes into the exponent, P = 2^(score + log2 s_v - M), with M the running maximum of the same, and the sum of the weights takes P / s_v: nothing is rounded on the way but P.
-// M follows only when a score passes it by 2^8, as then no column has to be compared across lanes for most tiles.
+// Codes of both types are exact in f16, and so are bf16 queries after a power of two per column; P is f16 in (0, 2^8], off by 2^-11 of itself.  The scale of a page's keys multiplies the
+// scores; that of its values goes into the exponent, P = 2^(score + log2 s_v - M), with M the running maximum of the same, and the sum of the weights takes P / s_v: nothing is
+// rounded on the way but P.  M follows only when a score passes it by 2^8, as then no column has to be compared across lanes for most tiles.
+//
+// Bounds: HBM for large batches (48 sessions of 3000 tokens, 32 heads, e4m3: 183 us, 6.5 TB/s); for many short units what a unit costs beside its tiles (128 sessions under a window of 1024, 8 heads: 74 us, floor 36;
+// a part's first copies, its queries and the joining of its warps are 7400 clocks beside 20000 for eight tiles a warp).
+// Why this way:
+// * tiles come as swizzled tensor copies, two in flight and two at work per warp: asked for lane by lane in the fragments' order, 16 bytes of eight rows an instruction, the same bytes came at 5.2 TB/s,
+//   in whole lines at 7.1 (nothing but copies);
+// * the scores of a tile and the values of the one in front do not wait for one another and are one stretch of code;
+// * two CTAs of four warps an SM: four of two warps are faster for short units (window 66 us, 64 ragged requests 84 -> 80) and slower for few (one session of 375 tokens 9.1 -> 12.3 us, one
+//   request of 131072 tokens 55 -> 59); three of four do not fit with the values' second place.
 constexpr int FEW_WARPS = 4, FEW_THREADS = FEW_WARPS * 32;
 constexpr int few_per_sm(int nt) { return 2; }      // CTAs, by their registers
 constexpr int DIRECT_TILES = 33;             // units of at most this many tiles are not cut where the chip holds all of them at once: no join
