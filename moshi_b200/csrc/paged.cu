@@ -433,8 +433,8 @@ __global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadP p) {
 // * two CTAs of four warps an SM: four of two warps are faster for short units (window 66 us, 64 ragged requests 84 -> 80) and slower for few (one session of 375 tokens 9.1 -> 12.3 us, one
 //   request of 131072 tokens 55 -> 59); three of four do not fit with the values' second place.
 constexpr int FEW_WARPS = 4, FEW_THREADS = FEW_WARPS * 32;
-constexpr int few_per_sm(int nt) { return 2; }      // CTAs, by their registers
-constexpr int DIRECT_TILES = 33;             // units of at most this many tiles are not cut where the chip holds all of them at once: no join
+constexpr int FEW_PER_SM = 2;                // CTAs
+constexpr int DIRECT_TILES = 64;             // units of more tiles are always cut
 constexpr int MIN_RUN = 8;                    // tiles of a CTA
 constexpr float SLACK = 8.f;
 
@@ -540,32 +540,7 @@ __device__ __forceinline__ Run run_of(const AttnP& p) {
   return r;
 }
 
-// int8 and eight columns: the codes of K go into the product as they are, and Q as three digits of 8 bits: 22 bits below the column's largest value, where f16 keeps 11 bits of each
-// value; sums are exact.  Three products of 32 dimensions are dearer than two of 16 by half, but the 160 instructions that make f16 of a tile's keys fall away.  More columns
-// share the conversion, and the digits' registers are not there.  (e4m3 by e4m3 is no instruction of its own: it takes as many products and conversions as f16.)
-constexpr bool few_digits(int fmt, int nt) { return fmt == INT8 && nt == 1; }
 constexpr int SEEN = 1, IN_PART = 0, HIDDEN = -1;      // a half of a tile: by all columns, by some, by none
-// four integers of up to 2^22 = 65536 x2 + 256 x1 + x0 with digits of -128 .. 127
-__device__ __forceinline__ void digits(float a, float b, float c, float d, uint32_t& d0, uint32_t& d1, uint32_t& d2) {
-  auto whole = [](float x) { return __float_as_int(x + 12582912.f) - 0x4b400000; };        // the last bits of a sum with 1.5 * 2^23
-  const int n[4] = {whole(a), whole(b), whole(c), whole(d)};
-  d0 = d1 = d2 = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int x0 = (int)(int8_t)n[i], n1 = (n[i] - x0) >> 8, x1 = (int)(int8_t)n1, x2 = (n1 - x1) >> 8;
-    d0 |= ((uint32_t)x0 & 255u) << (8 * i); d1 |= ((uint32_t)x1 & 255u) << (8 * i); d2 |= ((uint32_t)x2 & 255u) << (8 * i);
-  }
-}
-// sums n of up to 128 * 128 * 127 < 2^21 begin at the bits of 1.5 * 2^23, and so end as those of 1.5 * 2^23 + n
-constexpr uint32_t DIGIT_ZERO = 0x4b400000u;
-__device__ __forceinline__ float digit_sum(uint32_t a0, uint32_t a1, uint32_t a2) {
-  const float f0 = __uint_as_float(a0) - 12582912.f, f1 = __uint_as_float(a1) - 12582912.f, f2 = __uint_as_float(a2) - 12582912.f;
-  return fmaf(f2, 65536.f, fmaf(f1, 256.f, f0));
-}
-__device__ __forceinline__ void mma_s8(uint32_t* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 
 // Tiles lie in shared memory as the copies swizzle them: 16-byte piece n of row r.
 template <int D>
@@ -576,9 +551,8 @@ template <int D>
 __device__ __forceinline__ int token_of(int i) { return (D == 128 ? 0x37156240u : 0x67542310u) >> (4 * i) & 7; }
 
 template <int D, int FMT, int NT>
-__global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnP p) {
+__global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnP p) {
   constexpr int KS = D / 16, MT = D / 16, COLS = 8 * NT, SIDE = 32 * D;        // bytes of a tile's keys or values
-  constexpr bool DIGITS = few_digits(FMT, NT);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const ring = smem_raw + ((1024u - (tcp::smem_u32(smem_raw) & 1023u)) & 1023u);       // [warp]: two tiles of keys, two of values, as the copies swizzle them
   __shared__ __align__(8) uint64_t bars[FEW_WARPS][4];                        // a ring's places
@@ -722,8 +696,8 @@ __global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(c
     const int h = w.h, c0 = w.ct * COLS, n_cols = q.n * p.G, pf = w.pf, pl = w.pl, first = w.first, count = w.count, used = w.used;
     const Tiles<5> tiles = w.tiles;
 
-    // queries: lane (g, c) has of column 8 nt + g the dimensions 64 i + 16 c .. + 15, as f16 or as three digits of 8 bits
-    uint32_t qf[DIGITS ? 1 : NT][KS][2], qd[3][KS / 2][2];
+    // queries: lane (g, c) has of column 8 nt + g the dimensions 64 i + 16 c .. + 15
+    uint32_t qf[NT][KS][2];
     float fac[NT][2];                        // of columns 8 nt + 2 c, + 1: what turns a product of codes into a score in base 2
     int pos[NT][2];
 #pragma unroll
@@ -743,24 +717,15 @@ __global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(c
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const float power = top > 0.f ? power_of_two_in(top) : 1.f;
-      constexpr float LAND = DIGITS ? 2097152.f : 16384.f;       // the column's largest lands in [LAND, 2 LAND)
-      const float up = LAND / power;
-      if constexpr (DIGITS) {
+      const float up = 16384.f / power;      // the column's largest lands in [2^14, 2^15)
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const float2 u = unpack_bf16(raw[k][0]), v = unpack_bf16(raw[k][1]);
-          digits(u.x * up, u.y * up, v.x * up, v.y * up, qd[0][k >> 1][k & 1], qd[1][k >> 1][k & 1], qd[2][k >> 1][k & 1]);
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 v = unpack_bf16(raw[k][e]);
+          qf[nt][k][e] = pack_f16(v.x * up, v.y * up);
         }
-      } else {
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float2 v = unpack_bf16(raw[k][e]);
-            qf[DIGITS ? 0 : nt][k][e] = pack_f16(v.x * up, v.y * up);
-          }
-      }
-      const float back = top < INFINITY ? power * (1.f / LAND) : NAN;         // such a column's results are NaN, and no other's
+      const float back = top < INFINITY ? power * (1.f / 16384.f) : NAN;         // such a column's results are NaN, and no other's
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         fac[nt][e] = __shfl_sync(0xffffffffu, back, (2 * c + e) * 4) * p.scale2;
@@ -791,61 +756,33 @@ __global__ void __launch_bounds__(FEW_THREADS, few_per_sm(NT)) few_rows_kernel(c
     // scores in base 2, log2 of the values' scale added
     auto scores = [&](int i, const Tile& t, float (&sc)[2][NT][4]) {
       const uint8_t* from = my_ring + ((used + i) & 1) * SIDE;
-      if constexpr (DIGITS) {
-        uint32_t acc[2][3][4];
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int d = 0; d < 3; ++d)
+        for (int nt = 0; nt < NT; ++nt) sc[half][nt][0] = sc[half][nt][1] = sc[half][nt][2] = sc[half][nt][3] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[half][d][e] = DIGIT_ZERO;
-#pragma unroll
-        for (int b = 0; b < D / 64; ++b)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint8_t* f_h = from + half * (SIDE / 2);
-            const uint4 r0 = *reinterpret_cast<const uint4*>(f_h + piece<D>(key_row, 4 * b + c)), r1 = *reinterpret_cast<const uint4*>(f_h + piece<D>(key_row + 8, 4 * b + c));
-#pragma unroll
-            for (int d = 0; d < 3; ++d) {
-              mma_s8(acc[half][d], r0.x, r1.x, r0.y, r1.y, qd[d][2 * b][0], qd[d][2 * b][1]);
-              mma_s8(acc[half][d], r0.z, r1.z, r0.w, r1.w, qd[d][2 * b + 1][0], qd[d][2 * b + 1][1]);
-            }
-          }
+      for (int b = 0; b < D / 64; ++b)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const float by[2] = {t.x[half].y * fac[0][0], t.x[half].y * fac[0][1]};
+          const uint8_t* f_h = from + half * (SIDE / 2);
+          const uint4 r0 = *reinterpret_cast<const uint4*>(f_h + piece<D>(key_row, 4 * b + c)), r1 = *reinterpret_cast<const uint4*>(f_h + piece<D>(key_row + 8, 4 * b + c));
+          const uint32_t k0[4] = {r0.x, r0.y, r0.z, r0.w}, k1[4] = {r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[half][0][e] = fmaf(digit_sum(acc[half][0][e], acc[half][1][e], acc[half][2][e]), by[e & 1], t.x[half].z);
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t w0 = ready<FMT>(k0[k]), w1 = ready<FMT>(k1[k]);
+            const uint32_t a0 = half2_of<FMT, 0>(w0), a1 = half2_of<FMT, 0>(w1), a2 = half2_of<FMT, 1>(w0), a3 = half2_of<FMT, 1>(w1);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(sc[half][nt], a0, a1, a2, a3, qf[nt][4 * b + k][0], qf[nt][4 * b + k][1]);
+          }
         }
-      } else {
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) sc[half][nt][0] = sc[half][nt][1] = sc[half][nt][2] = sc[half][nt][3] = 0.f;
+        for (int nt = 0; nt < NT; ++nt) {
+          const float by[2] = {t.x[half].y * fac[nt][0], t.x[half].y * fac[nt][1]};
 #pragma unroll
-        for (int b = 0; b < D / 64; ++b)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint8_t* f_h = from + half * (SIDE / 2);
-            const uint4 r0 = *reinterpret_cast<const uint4*>(f_h + piece<D>(key_row, 4 * b + c)), r1 = *reinterpret_cast<const uint4*>(f_h + piece<D>(key_row + 8, 4 * b + c));
-            const uint32_t k0[4] = {r0.x, r0.y, r0.z, r0.w}, k1[4] = {r1.x, r1.y, r1.z, r1.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t w0 = ready<FMT>(k0[k]), w1 = ready<FMT>(k1[k]);
-              const uint32_t a0 = half2_of<FMT, 0>(w0), a1 = half2_of<FMT, 0>(w1), a2 = half2_of<FMT, 1>(w0), a3 = half2_of<FMT, 1>(w1);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma_f16(sc[half][nt], a0, a1, a2, a3, qf[nt][4 * b + k][0], qf[nt][4 * b + k][1]);
-            }
-          }
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float by[2] = {t.x[half].y * fac[nt][0], t.x[half].y * fac[nt][1]};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[half][nt][e] = fmaf(sc[half][nt][e], by[e & 1], t.x[half].z);
-          }
-      }
+          for (int e = 0; e < 4; ++e) sc[half][nt][e] = fmaf(sc[half][nt][e], by[e & 1], t.x[half].z);
+        }
     };
     uint32_t pb[2][NT][2];                   // weights of the tile whose values come next
     // weights out of scores, and O and the sums brought to the maximum that they refer to
@@ -1123,7 +1060,11 @@ Batch batch_of(const b200_paged_batch* b) {
 bool rows_fit(const void* p, long long ld, int heads, int dim) { return p && !(reinterpret_cast<uintptr_t>(p) & 15) && ld >= (long long)heads * dim && ld % 8 == 0; }
 int shift_of(int P) { return P == 16 ? 4 : P == 32 ? 5 : P == 64 ? 6 : 7; }
 
-// CTAs of 8 * nt columns, about one wave of them (four, three or two to an SM), fewer where the tables allow for less work than that.
+// Sequences of more than 16 columns (rows times heads of a group), at head size 64 of more than 32, go to the tensor cores' kernel of whole tiles, whose time hardly depends on how many of its 256 columns
+// there are; the only sequence of a step goes there with all its rows if it may have that many.  (32 heads of 128 on 8, 3000 tokens, here / there: 16 requests of 16 columns 40 / 69 us, of 24 87 / 69,
+// of 48 136 / 70; one request of 24 columns 34 / 19; 64 of 32 246 / 253, of 64 460 / 254.  24 heads of 64 on 4, 16 requests of 1000 to 6000 tokens and 30 columns: 29 / 48.)
+constexpr int few_cols(int dim) { return dim == 64 ? 32 : 16; }
+// CTAs of 8 * nt columns, a wave of them, fewer where the tables allow for less work than that.
 struct FewPlan { int nt, ctiles, ctas; long long units; bool direct; };
 FewPlan few_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks, int few_rows) {
   FewPlan f;
@@ -1133,8 +1074,11 @@ FewPlan few_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, in
   f.units = (long long)b->sequences * c->kv_heads * f.ctiles;
   long long keys = (long long)b->table_width * c->page_tokens;
   if (window > 0 && (long long)window + sinks + rows < keys) keys = (long long)window + sinks + rows;
-  const long long tiles = ceil_div64(keys, 32) + 1, runs = ceil_div64(f.units * (tiles + 4), MIN_RUN), wave = 148 * few_per_sm(f.nt);
-  f.direct = f.units <= wave && tiles <= DIRECT_TILES;
+  const long long tiles = ceil_div64(keys, 32) + 1, runs = ceil_div64(f.units * (tiles + 4), MIN_RUN), wave = 148 * FEW_PER_SM;
+  // A CTA a unit, and nothing to join, where the chip holds all units at once and the longest is not much longer than an equal share: 7 us and 0.25 a tile, against 10.5 and 0.34 for every 296th part of all
+  // tiles and 12 for each unit.  (One token, 32 heads on 8, uncut / cut: 1 request of 1000 tokens 14.0 / 12.5 us, 32 of them 19.1 / 25.6, of 2000 29.7 / 36.0, 8 of 2000 24.5 / 17.9; 1 session of 374
+  // tokens with 32 heads 9.2 / 12.2.)
+  f.direct = f.units <= wave && tiles <= DIRECT_TILES && 250 * tiles < 3500 + f.units * (tiles + UNIT_COST) * 115 / 100;
   f.ctas = (int)(f.direct ? f.units : runs < wave ? runs : wave);
   return f;
 }
@@ -1161,14 +1105,12 @@ int code_map(CUtensorMap* m, const void* codes, long long rows, int dim, int box
 
 namespace {
 
-// Sequences of more than 64 columns (rows times heads of a group) go to the tensor cores' kernel of whole tiles; the only sequence of a step goes there with all its rows if it may have that many.
-constexpr int FEW_COLS = 64;
 struct Route { int from_rows; FewPlan few; PromptPlan prompt; int64_t few_bytes, prompt_bytes; };
 Route route(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks) {
   Route r;
   memset(&r, 0, sizeof(r));
-  const bool many = (long long)b->max_rows * G > FEW_COLS;
-  r.from_rows = !many ? 0x7fffffff : b->sequences == 1 ? 1 : FEW_COLS / G + 1;
+  const bool many = (long long)b->max_rows * G > few_cols(c->dim);
+  r.from_rows = !many ? 0x7fffffff : b->sequences == 1 ? 1 : few_cols(c->dim) / G + 1;
   if (r.from_rows > 1) { r.few = few_plan(c, b, G, window, sinks, r.from_rows); r.few_bytes = (few_bytes(r.few, c->dim) + 15) / 16 * 16; }
   if (many) { r.prompt = prompt_plan(c, b, G, window, sinks); r.prompt_bytes = prompt_bytes(r.prompt, c->dim); }
   return r;
@@ -1192,16 +1134,17 @@ int launch_few(const AttnP& p, const FewPlan& f, cudaStream_t st) {
 }
 template <int D, int FMT>
 int launch_few_nt(const AttnP& p, const FewPlan& f, cudaStream_t st) {
-  if (f.nt == 1) return launch_few<D, FMT, 1>(p, f, st);
-  if (f.nt == 2) return launch_few<D, FMT, 2>(p, f, st);
-  return launch_few<D, FMT, 4>(p, f, st);
+  if constexpr (few_cols(D) > 16)
+    if (f.nt == 4) return launch_few<D, FMT, 4>(p, f, st);
+  return f.nt == 1 ? launch_few<D, FMT, 1>(p, f, st) : launch_few<D, FMT, 2>(p, f, st);
 }
 
 constexpr int WAVE = 148 * 3 / 2;
 template <int FMT, int D>
 int launch_append(AppendP& p, cudaStream_t st) {
-  // A page gets at most four rows of a sequence: a warp each, and all of its heads side by side (48 rows of 32 heads: 6.9 us as blocks of whole pages, 5.x as warps).
-  const bool few = p.b.max_rows <= 4;
+  // Up to 16 rows of a sequence: a warp a page, head and side (32 heads, 48 sequences of 1 / 8 / 16 rows: 7.8 / 9.7 / 13.7 us, as blocks of whole pages 28 / 29 / 30; 8 heads, 8 sequences of
+  // 32 / 64 rows: 6.8 / 9.6 us, as blocks 6.1 / 6.5).
+  const bool few = p.b.max_rows <= 16;
   const int threads = few ? APPEND_THREADS : p.P * D / 32;
   // as many heads to a block as leave the chip a wave of blocks, two to an SM
   p.heads_per_block = 1;

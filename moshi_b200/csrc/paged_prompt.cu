@@ -2,8 +2,8 @@
 //
 // A CTA owns one kv head and up to 256 rows (row of the sequence, query head of the group) as two tiles of 128, and walks the keys in tiles of 128 tokens.  Warps 8..14 bring the codes from memory
 // through registers into f16 tiles (exact for both types) in SWIZZLE_128B, keys K-major and values as they lie, tokens by dims; warp 15 issues S_i = Q_i K^T and O_i += P_i V as
-// tcgen05.mma with fp32 accumulators in TMEM (S_0, S_1, O_0, O_1); warps 0..3 and 4..7 hold a row per thread, with all its 128 scores, and put P as f16 over the scores,
-// from where the second product reads it.  While one tile's weights are made, the other's products run.
+// tcgen05.mma with fp32 accumulators in TMEM (one place for the scores, O_0, O_1); warps 0..3 and 4..7 hold a row per thread, with all its 128 scores, and put P as f16 into TMEM,
+// from where the second product reads it.  As soon as one tile's scores are in registers their place takes the other's.
 //
 // Scales as in paged.cu: that of a page's keys multiplies its 16 or more columns' scores, that of its values goes into the exponent.  O is rescaled only when a row's maximum grew by more than 2^8.
 #include "paged.cuh"
@@ -18,7 +18,7 @@ namespace {
 using namespace tcp;
 typedef __nv_bfloat16 bf16;
 
-constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 7, THREADS = (SOFT_WARPS + CONVERT_WARPS + 1) * 32, ROWS = 256, KEYS = 128, INFOS = 4;
+constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 7, THREADS = (SOFT_WARPS + CONVERT_WARPS + 1) * 32, ROWS = 256, KEYS = 128, INFOS = 8;
 constexpr float SLACK = 8.f;
 
 template <int D>
@@ -121,7 +121,7 @@ template <int D, int FMT>
 __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
   typedef Smem<D> L;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[17 + INFOS];
+  __shared__ __align__(8) uint64_t bars[19 + INFOS];
   __shared__ float4 info[INFOS][8];          // per 16 keys: keys' scale, log2 and reciprocal of the values'; there: whether the page is
   __shared__ __align__(16) uint32_t there[INFOS][8];
   __shared__ uint32_t tmem_at;
@@ -130,12 +130,12 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t bar = smem_u32(bars), k_full = bar, k_empty = bar + 16, v_full = bar + 32, v_empty = bar + 48, s_full = bar + 64, p_full = bar + 80, o_done = bar + 96, p_half = bar + 112, q_full = bar + 128, i_full = bar + 136;
+  const uint32_t bar = smem_u32(bars), k_full = bar, k_empty = bar + 16, v_full = bar + 32, v_empty = bar + 48, s_full = bar + 64, p_full = bar + 80, o_done = bar + 96, p_half = bar + 112, s_taken = bar + 128, q_full = bar + 144, i_full = bar + 152;
   if (threadIdx.x == 0) {
     quit = 0;
     for (int i = 0; i < 2; ++i) {
       mbar_init(k_full + 8 * i, 4); mbar_init(k_empty + 8 * i, 1); mbar_init(v_full + 8 * i, 4); mbar_init(v_empty + 8 * i, 1);
-      mbar_init(s_full + 8 * i, 1); mbar_init(p_half + 8 * i, 4); mbar_init(p_full + 8 * i, 4); mbar_init(o_done + 8 * i, 1);
+      mbar_init(s_full + 8 * i, 1); mbar_init(p_half + 8 * i, 4); mbar_init(s_taken + 8 * i, 4); mbar_init(p_full + 8 * i, 4); mbar_init(o_done + 8 * i, 1);
     }
     mbar_init(q_full, SOFT_WARPS);
     for (int i = 0; i < INFOS; ++i) mbar_init(i_full + 8 * i, 4);
@@ -236,44 +236,47 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
     constexpr uint32_t id_s = idesc_f16(KEYS, false), id_o = idesc_f16(D, true);
     auto scores = [&](int i, int x) {        // of tile x for queries i
       const uint32_t a = desc_low(base + L::Q + i * L::TILE), b = desc_low(base + L::K + (x & 1) * L::TILE);
-#pragma unroll
-      for (int half = 0; half < D / 64; ++half) umma_block<1>(tmem + 128 * i, a + half * (L::HALF >> 4), b - a, id_s, half > 0 ? 1u : 0u);
-      commit_elected(s_full + 8 * i);
-    };
-    bool ok = warp_wait(q_full, 0, &quit) && warp_wait(k_full, 0, &quit);
-    if (ok) {
       tc_fence_after();
-      for (int i = 0; i < tiles_q; ++i) scores(i, 0);
-      commit_elected(k_empty);
-    }
-    for (int x = 0; ok && x < n; ++x) {
-      const int st = x & 1;
-      for (int i = 0; ok && i < tiles_q; ++i) {
-        ok = i > 0 || warp_wait(v_full + 8 * st, (uint32_t)(x >> 1) & 1u, &quit);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {                                // of the keys: the second half's weights are made beside the first's product
-          ok = ok && warp_wait((half ? p_full : p_half) + 8 * i, (uint32_t)x & 1u, &quit);
-          if (!ok) break;
-          tc_fence_after();
-          if (elected()) {
+      for (int half = 0; half < D / 64; ++half) umma_block<1>(tmem, a + half * (L::HALF >> 4), b - a, id_s, half > 0 ? 1u : 0u);
+      commit_elected(s_full + 8 * i);
+      if (i == tiles_q - 1) commit_elected(k_empty + 8 * (x & 1));
+    };
+    auto sums = [&](int i, int x) {          // over tile x for queries i, half of the keys behind the other: the second half's weights are made beside the first's product
 #pragma unroll
-            for (int k = half * KEYS / 32; k < (half + 1) * KEYS / 32; ++k)
-              product_pv(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k, base + L::V + st * L::TILE + k * 2048, L::HALF, id_o, x > 0 || k > 0 ? 1u : 0u);
-          }
-          __syncwarp();
+      for (int half = 0; half < 2; ++half) {
+        if (!warp_wait((half ? p_full : p_half) + 8 * i, (uint32_t)x & 1u, &quit)) return false;
+        tc_fence_after();
+        if (elected()) {
+#pragma unroll
+          for (int k = half * KEYS / 32; k < (half + 1) * KEYS / 32; ++k)
+            product_pv(tmem + 256 + 128 * i, tmem + 128 + 64 * i + 8 * k, base + L::V + (x & 1) * L::TILE + k * 2048, L::HALF, id_o, x > 0 || k > 0 ? 1u : 0u);
         }
-        if (!ok) break;
-        commit_elected(o_done + 8 * i);
-        if (i == tiles_q - 1) commit_elected(v_empty + 8 * st);
-        if (x + 1 < n) {                     // the next scores lie over these weights
-          ok = (i > 0 || warp_wait(k_full + 8 * (st ^ 1), (uint32_t)((x + 1) >> 1) & 1u, &quit)) && warp_wait(o_done + 8 * i, (uint32_t)x & 1u, &quit);
-          if (!ok) break;
-          tc_fence_after();
-          scores(i, x + 1);
-          if (i == tiles_q - 1) commit_elected(k_empty + 8 * (st ^ 1));
-        }
+        __syncwarp();
       }
+      commit_elected(o_done + 8 * i);
+      if (i == tiles_q - 1) commit_elected(v_empty + 8 * (x & 1));
+      return true;
+    };
+    auto v_there = [&](int x) { return warp_wait(v_full + 8 * (x & 1), (uint32_t)(x >> 1) & 1u, &quit); };
+    // The scores' place is free as soon as a tile's weight warps have them in registers, and then takes the other tile's: the next scores of a tile are made while its weights still are.
+    // In turn: scores of 1, sum of 1 over the keys in front, scores of 0 over the next keys, sum of 0.
+    bool ok = warp_wait(q_full, 0, &quit) && warp_wait(k_full, 0, &quit);
+    if (ok) scores(0, 0);
+    for (int x = 0; ok && x < n; ++x) {
+      ok = warp_wait(s_taken, (uint32_t)x & 1u, &quit);
+      if (tiles_q > 1) {
+        if (ok) scores(1, x);
+        if (x > 0) ok = ok && sums(1, x - 1);
+        ok = ok && warp_wait(s_taken + 8, (uint32_t)x & 1u, &quit);
+      }
+      if (x + 1 < n) {
+        ok = ok && warp_wait(k_full + 8 * ((x + 1) & 1), (uint32_t)((x + 1) >> 1) & 1u, &quit);
+        if (ok) scores(0, x + 1);
+      }
+      ok = ok && v_there(x) && sums(0, x);
     }
+    if (tiles_q > 1) ok = ok && sums(1, n - 1);
     __syncwarp();
   }
   } else {
@@ -331,7 +334,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
     const bool has = row < u.rows;
     const int pos = has ? u.q.before + rr / p.G : -1, lo = p.window > 0 ? pos - p.window : -1;      // sees j <= pos, j > lo or j < sinks
     const int pf = u.q.before + (u.r0 + 128 * i) / p.G, pl = u.q.before + (u.r0 + min(128 * i + 128, u.rows) - 1) / p.G;      // of this tile of queries
-    const uint32_t lanes = (uint32_t)(q4 * 32) << 16, ts = tmem + lanes + 128 * i, to = tmem + lanes + 256 + 128 * i;
+    const uint32_t lanes = (uint32_t)(q4 * 32) << 16, ts = tmem + lanes, tp = tmem + lanes + 128 + 64 * i, to = tmem + lanes + 256 + 128 * i;
     const float fac = p.scale2 * power * (1.f / 16384.f);
     float m = -INFINITY, sum = 0.f;
     bool ok = true;
@@ -370,14 +373,19 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
         }
         if (c < 3) tmem_ld_wait32(r + 32 * c + 32);
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_taken + 8 * i);
       const bool grow = t > m + SLACK;
+      if (x > 0) {                           // the sum over the keys in front has read its weights and settled in O
+        ok = wait_or_quit(o_done + 8 * i, (uint32_t)(x - 1) & 1u, &quit);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        tc_fence_after();
+      }
       if (__any_sync(0xffffffffu, grow)) {
         const float factor = grow ? exp2_fast(m - t) : 1.f;
         if (grow) { m = t; sum *= factor; }
         if (x > 0) {
-          ok = wait_or_quit(o_done + 8 * i, (uint32_t)(x - 1) & 1u, &quit);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          tc_fence_after();
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {
             uint32_t o[16];
@@ -416,7 +424,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
           apart(part, s0, s1);
           sum = fmaf(s0 + s1, ip[b].z, sum);
         }
-        tmem_st16(ts + 16 * c, w);
+        tmem_st16(tp + 16 * c, w);
         if (c & 1) {
           tmem_st_wait();
           tc_fence_before();
@@ -548,7 +556,7 @@ PromptPlan prompt_plan(const b200_paged_cache* c, const b200_paged_batch* b, int
   if (window > 0 && (long long)window + sinks + ROWS / G < keys) keys = (long long)window + sinks + ROWS / G;
   const long long tiles = ceil_div64(keys, KEYS);
   long long n = f.units ? 148 / f.units : 1;
-  if (n > tiles / 4) n = tiles / 4;          // ranges of four tiles at least
+  if (n > tiles / 2) n = tiles / 2;          // ranges of two tiles at least
   f.nsplit = n < 1 ? 1 : (int)n;
   return f;
 }

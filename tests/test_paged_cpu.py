@@ -69,12 +69,12 @@ def kernels(fake, call, what):
     (dict(sequences=1, total_rows=1, table_width=6), ["few_rows"]),                               # few short units: uncut
     (dict(sequences=64, total_rows=64, table_width=6), ["few_rows", "join_kernel"]),
     (dict(window=512, sinks=4), ["few_rows"]),
-    (dict(total_rows=64, max_rows=16), ["few_rows", "join_kernel"]),                              # 64 columns
-    (dict(total_rows=68, max_rows=17), ["prompt_kernel", "prompt_join", "few_rows", "join_kernel"]),
+    (dict(total_rows=16, max_rows=4), ["few_rows", "join_kernel"]),                               # 16 columns
+    (dict(total_rows=20, max_rows=5), ["prompt_kernel", "prompt_join", "few_rows", "join_kernel"]),
     (dict(sequences=1, total_rows=17, max_rows=17), ["prompt_kernel", "prompt_join"]),           # the only sequence goes there with all its rows
     (dict(sequences=1, total_rows=5000, max_rows=5000), ["prompt_kernel"]),
     (dict(sequences=8, total_rows=5000, max_rows=900), ["prompt_kernel", "few_rows", "join_kernel"]),
-    (dict(dim=64, q_heads=8, q_ld=512, out_ld=512, total_rows=64, max_rows=64, sequences=1), ["few_rows", "join_kernel"]),
+    (dict(dim=64, q_heads=8, q_ld=512, out_ld=512, total_rows=16, max_rows=16, sequences=1), ["few_rows", "join_kernel"]),
     (dict(total_rows=0), []), (dict(max_rows=0), []),
 ], ids=str)
 @pytest.mark.parametrize("kv_dtype", [_lib.B200_KV_INT8, _lib.B200_KV_FP8_E4M3])
@@ -83,8 +83,8 @@ def test_which_kernels_attend(fake, changed, names, kv_dtype):
 
 
 def test_which_kernels_append_and_read(fake):
-    assert kernels(fake, Call(max_rows=4, total_rows=16), "append") == [(0, "append_few")]
-    assert kernels(fake, Call(max_rows=5, total_rows=16), "append") == [(0, "append_many")]
+    assert kernels(fake, Call(max_rows=16, total_rows=16), "append") == [(0, "append_few")]
+    assert kernels(fake, Call(max_rows=17, total_rows=40), "append") == [(0, "append_many")]
     assert kernels(fake, Call(no_rotary=1, q=None, out=None, q_heads=0), "append") == [(0, "append_few")]
     assert kernels(fake, Call(total_rows=0, k_ptr=None), "append") == []
     assert kernels(fake, Call(), "read") == [(0, "read_kernel")]
