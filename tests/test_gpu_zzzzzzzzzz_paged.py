@@ -541,6 +541,39 @@ def test_captured_append_and_attend():
     assert torch.equal(*results)
 
 
+def test_calls_side_by_side_on_two_streams():
+    """Steps of two batches over one cache at once, prompts beside single tokens, appends to pages of their own among them."""
+    c = Content([900, 1400, 300], 2, 128, 64, "int8", capacity=[1200, 1500, 400])
+    cache = c.cache()
+    jobs = []
+    for i, (s, new) in enumerate(((0, 250), (1, 1))):
+        g = torch.Generator().manual_seed(i)
+        kv, q = torch.randn(new, 2, 128, generator=g).bfloat16().cuda(), torch.randn(new, 8, 128, generator=g).bfloat16().cuda()
+        jobs.append((batch_of(c.table[s:s + 1], [c.lengths[s]], [new]), kv, q, torch.cuda.Stream(), []))
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for batch, kv, q, stream, outs in jobs:
+            with torch.cuda.stream(stream):
+                cache.append(batch, kv, kv)
+                outs.append(cache.attend(batch, q, window=700, sinks=5))
+    torch.cuda.synchronize()
+    other = c.cache()
+    for batch, kv, q, _, outs in jobs:
+        other.append(batch, kv, kv)
+        want = other.attend(batch, q, window=700, sinks=5)
+        assert all(torch.equal(x, want) for x in outs)
+    assert cache.error_flags() == 0
+
+
+@pytest.mark.parametrize("dim,new", [(64, 7), (64, 8), (64, 9), (128, 4), (128, 5)])
+@pytest.mark.parametrize("dtype", ["int8", "fp8_e4m3"])
+def test_columns_around_the_border_between_the_kernels(dim, new, dtype):
+    """Four heads a group: 28, 32 and 36 columns, 16 and 20; with a sequence of one row beside."""
+    check_attention([300, 1000, 64], [new, 1, 2], (8, 2), (dtype, dim, 16))
+    check_attention([300, 1000, 64], [new, 1, 2], (8, 2), (dtype, dim, 64), window=50, sinks=3)
+    check_attention([777], [new], (4, 1), (dtype, dim, 32))
+
+
 def test_another_stream_than_the_current_default():
     c = Content([700], 2, 128, 64, "int8")
     cache, q = c.cache(), torch.randn(1, 8, 128).bfloat16().cuda()
