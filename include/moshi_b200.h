@@ -563,7 +563,7 @@ int64_t b200_dlm_algorithmic_flops(b200_dlm* h, int tokens, int context);
  * recorded in the cache's flags. */
 typedef struct {
   void *k_dev, *v_dev;                /* codes [pages][kv_heads][page_tokens][dim], int8 or e4m3 (B200_KV_*), 16-byte border */
-  float *k_scale_dev, *v_scale_dev;   /* [pages][kv_heads]: a code stands for code * scale */
+  float *k_scale_dev, *v_scale_dev;   /* [pages][kv_heads]: a code stands for code * scale; 2^-60 .. 2^58, or 0 and all codes 0 */
   int32_t* flags_dev;                 /* one word; B200_PAGED_* are ORed into it */
   int32_t pages, page_tokens;         /* page_tokens 16, 32, 64 or 128 */
   int32_t kv_heads, dim;              /* dim 64 or 128 */

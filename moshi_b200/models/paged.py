@@ -111,7 +111,7 @@ class PagedKVCache:
 
     @classmethod
     def from_tensors(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> "PagedKVCache":
-        """A cache in the caller's memory; scales of pages in use are 0 or within 2^-60 .. 2^58."""
+        """A cache in the caller's memory.  Scales of pages in use lie within 2^-60 .. 2^58; where one is 0, all codes of that page and head are 0."""
         self = cls.__new__(cls)
         self._take(k, v, k_scale, v_scale)
         return self
