@@ -166,7 +166,7 @@ def within(dtype, x, got, s):
 
 @pytest.mark.parametrize("form", FORMS, ids=str)
 @pytest.mark.parametrize("pairing,rot", [("adjacent", 1.0), ("halves", 1.0), ("halves", 0.5), ("adjacent", 0.25), (None, 0)])
-@pytest.mark.parametrize("new", [[1] * 6, [3, 0, 4, 2, 1, 1], [70, 1, 0, 129, 16, 5]], ids=str)
+@pytest.mark.parametrize("new", [[1] * 6, [3, 0, 4, 2, 1, 1], [16, 9, 0, 5, 13, 1], [17, 1, 2, 0, 3, 16], [70, 1, 0, 129, 16, 5]], ids=str)
 def test_append(form, pairing, rot, new):
     dtype, dim, page = form
     before, hkv, hq, T = [0, 17, 63, 64, 1000, 100000], 3, 6, sum(new) + 5
