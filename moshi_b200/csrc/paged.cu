@@ -188,7 +188,8 @@ __device__ void append_queries(const AppendP& p, int block) {
       const int s = sequence_of_row(p.b, r);
       if (s < p.b.S) {
         const Seq q = sequence(p.b, s, p.P);
-        if (q.ok && r >= q.r0) pos = q.before + r - q.r0;
+        if (has_row(q, r)) pos = q.before + (r - q.r0);
+        else if (lane == 0) flag(p.flags, B200_PAGED_BAD_BATCH);
       }
     }
     if (lane == 0) row_pos[i] = pos;
@@ -370,11 +371,11 @@ __global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadP p) {
   const int s = sequence_of_row(p.b, r);
   if (s >= p.b.S) return;
   const Seq q = sequence(p.b, s, p.P);
-  if (!q.ok || r < q.r0) {
-    if (!q.ok && lane == 0) flag(p.flags, B200_PAGED_BAD_BATCH);
+  if (!has_row(q, r)) {
+    if (lane == 0) flag(p.flags, B200_PAGED_BAD_BATCH);
     return;
   }
-  const int pos = q.before + r - q.r0, page = p.b.table[s * p.b.table_ld + pos / p.P], slot = pos % p.P;
+  const int pos = q.before + (r - q.r0), page = p.b.table[s * p.b.table_ld + pos / p.P], slot = pos % p.P;
   if (page < 0 || page >= p.pages) {
     if (lane == 0) flag(p.flags, B200_PAGED_BAD_PAGE);
     return;

@@ -32,12 +32,14 @@ __device__ __forceinline__ Seq sequence(const Batch& b, int s, int P) {
   q.n = r1 - q.r0;
   return q;
 }
-// The sequence that row r belongs to, S if there is none; the whole warp asks together (one load latency, where a binary search has seven for 128 sequences).
+// The sequence that row r belongs to, S if there is none; the whole warp asks together (one load latency, where a binary search has seven for 128 sequences).  Of rows that do not rise it may be one
+// that does not have row r: has_row says so, and a position is asked for behind it only, as that is what sequence() has bounded.
 __device__ __forceinline__ int sequence_of_row(const Batch& b, int r) {
   int s = 0;
   for (int i = threadIdx.x & 31; i - (int)(threadIdx.x & 31) < b.S; i += 32) s += __popc(__ballot_sync(0xffffffffu, i < b.S && b.rows[i + 1] <= r));
   return r < b.rows[0] ? b.S : s;
 }
+__device__ __forceinline__ bool has_row(const Seq& q, int r) { return q.ok && r >= q.r0 && r - q.r0 < q.n; }
 
 // ---- codes ----
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {

@@ -1,0 +1,49 @@
+"""Rare calls of the paged 8-bit cache on the GPU, against 64-bit restatements (oracle/paged.py)."""
+import pytest
+import torch
+
+from moshi_b200 import _lib
+from moshi_b200.models import PagedBatch, PagedKVCache, RotaryTable, paged
+from oracle import paged as oracle
+
+from .paged_util import Content, batch_of
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32).cuda()
+
+
+@pytest.mark.parametrize("rows", [[0, 5, 1, 2], [0, 2, 0, 0], [0, 0, 9, 3], [0, 14, 14, 3]], ids=str)
+@pytest.mark.parametrize("dtype", ["int8", "fp8_e4m3"])
+def test_rows_that_no_sequence_has_are_left_out(rows, dtype):
+    """Rows out of order, under which a row is counted to a sequence that does not have it.  Lengths end where the tables do, and the table is a slice of a larger one whose other entries name a page of
+    its own: it is not read, and queries, keys and values of such rows stay as they are."""
+    T, S, width, page, dim = 14, 3, 2, 16, 64
+    cache = PagedKVCache(8, 2, dim, page, dtype)
+    for pool, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        pool.view(torch.int8)[:6], scale[:6] = 8, 1.0
+        pool.view(torch.int8)[6], scale[6] = 64, 4.0     # int8: 256; e4m3: 8
+    wide = torch.full((S + 4, width + 3), 6, dtype=torch.int32, device="cuda")
+    wide[:S, :width] = torch.arange(S * width, device="cuda").view(S, width)
+    before = [width * page - max(b - a, 0) for a, b in zip(rows, rows[1:])]
+    before[2] = width * page - 1 if rows[3] - rows[2] == 1 else width * page
+    batch = PagedBatch(wide[:S, :width], i32(before), i32(rows), T)
+    seen = [0] * T                                       # of rows that exactly one well-formed sequence has and is counted to
+    for r in range(T):
+        s = sum(x <= r for x in rows[1:])
+        seen[r] = s < S and rows[s] <= r < rows[s + 1] and 0 <= rows[s] and rows[s + 1] <= T and before[s] + rows[s + 1] - rows[s] <= width * page
+    k, v = (torch.full((T, 2, dim), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    _lib.check(_lib.lib().b200_paged_read(cache._ref, batch._ref, k.data_ptr(), v.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    one = 8.0 if dtype == "int8" else 2.0 ** -6
+    for got in (k, v):
+        assert [float(x) for x in got.float().amax((1, 2))] == [one if ok else 7.0 for ok in seen]
+        assert torch.equal(got.float().amin((1, 2)), got.float().amax((1, 2)))
+    assert cache.error_flags() == paged.BAD_BATCH
+    cache.clear_error_flags()
+    x, q = (torch.randn(T, h, dim).bfloat16().cuda() for h in (2, 4))
+    q_out = torch.full_like(q, 7.0)
+    cache.append(batch, x, x, q=q, q_out=q_out, rotary=RotaryTable(dim))
+    assert [bool((y == 7).all()) for y in q_out] == [not ok for ok in seen] and cache.error_flags() == paged.BAD_BATCH
+    assert bool((cache.k.view(torch.int8)[6] == 64).all())
