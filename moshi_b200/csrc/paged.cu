@@ -95,15 +95,8 @@ __device__ __forceinline__ Page page_of(const AppendP& p, int item, bool tell) {
   const Seq q = sequence(p.b, s, p.P);
   Page g;
   g.ok = false; g.seq = s;
-  if (!q.ok) {
-    if (tell) flag(p.flags, B200_PAGED_BAD_BATCH);
-    return g;
-  }
-  const int nth = item - (q.r0 / p.P + 2 * s);          // of the sequence's pages; rows out of order could make it negative
-  if (nth < 0) {
-    if (tell) flag(p.flags, B200_PAGED_BAD_BATCH);
-    return g;
-  }
+  const int nth = item - (q.r0 / p.P + 2 * s);          // of the sequence's pages; negative for numbers in front of the first sequence's, and for some of rows out of order
+  if (!q.ok || nth < 0) return g;
   const int block = q.before / p.P + nth;
   const long long first = (long long)block * p.P;
   if (q.n == 0 || first >= (long long)q.before + q.n) return g;
@@ -189,7 +182,6 @@ __device__ void append_queries(const AppendP& p, int block) {
       if (s < p.b.S) {
         const Seq q = sequence(p.b, s, p.P);
         if (has_row(q, r)) pos = q.before + (r - q.r0);
-        else if (lane == 0) flag(p.flags, B200_PAGED_BAD_BATCH);
       }
     }
     if (lane == 0) row_pos[i] = pos;
@@ -229,6 +221,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_few_kernel(const Append
   pdl_trigger();
   pdl_wait();
   constexpr int CHUNKS = D / 16, RPS = 32 / CHUNKS;
+  if (blockIdx.x == gridDim.x - 1) { record_sequences(p.b, p.P, p.flags, blockDim.x); return; }
   if ((int)blockIdx.x >= p.page_ctas) { append_queries<D>(p, (int)blockIdx.x - p.page_ctas); return; }
   const int lane = threadIdx.x & 31, task = (int)blockIdx.x * (APPEND_THREADS / 32) + (threadIdx.x >> 5);
   if (task >= p.items * p.H * 2) return;
@@ -284,6 +277,7 @@ __global__ void __launch_bounds__(512) append_many_kernel(const AppendP p) {
   pdl_trigger();
   pdl_wait();
   constexpr int CHUNKS = D / 16;
+  if (blockIdx.x == gridDim.x - 1) { record_sequences(p.b, p.P, p.flags, blockDim.x); return; }
   if ((int)blockIdx.x >= p.page_ctas) { append_queries<D>(p, (int)blockIdx.x - p.page_ctas); return; }
   __shared__ float tops[2][16];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
@@ -366,15 +360,13 @@ template <int FMT, int D>
 __global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadP p) {
   pdl_trigger();
   pdl_wait();
+  if (blockIdx.x == gridDim.x - 1) { record_sequences(p.b, p.P, p.flags, blockDim.x); return; }
   const int lane = threadIdx.x & 31, task = (int)blockIdx.x * (READ_THREADS / 32) + (threadIdx.x >> 5), r = task >> 1, side = task & 1;
   if (r >= p.b.T) return;
   const int s = sequence_of_row(p.b, r);
   if (s >= p.b.S) return;
   const Seq q = sequence(p.b, s, p.P);
-  if (!has_row(q, r)) {
-    if (lane == 0) flag(p.flags, B200_PAGED_BAD_BATCH);
-    return;
-  }
+  if (!has_row(q, r)) return;
   const int pos = q.before + (r - q.r0), page = p.b.table[s * p.b.table_ld + pos / p.P], slot = pos % p.P;
   if (page < 0 || page >= p.pages) {
     if (lane == 0) flag(p.flags, B200_PAGED_BAD_PAGE);
@@ -571,9 +563,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
   const int key_row = token_of<D>(g), val_row[2] = {token_of<D>(2 * c), token_of<D>(2 * c + 1)};
   pdl_trigger();
   pdl_wait();
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < p.b.S; i += FEW_THREADS)
-      if (!sequence(p.b, i, p.P).ok) flag(p.flags, B200_PAGED_BAD_BATCH);
+  if (blockIdx.x == 0) record_sequences(p.b, p.P, p.flags, FEW_THREADS);
   const Run run = run_of(p);
   if (run.s < 0) return;
 
@@ -1156,7 +1146,7 @@ int launch_append(AppendP& p, cudaStream_t st) {
   const int slots = threads / (D / 16);
   p.q_rows = 1;
   while (p.q_rows < 8 && 2 * p.q_rows <= slots && (long long)p.b.T * p.Hq >= 148ll * 8 * slots * p.q_rows) p.q_rows *= 2;
-  const dim3 grid((unsigned)(p.page_ctas + (p.Hq ? ceil_div(p.b.T, p.q_rows) : 0)));
+  const dim3 grid((unsigned)(p.page_ctas + (p.Hq ? ceil_div(p.b.T, p.q_rows) : 0) + 1));       // the last one looks at the sequences
   if (few) return launch_early(append_few_kernel<FMT, D>, grid, dim3(threads), 0, st, p);
   return launch_early(append_many_kernel<FMT, D>, grid, dim3(threads), 0, st, p);
 }
@@ -1215,7 +1205,7 @@ int b200_paged_read(const b200_paged_cache* cache, const b200_paged_batch* batch
   p.k_codes = static_cast<const uint8_t*>(cache->k_dev); p.v_codes = static_cast<const uint8_t*>(cache->v_dev); p.k_scale = cache->k_scale_dev; p.v_scale = cache->v_scale_dev;
   p.flags = cache->flags_dev; p.b = batch_of(batch); p.k = static_cast<__nv_bfloat16*>(k_out_dev); p.v = static_cast<__nv_bfloat16*>(v_out_dev);
   p.pages = cache->pages; p.P = cache->page_tokens; p.H = cache->kv_heads;
-  const dim3 grid((unsigned)ceil_div(batch->total_rows, READ_THREADS / 64));
+  const dim3 grid((unsigned)ceil_div(batch->total_rows, READ_THREADS / 64) + 1);        // the last one looks at the sequences
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool i8 = cache->kv_dtype == B200_KV_INT8;
   if (D == 128) { if (i8) EARLY_LAUNCH((read_kernel<INT8, 128>), grid, READ_THREADS, 0, st, p); else EARLY_LAUNCH((read_kernel<E4M3, 128>), grid, READ_THREADS, 0, st, p); }

@@ -40,6 +40,11 @@ __device__ __forceinline__ int sequence_of_row(const Batch& b, int r) {
   return r < b.rows[0] ? b.S : s;
 }
 __device__ __forceinline__ bool has_row(const Seq& q, int r) { return q.ok && r >= q.r0 && r - q.r0 < q.n; }
+// One block of every call looks at all sequences: those that are left out are recorded, whether or not they have rows or pages that another block comes across.
+__device__ __forceinline__ void record_sequences(const Batch& b, int P, int32_t* flags, int threads) {
+  for (int s = threadIdx.x; s < b.S; s += threads)
+    if (!sequence(b, s, P).ok) atomicOr(flags, B200_PAGED_BAD_BATCH);
+}
 
 // ---- codes ----
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {

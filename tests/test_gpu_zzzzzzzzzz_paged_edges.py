@@ -47,3 +47,40 @@ def test_rows_that_no_sequence_has_are_left_out(rows, dtype):
     cache.append(batch, x, x, q=q, q_out=q_out, rotary=RotaryTable(dim))
     assert [bool((y == 7).all()) for y in q_out] == [not ok for ok in seen] and cache.error_flags() == paged.BAD_BATCH
     assert bool((cache.k.view(torch.int8)[6] == 64).all())
+
+
+@pytest.mark.parametrize("first", [1, 15, 16, 17, 40, 200])
+@pytest.mark.parametrize("new", [(1, 2), (30, 17)], ids=str)
+def test_any_number_of_rows_in_front_of_the_first_sequence(first, new):
+    """They belong to nobody, like those behind the last: left as they are, and nothing is recorded."""
+    c = Content([41, 52], 2, 128, 16, "int8", capacity=[41 + new[0], 52 + new[1]])
+    cache, other, n = c.cache(), c.cache(), sum(new)
+    x, q = torch.randn(first + n + 3, 2, 128).bfloat16().cuda(), torch.randn(first + n + 3, 4, 128).bfloat16().cuda()
+    batch = PagedBatch(c.table.cuda(), i32([41, 52]), i32([first, first + new[0], first + n]), first + n + 3, max(new))
+    rotary = RotaryTable(128)
+    turned = cache.append(batch, x, x, q=q, rotary=rotary, q_out=torch.full_like(q, 7.0))
+    out = cache.attend(batch, turned, out=torch.full_like(q, 7.0))
+    k, v = cache.read(batch)
+    assert cache.error_flags() == 0
+    for t in (turned, out):
+        assert bool((t[:first] == 7).all()) and bool((t[first + n:] == 7).all())
+    mine = slice(first, first + n)
+    batch = batch_of(c.table, [41, 52], new)
+    q2 = other.append(batch, x[mine].clone(), x[mine].clone(), q=q[mine].clone(), rotary=rotary)
+    k2, v2 = other.read(batch)
+    assert torch.equal(q2, turned[mine]) and torch.equal(other.attend(batch, q2), out[mine]) and torch.equal(k2, k[mine]) and torch.equal(v2, v[mine])
+    assert torch.equal(other.k, cache.k) and torch.equal(other.v, cache.v)
+
+
+@pytest.mark.parametrize("rows,before", [([0, 40, 0, 0], [0, 0, 0]), ([5, 0, 0, 0], [0, 0, 0]), ([0, 2, 2, 4], [0, -1, 0]), ([0, 2, 2, 4], [0, 65, 0]), ([0, 0, 0, 41], [0, 0, 24]),
+                                         ([0, 1, 2, 41], [0, 0, 0])], ids=str)
+def test_every_call_records_every_sequence_that_does_not_fit(rows, before):
+    """Also one without rows, or one that the others' rows hide."""
+    cache = PagedKVCache(12, 2, 64, 16, "int8")
+    x, q = torch.randn(41, 2, 64).bfloat16().cuda(), torch.randn(41, 4, 64).bfloat16().cuda()
+    batch = PagedBatch(torch.arange(12, dtype=torch.int32, device="cuda").view(3, 4), i32(before), i32(rows), 41, 40)
+    fits = rows in ([0, 1, 2, 41],)
+    for call in (lambda: cache.append(batch, x, x), lambda: cache.append(batch, x, x, q=q), lambda: cache.attend(batch, q), lambda: cache.read(batch)):
+        call()
+        assert cache.error_flags() == (0 if fits else paged.BAD_BATCH)
+        cache.clear_error_flags()
