@@ -560,6 +560,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
   if (lane < 4) tcp::mbar_init(bar + 8 * lane, 1);
   if (threadIdx.x == 0) quit = 0;
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __syncthreads();                           // no warp waits before `quit` has its first value
   const int key_row = token_of<D>(g), val_row[2] = {token_of<D>(2 * c), token_of<D>(2 * c + 1)};
   pdl_trigger();
   pdl_wait();
