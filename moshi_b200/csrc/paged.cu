@@ -629,8 +629,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
       const bool all = j + 15 <= w.pf && (p.window <= 0 || w.pl - j < p.window || j + 16 <= p.sinks);
       x.x = __int_as_float(all ? SEEN : IN_PART);
       x.y = p.k_scale[(long long)page * p.H + w.h];
-      float vs = p.v_scale[(long long)page * p.H + w.h];
-      vs = vs > 0.f ? vs : 1.f;              // all codes of a page of zeros are 0
+      const float vs = value_scale(p.v_scale[(long long)page * p.H + w.h]);
       x.z = __log2f(vs); x.w = __frcp_rn(vs);
     }
     meta[warp][(2 * i + lane) & 63] = x;

@@ -97,6 +97,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ float power_of_two_in(float x) { return __uint_as_float(max(__float_as_uint(x) & 0x7f800000u, (127u - 100u) << 23)); }
 
 // ---- attention ----
+// What a page's values count as in the exponent.  A page of zeros has the scale 0 and adds nothing to the sums but its share of the weights' total: it counts as the least scale, so that the running maximum,
+// which is of score + log2(scale), stays that of the pages that have something to add.
+__device__ __forceinline__ float value_scale(float s) { return s > 0.f ? s : SCALE_MIN; }
 struct AttnP {
   const uint8_t *k, *v;
   const float *k_scale, *v_scale;

@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       const bool keys = !(task & 4);
       if (keys) {                            // what the weights need to know of these keys' pages
         if (lane < 2) {
-          const float vs = scales.y > 0.f ? scales.y : 1.f;                   // all codes of a page of zeros are 0
+          const float vs = value_scale(scales.y);
           there[i % INFOS][2 * w4 + lane] = page >= 0 ? 1u : 0u;
           info[i % INFOS][2 * w4 + lane] = page >= 0 ? make_float4(scales.x > 0.f ? scales.x : 1.f, __log2f(vs), __frcp_rn(vs), 0.f) : make_float4(1.f, 0.f, 0.f, 0.f);
         }

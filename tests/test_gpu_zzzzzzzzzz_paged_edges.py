@@ -84,3 +84,34 @@ def test_every_call_records_every_sequence_that_does_not_fit(rows, before):
         call()
         assert cache.error_flags() == (0 if fits else paged.BAD_BATCH)
         cache.clear_error_flags()
+
+
+@pytest.mark.parametrize("new", [1, 140])
+@pytest.mark.parametrize("size", [1.0, 1e-6, 1e-9])
+@pytest.mark.parametrize("dtype,dim,page", [("int8", 128, 64), ("fp8_e4m3", 64, 16)])
+def test_pages_of_zero_values_beside_small_values(new, size, dtype, dim, page):
+    """A page whose values are all 0 (its scale is 0) has its share of the weights and takes no bits from the others', however small their scales are; nor does it where its keys have the largest scores."""
+    c = Content([300 + new], 2, dim, page, dtype)
+    cache = c.cache()
+    cache.v_scale.mul_(size)
+    c.scales[1] = cache.v_scale.cpu()
+    for block in (0, 2):
+        pg = int(c.table[0, block])
+        cache.v.view(torch.int8)[pg], cache.v_scale[pg], c.codes[1][pg], c.scales[1][pg] = 0, 0, 0, 0
+    for grow in (1.0, 3.0):                              # of the zeros' keys
+        pg = int(c.table[0, 2])
+        cache.k_scale[pg] *= grow
+        c.scales[0][pg] *= grow
+        q = torch.randn(new, 4, dim, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+        want, tol = oracle.attend(q.double().cpu(), *c.kvt(0), 300, dim ** -0.5)
+        off = (cache.attend(batch_of(c.table, [300], [new]), q).double().cpu() - want).abs()
+        assert bool((off <= tol).all()), float((off / tol).max())
+
+
+@pytest.mark.parametrize("new", [1, 140])
+def test_nothing_but_zero_values(new):
+    c = Content([300 + new], 2, 128, 64, "int8")
+    cache = c.cache()
+    cache.v.zero_(), cache.v_scale.zero_()
+    out = cache.attend(batch_of(c.table, [300], [new]), torch.randn(new, 4, 128).bfloat16().cuda())
+    assert bool((out == 0).all()) and cache.error_flags() == 0
