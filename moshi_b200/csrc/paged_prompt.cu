@@ -79,6 +79,16 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// magnitudes of eight bf16: the largest of the even ones and that of the odd ones
+__device__ __forceinline__ uint32_t largest8(const uint4& x) {
+  constexpr uint32_t M = 0x7fff7fffu;
+  return max2(max2(x.x & M, x.y & M), max2(x.z & M, x.w & M));
+}
 // bits 0 .. x of 32
 __device__ __forceinline__ uint32_t upto(int x) { return x < 0 ? 0u : x > 31 ? 0xffffffffu : 0xffffffffu >> (31 - x); }
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* quit) { return __all_sync(0xffffffffu, wait_or_quit(bar, parity, quit)); }
@@ -130,7 +140,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
   __shared__ __align__(16) uint32_t there[INFOS][8];
   __shared__ uint32_t tmem_at;
   __shared__ volatile int quit;
-  __shared__ float tops[SOFT_WARPS];
+  __shared__ float factors[ROWS];            // of a row: what turns a product of codes into a score in base 2, but for the keys' scale
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -285,12 +295,10 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-    // ---- queries: f16 after one power of two for all of them ----
+    // ---- queries: f16 after a power of two for each row, as rows and heads of very different size may lie side by side ----
     constexpr int PIECES = D / 8, MINE = 2 * 128 * PIECES / (SOFT_WARPS * 32);          // 16-byte pieces of a row, and of this thread
-    float power;
     {
       uint4 raw[MINE];
-      float top = 0.f;
       // the thread has piece c of every APART-th row from `at` on; token and head of a row by counting, not by division
       constexpr int APART = SOFT_WARPS * 32 / PIECES;
       const int c = threadIdx.x % PIECES, at = threadIdx.x / PIECES, step_i = APART / p.G, step_g = APART - step_i * p.G;
@@ -302,26 +310,32 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
         i += step_i; g += step_g;
         if (g >= p.G) { g -= p.G; ++i; }
       }
+      // magnitudes as 16-bit numbers, which order like the values; two rows a word, k and k + MINE / 2
+      uint32_t top[MINE / 2];
 #pragma unroll
-      for (int k = 0; k < MINE; ++k) {
-        const uint32_t v[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float a = fabsf(__uint_as_float(v[i] << 16)), b = fabsf(__uint_as_float(v[i] & 0xffff0000u));
-          if (a < INFINITY) top = fmaxf(top, a);
-          if (b < INFINITY) top = fmaxf(top, b);
-        }
+      for (int k = 0; k < MINE / 2; ++k) {
+        const uint32_t a = largest8(raw[k]), b = largest8(raw[k + MINE / 2]);
+        top[k] = max2(prmt(a, b, 0x5410u), prmt(a, b, 0x7632u));
       }
-      top = warp_max(top);
-      if (lane == 0) tops[warp] = top;
-      asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
+      // The lanes of a row have as many rows as they are: each step halves the rows that a lane answers for, until lane c has the c-th one's.
+      static_assert(MINE == PIECES, "a row's lanes share its rows out");
 #pragma unroll
-      for (int i = 0; i < SOFT_WARPS; ++i) top = fmaxf(top, tops[i]);
-      power = top > 0.f ? power_of_two_in(top) : 1.f;
-      const float up = 16384.f / power;
+      for (int h = MINE / 4; h > 0; h /= 2)
+#pragma unroll
+        for (int k = 0; k < h; ++k) {
+          const bool upper = lane & h;
+          const uint32_t theirs = __shfl_xor_sync(0xffffffffu, upper ? top[k] : top[k + h], h);
+          top[k] = max2(upper ? top[k + h] : top[k], theirs);
+        }
+      top[0] = max2(top[0], __shfl_xor_sync(0xffffffffu, top[0], MINE / 2));
+      const uint32_t largest = lane & MINE / 2 ? top[0] & 0xffff0000u : top[0] << 16;
+      const float power = largest ? power_of_two_in(__uint_as_float(largest)) : 1.f, up_mine = __uint_as_float((268u << 23) - __float_as_uint(power));      // 2^14 / power
+      factors[at + c * APART] = power * (1.f / 16384.f) * p.scale2;
+      asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");      // all rows' factors
 #pragma unroll
       for (int k = 0; k < MINE; ++k) {
         const int r = at + k * APART;
+        const float up = __shfl_sync(0xffffffffu, up_mine, k, PIECES);
         const uint32_t v[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
         uint32_t o[4];
 #pragma unroll
@@ -339,7 +353,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
     const int pos = has ? u.q.before + rr / p.G : -1, lo = p.window > 0 ? pos - p.window : -1;      // sees j <= pos, j > lo or j < sinks
     const int pf = u.q.before + (u.r0 + 128 * i) / p.G, pl = u.q.before + (u.r0 + min(128 * i + 128, u.rows) - 1) / p.G;      // of this tile of queries
     const uint32_t lanes = (uint32_t)(q4 * 32) << 16, ts = tmem + lanes, tp = tmem + lanes + 128 + 64 * i, to = tmem + lanes + 256 + 128 * i;
-    const float fac = p.scale2 * power * (1.f / 16384.f);
+    const float fac = factors[row];
     float m = -INFINITY, sum = 0.f;
     bool ok = true;
     for (int x = 0; x < n; ++x) {

@@ -115,3 +115,27 @@ def test_nothing_but_zero_values(new):
     cache.v.zero_(), cache.v_scale.zero_()
     out = cache.attend(batch_of(c.table, [300], [new]), torch.randn(new, 4, 128).bfloat16().cuda())
     assert bool((out == 0).all()) and cache.error_flags() == 0
+
+
+@pytest.mark.parametrize("new", [1, 140])
+@pytest.mark.parametrize("heads", [(8, 2), (6, 1)], ids=str)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_large_query_leaves_its_neighbours_alone(new, heads, dim):
+    """Rows and heads of very different size in one step: each has its own result, whatever lies beside it."""
+    c = Content([500 + new], heads[1], dim, 64, "int8")
+    cache, batch = c.cache(), batch_of(c.table, [500], [new])
+    q = torch.randn(new, heads[0], dim, generator=torch.Generator().manual_seed(2)).bfloat16()
+    want, tol = oracle.attend(q.double(), *c.kvt(0), 500, dim ** -0.5)
+    small, tol_small = oracle.attend(q[:, 0].double()[:, None] * 2.0 ** -30, *(x[:, :1] for x in c.kvt(0)), 500, dim ** -0.5 * 2.0 ** 30)
+    large = q.clone()
+    large[:, 1] *= 2.0 ** 40
+    large[new // 2, 3] *= 2.0 ** 100
+    got = cache.attend(batch, large.cuda()).double().cpu()
+    plain = torch.ones(new, heads[0], dtype=torch.bool)
+    plain[:, 1] = plain[new // 2, 3] = False
+    assert bool(((got - want).abs() <= tol)[plain].all())
+    assert bool(got.isfinite().all())
+    tiny = q.clone()
+    tiny[:, 0] *= 2.0 ** -30
+    got = cache.attend(batch, tiny.cuda(), scale=dim ** -0.5 * 2.0 ** 30).double().cpu()
+    assert bool(((got[:, :1] - small).abs() <= tol_small).all())
