@@ -329,8 +329,16 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
         }
       top[0] = max2(top[0], __shfl_xor_sync(0xffffffffu, top[0], MINE / 2));
       const uint32_t largest = lane & MINE / 2 ? top[0] & 0xffff0000u : top[0] << 16;
-      const float power = largest ? power_of_two_in(__uint_as_float(largest)) : 1.f, up_mine = __uint_as_float((268u << 23) - __float_as_uint(power));      // 2^14 / power
-      factors[at + c * APART] = power * (1.f / 16384.f) * p.scale2;
+      // A row that is not finite gets NaN, and no other: it asks as zeros, whose weights say whether it sees anything at all, and its factor tells the end of it.
+      const bool odd = largest >= 0x7f800000u;
+      const float power = largest ? power_of_two_in(__uint_as_float(largest)) : 1.f;
+      const float up_mine = __uint_as_float((268u << 23) - __float_as_uint(power));            // 2^14 / power
+      factors[at + c * APART] = odd ? NAN : power * (1.f / 16384.f) * p.scale2;
+      if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+        for (int k = 0; k < MINE; ++k)
+          if (__shfl_sync(0xffffffffu, odd, k, PIECES)) raw[k] = make_uint4(0, 0, 0, 0);
+      }
       asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");      // all rows' factors
 #pragma unroll
       for (int k = 0; k < MINE; ++k) {
@@ -382,7 +390,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
         }
 #pragma unroll
         for (int b = 2 * c; b < 2 * c + 2; ++b) {
-          by[b] = fmaxf(ip[b].x * fac, FLT_MIN);
+          by[b] = fmaxf(ip[b].x * fac, FLT_MIN);                              // also where fac is NaN
           lv[b] = ip[b].y;
           float mx[2] = {__uint_as_float(r[16 * b]), __uint_as_float(r[16 * b + 1])};
 #pragma unroll
@@ -457,6 +465,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
     }
     if (ok) {
       tc_fence_after();
+      if (sum != 0.f && isnan(factors[row])) sum = NAN;
       const float inv = sum != 0.f ? 1.f / sum : 0.f;
       if (p.nsplit > 1) {
         const long long at = (long long)blockIdx.x * ROWS + row;

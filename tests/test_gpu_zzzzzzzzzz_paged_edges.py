@@ -139,3 +139,22 @@ def test_a_large_query_leaves_its_neighbours_alone(new, heads, dim):
     tiny[:, 0] *= 2.0 ** -30
     got = cache.attend(batch, tiny.cuda(), scale=dim ** -0.5 * 2.0 ** 30).double().cpu()
     assert bool(((got[:, :1] - small).abs() <= tol_small).all())
+
+
+@pytest.mark.parametrize("new,before", [(1, 0), (1, 3000), (140, 0), (140, 3000)])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_queries_that_are_not_finite_give_nan_whatever_they_meet(new, before, value):
+    """Also where every product with a key is minus infinity: one key alone, or keys of one sign."""
+    c = Content([before + new], 2, 128, 64, "int8")
+    c.codes[0][..., 5] = -c.codes[0][..., 5].abs() - 1
+    cache, batch = c.cache(), batch_of(c.table, [before], [new])
+    q = torch.randn(new, 8, 128, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    want = cache.attend(batch, q)
+    spoilt = torch.zeros(new, 8, dtype=torch.bool, device="cuda")
+    for row, head in ((0, 2), (0, 7), (new // 2, 4), (new - 1, 0)):
+        q[row, head, 5] = value
+        spoilt[row, head] = True
+    got = cache.attend(batch, q)
+    assert bool(got[spoilt].isnan().all()) and torch.equal(got[~spoilt], want[~spoilt])
+    table = torch.full_like(c.table, -1)                 # a row that sees nothing gets zeros, whatever it asks
+    assert bool((cache.attend(batch_of(table, [before], [new]), q) == 0).all()) and cache.error_flags() == paged.BAD_PAGE
