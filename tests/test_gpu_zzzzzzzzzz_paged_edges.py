@@ -158,3 +158,24 @@ def test_queries_that_are_not_finite_give_nan_whatever_they_meet(new, before, va
     assert bool(got[spoilt].isnan().all()) and torch.equal(got[~spoilt], want[~spoilt])
     table = torch.full_like(c.table, -1)                 # a row that sees nothing gets zeros, whatever it asks
     assert bool((cache.attend(batch_of(table, [before], [new]), q) == 0).all()) and cache.error_flags() == paged.BAD_PAGE
+
+
+@pytest.mark.parametrize("new", [1, 140])
+@pytest.mark.parametrize("dtype", ["int8", "fp8_e4m3"])
+@pytest.mark.parametrize("power", [18, 20, 21, 22, 23])
+def test_scores_whose_last_bit_is_several_units(new, dtype, power):
+    """Scores of 2^(power + 6) and more in base 2, which climb by their last bit from 128 tokens to the next.  `scale` is what makes scale * log2(e) round to 1, so that all scores are exact in 32 bits."""
+    scale, dim, page = 0.6931471824645996, 64, 128
+    c = Content([1000 + new], 2, dim, page, dtype)
+    for b, pg in enumerate(c.table[0].tolist()):
+        c.scales[0][pg] = 2.0 ** power * (1 + b * 2.0 ** -23)
+    c.scales[1].fill_(1.0)
+    c.codes[0] = torch.zeros_like(c.codes[0])
+    c.codes[0][..., 0] = 64
+    q = torch.zeros(new, 4, dim)
+    q[..., 0] = 1.0
+    got = c.cache().attend(batch_of(c.table, [1000], [new]), q.bfloat16().cuda(), scale=scale).double().cpu()
+    k, v, top = c.kvt(0)
+    want, _ = oracle.attend(q.double(), k, v, top, 1000, scale)
+    # weights in f16 and the result's rounding; `scale` misses ln 2 by 2e-9 of it, and scores that count differ by 2^6 at most
+    assert bool(((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * v.abs().amax()).all()), float((got - want).abs().max())
