@@ -413,9 +413,9 @@ __global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadP p) {
 // cache bytes.  Which dimension of K is which k of the product is free as long as Q has the same order, and so is which dimension of V is which row of O^T, and which token is which row of S^T and
 // k of the other product: a lane reads its fragments as 16 neighbouring codes.  P^T comes out of S^T by movmatrix.
 //
-// Codes of both types are exact in f16, and so are bf16 queries after a power of two per column; P is f16 in (0, 2^8], off by 2^-11 of itself.  The scale of a page's keys multiplies the
-// scores; that of its values goes into the exponent, P = 2^(score + log2 s_v - M), with M the running maximum of the same, and the sum of the weights takes P / s_v: nothing is
-// rounded on the way but P.  M follows only when a score passes it by 2^8, as then no column has to be compared across lanes for most tiles.
+// Codes of both types are exact in f16, and so are bf16 queries after a power of two per column; the scale of a page's keys multiplies the
+// scores; that of its values goes into the exponent, P = 2^(score + log2 s_v - M), with M behind the running maximum of the same, and the sum of the weights takes P / s_v: nothing is
+// rounded on the way but P, which is f16.  M follows only when a score passes it by 2^15, as then no column has to be compared across lanes for most tiles.
 //
 // Bounds: HBM for large batches (48 sessions of 3000 tokens, 32 heads, e4m3: 185 us, 6.4 TB/s); for many short units what a unit costs beside its tiles (128 sessions under a window of 1024, 8 heads: 72 us, floor 36;
 // a part's first copies, its queries and the joining of its warps are 7400 clocks beside 20000 for eight tiles a warp).
@@ -429,7 +429,6 @@ constexpr int FEW_WARPS = 4, FEW_THREADS = FEW_WARPS * 32;
 constexpr int FEW_PER_SM = 2;                // CTAs
 constexpr int DIRECT_TILES = 64;             // units of more tiles are always cut
 constexpr int MIN_RUN = 8;                    // tiles of a CTA
-constexpr float SLACK = 8.f;
 
 __device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -808,7 +807,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
             y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
             y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
             y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
-            const float now = fmaxf(m[nt][e], y), by = now == -INFINITY ? 1.f : exp2_fast(m[nt][e] - now);
+            const float now = fmaxf(m[nt][e], y - UNDER), by = now == -INFINITY ? 1.f : exp2_fast(m[nt][e] - now);
             m[nt][e] = now;
             l[nt][e] *= by;
 #pragma unroll

@@ -100,6 +100,9 @@ __device__ __forceinline__ float power_of_two_in(float x) { return __uint_as_flo
 // What a page's values count as in the exponent.  A page of zeros has the scale 0 and adds nothing to the sums but its share of the weights' total: it counts as the least scale, so that the running maximum,
 // which is of score + log2(scale), stays that of the pages that have something to add.
 __device__ __forceinline__ float value_scale(float s) { return s > 0.f ? s : SCALE_MIN; }
+// Weights are P = 2^(score + log2(value scale) - M) in f16, whose numbers go from 2^-24 to 65504.  M is set 2^UNDER below the largest exponent and follows when one passes it by 2^SLACK: P reaches 2^15, and
+// a weight (times its value's scale) is off by 2^-11 of itself or, under 2^-21 of the largest one, by 2^-32 of that.
+constexpr float UNDER = 7.f, SLACK = 15.f;
 struct AttnP {
   const uint8_t *k, *v;
   const float *k_scale, *v_scale;

@@ -5,7 +5,7 @@
 // tcgen05.mma with fp32 accumulators in TMEM (one place for the scores, O_0, O_1); warps 0..3 and 4..7 hold a row per thread, with all its 128 scores, and put P as f16 into TMEM,
 // from where the second product reads it.  As soon as one tile's scores are in registers their place takes the other's.
 //
-// Scales as in paged.cu: that of a page's keys multiplies its 16 or more columns' scores, that of its values goes into the exponent.  O is rescaled only when a row's maximum grew by more than 2^8.
+// Scales as in paged.cu: that of a page's keys multiplies its 16 or more columns' scores, that of its values goes into the exponent.  O is rescaled only when a weight would pass 2^15.
 //
 // Bounds: the chain of a tile through its weight warps; the tensor pipe and the exponentials' unit are each active half the time (2048 rows on 6100 tokens, 32 heads on 8: 280 us, 0.86 PFLOP/s; a
 // window of 1024 over 6000 rows of 16 heads on 4: 104 us).  A row's scores are read from TMEM once, and stay in 184 registers that setmaxnreg takes from the other warps
@@ -23,7 +23,6 @@ using namespace tcp;
 typedef __nv_bfloat16 bf16;
 
 constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 7, THREADS = (SOFT_WARPS + CONVERT_WARPS + 1) * 32, ROWS = 256, KEYS = 128, INFOS = 8;
-constexpr float SLACK = 8.f;
 
 template <int D>
 struct Smem {
@@ -409,8 +408,8 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
         tc_fence_after();
       }
       if (__any_sync(0xffffffffu, grow)) {
-        const float factor = grow ? exp2_fast(m - t) : 1.f;
-        if (grow) { m = t; sum *= factor; }
+        const float now = t - UNDER, factor = grow ? exp2_fast(m - now) : 1.f;
+        if (grow) { m = now; sum *= factor; }
         if (x > 0) {
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {

@@ -56,8 +56,8 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, top: torch.Tensor,
     result, and how far from it 32-bit scores and sums with weights in f16, rounded to bf16 at the end, may be:
     half a step of the result; on the weights' side half a step of f16 (2^-11) and twice the scores' error (a softmax weight moves by it, and so does their sum), with 2^-18 of
     the largest sum of |q k| and 2^-18 for the exponential, each many times what 32-bit sums of 128 terms are off by; and what f16 drops of small weights.  The weight of token j is held as
-    p_j s_j / M, s_j its scale, M at most the largest p_j s_j: off by 2^-25 at most where f16 has its least step of 2^-24.  It multiplies codes of up to top_j / s_j, so all of them
-    together are off by 2^-25 * tokens * M * (largest code) <= 2^-25 * tokens * max(p_j top_j)."""
+    p_j s_j / M, s_j its scale, M at most 2^-7 of the largest p_j s_j: off by 2^-25 at most where f16 has its least step of 2^-24.  It multiplies codes of up to top_j / s_j, so all of them
+    together are off by 2^-25 * tokens * M * (largest code) <= 2^-32 * tokens * max(p_j top_j)."""
     rows, heads, _ = q.shape
     out, tol = torch.zeros_like(q), torch.zeros_like(q)
     seen = visible(torch.arange(first, first + rows), k.shape[0], window, sinks)
@@ -68,6 +68,6 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, top: torch.Tensor,
         w = torch.nan_to_num((s - s.amax(1, keepdim=True)).exp())
         w = w / w.sum(1, keepdim=True).clamp_min(1e-300)
         out[:, h] = w @ vh
-        dropped = 2.0 ** -25 * k.shape[0] * (w * top[:, h * v.shape[1] // heads]).amax(1, keepdim=True)
+        dropped = 2.0 ** -32 * k.shape[0] * (w * top[:, h * v.shape[1] // heads]).amax(1, keepdim=True)
         tol[:, h] = 2.0 ** -8 * out[:, h].abs() + (2.0 ** -11 + 2.0 ** -17 * (1 + size)) * (w @ vh.abs()) + dropped
     return out, tol

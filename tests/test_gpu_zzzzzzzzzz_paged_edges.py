@@ -179,3 +179,27 @@ def test_scores_whose_last_bit_is_several_units(new, dtype, power):
     want, _ = oracle.attend(q.double(), k, v, top, 1000, scale)
     # weights in f16 and the result's rounding; `scale` misses ln 2 by 2e-9 of it, and scores that count differ by 2^6 at most
     assert bool(((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * v.abs().amax()).all()), float((got - want).abs().max())
+
+
+@pytest.mark.parametrize("new", [1, 20, 140])
+@pytest.mark.parametrize("before,far", [(200, 0), (200, 100), (3000, 0), (3000, 2990)])
+@pytest.mark.parametrize("dtype,dim", [("int8", 128), ("fp8_e4m3", 64)])
+def test_weights_far_under_the_largest(new, before, far, dtype, dim):
+    """One token has nearly all of the weight and a value of 0, the others 2^-26 of it each: what they add is the result."""
+    c = Content([before + new], 2, dim, 64, dtype)
+    page, slot = int(c.table[0, far // 64]), far % 64
+    top = oracle.Q_MAX[dtype]
+    c.codes[0][..., 0] = 0
+    c.codes[0][page, :, slot], c.codes[0][page, :, slot, 0] = 0, top
+    c.codes[1] = c.codes[1].abs()
+    c.codes[1][page, :, slot] = 0
+    c.scales[0].fill_(1 / top), c.scales[1].fill_(1 / top)
+    q = torch.randn(new, 4, dim, generator=torch.Generator().manual_seed(2))
+    q[..., 0] = 26 * 0.6931 * dim ** 0.5
+    q = q.bfloat16()
+    k, v, most = c.kvt(0)
+    scale = dim ** -0.5
+    want, tol = oracle.attend(q.double(), k, v, most, before, scale)
+    off = (c.cache().attend(batch_of(c.table, [before], [new]), q.cuda()).double().cpu() - want).abs()
+    assert float((tol / want.clamp_min(1e-30)).median()) < 0.2
+    assert bool((off <= tol).all()), (float((off / tol).max()), float((off / want.clamp_min(1e-30)).max()))
