@@ -796,7 +796,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           top[nt][e] = fmaxf(fmaxf(sc[0][nt][e], sc[0][nt][e + 2]), fmaxf(sc[1][nt][e], sc[1][nt][e + 2]));
-          grow |= top[nt][e] - m[nt][e] > SLACK;     // the difference, as it is exact: above 2^27 the sum may round to the score itself
+          grow |= top[nt][e] > __fadd_rd(m[nt][e], SLACK);      // rounded down: above 2^27 the sum would else round to the score itself, and its weight to infinity
         }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll

@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(s_taken + 8 * i);
-      const bool grow = t - m > SLACK;       // the difference, as it is exact: above 2^27 the sum may round to the score itself
+      const bool grow = t > __fadd_rd(m, SLACK);       // rounded down: above 2^27 the sum would else round to the score itself, and its weight to infinity
       if (x > 0) {                           // the sum over the keys in front has read its weights and settled in O
         ok = wait_or_quit(o_done + 8 * i, (uint32_t)(x - 1) & 1u, &quit);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
