@@ -211,8 +211,10 @@ class PagedKVCache:
         return k, v
 
     def error_flags(self) -> int:
-        """What the kernels found wrong since the last ``clear_error_flags`` (waits for the device): BAD_BATCH, BAD_PAGE, NOT_FINITE, WAIT."""
+        """What the kernels found wrong since the last ``clear_error_flags``: BAD_BATCH, BAD_PAGE, NOT_FINITE, WAIT.  Waits for all streams of the device."""
+        torch.cuda.synchronize(self.device)
         return int(self.flags.item())
 
     def clear_error_flags(self) -> None:
+        """Behind what the current stream has been given, and before what it is given next."""
         self.flags.zero_()

@@ -203,3 +203,21 @@ def test_weights_far_under_the_largest(new, before, far, dtype, dim):
     off = (c.cache().attend(batch_of(c.table, [before], [new]), q.cuda()).double().cpu() - want).abs()
     assert float((tol / want.clamp_min(1e-30)).median()) < 0.2
     assert bool((off <= tol).all()), (float((off / tol).max()), float((off / want.clamp_min(1e-30)).max()))
+
+
+def test_error_flags_wait_for_every_stream():
+    """What a kernel records on another stream than the current one counts, however late it comes."""
+    cache = PagedKVCache(4, 2, 64, 16, "int8")
+    x = torch.zeros(1, 2, 64, dtype=torch.bfloat16, device="cuda")
+    batch = batch_of(torch.zeros(1, 2, dtype=torch.int32), [-1], [1])
+    cache.append(batch, x, x)                            # the kernel is loaded
+    assert cache.error_flags() == paged.BAD_BATCH
+    cache.clear_error_flags()
+    assert cache.error_flags() == 0
+    torch.cuda._sleep(1000)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(400_000_000)                   # 0.2 s
+        cache.append(batch, x, x)
+    assert cache.error_flags() == paged.BAD_BATCH
