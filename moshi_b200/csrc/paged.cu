@@ -128,7 +128,8 @@ __device__ __forceinline__ float scale_for(float top, int older, float s_old, in
 }
 template <int FMT>
 __device__ __forceinline__ void store16(uint8_t* row, const Chunk& c, const float* x, float scale) {
-  // x / scale, rounded like a division: a product with the reciprocal, and what it left over once more.  (Scales lie between 2^-60 and 2^58 and |x| <= 2^64: nothing over- or underflows.)
+  // x / scale, rounded like a division, by Markstein's correction (IBM Journal of Research and Development 34, 1990): a product with the rounded reciprocal, and what it left over, exact in an FMA, once more.
+  // (Scales lie between 2^-60 and 2^58 and |x| <= 2^64: nothing overflows, and what underflows is 0 as a code.)
   const float div = scale > 0.f ? scale : 1.f, inv = 1.f / div;
   float y[16];
 #pragma unroll

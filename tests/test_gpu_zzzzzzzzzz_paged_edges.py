@@ -221,3 +221,31 @@ def test_error_flags_wait_for_every_stream():
         torch.cuda._sleep(400_000_000)                   # 0.2 s
         cache.append(batch, x, x)
     assert cache.error_flags() == paged.BAD_BATCH
+
+
+@pytest.mark.parametrize("dtype", ["int8", "fp8_e4m3"])
+@pytest.mark.parametrize("new", [15, 24])
+def test_codes_are_those_of_a_division(dtype, new):
+    """x / scale in 32 bits, rounded once, and that to the nearest code: over all scales, values that end up between two codes among them."""
+    page, dim, pages, heads = 32, 128, 238, 2
+    top = oracle.Q_MAX[dtype]
+    g = torch.Generator().manual_seed(4)
+    cache = PagedKVCache(pages, heads, dim, page, dtype)
+    # a page holds one row already, under a scale of any size from 2^-60 to 2^58
+    scale = torch.ldexp(1 + torch.rand(pages, heads, generator=g) * (torch.arange(pages) % 2)[:, None], torch.arange(pages).div(2, rounding_mode="floor")[:, None] - 60).clamp_max(2.0 ** 58).float()
+    cache.v_scale.copy_(scale), cache.k_scale.copy_(scale)
+    y = (torch.rand(pages, new, heads, dim, generator=g) * 2 - 1) * top
+    y[:, ::3] = y[:, ::3].round() + 0.5
+    if dtype == "fp8_e4m3":
+        y[:, 1::3] *= torch.exp2(-12 * torch.rand(pages, (new + 1) // 3, heads, 1, generator=g))[:, :y[:, 1::3].shape[1]]
+    x = (y.clamp(-0.99 * top, 0.99 * top) * scale[:, None, :, None]).bfloat16()
+    x = torch.where(x.float().abs() <= top * scale[:, None, :, None], x, torch.zeros_like(x)).clamp(-2.0 ** 64, 2.0 ** 64)
+    batch = batch_of(torch.arange(pages, dtype=torch.int32)[:, None], [1] * pages, [new] * pages)
+    cache.append(batch, *(x.flatten(0, 1).cuda() for _ in range(2)))
+    assert cache.error_flags() == 0
+    for pool, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        assert torch.equal(s.cpu(), scale)
+        quotient = (x.float() / scale[:, None, :, None]).transpose(1, 2)
+        want = quotient.round() if dtype == "int8" else quotient.to(torch.float8_e4m3fn).float()
+        got = pool[:, :, 1:1 + new].float().cpu()
+        assert torch.equal(got, want), (got - want).abs().max()
