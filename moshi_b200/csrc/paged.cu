@@ -8,8 +8,6 @@
 // same sign: 0.1 % a token never changes a code, and after 64 tokens the largest are 8 steps off.)  For e4m3 halving is exact but for subnormals.
 #include "paged.cuh"
 
-#include "tc_prims.cuh"
-
 namespace b200 {
 namespace paged {
 
@@ -87,14 +85,14 @@ __device__ __forceinline__ void rotate16(float* x, const Turn& t, int halves) {
 
 // Which sequence and page the step's touched page number `item` is.  They are numbered without a pass over the sequences: sequence s has the numbers from rows[s] / P + 2 s on, and n rows
 // from any place in a page on touch at most n / P + 2 pages.  The whole warp asks together.
-struct Page { int seq, first, page, o, e, r; bool ok; };      // position of its first slot; slots o .. e - 1 are the step's, from batch row r on
+struct Page { int first, page, o, e, r; bool ok; };      // position of its first slot; slots o .. e - 1 are the step's, from batch row r on
 __device__ __forceinline__ Page page_of(const AppendP& p, int item, bool tell) {
   const int lane = threadIdx.x & 31;
   int s = 0;                                            // the last sequence whose numbers begin at or in front of `item`
   for (int i = lane + 1; i - lane - 1 < p.b.S - 1; i += 32) s += __popc(__ballot_sync(0xffffffffu, i < p.b.S && (long long)p.b.rows[i] / p.P + 2ll * i <= item));
   const Seq q = sequence(p.b, s, p.P);
   Page g;
-  g.ok = false; g.seq = s;
+  g.ok = false;
   const int nth = item - (q.r0 / p.P + 2 * s);          // of the sequence's pages; negative for numbers in front of the first sequence's, and for some of rows out of order
   if (!q.ok || nth < 0) return g;
   const int block = q.before / p.P + nth;
@@ -460,9 +458,9 @@ __device__ __forceinline__ void store_row(const AttnP& p, const Seq& q, int h, i
 }
 
 // ---- the flattened work ----
-// The tiles of all units (sequence, column tile, kv head) one behind the other are cut into equal runs, one per CTA: lengths of a batch may differ as they like.  A unit that lies in several runs
+// The tiles of all units (sequence, kv head) one behind the other are cut into equal runs, one per CTA: lengths of a batch may differ as they like.  A unit that lies in several runs
 // is joined by join_kernel; a run has at most two parts of such units, one that the run begins inside of and one that it ends inside of.
-__device__ __forceinline__ int units_of(const AttnP& p, const Seq& q) { return !q.ok || q.n == 0 || q.n >= p.from_rows ? 0 : p.H * ((q.n * p.G + p.cols - 1) / p.cols); }
+__device__ __forceinline__ int units_of(const AttnP& p, const Seq& q) { return !q.ok || q.n == 0 || q.n >= p.from_rows ? 0 : p.H; }
 // What joining the warps, the first loads and the queries cost a unit, in tiles: a run of many short units is shorter.
 constexpr int UNIT_COST = 12;
 __device__ __forceinline__ int tiles_of(const AttnP& p, const Seq& q) { return Tiles<5>(q.before, q.before + q.n - 1, p.window, p.sinks).n; }
@@ -475,7 +473,7 @@ struct Run { long long from, to, base; int s; };      // this CTA's tiles; the s
 // by all threads of the block
 __device__ __forceinline__ Run run_of(const AttnP& p) {
   if (p.direct) {                            // a CTA a unit
-    const int per = p.H * p.ctiles, s = (int)blockIdx.x / per, u = (int)blockIdx.x - s * per;
+    const int s = (int)blockIdx.x / p.H, u = (int)blockIdx.x - s * p.H;
     const Seq q = sequence(p.b, s, p.P);
     Run r;
     r.s = u < units_of(p, q) ? s : -1; r.base = 0;
@@ -571,7 +569,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
   // A part of a unit: its places of u0 .. u1 - 1 are the run's, of which the first UNIT_COST are no tiles.
   struct Part {
     Seq q;
-    int s, h, ct, u0, u1, n_pos, pf, pl, first, count, used;                  // this warp's tiles; used: how many went through its ring before
+    int s, h, u0, u1, n_pos, pf, pl, first, count, used;                  // this warp's tiles; used: how many went through its ring before
     Tiles<5> tiles;
   };
   long long f = run.from, base = run.base;
@@ -586,13 +584,12 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
       n_at = units_at ? tiles_of(p, q_at) + UNIT_COST : 1;
     }
     const long long at = f - base;
-    const int unit = at < 0x7fffffffll ? (int)((uint32_t)at / (uint32_t)n_at) : (int)(at / n_at);
-    const int u0 = (int)(at - (long long)unit * n_at), u1 = (int)min((long long)n_at, u0 + (run.to - f));
+    const int h = at < 0x7fffffffll ? (int)((uint32_t)at / (uint32_t)n_at) : (int)(at / n_at);
+    const int u0 = (int)(at - (long long)h * n_at), u1 = (int)min((long long)n_at, u0 + (run.to - f));
     f += u1 - u0;
-    const int h = unit % p.H, ct = unit / p.H, n_cols = q_at.n * p.G;
-    const int pf = q_at.before + ct * COLS / p.G, pl = q_at.before + (min(ct * COLS + COLS, n_cols) - 1) / p.G;
-    Part w{q_at, s_at, h, ct, u0, u1, n_at, pf, pl, 0, 0, used, Tiles<5>(pf, pl, p.window, p.sinks)};
-    const int t0 = min(max(u0 - UNIT_COST, 0), w.tiles.n), t1 = min(max(u1 - UNIT_COST, 0), w.tiles.n);       // a column tile may see fewer keys than its sequence
+    const int pf = q_at.before, pl = q_at.before + q_at.n - 1;
+    Part w{q_at, s_at, h, u0, u1, n_at, pf, pl, 0, 0, used, Tiles<5>(pf, pl, p.window, p.sinks)};
+    const int t0 = max(u0 - UNIT_COST, 0), t1 = max(u1 - UNIT_COST, 0);
     w.first = t0 + warp;
     w.count = w.first < t1 ? (t1 - w.first + FEW_WARPS - 1) / FEW_WARPS : 0;
     return w;
@@ -648,7 +645,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
   };
   uint32_t raw[KS][2];                       // eight columns' queries of the part to come, as they are in memory
   auto load_queries = [&](const Part& w, int nt) {
-    const int col = w.ct * COLS + nt * 8 + g;
+    const int col = nt * 8 + g;
     const bool has = col < w.q.n * p.G;
     const int i = has ? col / p.G : 0;
     const bf16* row = p.q + (long long)(w.q.r0 + i) * p.q_ld + (long long)(w.h * p.G + (has ? col - i * p.G : 0)) * D;
@@ -684,7 +681,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
   start(w);
   for (;;) {
     const Seq q = w.q;
-    const int h = w.h, c0 = w.ct * COLS, n_cols = q.n * p.G, pf = w.pf, pl = w.pl, first = w.first, count = w.count, used = w.used;
+    const int h = w.h, n_cols = q.n * p.G, pf = w.pf, pl = w.pl, first = w.first, count = w.count, used = w.used;
     const Tiles<5> tiles = w.tiles;
 
     // queries: lane (g, c) has of column 8 nt + g the dimensions 64 i + 16 c .. + 15
@@ -720,7 +717,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         fac[nt][e] = __shfl_sync(0xffffffffu, back, (2 * c + e) * 4) * p.scale2;
-        const int cc = c0 + nt * 8 + 2 * c + e;
+        const int cc = nt * 8 + 2 * c + e;
         pos[nt][e] = cc < n_cols ? q.before + cc / p.G : -1;
       }
     }
@@ -911,11 +908,11 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
     const int slot = 2 * (int)blockIdx.x + (now.u0 == 0 ? 1 : 0);
     if (!p.direct && now.u0 == 0 && threadIdx.x == 0) {                       // where the unit's parts are: this run's and so many after it
       const long long runs = run.to - run.from, left = now.n_pos - now.u1;
-      p.parts[((long long)now.s * p.ctiles + now.ct) * p.H + now.h] = make_int2((int)blockIdx.x, alone ? 0 : (int)((left + runs - 1) / runs));
+      p.parts[(long long)now.s * p.H + now.h] = make_int2((int)blockIdx.x, alone ? 0 : (int)((left + runs - 1) / runs));
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      if (c0 + nt * 8 >= n_cols) break;
+      if (nt * 8 >= n_cols) break;
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -934,7 +931,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
       const int d0 = (threadIdx.x & 15) * PER;
 #pragma unroll
       for (int col = threadIdx.x >> 4; col < 8; col += FEW_THREADS / 16) {
-        const int cc = c0 + nt * 8 + col;
+        const int cc = nt * 8 + col;
         if (cc >= n_cols) break;
         float top = -INFINITY, sum = 0.f, acc[PER];
 #pragma unroll
@@ -974,9 +971,9 @@ __global__ void __launch_bounds__(128) join_kernel(const AttnP p) {
   constexpr int COLS = 8 * NT, PER = D / 16;
   __shared__ float o_s[8][D + 4], m_s[8], l_s[8];
   const int most = min(COLS, p.b.max_rows * p.G);       // columns of a unit
-  const int col = (int)(blockIdx.x % most), team = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * PER;
+  const int cc = (int)(blockIdx.x % most), team = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * PER;
   const long long unit = blockIdx.x / most;
-  const int h = (int)(unit % p.H), ct = (int)(unit / p.H % p.ctiles), s = (int)(unit / p.H / p.ctiles), cc = ct * COLS + col;
+  const int h = (int)(unit % p.H), s = (int)(unit / p.H);
   const Seq q = sequence(p.b, s, p.P);
   if (units_of(p, q) == 0 || cc >= q.n * p.G) return;
   const int2 parts = p.parts[unit];
@@ -988,7 +985,7 @@ __global__ void __launch_bounds__(128) join_kernel(const AttnP p) {
   for (int e = 0; e < PER; ++e) acc[e] = 0.f;
 #pragma unroll 2
   for (int i = team; i <= parts.y; i += 8) {
-    const long long at = (long long)(2 * (parts.x + i) + (i == 0 ? 1 : 0)) * COLS + col;
+    const long long at = (long long)(2 * (parts.x + i) + (i == 0 ? 1 : 0)) * COLS + cc;
     const float2 y = ml[at];
     const float now = fmaxf(top, y.x), keep = now == -INFINITY ? 0.f : exp2_fast(top - now), by = now == -INFINITY ? 0.f : exp2_fast(y.x - now);
     const float4* o = reinterpret_cast<const float4*>(p.part_o + at * D + d0);
@@ -1057,13 +1054,12 @@ int shift_of(int P) { return P == 16 ? 4 : P == 32 ? 5 : P == 64 ? 6 : 7; }
 // of 48 136 / 70; one request of 24 columns 34 / 19; 64 of 32 246 / 253, of 64 460 / 254.  24 heads of 64 on 4, 16 requests of 1000 to 6000 tokens and 30 columns: 29 / 48.)
 constexpr int few_cols(int dim) { return dim == 64 ? 32 : 16; }
 // CTAs of 8 * nt columns, a wave of them, fewer where the tables allow for less work than that.
-struct FewPlan { int nt, ctiles, ctas; long long units; bool direct; };
+struct FewPlan { int nt, ctas; long long units; bool direct; };
 FewPlan few_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks, int few_rows) {
   FewPlan f;
   const long long rows = few_rows <= b->max_rows ? few_rows - 1 : b->max_rows, cols = rows * G;
   f.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
-  f.ctiles = (int)ceil_div64(cols, 8 * f.nt);
-  f.units = (long long)b->sequences * c->kv_heads * f.ctiles;
+  f.units = (long long)b->sequences * c->kv_heads;       // few_cols, and so all rows of a sequence that come here, fit into one
   long long keys = (long long)b->table_width * c->page_tokens;
   if (window > 0 && (long long)window + sinks + rows < keys) keys = (long long)window + sinks + rows;
   const long long tiles = ceil_div64(keys, 32) + 1, runs = ceil_div64(f.units * (tiles + 4), MIN_RUN), wave = 148 * FEW_PER_SM;
@@ -1077,9 +1073,8 @@ FewPlan few_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, in
 // sums and (maximum, sum of the weights) of two parts per CTA, and where each unit's parts are
 int64_t few_bytes(const FewPlan& f, int D) { return f.direct ? 0 : (int64_t)f.ctas * 2 * 8 * f.nt * (D + 2) * 4 + f.units * 8; }
 
-}  // namespace
-
-int code_map(CUtensorMap* m, const void* codes, long long rows, int dim, int box_rows) {
+// A tensor map over a cache's codes, [rows][dim], boxes of 16 whole rows, swizzled by 128 bytes (dim 64: by 64).
+int code_map(CUtensorMap* m, const void* codes, long long rows, int dim) {
   static const EncodeFn fn = [] {
     void* f = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -1088,14 +1083,12 @@ int code_map(CUtensorMap* m, const void* codes, long long rows, int dim, int box
   }();
   if (!fn) B200_FAIL(B200_ERR_CUDA, "cuTensorMapEncodeTiled not available");
   cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)dim};
-  cuuint32_t box[2] = {(cuuint32_t)dim, (cuuint32_t)box_rows}, est[2] = {1, 1};
+  cuuint32_t box[2] = {(cuuint32_t)dim, 16}, est[2] = {1, 1};
   const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, est, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) B200_FAIL(B200_ERR_CUDA, "paged cache: tensor map of %lld rows of %d codes refused (%d)", rows, dim, (int)r);
   return B200_OK;
 }
-
-namespace {
 
 struct Route { int from_rows; FewPlan few; PromptPlan prompt; int64_t few_bytes, prompt_bytes; };
 Route route(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks) {
@@ -1113,8 +1106,8 @@ int launch_few(const AttnP& p, const FewPlan& f, cudaStream_t st) {
   constexpr int ring = FEW_WARPS * 4 * 32 * D, sums = FEW_WARPS * 8 * (D + 4) * 4, smem = ring + sums + 1024;
   static std::atomic<uint64_t> limits{0};
   CUtensorMap map_k, map_v;
-  B200_TRY(code_map(&map_k, p.k, (long long)p.pages * p.H * p.P, D, 16));
-  B200_TRY(code_map(&map_v, p.v, (long long)p.pages * p.H * p.P, D, 16));
+  B200_TRY(code_map(&map_k, p.k, (long long)p.pages * p.H * p.P, D));
+  B200_TRY(code_map(&map_v, p.v, (long long)p.pages * p.H * p.P, D));
   B200_TRY(allow_smem(limits, smem, few_rows_kernel<D, FMT, NT>));
   // all of an SM's L1 as shared memory, also for what runs in between: left to the driver an SM keeps what the kernel in front left, and then holds one CTA and not two
   static std::atomic<uint64_t> shares{0};
@@ -1248,7 +1241,7 @@ int b200_paged_attention(const b200_paged_cache* cache, const b200_paged_batch* 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int fmt = cache->kv_dtype == B200_KV_INT8 ? INT8 : E4M3;
   p.from_rows = r.from_rows;
-  p.cols = p.ctiles = p.direct = p.q_tiles = p.nsplit = 0; p.part_o = p.part_ml = nullptr; p.parts = nullptr;
+  p.direct = p.q_tiles = p.nsplit = 0; p.part_o = p.part_ml = nullptr; p.parts = nullptr;
   if (r.prompt.units) {
     AttnP x = p;
     x.q_tiles = r.prompt.q_tiles; x.nsplit = r.prompt.nsplit;
@@ -1260,11 +1253,11 @@ int b200_paged_attention(const b200_paged_cache* cache, const b200_paged_batch* 
   }
   if (r.few.units) {
     const FewPlan& f = r.few;
-    p.cols = 8 * f.nt; p.ctiles = f.ctiles; p.direct = f.direct;
+    p.direct = f.direct;
     if (!f.direct) {
       p.part_o = static_cast<float*>(work_dev);
-      p.part_ml = p.part_o + (long long)f.ctas * 2 * p.cols * D;
-      p.parts = reinterpret_cast<int2*>(p.part_ml + (long long)f.ctas * 2 * p.cols * 2);
+      p.part_ml = p.part_o + (long long)f.ctas * 2 * 8 * f.nt * D;
+      p.parts = reinterpret_cast<int2*>(p.part_ml + (long long)f.ctas * 2 * 8 * f.nt * 2);
     }
     if (D == 128) B200_TRY((fmt == INT8 ? launch_few_nt<128, INT8>(p, f, st) : launch_few_nt<128, E4M3>(p, f, st)));
     else B200_TRY((fmt == INT8 ? launch_few_nt<64, INT8>(p, f, st) : launch_few_nt<64, E4M3>(p, f, st)));

@@ -115,10 +115,9 @@ struct AttnP {
   int window, sinks;
   float scale2;                              // score scale * log2(e)
   // few rows
-  int cols, ctiles;                          // columns of a unit, units of a sequence and kv head
   int direct;                                // a CTA per unit
-  float *part_o, *part_ml;                   // [CTAs][2][cols][D], [CTAs][2][cols][2]
-  int2* parts;                               // [sequences][ctiles][H]: first CTA and number of further ones of a unit
+  float *part_o, *part_ml;                   // [CTAs][2][columns][D], [CTAs][2][columns][2]
+  int2* parts;                               // [sequences][H]: first CTA and number of further ones of a unit
   // many rows
   int from_rows;                             // sequences of at least this many rows
   int q_tiles, nsplit;                       // units of a sequence and kv head; ranges of the keys
@@ -157,9 +156,6 @@ __device__ __forceinline__ bool wait_or_quit(uint32_t bar, uint32_t parity, vola
     }
   }
 }
-// paged.cu: a tensor map over a cache's codes, [rows][dim], boxes of box_rows whole rows, swizzled by 128 bytes (dim 64: by 64)
-int code_map(CUtensorMap* m, const void* codes, long long rows, int dim, int box_rows);
-
 // paged_prompt.cu
 struct PromptPlan { int q_tiles, nsplit; long long units; };
 PromptPlan prompt_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks);
