@@ -249,3 +249,19 @@ def test_codes_are_those_of_a_division(dtype, new):
         want = quotient.round() if dtype == "int8" else quotient.to(torch.float8_e4m3fn).float()
         got = pool[:, :, 1:1 + new].float().cpu()
         assert torch.equal(got, want), (got - want).abs().max()
+
+
+@pytest.mark.parametrize("new", [1, 5, 140])
+@pytest.mark.parametrize("dtype", ["int8", "fp8_e4m3"])
+def test_far_positions_under_a_window(new, dtype):
+    """Two billion tokens in, all of them on one page: what a session sees that is as far from a page's border and much younger."""
+    page, near = 128, 1700
+    far = near + page * 15_600_000
+    cache = Content([page], 2, 128, page, dtype, spare=0).cache()
+    q = torch.randn(new, 8, 128, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    table = torch.zeros(1, -(-(far + new) // page), dtype=torch.int32, device="cuda")
+    for window, sinks in ((500, 0), (333, 3), (1, 200), (1500, 130)):
+        a, b = (cache.attend(PagedBatch(table, i32([before]), i32([0, new]), new), q, window=window, sinks=sinks).float() for before in (near, far))
+        # each within half a step of bf16 and 2^-11 and less of what it sums up, which is 3 at most a value
+        assert bool(((a - b).abs() <= 2.0 ** -7 * torch.maximum(a.abs(), b.abs()) + 2.0 ** -9 * 3).all())
+    assert cache.error_flags() == 0
