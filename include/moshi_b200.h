@@ -569,21 +569,21 @@ typedef struct {
   int32_t kv_heads, dim;              /* dim 64 or 128 */
   int32_t kv_dtype, device;
 } b200_paged_cache;
-enum { B200_PAGED_BAD_BATCH = 1,      /* rows out of order or past total_rows / max_rows, negative lengths, or tokens past the table: the sequence was left out */
+enum { B200_PAGED_BAD_BATCH = 1,      /* rows out of order or past total_rows / max_rows, negative lengths, or tokens past the table: the sequence was left out (every call looks at all of them) */
        B200_PAGED_BAD_PAGE = 2,       /* a table names a page that the cache does not have: its tokens were left out */
        B200_PAGED_NOT_FINITE = 4,     /* an appended value is NaN, infinite or above 2^64: stored as 0 */
        B200_PAGED_WAIT = 8 };         /* a kernel waited ten seconds for its own copies in vain: the results are incomplete */
 
 /* A step: sequence s adds the rows rows[s] .. rows[s + 1] - 1 of the call's tensors (none, one or many) behind its before[s] tokens; token t of it lies in page
- * table[s][t / page_tokens].  Rows from rows[sequences] on belong to nobody and are left as they are. */
+ * table[s][t / page_tokens].  Rows in front of rows[0] and from rows[sequences] on belong to nobody and are left as they are in every result. */
 typedef struct {
   const int32_t *table_dev;           /* [sequences][table_ld], table_width of them used */
   const int32_t *before_dev;          /* [sequences] tokens in front of the step */
-  const int32_t *rows_dev;            /* [sequences + 1], rising from 0 on */
+  const int32_t *rows_dev;            /* [sequences + 1], none negative, none less than the one in front */
   int64_t table_ld;
   int32_t sequences, table_width;
   int32_t total_rows;                 /* rows of the call's tensors */
-  int32_t max_rows;                   /* no sequence has more than this in the step */
+  int32_t max_rows;                   /* no sequence has more than this in the step; work is laid out by it, so a number far above the truth costs time */
 } b200_paged_batch;
 typedef struct {
   const uint64_t* turns_dev;          /* [rot_dims / 2]: frequency / (2 pi), turns per position, as a fraction of 2^64 */
@@ -591,18 +591,18 @@ typedef struct {
 } b200_rotary;
 
 /* Appends k, v bf16 [total_rows][kv_heads * dim] (k_ld, v_ld elements from row to row, multiples of 8), keys rotated by their positions (rotary NULL: not), and rotates the queries q
- * [total_rows][q_heads * dim] into q_out (q NULL: none; q_out may be q).  Scales: the rows that begin a page give it max|x| / 127 (e4m3: / 448), at least 2^-60; rows
+ * [total_rows][q_heads * dim] into q_out (q NULL: none; q_out may be q; at most 8192 heads).  Scales: the rows that begin a page give it max|x| / 127 (e4m3: / 448), at least 2^-60; rows
  * that come later double it until they fit, and the page's older codes are rounded to the new scale.  Appending the same rows again changes nothing.  A page
  * that is written to must belong to one sequence of the batch only. */
 int b200_paged_append(const b200_paged_cache* cache, const b200_paged_batch* batch, const void* k_dev, int64_t k_ld, const void* v_dev, int64_t v_ld,
                       const void* q_dev, int64_t q_ld, void* q_out_dev, int64_t q_out_ld, int q_heads, const b200_rotary* rotary, void* stream);
 /* Attention of the step's rows over the cache, behind b200_paged_append with the same batch: the row at position p sees the tokens j <= p of its sequence and, where
- * window > 0, of these only p - j < window or j < sinks.  q, out bf16 [total_rows][q_heads * dim]; query head h reads cache head h / (q_heads / kv_heads).
- * A row that sees nothing gets zeros.  work_dev: b200_paged_attention_bytes(...) bytes that this call alone uses (0: may be null). */
+ * window > 0, of these only p - j < window or j < sinks.  q, out bf16 [total_rows][q_heads * dim]; query head h reads cache head h / (q_heads / kv_heads), at most 256 of them one; scale > 0.
+ * A row that sees nothing gets zeros, one that sees something with a query that is not finite NaN.  Where max_rows is 0 nothing is launched, and nothing recorded.  work_dev: b200_paged_attention_bytes(...) bytes that this call alone uses (0: may be null). */
 int64_t b200_paged_attention_bytes(const b200_paged_cache* cache, const b200_paged_batch* batch, int q_heads, int window, int sinks);
 int b200_paged_attention(const b200_paged_cache* cache, const b200_paged_batch* batch, const void* q_dev, int64_t q_ld, void* out_dev, int64_t out_ld, int q_heads,
                          float scale, int window, int sinks, void* work_dev, int64_t work_bytes, void* stream);
-/* What the cache holds of the batch's rows (positions before[s] + i): k, v bf16 [total_rows][kv_heads][dim]. */
+/* What the cache holds of the batch's rows (positions before[s] + i): k, v bf16 [total_rows][kv_heads][dim].  Rows of nobody, of sequences that are left out and on bad pages are not written. */
 int b200_paged_read(const b200_paged_cache* cache, const b200_paged_batch* batch, void* k_out_dev, void* v_out_dev, void* stream);
 
 /* ------------------------------------------------------------------------------------------ */

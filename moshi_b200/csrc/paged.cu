@@ -416,14 +416,14 @@ __global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadP p) {
 // scores; that of its values goes into the exponent, P = 2^(score + log2 s_v - M), with M behind the running maximum of the same, and the sum of the weights takes P / s_v: nothing is
 // rounded on the way but P, which is f16.  M follows only when a score passes it by 2^15, as then no column has to be compared across lanes for most tiles.
 //
-// Bounds: HBM for large batches (48 sessions of 3000 tokens, 32 heads, e4m3: 185 us, 6.4 TB/s); for many short units what a unit costs beside its tiles (128 sessions under a window of 1024, 8 heads: 72 us, floor 36;
+// Bounds: HBM for large batches (48 sessions of 3000 tokens, 32 heads, e4m3: 184 us, 6.4 TB/s); for many short units what a unit costs beside its tiles (128 sessions under a window of 1024, 8 heads: 68 us, floor 36;
 // a part's first copies, its queries and the joining of its warps are 7400 clocks beside 20000 for eight tiles a warp).
 // Why this way:
 // * tiles come as swizzled tensor copies, two in flight and two at work per warp: asked for lane by lane in the fragments' order, 16 bytes of eight rows an instruction, the same bytes came at 5.2 TB/s,
 //   in whole lines at 7.1 (nothing but copies);
 // * the scores of a tile and the values of the one in front do not wait for one another and are one stretch of code;
-// * two CTAs of four warps an SM: four of two warps are faster for short units (window 66 us, 64 ragged requests 84 -> 80) and slower for few (one session of 375 tokens 9.1 -> 12.3 us, one
-//   request of 131072 tokens 55 -> 59); three of four do not fit with the values' second place.
+// * two CTAs of four warps an SM: four of two warps are faster for short units (that window 68 -> 62 us) and slower for few (one session of 375 tokens 8.5 -> 11.6 us, one request of 131072 tokens
+//   53 -> 55); three of four do not fit with the values' second place.
 constexpr int FEW_WARPS = 4, FEW_THREADS = FEW_WARPS * 32;
 constexpr int FEW_PER_SM = 2;                // CTAs
 constexpr int DIRECT_TILES = 64;             // units of more tiles are always cut
@@ -1050,8 +1050,9 @@ bool rows_fit(const void* p, long long ld, int heads, int dim) { return p && !(r
 int shift_of(int P) { return P == 16 ? 4 : P == 32 ? 5 : P == 64 ? 6 : 7; }
 
 // Sequences of more than 16 columns (rows times heads of a group), at head size 64 of more than 32, go to the tensor cores' kernel of whole tiles, whose time hardly depends on how many of its 256 columns
-// there are; the only sequence of a step goes there with all its rows if it may have that many.  (32 heads of 128 on 8, 3000 tokens, here / there: 16 requests of 16 columns 40 / 69 us, of 24 87 / 69,
-// of 48 136 / 70; one request of 24 columns 34 / 19; 64 of 32 246 / 253, of 64 460 / 254.  24 heads of 64 on 4, 16 requests of 1000 to 6000 tokens and 30 columns: 29 / 48.)
+// there are; the only sequence of a step goes there with all its rows if it may have that many.  (Here / there, 3000 tokens.  32 heads of 128 on 8: 16 requests of 16 columns 39 / 65 us, 64 of them 105 / 233, one 17.5 / 14.8;
+// of 24 columns, as several units a sequence, 87 / 66, of 48 136 / 66.  24 heads of 64 on 4: 16 requests of 18, 24 and 30 columns 26, 26 and 28 / 31, of 24 on 1000 tokens 20 / 19, of 30 on 10000 50 / 81,
+// 64 of 24 61 / 100, one 19 / 13; 32 heads on 8, 32 columns: 16 requests 42 / 53, 4 of them 23 / 21.5.)
 constexpr int few_cols(int dim) { return dim == 64 ? 32 : 16; }
 // CTAs of 8 * nt columns, a wave of them, fewer where the tables allow for less work than that.
 struct FewPlan { int nt, ctas; long long units; bool direct; };
@@ -1064,8 +1065,8 @@ FewPlan few_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, in
   if (window > 0 && (long long)window + sinks + rows < keys) keys = (long long)window + sinks + rows;
   const long long tiles = ceil_div64(keys, 32) + 1, runs = ceil_div64(f.units * (tiles + 4), MIN_RUN), wave = 148 * FEW_PER_SM;
   // A CTA a unit, and nothing to join, where the chip holds all units at once and the longest is not much longer than an equal share: 7 us and 0.25 a tile, against 10.5 and 0.34 for every 296th part of all
-  // tiles and 12 for each unit.  (One token, 32 heads on 8, uncut / cut: 1 request of 1000 tokens 14.0 / 12.5 us, 32 of them 19.1 / 25.6, of 2000 29.7 / 36.0, 8 of 2000 24.5 / 17.9; 1 session of 374
-  // tokens with 32 heads 9.2 / 12.2.)
+  // tiles and 12 for each unit.  (One token, 32 heads on 8, uncut / cut: 1 request of 1000 tokens 13.4 / 11.3 us, 32 of them 18.2 / 23.7, 8 of 2000 23.3 / 16.7, 32 of them, past the limit, 28.8 / 34.6; 1
+  // session of 374 tokens with 32 heads 8.7 / 11.3.)
   f.direct = f.units <= wave && tiles <= DIRECT_TILES && 250 * tiles < 3500 + f.units * (tiles + UNIT_COST) * 115 / 100;
   f.ctas = (int)(f.direct ? f.units : runs < wave ? runs : wave);
   return f;

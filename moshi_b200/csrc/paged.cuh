@@ -101,7 +101,8 @@ __device__ __forceinline__ float power_of_two_in(float x) { return __uint_as_flo
 // which is of score + log2(scale), stays that of the pages that have something to add.
 __device__ __forceinline__ float value_scale(float s) { return s > 0.f ? s : SCALE_MIN; }
 // Weights are P = 2^(score + log2(value scale) - M) in f16, whose numbers go from 2^-24 to 65504.  M is set 2^UNDER below the largest exponent and follows when one passes it by 2^SLACK: P reaches 2^15, and
-// a weight (times its value's scale) is off by 2^-11 of itself or, under 2^-21 of the largest one, by 2^-32 of that.
+// a weight (times its value's scale) is off by 2^-11 of itself or, under 2^-21 of the largest one, by 2^-32 of that.  exp2 ends at 2^-126: of pages whose value scales lie as far apart as 2^118, the whole
+// range that scales have, the lower ones' weights count in the total down to 2^-15 of the largest.
 constexpr float UNDER = 7.f, SLACK = 15.f;
 struct AttnP {
   const uint8_t *k, *v;

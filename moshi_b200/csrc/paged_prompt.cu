@@ -7,8 +7,8 @@
 //
 // Scales as in paged.cu: that of a page's keys multiplies its 16 or more columns' scores, that of its values goes into the exponent.  O is rescaled only when a weight would pass 2^15.
 //
-// Bounds: the chain of a tile through its weight warps; the tensor pipe and the exponentials' unit are each active half the time (2048 rows on 6100 tokens, 32 heads on 8: 280 us, 0.86 PFLOP/s; a
-// window of 1024 over 6000 rows of 16 heads on 4: 104 us).  A row's scores are read from TMEM once, and stay in 184 registers that setmaxnreg takes from the other warps
+// Bounds: the chain of a tile through its weight warps; the tensor pipe and the exponentials' unit are each active half the time (2048 rows on 6100 tokens, 32 heads on 8: 281 to 285 us, 0.84 PFLOP/s; a
+// window of 1024 over 6000 rows of 16 heads on 4: 103 us).  The same statements in another order were up to 4 % slower.  A row's scores are read from TMEM once, and stay in 184 registers that setmaxnreg takes from the other warps
 // (read twice, in 96, the first of these took 389 us when this took 365).
 #include "paged.cuh"
 

@@ -265,3 +265,26 @@ def test_far_positions_under_a_window(new, dtype):
         # each within half a step of bf16 and 2^-11 and less of what it sums up, which is 3 at most a value
         assert bool(((a - b).abs() <= 2.0 ** -7 * torch.maximum(a.abs(), b.abs()) + 2.0 ** -9 * 3).all())
     assert cache.error_flags() == 0
+
+
+@pytest.mark.parametrize("dtype,dim,page", [("int8", 128, 64), ("fp8_e4m3", 64, 16)])
+def test_a_step_in_two_batches_over_the_same_tensors(dtype, dim, page):
+    """A portion of a prompt and single rows, each with a plan of its own: the other's rows belong to nobody, and are left as they are."""
+    new, before = [150, 1, 1, 1, 0, 1], [700, 300, 64, 63, 5, 0]
+    c = Content(before, 2, dim, page, dtype, capacity=[b + n for b, n in zip(before, new)])
+    one, two = c.cache(), c.cache()
+    q, k, v = (torch.randn(sum(new), h, dim).bfloat16().cuda() for h in (8, 2, 2))
+    batch, rotary = batch_of(c.table, before, new), RotaryTable(dim)
+    want_q = one.append(batch, k, v, q=q, rotary=rotary)
+    assert torch.equal(one.append(batch, k, v, q=q, rotary=rotary), want_q)
+    got_q, out, T = torch.full_like(q, 7.0), torch.full_like(q, 7.0), batch.total_rows
+    parts = [PagedBatch(batch.table[:1], batch.before[:1], batch.rows[:2], T, 150), PagedBatch(batch.table[1:], batch.before[1:], batch.rows[1:], T, 1)]
+    for b in parts:
+        two.append(b, k, v, q=q, rotary=rotary, q_out=got_q)
+    for b in parts:
+        two.attend(b, got_q, out=out)
+    assert torch.equal(got_q, want_q) and one.error_flags() == two.error_flags() == 0
+    assert all(torch.equal(a.view(torch.int8), b.view(torch.int8)) for a, b in ((one.k, two.k), (one.v, two.v)))       # as bytes: unwritten places are NaN
+    # the same rows cut into other ranges: 32-bit sums in another order, weights in f16, and half a step of bf16 each
+    want = one.attend(batch, want_q).float()
+    assert bool(((out.float() - want).abs() <= 2.0 ** -7 * torch.maximum(out.float().abs(), want.abs()) + 2.0 ** -9 * 3).all())
