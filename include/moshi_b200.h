@@ -572,7 +572,9 @@ typedef struct {
 enum { B200_PAGED_BAD_BATCH = 1,      /* rows out of order or past total_rows / max_rows, negative lengths, or tokens past the table: the sequence was left out (every call looks at all of them) */
        B200_PAGED_BAD_PAGE = 2,       /* a table names a page that the cache does not have: its tokens were left out */
        B200_PAGED_NOT_FINITE = 4,     /* an appended value is NaN, infinite or above 2^64: stored as 0 */
-       B200_PAGED_WAIT = 8 };         /* a kernel waited ten seconds for its own copies in vain: the results are incomplete */
+       B200_PAGED_WAIT = 8,           /* a kernel waited ten seconds for its own copies in vain: the results are incomplete */
+       B200_PAGED_BAD_TREE = 16,      /* a drafted token's parent is not one in front of it: it was taken as a child of the last cached token */
+       B200_PAGED_NO_PAGES = 32 };    /* a pool has fewer free pages than were asked for: nobody got any */
 
 /* A step: sequence s adds the rows rows[s] .. rows[s + 1] - 1 of the call's tensors (none, one or many) behind its before[s] tokens; token t of it lies in page
  * table[s][t / page_tokens].  Rows in front of rows[0] and from rows[sequences] on belong to nobody and are left as they are in every result. */
@@ -596,6 +598,16 @@ typedef struct {
  * that is written to must belong to one sequence of the batch only. */
 int b200_paged_append(const b200_paged_cache* cache, const b200_paged_batch* batch, const void* k_dev, int64_t k_ld, const void* v_dev, int64_t v_ld,
                       const void* q_dev, int64_t q_ld, void* q_out_dev, int64_t q_out_ld, int q_heads, const b200_rotary* rotary, void* stream);
+/* The same with rows at positions of their own: a drafted token's is its depth in the tree, an image's patches have several (time, height, width).  Pair j of the rotated dimensions is turned by
+ * positions[pair_axis[j]][row], any 32-bit numbers, for keys and queries; where a row is stored does not go by it.  rotary must be given. */
+typedef struct {
+  const int32_t* positions_dev;       /* [axes][ld], total_rows of them used */
+  int64_t ld;
+  const uint8_t* pair_axis_dev;       /* [rot_dims / 2], each below axes, 8-byte border; may be null where axes is 1 */
+  int32_t axes;                       /* 1 .. 4 */
+} b200_paged_positions;
+int b200_paged_append_at(const b200_paged_cache* cache, const b200_paged_batch* batch, const void* k_dev, int64_t k_ld, const void* v_dev, int64_t v_ld, const void* q_dev, int64_t q_ld,
+                         void* q_out_dev, int64_t q_out_ld, int q_heads, const b200_rotary* rotary, const b200_paged_positions* positions, void* stream);
 /* Attention of the step's rows over the cache, behind b200_paged_append with the same batch: the row at position p sees the tokens j <= p of its sequence and, where
  * window > 0, of these only p - j < window or j < sinks.  q, out bf16 [total_rows][q_heads * dim]; query head h reads cache head h / (q_heads / kv_heads), at most 256 of them one; scale > 0.
  * A row that sees nothing gets zeros, one that sees something with a query that is not finite NaN.  Where max_rows is 0 nothing is launched, and nothing recorded.  work_dev: b200_paged_attention_bytes(...) bytes that this call alone uses (0: may be null). */
@@ -604,6 +616,48 @@ int b200_paged_attention(const b200_paged_cache* cache, const b200_paged_batch* 
                          float scale, int window, int sinks, void* work_dev, int64_t work_bytes, void* stream);
 /* What the cache holds of the batch's rows (positions before[s] + i): k, v bf16 [total_rows][kv_heads][dim].  Rows of nobody, of sequences that are left out and on bad pages are not written. */
 int b200_paged_read(const b200_paged_cache* cache, const b200_paged_batch* batch, void* k_out_dev, void* v_out_dev, void* stream);
+
+/* ---- trees of drafted tokens ---- (csrc/paged_tree.cu, paged_pool.cu)
+ * The rows of a sequence's step are a tree: row i comes behind row parents[rows[s] + i] of the same sequence, which has a lower number, or, -1, behind the last cached token.  They lie in the cache one
+ * behind the other like any step's rows; their positions are before + depth.  At most 1024 of a sequence (max_rows). */
+typedef struct {
+  uint32_t* seen_dev;                 /* [total_rows][words]: bit i of a row: it sees the sequence's i-th row of the step (itself, and those that it comes behind) */
+  int32_t* position_dev;              /* [total_rows] */
+  int32_t words;                      /* 32 * words >= max_rows, at most 32 */
+} b200_paged_tree;
+/* Fills a tree from parents; all layers of a step share it.  Rows of no sequence are left as they are.  Reads the batch's before and rows only.  flags_dev: as a cache's. */
+int b200_paged_tree_build(const b200_paged_batch* batch, const b200_paged_tree* tree, const int32_t* parents_dev, int32_t* flags_dev, int device, void* stream);
+/* b200_paged_attention of a tree's rows: of what is cached a row at position p sees token j where window is 0, p - j < window or j < sinks; of the step's rows those of its mask for whose positions the same holds. */
+int64_t b200_paged_tree_attention_bytes(const b200_paged_cache* cache, const b200_paged_batch* batch, int q_heads, int window, int sinks);
+int b200_paged_tree_attention(const b200_paged_cache* cache, const b200_paged_batch* batch, const b200_paged_tree* tree, const void* q_dev, int64_t q_ld, void* out_dev, int64_t out_ld, int q_heads,
+                              float scale, int window, int sinks, void* work_dev, int64_t work_bytes, void* stream);
+/* The rows of a step that are kept move to the front, in n_caches caches that are alike (one per layer): sequence s keeps its rows kept[rows[s] + i], i < counts[s], which rise (else it is left out), and
+ * row i of them lies in place before[s] + i afterwards; what lies behind is of no use any more.  Within a page codes move as they are.  A row that comes from another page is rounded once more, to the scale of
+ * the page that it moves to, which is doubled until the row fits, or is the rows' own where nothing else of use is left there.  The first cache's flags are used. */
+int b200_paged_keep(const b200_paged_cache* caches, int n_caches, const b200_paged_batch* batch, const int32_t* kept_dev, const int32_t* counts_dev, void* stream);
+
+/* ---- the pages of a pool ---- (csrc/paged_pool.cu)
+ * Who holds which pages, on the device: sequence s has lengths[s] tokens and holds the pages table[s][0 .. held[s] - 1], enough for them; refs counts the sequences that hold a page, 0: it is free.  The calls
+ * keep to that; what does not fit together is left out and recorded in the flags.  work_dev: b200_page_pool_bytes(...) bytes that this call alone uses. */
+typedef struct {
+  int32_t *table_dev;                 /* [sequences][table_ld], table_width of them used; -1 behind what is held */
+  int32_t *lengths_dev, *held_dev;    /* [sequences] */
+  int32_t *refs_dev;                  /* [pages] */
+  int32_t *flags_dev;                 /* one word */
+  int64_t table_ld;
+  int32_t sequences, table_width;     /* at most 4096 sequences */
+  int32_t pages, page_tokens;
+  int32_t device;
+} b200_page_pool;
+int64_t b200_page_pool_bytes(const b200_page_pool* pool);
+/* All at once, sequence i becomes what sequence source[i] was: its tokens' pages are held by one more; -1: it becomes empty.  So requests are forked, beams change places, and pages are given back.  Pages
+ * that were held in reserve are given back too.  A source that is no sequence leaves the sequence what it is. */
+int b200_page_pool_rearrange(const b200_page_pool* pool, const int32_t* source_dev, void* work_dev, int64_t work_bytes, void* stream);
+/* Sequence s gets pages for add[s] >= 0 tokens behind its lengths[s].  Where the page of the first of them is partly filled and shared it gets a copy of its own, in all caches; of the sequences that share one in
+ * this call, the last keeps it if nobody else holds it.  Free pages go out by rising numbers, to sequences by rising numbers, a copy before the sequence's other pages.  If there are too few nobody gets any. */
+int b200_page_pool_reserve(const b200_page_pool* pool, const b200_paged_cache* caches, int n_caches, const int32_t* add_dev, void* work_dev, int64_t work_bytes, void* stream);
+/* Pages in use move to the lowest numbers, in all caches: those at or above the number of pages in use go, by rising numbers, into the free ones below it. */
+int b200_page_pool_compact(const b200_page_pool* pool, const b200_paged_cache* caches, int n_caches, void* work_dev, int64_t work_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------ */
 /* Kernel-level entry points (used by the parity tests; same kernels the handles launch)        */

@@ -81,6 +81,19 @@ class RotaryC(C.Structure):
     _fields_ = [("turns", C.c_void_p), ("rot_dims", C.c_int32), ("pairing", C.c_int32)]
 
 
+class PagedPositionsC(C.Structure):
+    _fields_ = [("positions", C.c_void_p), ("ld", C.c_int64), ("pair_axis", C.c_void_p), ("axes", C.c_int32)]
+
+
+class PagedTreeC(C.Structure):
+    _fields_ = [("seen", C.c_void_p), ("position", C.c_void_p), ("words", C.c_int32)]
+
+
+class PagePoolC(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("lengths", C.c_void_p), ("held", C.c_void_p), ("refs", C.c_void_p), ("flags", C.c_void_p), ("table_ld", C.c_int64),
+                ("sequences", C.c_int32), ("table_width", C.c_int32), ("pages", C.c_int32), ("page_tokens", C.c_int32), ("device", C.c_int32)]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _L = C.c_int64
@@ -178,7 +191,16 @@ _PROTOTYPES: dict[str, tuple[tp.Any, list]] = {
     "b200_paged_append": (_I, [_P, _P, _P, _L, _P, _L, _P, _L, _P, _L, _I, _P, _P]),
     "b200_paged_attention_bytes": (_L, [_P, _P, _I, _I, _I]),
     "b200_paged_attention": (_I, [_P, _P, _P, _L, _P, _L, _I, C.c_float, _I, _I, _P, _L, _P]),
+    "b200_paged_append_at": (_I, [_P, _P, _P, _L, _P, _L, _P, _L, _P, _L, _I, _P, _P, _P]),
     "b200_paged_read": (_I, [_P, _P, _P, _P, _P]),
+    "b200_paged_tree_build": (_I, [_P, _P, _P, _P, _I, _P]),
+    "b200_paged_tree_attention_bytes": (_L, [_P, _P, _I, _I, _I]),
+    "b200_paged_tree_attention": (_I, [_P, _P, _P, _P, _L, _P, _L, _I, C.c_float, _I, _I, _P, _L, _P]),
+    "b200_paged_keep": (_I, [_P, _I, _P, _P, _P, _P]),
+    "b200_page_pool_bytes": (_L, [_P]),
+    "b200_page_pool_rearrange": (_I, [_P, _P, _P, _L, _P]),
+    "b200_page_pool_reserve": (_I, [_P, _P, _I, _P, _P, _L, _P]),
+    "b200_page_pool_compact": (_I, [_P, _P, _I, _P, _L, _P]),
     # kernel-level
     "b200_op_linear_bf16": (_I, [_P, _P, _P, _I, _I, _I, _P]),
     "b200_op_packed_bytes": (C.c_int64, [_I, _I, _I, _I]),

@@ -37,6 +37,10 @@ struct AppendP {
   long long k_ld, v_ld, q_ld, q_out_ld;
   const uint64_t* turns;                     // per pair of dimensions: turns per position as a 64-bit fraction; null: no rotation
   int rot, halves;                           // rotated dimensions; pairs are (j, j + rot / 2), else (2j, 2j + 1)
+  const int32_t* positions;                  // positions of the rows' own: [axes][positions_ld]
+  const uint8_t* pair_axis;                  // per pair: the axis whose position turns it; null: the first
+  long long positions_ld;
+  int axes;
   int pages, P, H, Hq, items, heads_per_block, page_ctas, q_rows;            // items: numbers of touched pages
 };
 
@@ -60,6 +64,26 @@ __device__ __forceinline__ void turn_of(Turn& t, const uint64_t* turns, int j, i
     const int part = (int)((turns[8 * j + i] * (uint64_t)pos) >> 32);
     sincospif((float)part * 4.656612873077393e-10f, &t.sn[i], &t.cs[i]);      // 2^-31: half turns
   }
+}
+// The same at positions of row r's own, one for each axis.
+__device__ __forceinline__ void turn_of_row(Turn& t, const AppendP& p, int j, int r) {
+  int at[4];
+#pragma unroll
+  for (int a = 0; a < 4; ++a) at[a] = a < p.axes ? p.positions[a * p.positions_ld + r] : 0;
+  const uint2 which = p.pair_axis ? *reinterpret_cast<const uint2*>(p.pair_axis + 8 * j) : make_uint2(0, 0);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t a = (i < 4 ? which.x : which.y) >> (8 * (i & 3)) & 255u;
+    const int pos = a == 1 ? at[1] : a == 2 ? at[2] : a == 3 ? at[3] : at[0];
+    const int part = (int)((p.turns[8 * j + i] * (uint64_t)(int64_t)pos) >> 32);         // whole turns drop out of negative products likewise
+    sincospif((float)part * 4.656612873077393e-10f, &t.sn[i], &t.cs[i]);
+  }
+}
+// OWN: the rows have positions of their own, else a row's position is its place in the sequence.
+template <bool OWN>
+__device__ __forceinline__ void turn(Turn& t, const AppendP& p, int j, int pos, int r) {
+  if constexpr (OWN) turn_of_row(t, p, j, r);
+  else turn_of(t, p.turns, j, pos);
 }
 __device__ __forceinline__ void unpack16(float* x, const uint4* raw) {
   const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
@@ -167,7 +191,7 @@ __device__ __forceinline__ float largest16(const float* x) {
 }
 
 // Queries: rotate, round, store.  `slots` rows of a head side by side in the block; q_rows rows of the batch, whose angles serve all heads.
-template <int D>
+template <int D, bool OWN>
 __device__ void append_queries(const AppendP& p, int block) {
   constexpr int CHUNKS = D / 16;
   __shared__ int row_pos[8];
@@ -190,7 +214,7 @@ __device__ void append_queries(const AppendP& p, int block) {
   if (pos < 0) return;
   const Chunk c(j, p.rot, p.halves);
   Turn t;
-  if (c.turned) turn_of(t, p.turns, j, pos);
+  if (c.turned) turn<OWN>(t, p, j, pos, r);
   constexpr int ROUND = 4;                   // heads asked for together: results may lie over the queries, so the compiler keeps loads behind stores
   for (int h0 = slot % slots; h0 < p.Hq; h0 += ROUND * slots) {
     uint4 raw[ROUND][2];
@@ -215,13 +239,13 @@ __device__ void append_queries(const AppendP& p, int block) {
 // Few rows a sequence: a warp per (page that the step touches, kv head, side); rows past the first sweep of the warp are read twice, for the scale and for the codes.
 // Bounds: the launch and a chain of four dependent reads (rows, table, scale, codes): 48 sequences of one row, 32 heads and their queries 8.6 us.
 constexpr int APPEND_THREADS = 256;
-template <int FMT, int D>
+template <int FMT, int D, bool OWN>
 __global__ void __launch_bounds__(APPEND_THREADS) append_few_kernel(const AppendP p) {
   pdl_trigger();
   pdl_wait();
   constexpr int CHUNKS = D / 16, RPS = 32 / CHUNKS;
   if (blockIdx.x == gridDim.x - 1) { record_sequences(p.b, p.P, p.flags, blockDim.x); return; }
-  if ((int)blockIdx.x >= p.page_ctas) { append_queries<D>(p, (int)blockIdx.x - p.page_ctas); return; }
+  if ((int)blockIdx.x >= p.page_ctas) { append_queries<D, OWN>(p, (int)blockIdx.x - p.page_ctas); return; }
   const int lane = threadIdx.x & 31, task = (int)blockIdx.x * (APPEND_THREADS / 32) + (threadIdx.x >> 5);
   if (task >= p.items * p.H * 2) return;
   const bool keys = !(task & 1);
@@ -240,7 +264,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_few_kernel(const Append
     load16(x, src + (g.r + slot - g.o) * ld, c);
     if (c.turned) {
       Turn t;
-      turn_of(t, p.turns, j, g.first + slot);
+      turn<OWN>(t, p, j, g.first + slot, g.r + slot - g.o);
       if (p.halves) rotate16(x, t, 1); else rotate16(x, t, 0);
     }
     odd |= only_finite(x);
@@ -271,13 +295,13 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_few_kernel(const Append
 // Many rows: a block of P * D / 32 threads, two chunks each, has a page and goes through some of its heads, keys and values; the next head's rows are on their way while one is worked on, and
 // the angles of the page's positions serve all heads.  Everything is read once, as the scale has to be known before the first code.
 // Bounds: bytes, once the chain of reads in front is shared by several heads: 7887 rows of 8 heads 24 us (48 MB), with 32 heads of queries 41 (177 MB, 4.3 TB/s).  A head to a block took 40 and 69.
-template <int FMT, int D>
+template <int FMT, int D, bool OWN>
 __global__ void __launch_bounds__(512) append_many_kernel(const AppendP p) {
   pdl_trigger();
   pdl_wait();
   constexpr int CHUNKS = D / 16;
   if (blockIdx.x == gridDim.x - 1) { record_sequences(p.b, p.P, p.flags, blockDim.x); return; }
-  if ((int)blockIdx.x >= p.page_ctas) { append_queries<D>(p, (int)blockIdx.x - p.page_ctas); return; }
+  if ((int)blockIdx.x >= p.page_ctas) { append_queries<D, OWN>(p, (int)blockIdx.x - p.page_ctas); return; }
   __shared__ float tops[2][16];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   const int groups = (p.H + p.heads_per_block - 1) / p.heads_per_block, item = (int)blockIdx.x / groups, h0 = ((int)blockIdx.x - item * groups) * p.heads_per_block;
@@ -290,7 +314,7 @@ __global__ void __launch_bounds__(512) append_many_kernel(const AppendP p) {
   Turn t[2];
   if (ck.turned) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) turn_of(t[k], p.turns, j, g.first + slot[k]);
+    for (int k = 0; k < 2; ++k) turn<OWN>(t[k], p, j, g.first + slot[k], mine[k] ? g.r + slot[k] - g.o : g.r);
   }
   uint4 raw[2][2];
   float s_next;
@@ -1126,7 +1150,7 @@ int launch_few_nt(const AttnP& p, const FewPlan& f, cudaStream_t st) {
 }
 
 constexpr int WAVE = 148 * 3 / 2;
-template <int FMT, int D>
+template <int FMT, int D, bool OWN>
 int launch_append(AppendP& p, cudaStream_t st) {
   // Up to 16 rows of a sequence: a warp a page, head and side (32 heads, 48 sequences of 1 / 8 / 16 rows: 7.8 / 9.7 / 13.7 us, as blocks of whole pages 28 / 29 / 30; 8 heads, 8 sequences of
   // 32 / 64 rows: 6.8 / 9.6 us, as blocks 6.1 / 6.5).
@@ -1141,11 +1165,33 @@ int launch_append(AppendP& p, cudaStream_t st) {
   p.q_rows = 1;
   while (p.q_rows < 8 && 2 * p.q_rows <= slots && (long long)p.b.T * p.Hq >= 148ll * 8 * slots * p.q_rows) p.q_rows *= 2;
   const dim3 grid((unsigned)(p.page_ctas + (p.Hq ? ceil_div(p.b.T, p.q_rows) : 0) + 1));       // the last one looks at the sequences
-  if (few) return launch_early(append_few_kernel<FMT, D>, grid, dim3(threads), 0, st, p);
-  return launch_early(append_many_kernel<FMT, D>, grid, dim3(threads), 0, st, p);
+  if (few) return launch_early(append_few_kernel<FMT, D, OWN>, grid, dim3(threads), 0, st, p);
+  return launch_early(append_many_kernel<FMT, D, OWN>, grid, dim3(threads), 0, st, p);
 }
 
 }  // namespace
+
+int checked_cache(const b200_paged_cache* cache, const char* what) { return check_cache(cache, what); }
+int checked(const b200_paged_cache* cache, const b200_paged_batch* batch, const char* what) {
+  B200_TRY(check_cache(cache, what));
+  return check_batch(cache, batch, what);
+}
+int attention_arguments(AttnP* p, const b200_paged_cache* cache, const b200_paged_batch* batch, const void* q_dev, int64_t q_ld, void* out_dev, int64_t out_ld, int q_heads, float scale, int window,
+                        int sinks, const char* what) {
+  B200_TRY(checked(cache, batch, what));
+  const int D = cache->dim, H = cache->kv_heads;
+  if (q_heads < H || q_heads % H || q_heads / H > 256) B200_FAIL(B200_ERR_SHAPE, "%s: %d query heads on %d heads of the cache", what, q_heads, H);
+  if (!(scale > 0.f && scale < INFINITY) || window < 0 || sinks < 0) B200_FAIL(B200_ERR_INVALID, "%s: scale %g, window %d, %d first tokens", what, (double)scale, window, sinks);
+  if (batch->total_rows && batch->max_rows && (!rows_fit(q_dev, q_ld, q_heads, D) || !rows_fit(out_dev, out_ld, q_heads, D)))
+    B200_FAIL(B200_ERR_INVALID, "%s: queries and results must begin on a 16-byte border, rows %lld and %lld elements apart", what, (long long)q_ld, (long long)out_ld);
+  memset(p, 0, sizeof(*p));
+  p->k = static_cast<const uint8_t*>(cache->k_dev); p->v = static_cast<const uint8_t*>(cache->v_dev); p->k_scale = cache->k_scale_dev; p->v_scale = cache->v_scale_dev;
+  p->flags = cache->flags_dev; p->b = batch_of(batch); p->q = static_cast<const __nv_bfloat16*>(q_dev); p->out = static_cast<__nv_bfloat16*>(out_dev);
+  p->q_ld = q_ld; p->out_ld = out_ld; p->pages = cache->pages; p->P = cache->page_tokens; p->page_shift = shift_of(p->P); p->H = H; p->G = q_heads / H;
+  p->window = window; p->sinks = sinks; p->scale2 = scale * LOG2E;
+  return B200_OK;
+}
+
 }  // namespace paged
 }  // namespace b200
 
@@ -1153,8 +1199,8 @@ using namespace b200;
 
 extern "C" {
 
-int b200_paged_append(const b200_paged_cache* cache, const b200_paged_batch* batch, const void* k_dev, int64_t k_ld, const void* v_dev, int64_t v_ld,
-                      const void* q_dev, int64_t q_ld, void* q_out_dev, int64_t q_out_ld, int q_heads, const b200_rotary* rotary, void* stream) {
+static int append(const b200_paged_cache* cache, const b200_paged_batch* batch, const void* k_dev, int64_t k_ld, const void* v_dev, int64_t v_ld,
+                  const void* q_dev, int64_t q_ld, void* q_out_dev, int64_t q_out_ld, int q_heads, const b200_rotary* rotary, const b200_paged_positions* at, void* stream) {
   using namespace b200::paged;
   B200_TRY(check_cache(cache, "paged_append"));
   B200_TRY(check_batch(cache, batch, "paged_append"));
@@ -1166,6 +1212,8 @@ int b200_paged_append(const b200_paged_cache* cache, const b200_paged_batch* bat
     B200_FAIL(B200_ERR_INVALID, "paged_append: %d query heads, rows %lld and %lld elements apart, on a 16-byte border", q_heads, (long long)q_ld, (long long)q_out_ld);
   if (rotary && (!rotary->turns_dev || rotary->rot_dims < 16 || rotary->rot_dims % 16 || rotary->rot_dims > D || (rotary->pairing != B200_ROT_HALVES && rotary->pairing != B200_ROT_ADJACENT)))
     B200_FAIL(B200_ERR_INVALID, "paged_append: %d rotated dimensions (a multiple of 16, up to the head size), pairing %d", rotary->rot_dims, rotary->pairing);
+  if (at && (!rotary || !at->positions_dev || at->axes < 1 || at->axes > 4 || at->ld < batch->total_rows || (at->axes > 1 && !at->pair_axis_dev) || (reinterpret_cast<uintptr_t>(at->pair_axis_dev) & 7)))
+    B200_FAIL(B200_ERR_INVALID, "paged_append: positions of %d axes (1 to 4), %lld apart, of %d rows, with a rotation and an axis for each of its pairs on an 8-byte border", at->axes, (long long)at->ld, batch->total_rows);
   DeviceGuard guard(cache->device);
   AppendP p;
   p.k_codes = static_cast<uint8_t*>(cache->k_dev); p.v_codes = static_cast<uint8_t*>(cache->v_dev); p.k_scale = cache->k_scale_dev; p.v_scale = cache->v_scale_dev;
@@ -1173,6 +1221,7 @@ int b200_paged_append(const b200_paged_cache* cache, const b200_paged_batch* bat
   p.k = static_cast<const __nv_bfloat16*>(k_dev); p.v = static_cast<const __nv_bfloat16*>(v_dev); p.q = static_cast<const __nv_bfloat16*>(q_dev);
   p.q_out = static_cast<__nv_bfloat16*>(q_out_dev); p.k_ld = k_ld; p.v_ld = v_ld; p.q_ld = q_ld; p.q_out_ld = q_out_ld;
   p.turns = rotary ? rotary->turns_dev : nullptr; p.rot = rotary ? rotary->rot_dims : 0; p.halves = rotary ? rotary->pairing == B200_ROT_HALVES : 0;
+  p.positions = at ? at->positions_dev : nullptr; p.pair_axis = at ? at->pair_axis_dev : nullptr; p.positions_ld = at ? at->ld : 0; p.axes = at ? at->axes : 0;
   p.pages = cache->pages; p.P = cache->page_tokens; p.H = cache->kv_heads; p.Hq = q_dev ? q_heads : 0;
   const long long items = (long long)batch->total_rows / p.P + 2ll * batch->sequences;
   if (items * p.H * 2 > (1ll << 30)) B200_FAIL(B200_ERR_SHAPE, "paged_append: %d rows of %d sequences with %d heads in one call", batch->total_rows, batch->sequences, p.H);
@@ -1180,10 +1229,24 @@ int b200_paged_append(const b200_paged_cache* cache, const b200_paged_batch* bat
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool i8 = cache->kv_dtype == B200_KV_INT8;
   int rc;
-  if (D == 128) rc = i8 ? launch_append<INT8, 128>(p, st) : launch_append<E4M3, 128>(p, st);
-  else rc = i8 ? launch_append<INT8, 64>(p, st) : launch_append<E4M3, 64>(p, st);
+  if (at) {
+    if (D == 128) rc = i8 ? launch_append<INT8, 128, true>(p, st) : launch_append<E4M3, 128, true>(p, st);
+    else rc = i8 ? launch_append<INT8, 64, true>(p, st) : launch_append<E4M3, 64, true>(p, st);
+  } else {
+    if (D == 128) rc = i8 ? launch_append<INT8, 128, false>(p, st) : launch_append<E4M3, 128, false>(p, st);
+    else rc = i8 ? launch_append<INT8, 64, false>(p, st) : launch_append<E4M3, 64, false>(p, st);
+  }
   B200_TRY(rc);
   return check_launch("paged_append");
+}
+int b200_paged_append(const b200_paged_cache* cache, const b200_paged_batch* batch, const void* k_dev, int64_t k_ld, const void* v_dev, int64_t v_ld,
+                      const void* q_dev, int64_t q_ld, void* q_out_dev, int64_t q_out_ld, int q_heads, const b200_rotary* rotary, void* stream) {
+  return append(cache, batch, k_dev, k_ld, v_dev, v_ld, q_dev, q_ld, q_out_dev, q_out_ld, q_heads, rotary, nullptr, stream);
+}
+int b200_paged_append_at(const b200_paged_cache* cache, const b200_paged_batch* batch, const void* k_dev, int64_t k_ld, const void* v_dev, int64_t v_ld, const void* q_dev, int64_t q_ld,
+                         void* q_out_dev, int64_t q_out_ld, int q_heads, const b200_rotary* rotary, const b200_paged_positions* positions, void* stream) {
+  if (!positions) B200_FAIL(B200_ERR_INVALID, "paged_append_at: no positions");
+  return append(cache, batch, k_dev, k_ld, v_dev, v_ld, q_dev, q_ld, q_out_dev, q_out_ld, q_heads, rotary, positions, stream);
 }
 
 int b200_paged_read(const b200_paged_cache* cache, const b200_paged_batch* batch, void* k_out_dev, void* v_out_dev, void* stream) {
@@ -1219,20 +1282,11 @@ int64_t b200_paged_attention_bytes(const b200_paged_cache* cache, const b200_pag
 int b200_paged_attention(const b200_paged_cache* cache, const b200_paged_batch* batch, const void* q_dev, int64_t q_ld, void* out_dev, int64_t out_ld, int q_heads,
                          float scale, int window, int sinks, void* work_dev, int64_t work_bytes, void* stream) {
   using namespace b200::paged;
-  B200_TRY(check_cache(cache, "paged_attention"));
-  B200_TRY(check_batch(cache, batch, "paged_attention"));
-  const int D = cache->dim, H = cache->kv_heads;
-  if (q_heads < H || q_heads % H || q_heads / H > 256) B200_FAIL(B200_ERR_SHAPE, "paged_attention: %d query heads on %d heads of the cache", q_heads, H);
-  if (!(scale > 0.f && scale < INFINITY) || window < 0 || sinks < 0) B200_FAIL(B200_ERR_INVALID, "paged_attention: scale %g, window %d, %d first tokens", (double)scale, window, sinks);
-  if (batch->total_rows == 0 || batch->max_rows == 0) return B200_OK;
-  if (!rows_fit(q_dev, q_ld, q_heads, D) || !rows_fit(out_dev, out_ld, q_heads, D))
-    B200_FAIL(B200_ERR_INVALID, "paged_attention: queries and results must begin on a 16-byte border, rows %lld and %lld elements apart", (long long)q_ld, (long long)out_ld);
-  DeviceGuard guard(cache->device);
   AttnP p;
-  p.k = static_cast<const uint8_t*>(cache->k_dev); p.v = static_cast<const uint8_t*>(cache->v_dev); p.k_scale = cache->k_scale_dev; p.v_scale = cache->v_scale_dev;
-  p.flags = cache->flags_dev; p.b = batch_of(batch); p.q = static_cast<const __nv_bfloat16*>(q_dev); p.out = static_cast<__nv_bfloat16*>(out_dev);
-  p.q_ld = q_ld; p.out_ld = out_ld; p.pages = cache->pages; p.P = cache->page_tokens; p.page_shift = shift_of(p.P); p.H = H; p.G = q_heads / H;
-  p.window = window; p.sinks = sinks; p.scale2 = scale * LOG2E;
+  B200_TRY(attention_arguments(&p, cache, batch, q_dev, q_ld, out_dev, out_ld, q_heads, scale, window, sinks, "paged_attention"));
+  if (batch->total_rows == 0 || batch->max_rows == 0) return B200_OK;
+  DeviceGuard guard(cache->device);
+  const int D = cache->dim;
   const Route r = route(cache, batch, p.G, window, sinks);
   if (r.few.units > 0x7fffffffll / 64 || r.prompt.units * (r.prompt.nsplit ? r.prompt.nsplit : 1) > 0x7fffffffll / 64 || (long long)batch->max_rows * p.G > 0x3fffffffll)
     B200_FAIL(B200_ERR_SHAPE, "paged_attention: %d sequences of up to %d rows with %d heads in one call", batch->sequences, batch->max_rows, q_heads);
@@ -1242,7 +1296,6 @@ int b200_paged_attention(const b200_paged_cache* cache, const b200_paged_batch* 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int fmt = cache->kv_dtype == B200_KV_INT8 ? INT8 : E4M3;
   p.from_rows = r.from_rows;
-  p.direct = p.q_tiles = p.nsplit = 0; p.part_o = p.part_ml = nullptr; p.parts = nullptr;
   if (r.prompt.units) {
     AttnP x = p;
     x.q_tiles = r.prompt.q_tiles; x.nsplit = r.prompt.nsplit;

@@ -1,4 +1,5 @@
-// What the kernels of the paged 8-bit cache share (paged.cu: append, read, attention of few rows; paged_prompt.cu: attention of many rows of a sequence).
+// What the kernels of the paged 8-bit cache share (paged.cu: append, read, attention of few rows; paged_prompt.cu: attention of many rows of a sequence; paged_tree.cu: of trees of drafted tokens;
+// paged_pool.cu: kept rows and the pages of a pool).
 #pragma once
 
 #include <cuda.h>
@@ -157,6 +158,11 @@ __device__ __forceinline__ bool wait_or_quit(uint32_t bar, uint32_t parity, vola
     }
   }
 }
+// paged.cu: what a call's host arguments have to be; attention's in its kernels' form
+int checked_cache(const b200_paged_cache* cache, const char* what);
+int checked(const b200_paged_cache* cache, const b200_paged_batch* batch, const char* what);
+int attention_arguments(AttnP* p, const b200_paged_cache* cache, const b200_paged_batch* batch, const void* q_dev, int64_t q_ld, void* out_dev, int64_t out_ld, int q_heads, float scale, int window,
+                        int sinks, const char* what);
 // paged_prompt.cu
 struct PromptPlan { int q_tiles, nsplit; long long units; };
 PromptPlan prompt_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks);

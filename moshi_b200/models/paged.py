@@ -7,8 +7,21 @@ and its table of pages; ``RotaryTable`` holds the position rotation.  A layer's 
     q = cache.append(batch, k, v, q=q, rotary=rotary)
     out = cache.attend(batch, q, window=4096, sinks=4)
 
+Drafted tokens are checked as a tree (``PagedTree``): append at its positions, attend with its masks, and keep the accepted path; ``PagePool`` keeps account of who holds which pages, on the device, for
+forks, beams and requests that come and go::
+
+    pool = PagePool(caches, sequences, width)              # the caches of all layers
+    pool.reserve(add)                                      # pages for the step's rows
+    batch = PagedBatch(pool.table, pool.lengths, rows, total_rows, max_rows)
+    tree = PagedTree(batch, parents)
+    for cache in caches:
+        q = cache.append(batch, k, v, q=q, rotary=rotary, positions=tree.positions)
+        out = cache.attend(batch, q, tree=tree)
+    pool.keep(batch, kept, counts)
+    pool.lengths += counts
+
 The calls enqueue on the current stream and wait for nothing, so that they may be captured into a graph.  They are for inference: there are no gradients, and inputs that ask for
-one are refused.  Pages are handed out by the caller; a page that is written to must belong to one sequence of the batch only (pages that are only read may be shared).  A step
+one are refused.  Pages are handed out by the caller or a pool; a page that is written to must belong to one sequence of the batch only (pages that are only read may be shared).  A step
 of prompts and single rows is quicker as two batches over the same tensors, ``PagedBatch(table[:n], before[:n], rows[:n + 1], ...)`` and ``PagedBatch(table[n:], before[n:], rows[n:],
 ...)``, each with its own ``max_rows``: the other's rows belong to nobody and are left as they are.
 """
@@ -26,7 +39,9 @@ _KV = {"int8": (torch.int8, _lib.B200_KV_INT8), "fp8_e4m3": (torch.float8_e4m3fn
 _NAMES = {dtype: name for name, (dtype, _) in _KV.items()}
 # floor(2^192 / (2 pi))
 _TURN = (1 << 192) * 10 ** 60 // (2 * 3141592653589793238462643383279502884197169399375105820974944)
-BAD_BATCH, BAD_PAGE, NOT_FINITE, WAIT = 1, 2, 4, 8
+BAD_BATCH, BAD_PAGE, NOT_FINITE, WAIT, BAD_TREE, NO_PAGES = 1, 2, 4, 8, 16, 32
+MAX_NODES = 1024                                # of a tree
+MAX_AXES = 4
 
 
 def _cuda(device: torch.device | str) -> torch.device:
@@ -54,9 +69,11 @@ def turns_of(freqs: tp.Iterable[float]) -> list[int]:
 
 class RotaryTable:
     """Frequencies of a position rotation: ``base ** (-2 j / rot_dims)`` radians per position for the pair j, or ``freqs`` (rot_dims / 2 numbers).  ``pairing``: "adjacent" turns
-    dimensions (2j, 2j + 1), "halves" (j, j + rot_dims / 2); dimensions from ``rot_dims`` on stay as they are."""
+    dimensions (2j, 2j + 1), "halves" (j, j + rot_dims / 2); dimensions from ``rot_dims`` on stay as they are.  ``axes``: for each pair the axis (0 .. 3) whose position turns it, where rows have positions of
+    several (time, height, width); those are given to every ``append``."""
 
-    def __init__(self, rot_dims: int, base: float = 10000.0, pairing: str = "adjacent", freqs: tp.Sequence[float] | None = None, device: torch.device | str = "cuda"):
+    def __init__(self, rot_dims: int, base: float = 10000.0, pairing: str = "adjacent", freqs: tp.Sequence[float] | None = None, device: torch.device | str = "cuda",
+                 axes: tp.Sequence[int] | None = None):
         if rot_dims < 16 or rot_dims % 16:
             raise ValueError(f"rot_dims {rot_dims}: a multiple of 16")
         if pairing not in ROT_PAIRINGS:
@@ -64,12 +81,17 @@ class RotaryTable:
         freqs = [base ** (-2.0 * j / rot_dims) for j in range(rot_dims // 2)] if freqs is None else [float(f) for f in freqs]
         if len(freqs) != rot_dims // 2:
             raise ValueError(f"{len(freqs)} frequencies for {rot_dims} dimensions")
+        axes = [0] * len(freqs) if axes is None else [int(a) for a in axes]
+        if len(axes) != len(freqs) or min(axes) < 0 or max(axes) >= MAX_AXES:
+            raise ValueError(f"axes {axes}: one of 0 .. {MAX_AXES - 1} for each of {len(freqs)} pairs")
         turns = turns_of(freqs)
         self.device = _cuda(device)
         self.rot_dims, self.pairing = rot_dims, pairing
         self.turns = torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64, device=self.device)
         self._c = _lib.RotaryC(self.turns.data_ptr(), rot_dims, ROT_PAIRINGS[pairing])
         self._ref = C.addressof(self._c)
+        self.axes = max(axes) + 1
+        self.pair_axis = torch.tensor(axes, dtype=torch.uint8, device=self.device) if self.axes > 1 else None
 
 
 class PagedBatch:
@@ -96,6 +118,42 @@ class PagedBatch:
         self._index, self._work = table.device.index, {}
         self._c = _lib.PagedBatchC(table.data_ptr(), before.data_ptr(), rows.data_ptr(), max(table.stride(0), table.shape[1]), S, table.shape[1], total_rows, self.max_rows)
         self._ref = C.addressof(self._c)
+
+
+class PagedTree:
+    """The rows of a batch as trees of drafted tokens.  ``parents`` i32 [total_rows]: row i of a sequence comes behind its row parents[rows[s] + i], which has a lower number, or, -1, behind the last cached token; a
+    parent that is neither counts as -1 and is recorded.  At most 1024 rows of a sequence.  A row's position is before + depth (``positions`` i32 [total_rows], for ``append``); it sees what
+    is cached, itself and those that it comes behind (``seen`` i32 [total_rows, words], bit i for the sequence's row i).  All layers of a step share a tree; once ``parents`` or the batch's tensors have been refilled,
+    ``update`` fills it anew on the current stream."""
+
+    def __init__(self, batch: PagedBatch, parents: torch.Tensor):
+        if parents.dtype != torch.int32 or parents.shape != (batch.total_rows,) or parents.device != batch.device or (parents.numel() > 1 and parents.stride(0) != 1):
+            raise ValueError(f"parents: i32 [{batch.total_rows}], dense, on {batch.device}; got {parents.dtype}, {tuple(parents.shape)}, {parents.device}")
+        if batch.max_rows > MAX_NODES:
+            raise ValueError(f"trees of up to {batch.max_rows} rows: {MAX_NODES} at most")
+        words = max(1, -(-batch.max_rows // 32))
+        self.batch, self.parents = batch, parents
+        self.seen = torch.zeros(batch.total_rows, words, dtype=torch.int32, device=batch.device)
+        self.positions = torch.zeros(batch.total_rows, dtype=torch.int32, device=batch.device)
+        self.flags = torch.zeros(1, dtype=torch.int32, device=batch.device)
+        self._c = _lib.PagedTreeC(self.seen.data_ptr(), self.positions.data_ptr(), words)
+        self._ref = C.addressof(self._c)
+        self._build = _entry("b200_paged_tree_build")
+        self.update()
+
+    def update(self) -> None:
+        rc = self._build(self.batch._ref, self._ref, self.parents.data_ptr(), self.flags.data_ptr(), self.batch._index, _stream(self.batch._index)) if self.batch.total_rows else 0
+        if rc:
+            _lib.check(rc)
+
+    def error_flags(self) -> int:
+        """BAD_BATCH, BAD_TREE of updates since the last ``clear_error_flags``.  Waits for all streams of the device."""
+        torch.cuda.synchronize(self.batch.device)
+        return int(self.flags.item())
+
+    def clear_error_flags(self) -> None:
+        """Behind what the current stream has been given, and before what it is given next."""
+        self.flags.zero_()
 
 
 class PagedKVCache:
@@ -136,6 +194,7 @@ class PagedKVCache:
         self._c = _lib.PagedCacheC(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.flags.data_ptr(), self.pages, self.page_tokens, self.kv_heads, self.head_dim, _KV[self.dtype][1], self.device.index)
         self._ref = C.addressof(self._c)
         self._append, self._attend, self._bytes, self._read = (_entry(f"b200_paged_{n}") for n in ("append", "attention", "attention_bytes", "read"))
+        self._append_at, self._attend_tree, self._tree_bytes, self._keep = (_entry(f"b200_paged_{n}") for n in ("append_at", "tree_attention", "tree_attention_bytes", "keep"))
 
     def _rows(self, name: str, t: torch.Tensor, batch: PagedBatch, heads: int) -> int:
         """Checks a step's tensor [total_rows, heads, head_dim]; its elements from row to row."""
@@ -157,9 +216,10 @@ class PagedKVCache:
         return t.shape[1]
 
     def append(self, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None, rotary: RotaryTable | None = None,
-               q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+               q_out: torch.Tensor | None = None, positions: torch.Tensor | None = None) -> torch.Tensor | None:
         """Stores the step's keys and values, bf16 [total_rows, kv_heads, head_dim] (rows may lie apart, as in a projection of all three), keys rotated by their positions.  Returns
-        the queries ``q`` [total_rows, q_heads, head_dim] rotated likewise, in ``q_out`` (which may be ``q``) or a new tensor."""
+        the queries ``q`` [total_rows, q_heads, head_dim] rotated likewise, in ``q_out`` (which may be ``q``) or a new tensor.  ``positions`` i32 [total_rows] or [axes, total_rows]: positions of the rows' own
+        for the rotation, as a tree's tokens have (``PagedTree.positions``) or an image's patches; where a row is stored does not go by them."""
         k_ld, v_ld = self._rows("k", k, batch, self.kv_heads), self._rows("v", v, batch, self.kv_heads)
         if rotary is not None and (rotary.device != self.device or rotary.rot_dims > self.head_dim):
             raise ValueError(f"{rotary.rot_dims} rotated dimensions on {rotary.device} for heads of {self.head_dim} on {self.device}")
@@ -174,16 +234,33 @@ class PagedKVCache:
             q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")
-        rc = self._append(self._ref, batch._ref, k.data_ptr(), k_ld, v.data_ptr(), v_ld, q_ptr, q_ld, o_ptr, o_ld, heads, rotary._ref if rotary is not None else None,
-                          _stream(self._index))
+        if positions is not None:
+            at = self._positions(batch, rotary, positions)
+            rc = self._append_at(self._ref, batch._ref, k.data_ptr(), k_ld, v.data_ptr(), v_ld, q_ptr, q_ld, o_ptr, o_ld, heads, rotary._ref, C.addressof(at), _stream(self._index))
+        elif rotary is not None and rotary.axes > 1:
+            raise ValueError(f"a rotation of {rotary.axes} axes needs the rows' positions")
+        else:
+            rc = self._append(self._ref, batch._ref, k.data_ptr(), k_ld, v.data_ptr(), v_ld, q_ptr, q_ld, o_ptr, o_ld, heads, rotary._ref if rotary is not None else None,
+                              _stream(self._index))
         if rc:
             _lib.check(rc)
         return q_out
 
-    def attend(self, batch: PagedBatch, q: torch.Tensor, scale: float | None = None, window: int = 0, sinks: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    def _positions(self, batch: PagedBatch, rotary: RotaryTable | None, t: torch.Tensor) -> _lib.PagedPositionsC:
+        if rotary is None:
+            raise ValueError("positions without a rotary table")
+        if t.dim() == 1 and rotary.axes == 1:
+            t = t[None]
+        if t.dtype is not torch.int32 or t.shape != (rotary.axes, batch.total_rows) or t.get_device() != self._index or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+            raise ValueError(f"positions: i32 {[rotary.axes, batch.total_rows]}, dense along the rows, on {self.device}; got {t.dtype} {list(t.shape)}, strides {t.stride()}, {t.device}")
+        return _lib.PagedPositionsC(t.data_ptr(), max(t.stride(0), batch.total_rows), rotary.pair_axis.data_ptr() if rotary.pair_axis is not None else None, rotary.axes)
+
+    def attend(self, batch: PagedBatch, q: torch.Tensor, scale: float | None = None, window: int = 0, sinks: int = 0, out: torch.Tensor | None = None,
+               tree: PagedTree | None = None) -> torch.Tensor:
         """Attention of the step's rows over what their sequences have cached, the step's own rows included (``append`` comes first): the row at position p sees tokens j <= p
         and, with a ``window``, of these only p - j < window and the first ``sinks`` tokens.  q bf16 [total_rows, q_heads, head_dim], q_heads a multiple of kv_heads; scores are
-        multiplied by ``scale`` > 0 (default head_dim ** -0.5).  Rows that belong to no sequence are left as they are in ``out``; a query that is not finite gives NaN in its own row and head."""
+        multiplied by ``scale`` > 0 (default head_dim ** -0.5).  With a ``tree`` of this batch a row sees what is cached in front of the step and, of the step's rows, itself and those that it comes behind; window and
+        first tokens then go by the tree's positions.  Rows that belong to no sequence are left as they are in ``out``; a query that is not finite gives NaN in its own row and head."""
         heads = self._heads("q", q)
         q_ld = self._rows("q", q, batch, heads)
         if out is None:
@@ -192,11 +269,19 @@ class PagedKVCache:
             o_ld = self._rows("out", out, batch, heads)
         if not 0 <= window < 1 << 31 or not 0 <= sinks < 1 << 31:
             raise ValueError(f"window {window}, {sinks} first tokens")
-        of = (self._shape, heads, window, sinks)
+        if tree is not None and tree.batch is not batch:
+            raise ValueError("the tree is of another batch")
+        of = (self._shape, heads, window, sinks, tree is None)
         n = batch._work.get(of)                       # a size, by sizes alone; the layers of a step ask for the same
         if n is None:
-            n = batch._work[of] = self._bytes(self._ref, batch._ref, heads, window, sinks)
+            n = batch._work[of] = (self._bytes if tree is None else self._tree_bytes)(self._ref, batch._ref, heads, window, sinks)
         work = q.new_empty((n + 1) // 2) if n else None
+        if tree is not None:
+            rc = self._attend_tree(self._ref, batch._ref, tree._ref, q.data_ptr(), q_ld, out.data_ptr(), o_ld, heads, self.head_dim ** -0.5 if scale is None else scale, window, sinks,
+                                   work.data_ptr() if n else None, n, _stream(self._index))
+            if rc:
+                _lib.check(rc)
+            return out
         rc = self._attend(self._ref, batch._ref, q.data_ptr(), q_ld, out.data_ptr(), o_ld, heads, self.head_dim ** -0.5 if scale is None else scale, window, sinks,
                           work.data_ptr() if n else None, n, _stream(self._index))
         if rc:
@@ -213,8 +298,92 @@ class PagedKVCache:
             _lib.check(rc)
         return k, v
 
+    def keep(self, batch: PagedBatch, kept: torch.Tensor, counts: torch.Tensor) -> None:
+        """Of the step's rows sequence s keeps counts[s] (i32 [sequences]), those of the numbers kept[rows[s]], kept[rows[s] + 1], .. (i32 [total_rows]) among its own, which rise: the accepted path of a
+        tree.  They move to the places from before[s] on, and what lies behind them is of no use any more.  Codes move as they are within a page; to another page's scale they are rounded once more."""
+        _keep([self], self._ref, 1, batch, kept, counts)
+
     def error_flags(self) -> int:
         """What the kernels found wrong since the last ``clear_error_flags``: BAD_BATCH, BAD_PAGE, NOT_FINITE, WAIT.  Waits for all streams of the device."""
+        torch.cuda.synchronize(self.device)
+        return int(self.flags.item())
+
+    def clear_error_flags(self) -> None:
+        """Behind what the current stream has been given, and before what it is given next."""
+        self.flags.zero_()
+
+
+def _keep(caches: tp.Sequence[PagedKVCache], ref, n: int, batch: PagedBatch, kept: torch.Tensor, counts: torch.Tensor) -> None:
+    cache = caches[0]
+    for name, t, size in (("kept", kept, batch.total_rows), ("counts", counts, batch.sequences)):
+        if t.dtype is not torch.int32 or t.shape != (size,) or t.get_device() != cache._index or (size > 1 and t.stride(0) != 1):
+            raise ValueError(f"{name}: i32 [{size}], dense, on {cache.device}; got {t.dtype} {list(t.shape)}, {t.device}")
+    if batch._index != cache._index:
+        raise ValueError(f"the batch on {batch.device}, the cache on {cache.device}")
+    rc = cache._keep(ref, n, batch._ref, kept.data_ptr(), counts.data_ptr(), _stream(cache._index))
+    if rc:
+        _lib.check(rc)
+
+
+class PagePool:
+    """Who holds which pages, on the device, for sequences whose tokens lie in ``caches`` (one per layer, alike).  ``table`` i32 [sequences, width], -1 behind what a sequence holds; ``lengths`` i32 [sequences]: tokens that
+    it has (the caller's to raise, by what a step has left); ``held``: pages that it holds, enough for them; ``refs`` i32 [pages]: sequences that hold a page.  A pool begins empty.  ``table`` and
+    ``lengths`` are what a ``PagedBatch`` takes.  The calls may be captured; none waits."""
+
+    def __init__(self, caches: tp.Sequence[PagedKVCache], sequences: int, width: int):
+        caches = list(caches)
+        if not caches or any((c.device, c.pages, c._shape, c.dtype) != (caches[0].device, caches[0].pages, caches[0]._shape, caches[0].dtype) for c in caches):
+            raise ValueError("a pool's caches are alike: device, pages, sizes and type")
+        if not 1 <= sequences <= 4096 or width < 1:
+            raise ValueError(f"{sequences} sequences (1 .. 4096) of {width} pages")
+        self.caches, self.device, self.sequences, self.width, self.pages = caches, caches[0].device, int(sequences), int(width), caches[0].pages
+        i32 = dict(dtype=torch.int32, device=self.device)
+        self.table = torch.full((sequences, width), -1, **i32)
+        self.lengths, self.held, self.refs, self.flags = (torch.zeros(n, **i32) for n in (sequences, sequences, self.pages, 1))
+        self._c = _lib.PagePoolC(self.table.data_ptr(), self.lengths.data_ptr(), self.held.data_ptr(), self.refs.data_ptr(), self.flags.data_ptr(), width, sequences, width, self.pages,
+                                 caches[0].page_tokens, self.device.index)
+        self._ref, self._index = C.addressof(self._c), self.device.index
+        self._of = (_lib.PagedCacheC * len(caches))(*(c._c for c in caches))
+        self._caches = C.addressof(self._of)
+        self._rearrange, self._reserve, self._compact = (_entry(f"b200_page_pool_{n}") for n in ("rearrange", "reserve", "compact"))
+        self._bytes = _entry("b200_page_pool_bytes")(self._ref)
+
+    def _work(self) -> torch.Tensor:
+        return torch.empty(self._bytes, dtype=torch.uint8, device=self.device)
+
+    def _of_sequences(self, name: str, t: torch.Tensor) -> int:
+        if t.dtype is not torch.int32 or t.shape != (self.sequences,) or t.get_device() != self._index or (self.sequences > 1 and t.stride(0) != 1):
+            raise ValueError(f"{name}: i32 [{self.sequences}], dense, on {self.device}; got {t.dtype} {list(t.shape)}, {t.device}")
+        return t.data_ptr()
+
+    def rearrange(self, source: torch.Tensor) -> None:
+        """All at once, sequence i becomes what sequence source[i] was (i32 [sequences]), -1: empty.  Forks requests (their pages are shared), moves beams, gives pages back; so are pages that were held in reserve."""
+        at, work = self._of_sequences("source", source), self._work()
+        rc = self._rearrange(self._ref, at, work.data_ptr(), self._bytes, _stream(self._index))
+        if rc:
+            _lib.check(rc)
+
+    def reserve(self, add: torch.Tensor) -> None:
+        """Pages for add[s] tokens (i32 [sequences]) behind the lengths[s] that sequence s has: by rising numbers, to sequences by rising numbers.  Where the next token goes to a partly filled page that others hold too, the
+        sequence gets a copy of it first, in all caches (of those in this call that share it, the last keeps it if nobody else holds it).  With too few free pages nobody gets any, and NO_PAGES is recorded."""
+        at, work = self._of_sequences("add", add), self._work()
+        rc = self._reserve(self._ref, self._caches, len(self.caches), at, work.data_ptr(), self._bytes, _stream(self._index))
+        if rc:
+            _lib.check(rc)
+
+    def compact(self) -> None:
+        """Moves the pages in use to the lowest numbers, in all caches."""
+        work = self._work()
+        rc = self._compact(self._ref, self._caches, len(self.caches), work.data_ptr(), self._bytes, _stream(self._index))
+        if rc:
+            _lib.check(rc)
+
+    def keep(self, batch: PagedBatch, kept: torch.Tensor, counts: torch.Tensor) -> None:
+        """``PagedKVCache.keep`` in all caches at once; what is found wrong is recorded in the first one's flags.  ``lengths`` stay as they are."""
+        _keep(self.caches, self._caches, len(self.caches), batch, kept, counts)
+
+    def error_flags(self) -> int:
+        """BAD_BATCH, BAD_PAGE, NO_PAGES of calls since the last ``clear_error_flags``.  Waits for all streams of the device."""
         torch.cuda.synchronize(self.device)
         return int(self.flags.item())
 
