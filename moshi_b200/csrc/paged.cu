@@ -1045,9 +1045,6 @@ __global__ void __launch_bounds__(128) join_kernel(const AttnP p) {
 // =========================================================================================================================
 // host
 // =========================================================================================================================
-typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 int check_cache(const b200_paged_cache* c, const char* what) {
   if (!c || !c->k_dev || !c->v_dev || !c->k_scale_dev || !c->v_scale_dev || !c->flags_dev) B200_FAIL(B200_ERR_INVALID, "%s: null pointer in the cache", what);
   if (c->kv_dtype != B200_KV_INT8 && c->kv_dtype != B200_KV_FP8_E4M3) B200_FAIL(B200_ERR_INVALID, "%s: kv_dtype %d", what, c->kv_dtype);
@@ -1097,23 +1094,6 @@ FewPlan few_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, in
 }
 // sums and (maximum, sum of the weights) of two parts per CTA, and where each unit's parts are
 int64_t few_bytes(const FewPlan& f, int D) { return f.direct ? 0 : (int64_t)f.ctas * 2 * 8 * f.nt * (D + 2) * 4 + f.units * 8; }
-
-// A tensor map over a cache's codes, [rows][dim], boxes of 16 whole rows, swizzled by 128 bytes (dim 64: by 64).
-int code_map(CUtensorMap* m, const void* codes, long long rows, int dim) {
-  static const EncodeFn fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
-    return reinterpret_cast<EncodeFn>(f);
-  }();
-  if (!fn) B200_FAIL(B200_ERR_CUDA, "cuTensorMapEncodeTiled not available");
-  cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)dim};
-  cuuint32_t box[2] = {(cuuint32_t)dim, 16}, est[2] = {1, 1};
-  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, est, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) B200_FAIL(B200_ERR_CUDA, "paged cache: tensor map of %lld rows of %d codes refused (%d)", rows, dim, (int)r);
-  return B200_OK;
-}
 
 struct Route { int from_rows; FewPlan few; PromptPlan prompt; int64_t few_bytes, prompt_bytes; };
 Route route(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks) {
@@ -1171,6 +1151,23 @@ int launch_append(AppendP& p, cudaStream_t st) {
 
 }  // namespace
 
+int code_map(CUtensorMap* m, const void* codes, long long rows, int dim) {
+  typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  if (!fn) B200_FAIL(B200_ERR_CUDA, "cuTensorMapEncodeTiled not available");
+  cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)dim};
+  cuuint32_t box[2] = {(cuuint32_t)dim, 16}, est[2] = {1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, est, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) B200_FAIL(B200_ERR_CUDA, "paged cache: tensor map of %lld rows of %d codes refused (%d)", rows, dim, (int)r);
+  return B200_OK;
+}
 int checked_cache(const b200_paged_cache* cache, const char* what) { return check_cache(cache, what); }
 int checked(const b200_paged_cache* cache, const b200_paged_batch* batch, const char* what) {
   B200_TRY(check_cache(cache, what));

@@ -22,6 +22,7 @@ __device__ __forceinline__ void tmem_ld_wait32(uint32_t* r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : R32(r, 0), R32(r, 8), R32(r, 16), R32(r, 24) :: "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait16(uint32_t* r) { asm volatile("tcgen05.wait::ld.sync.aligned;" : R32(r, 0), R32(r, 8) :: "memory"); }
+__device__ __forceinline__ void tmem_ld_wait8(uint32_t* r) { asm volatile("tcgen05.wait::ld.sync.aligned;" : R32(r, 0) :: "memory"); }
 #undef R32
 #define R8(r, o) "r"((r)[o]), "r"((r)[o + 1]), "r"((r)[o + 2]), "r"((r)[o + 3]), "r"((r)[o + 4]), "r"((r)[o + 5]), "r"((r)[o + 6]), "r"((r)[o + 7])
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {

@@ -1,12 +1,13 @@
 // Attention of trees of drafted tokens over the paged 8-bit cache: a row sees what its sequence has cached in front of the step, and of the step's own tokens itself and those that it comes behind.
 //
-// Columns are (row of the sequence, query head of the group).  A unit is C = 32, 64 or 128 of them with one kv head, and a CTA walks its keys in tiles of 128 tokens.  The tensor cores' tiles have 128 rows,
-// and a tree has 20 to 100 columns as often as not: the rows are R = 128 / C copies of the columns, of which each weighs C of a tile's 128 keys.  So all threads of the weights have work whatever C is, with a
+// Columns are (row of the sequence, query head of the group).  A unit is C = 32, 64 or 128 of them with one kv head, and a CTA walks its keys in tiles of 64 tokens.  The tensor cores' tiles have 128 rows,
+// and a tree has 20 to 100 columns as often as not: the rows are R = 128 / C copies of the columns, of which each weighs 64 / R of a tile's keys.  So all threads of the weights have work whatever C is, with a
 // running maximum of their own; the products of a copy's rows with the other copies' keys are thrown away (scores) or made of zeros (P is block-diagonal, and the zeros are written once).  Tiles go to
 // two groups of weight warps in turn, with a sum O of each, so that the scores of one tile, the weights of another and the sum over a third are made at the same time.  At a unit's end its 2 R sums
 // are joined through shared memory.
 //
-// Units lie one behind the other and are cut into equal runs, one per CTA, as in paged.cu.  Codes, scales, f16 tiles and the lazy maximum are those of paged_prompt.cu.
+// Codes come as swizzled tensor copies (a producer warp, 72 KB on their way); six warps turn them into f16 tiles; one issues the products: S = Q K^T with Q in TMEM, O += P V with P there.  Units lie
+// one behind the other and are cut into equal runs, one per CTA, as in paged.cu.  Codes, scales, f16 tiles and the lazy maximum are those of paged_prompt.cu.
 #include "paged_tc.cuh"
 
 #include <cfloat>
@@ -66,8 +67,8 @@ __global__ void __launch_bounds__(128) tree_build_kernel(const BuildP p) {
 // =========================================================================================================================
 // attention
 // =========================================================================================================================
-constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 7, THREADS = (SOFT_WARPS + CONVERT_WARPS + 1) * 32, KEYS = 128, INFOS = 8;
-constexpr int UNIT_COST = 6, MIN_RUN = 6;    // in tiles: what a unit costs beside its own, and the least of a CTA
+constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 6, PRODUCER = 14, ISSUER = 15, THREADS = 16 * 32, SHIFT = 6, KEYS = 1 << SHIFT, STAGES = 4, INFOS = 16;
+constexpr int UNIT_COST = 10, MIN_RUN = 10;  // in tiles: what a unit costs beside its own, and the least of a CTA
 
 struct TreeP : AttnP {
   const uint32_t* seen;                      // [rows][words]: bit i of a row: it sees the sequence's i-th token of the step
@@ -78,15 +79,19 @@ struct TreeP : AttnP {
 
 template <int D>
 struct TreeSmem {
-  static constexpr uint32_t TILE = 128 * D * 2, HALF = 128 * 128;             // 128 rows of f16, in halves of 64 dims
-  static constexpr uint32_t Q = 0, K = TILE, V = 3 * TILE, JOIN = 5 * TILE, BYTES = JOIN + 256 * 128 + 1024;
+  static constexpr int SLOTS = CONVERT_WARPS * (D == 128 ? 3 : 6);            // places of 32 tokens' codes; a place is always the same warp's
+  static constexpr uint32_t HALF = KEYS * 128, TILE = HALF * (D / 64);        // a tile's f16 rows, in halves of 64 dims
+  static constexpr uint32_t SLOT = 32 * D, K = 0, V = K + STAGES * TILE, CODES = V + STAGES * TILE, JOIN = CODES + SLOTS * SLOT, BYTES = JOIN + 256 * D / 2 + 1024;
 };
+// What is to be known of a tile: its first token, first and last position of the unit's rows, whether every row sees all of it (1) and whether all its tokens are there and may be seen (2); and of each 16
+// tokens: keys' scale, log2 and reciprocal of the values', 1 where there is a page.
+struct TileInfo { int j0, pf, pl, whole; float4 group[KEYS / 16]; };
 
 // ---- the flattened work ----
 template <int C>
 __device__ __forceinline__ int units_of(const AttnP& p, const Seq& q) { return !q.ok || q.n == 0 ? 0 : p.H * ((q.n * p.G + C - 1) / C); }
 // all units of a sequence take its whole range, from the first row's window on
-__device__ __forceinline__ int places_of(const AttnP& p, const Seq& q) { return Tiles<7>(q.before, q.before + q.n - 1, p.window, p.sinks).n + UNIT_COST; }
+__device__ __forceinline__ int places_of(const AttnP& p, const Seq& q) { return Tiles<SHIFT>(q.before, q.before + q.n - 1, p.window, p.sinks).n + UNIT_COST; }
 template <int C>
 __device__ __forceinline__ long long work_of(const AttnP& p, int s) {
   const Seq q = sequence(p.b, s, p.P);
@@ -143,62 +148,104 @@ __device__ Run run_of(const AttnP& p) {
   return r;
 }
 // A part of a unit: places u0 .. u1 - 1 of n_pos, of which the first UNIT_COST are no tiles; tiles t0 .. t0 + n - 1 of the sequence's.
-struct Part { Seq q; int s, h, ct, u0, u1, n_pos, t0, n; };
-template <int C>
+struct Part {
+  Seq q;
+  int s, h, ct, u0, u1, n_pos, t0, n;
+  int first, from;                           // of the sequence's tiles: those in front of `first` are the first ones' (Tiles)
+  __device__ __forceinline__ int tile(int x) const { const int i = t0 + x; return i < first ? i : from + i - first; }
+};
+// A warp's way through its CTA's parts.  It lies in shared memory, as every warp's roles have other uses for 20 registers.
 struct Walk {
   long long f, to, base;
   int s, units, places;
   Seq q;
-  __device__ __forceinline__ void at(const AttnP& p) {
-    q = sequence(p.b, s, p.P);
-    units = units_of<C>(p, q);
-    places = units ? places_of(p, q) : 1;
-  }
-  __device__ __forceinline__ Walk(const AttnP& p, const Run& r) : f(r.from), to(r.to), base(r.base), s(r.s) { at(p); }
-  __device__ __forceinline__ bool next(const AttnP& p, Part& x) {
-    if (f >= to) return false;
-    while (f >= base + (long long)units * places && s + 1 < p.b.S) {          // the next sequence that has work
-      base += (long long)units * places;
-      ++s;
-      at(p);
-    }
-    const long long o = f - base;
-    const int u = o < 0x7fffffffll ? (int)((uint32_t)o / (uint32_t)places) : (int)(o / places), cts = units / p.H;
-    x.q = q; x.s = s; x.h = u / cts; x.ct = u - x.h * cts; x.n_pos = places;
-    x.u0 = (int)(o - (long long)u * places); x.u1 = (int)min((long long)places, x.u0 + (to - f));
-    f += x.u1 - x.u0;
-    x.t0 = max(x.u0 - UNIT_COST, 0); x.n = max(x.u1 - UNIT_COST, 0) - x.t0;
-    return true;
-  }
+  Part part[2];                              // the last one at `now`, the one in front of it beside it
+  int now;
 };
+template <int C>
+__device__ __forceinline__ void walk_to(Walk& w, const AttnP& p, int s) {
+  w.s = s;
+  w.q = sequence(p.b, s, p.P);
+  w.units = units_of<C>(p, w.q);
+  w.places = w.units ? places_of(p, w.q) : 1;
+}
+// by one lane
+template <int C>
+__device__ __forceinline__ bool walk_on(Walk& w, const AttnP& p) {
+  if (w.f >= w.to) return false;
+  while (w.f >= w.base + (long long)w.units * w.places && w.s + 1 < p.b.S) {  // the next sequence that has work
+    w.base += (long long)w.units * w.places;
+    walk_to<C>(w, p, w.s + 1);
+  }
+  w.now ^= 1;
+  Part& x = w.part[w.now];
+  const long long o = w.f - w.base;
+  const int u = o < 0x7fffffffll ? (int)((uint32_t)o / (uint32_t)w.places) : (int)(o / w.places), cts = w.units / p.H;
+  x.q = w.q; x.s = w.s; x.h = u / cts; x.ct = u - x.h * cts; x.n_pos = w.places;
+  x.u0 = (int)(o - (long long)u * w.places); x.u1 = (int)min((long long)w.places, x.u0 + (w.to - w.f));
+  w.f += x.u1 - x.u0;
+  const Tiles<SHIFT> tiles(w.q.before, w.q.before + w.q.n - 1, p.window, p.sinks);
+  x.first = tiles.first; x.from = tiles.from;
+  x.t0 = max(x.u0 - UNIT_COST, 0); x.n = max(x.u1 - UNIT_COST, 0) - x.t0;
+  return true;
+}
+// by the whole warp: the next part, null behind the last
+template <int C>
+__device__ __forceinline__ const Part* next_part(Walk& w, const AttnP& p) {
+  __syncwarp();                              // the part before the one in front has been read
+  bool more = false;
+  if ((threadIdx.x & 31) == 0) more = walk_on<C>(w, p);
+  more = __shfl_sync(0xffffffffu, more, 0);
+  __syncwarp();                              // what lane 0 has written is there for all
+  return more ? &w.part[w.now] : nullptr;
+}
 
-// registers of a weight thread and of the others: together those that the block was launched with
-template <int C> constexpr int soft_regs() { return C == 128 ? 176 : 128; }
+// D[128 rows][n] (+)= A B^T over 16 of k: A in TMEM (8 columns of two f16), B's rows [n][64 of k] in shared memory, swizzled
+__device__ __forceinline__ void product_tk(uint32_t d, uint32_t a, uint32_t b_smem, uint32_t idesc, uint32_t accumulate) {
+  const uint64_t desc = (uint64_t)desc_low(b_smem) | (uint64_t)DESC_HIGH << 32;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+#define R8(r, o) "r"((r)[o]), "r"((r)[o + 1]), "r"((r)[o + 2]), "r"((r)[o + 3]), "r"((r)[o + 4]), "r"((r)[o + 5]), "r"((r)[o + 6]), "r"((r)[o + 7])
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), R8(r, 0) : "memory");
+}
+#undef R8
+// registers of a weight thread; with those of the others they are what the block was launched with
+template <int C> constexpr int soft_regs() { return C == 128 ? 168 : 144; }
 
 template <int D, int FMT, int C>
-__global__ void __launch_bounds__(THREADS, 1) tree_kernel(const TreeP p) {
+__global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TreeP p) {
   typedef TreeSmem<D> L;
-  constexpr int R = 128 / C;
+  constexpr int R = 128 / C, HOLD = KEYS / R, SLOTS = L::SLOTS;               // HOLD: scores of a weight thread
+  // TMEM: scores and weights of the two groups of warps, their sums, the queries
+  constexpr uint32_t P_AT = 2 * KEYS, O_AT = P_AT + KEYS, Q_AT = 512 - D / 2;
+  static_assert(O_AT + 2 * D <= Q_AT, "TMEM");
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[17 + INFOS];
-  __shared__ float4 info[INFOS][8];          // per 16 keys: keys' scale, log2 and reciprocal of the values'; there: whether the page is
-  __shared__ __align__(16) uint32_t there[INFOS][8];
+  __shared__ __align__(8) uint64_t bars[2 * SLOTS + 4 * STAGES + 9 + INFOS];
+  __shared__ __align__(16) TileInfo infos[INFOS];
   __shared__ uint32_t tmem_at;
   __shared__ volatile int quit;              // somebody has waited too long: nobody waits any more, and all go through to the end
+  __shared__ int end;                        // number of the converters' jobs, once it is known
   __shared__ float factors[C];               // of a column: what turns a product of codes into a score in base 2, but for the keys' scale
   __shared__ float2 ml[256], total[C];
+  __shared__ Walk walks[THREADS / 32];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t bar = smem_u32(bars), k_full = bar, k_empty = bar + 16, v_full = bar + 32, v_empty = bar + 48, s_full = bar + 64, p_full = bar + 80, o_done = bar + 96, s_taken = bar + 112, q_full = bar + 128, i_full = bar + 136;
+  const uint32_t bar = smem_u32(bars), c_full = bar, c_empty = c_full + 8 * SLOTS, k_full = c_empty + 8 * SLOTS, k_empty = k_full + 8 * STAGES, v_full = k_empty + 8 * STAGES, v_empty = v_full + 8 * STAGES,
+                 s_full = v_empty + 8 * STAGES, p_full = s_full + 16, o_done = p_full + 16, s_taken = o_done + 16, q_full = s_taken + 16, i_full = q_full + 8;
   if (threadIdx.x == 0) {
     quit = 0;
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(k_full + 8 * i, 4); mbar_init(k_empty + 8 * i, 1); mbar_init(v_full + 8 * i, 4); mbar_init(v_empty + 8 * i, 1);
-      mbar_init(s_full + 8 * i, 1); mbar_init(s_taken + 8 * i, 4); mbar_init(p_full + 8 * i, 4); mbar_init(o_done + 8 * i, 1);
-    }
-    mbar_init(q_full, SOFT_WARPS);
-    for (int i = 0; i < INFOS; ++i) mbar_init(i_full + 8 * i, 4);
+    end = 0x7fffffff;
+    for (int i = 0; i < SLOTS; ++i) { mbar_init(c_full + 8 * i, 1); mbar_init(c_empty + 8 * i, 1); }
+    for (int i = 0; i < STAGES; ++i) { mbar_init(k_full + 8 * i, 2); mbar_init(k_empty + 8 * i, 1); mbar_init(v_full + 8 * i, 2); mbar_init(v_empty + 8 * i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(s_full + 8 * i, 1); mbar_init(s_taken + 8 * i, 4); mbar_init(p_full + 8 * i, 4); mbar_init(o_done + 8 * i, 1); }
+    mbar_init(q_full, 4);
+    for (int i = 0; i < INFOS; ++i) mbar_init(i_full + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   pdl_trigger();
@@ -207,183 +254,206 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const TreeP p) {
   if (threadIdx.x == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
   const Run run = run_of<C>(p);
   if (run.s < 0) return;                     // the whole block
-  if (warp == SOFT_WARPS + CONVERT_WARPS) tmem_alloc(smem_u32(&tmem_at), 512);
+  if (warp == ISSUER) tmem_alloc(smem_u32(&tmem_at), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_at;
-  Walk<C> walk(p, run);
-  Part u;
+  Walk& walk = walks[warp];
+  if (lane == 0 && (warp < SOFT_WARPS || warp >= PRODUCER)) {
+    walk.f = run.from; walk.to = run.to; walk.base = run.base; walk.now = 0;
+    walk_to<C>(walk, p, run.s);
+  }
 
-  // Tiles are numbered through all parts, g = 0, 1, ..: tile g has the places g & 1 of keys and values, and the weight warps g & 1.
+  // Tiles are numbered through all parts, g = 0, 1, ..: tile g has the places g % STAGES of keys and values, and the weight warps g & 1; its codes are the jobs 4 g .. 4 g + 3, 32 tokens of keys or values each.
   if (warp >= SOFT_WARPS) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(256 - soft_regs<C>()));
-  if (warp < SOFT_WARPS + CONVERT_WARPS) {
-    // ---- codes into f16 tiles: 32 tokens of a tile's keys or values at a time, eight such tasks a tile, which the warps take in turn ----
-    constexpr int LANES = D / 16, STEP = 32 / LANES, LOADS = 32 / STEP;       // lanes a row, rows a load, loads
-    const int row = lane / LANES, c = lane % LANES;
+  if (warp < PRODUCER) {
+    // ---- codes into f16 tiles ----
+    constexpr int LANES = D / 16, STEP = 32 / LANES;     // lanes a row, rows at a time
+    const int c = lane % LANES;
     // lanes of a row's second 64 dims take the neighbouring row, so that eight lanes' pieces of the f16 tile lie in different banks
-    const int r_in = row ^ (D == 128 ? c >> 2 : 0);
-    struct Job { int task, j0, h, pf, pl, page; };      // task: numbered through all tiles, -1: none; page: lane l's, of tokens j0 + (l & 1) * 16 ..
-    int at = warp - SOFT_WARPS, first = 0, count = 0;   // the next task, and the part's
-    u.n = 0;
-    auto next_job = [&]() {
-      Job x;
-      x.task = -1;
-      while (at >= first + count) {
-        first += count;
-        if (!walk.next(p, u)) { count = 0; return x; }
-        count = 8 * u.n;
-      }
-      const int t = at - first;
-      const Tiles<7> tiles(u.q.before, u.q.before + u.q.n - 1, p.window, p.sinks);
-      x.task = at; x.h = u.h; x.pf = u.q.before; x.pl = u.q.before + u.q.n - 1;
-      x.j0 = (tiles[u.t0 + (t >> 3)] << 7) + 32 * (t & 3);
-      const int j = x.j0 + 16 * (lane & 1);
-      x.page = -1;
-      if (j <= x.pl && (p.window <= 0 || x.pf - j - 15 < p.window || j < p.sinks)) {
-        x.page = p.b.table[u.s * p.b.table_ld + (j >> p.page_shift)];
-        if (x.page < 0 || x.page >= p.pages) { x.page = -1; atomicOr(p.flags, B200_PAGED_BAD_PAGE); }
-      }
-      at += CONVERT_WARPS;
-      return x;
-    };
-    uint4 held[LOADS];                       // of the job to come
-    float2 scales = make_float2(0.f, 1.f);
-    auto load = [&](const Job& x) {
-      if (x.task < 0) return;
-      const bool keys = !(x.task & 4);
-      const uint8_t* codes = keys ? p.k : p.v;
-      if (keys && x.page >= 0) scales = make_float2(p.k_scale[(long long)x.page * p.H + x.h], p.v_scale[(long long)x.page * p.H + x.h]);
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int pg = __shfl_sync(0xffffffffu, x.page, half), j1 = x.j0 + 16 * half;
-        const uint8_t* from = codes + (((long long)pg * p.H + x.h) * p.P + (j1 & (p.P - 1)) + r_in) * D + 16 * c;
-        // values that no row sees may be anything; keys are masked
-        const bool all = keys || (j1 + 15 <= x.pl && (p.window <= 0 || x.pf - j1 < p.window || j1 + 16 <= p.sinks));
-#pragma unroll
-        for (int i = 0; i < LOADS / 2; ++i) {
-          const int j = j1 + i * STEP + r_in;
-          const bool seen = pg >= 0 && (all || (j <= x.pl && (p.window <= 0 || x.pf - j < p.window || j < p.sinks)));
-          held[half * (LOADS / 2) + i] = seen ? *reinterpret_cast<const uint4*>(from + i * STEP * D) : make_uint4(0, 0, 0, 0);
+    const int r_in = lane / LANES ^ (D == 128 ? c >> 2 : 0);
+    for (int j = warp - SOFT_WARPS;; j += CONVERT_WARPS) {
+      const int slot = j % SLOTS, g = j >> 2, st = g % STAGES, half = j & 1;
+      const bool values = j & 2;
+      warp_wait(c_full + 8 * slot, (uint32_t)(j / SLOTS) & 1u, &quit);
+      if (__any_sync(0xffffffffu, quit || j >= *(volatile int*)&end)) break;
+      warp_wait((values ? v_empty : k_empty) + 8 * st, ((uint32_t)(g / STAGES) & 1u) ^ 1u, &quit);
+      const TileInfo& t = infos[g % INFOS];
+      const bool all = !values || (t.whole & 2);         // values that no row sees may be anything; keys are masked
+      const uint8_t* from = smem + L::CODES + slot * L::SLOT;
+      uint8_t* const to = smem + (values ? L::V : L::K) + st * L::TILE + (c >> 2) * L::HALF;
+#pragma unroll 4
+      for (int i = 0; i < 32 / STEP; ++i) {
+        const int r = i * STEP + r_in, n = 32 * half + r;
+        uint4 x = *reinterpret_cast<const uint4*>(from + (D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ (r >> 1 & 3)) << 4)));
+        if (!all) {
+          const int token = t.j0 + n;
+          if (!(t.group[n >> 4].w != 0.f && token <= t.pl && (p.window <= 0 || t.pf - token < p.window || token < p.sinks))) x = make_uint4(0, 0, 0, 0);
         }
-      }
-    };
-    Job job = next_job();
-    load(job);
-    Job then = next_job();
-    while (job.task >= 0) {
-      const int g = job.task >> 3, st = g & 1, w4 = job.task & 3;
-      const bool keys = !(job.task & 4);
-      if (keys) {                            // what the weights need to know of these keys' pages
-        if (lane < 2) {
-          const float vs = value_scale(scales.y);
-          there[g % INFOS][2 * w4 + lane] = job.page >= 0 ? 1u : 0u;
-          info[g % INFOS][2 * w4 + lane] = job.page >= 0 ? make_float4(scales.x > 0.f ? scales.x : 1.f, __log2f(vs), __frcp_rn(vs), 0.f) : make_float4(1.f, 0.f, 0.f, 0.f);
-        }
-        __syncwarp();
-      }
-      warp_wait((keys ? k_empty : v_empty) + 8 * st, ((uint32_t)(g >> 1) & 1u) ^ 1u, &quit);
-      if (keys && lane == 0) mbar_arrive(i_full + 8 * (g % INFOS));
-      uint8_t* const dst = smem + (keys ? L::K : L::V) + st * L::TILE + (c >> 2) * L::HALF;
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int t = 32 * w4 + i * STEP + r_in;
-        const uint32_t w[4] = {ready<FMT>(held[i].x), ready<FMT>(held[i].y), ready<FMT>(held[i].z), ready<FMT>(held[i].w)};
-        uint8_t* r = dst + t * 128;
-        *reinterpret_cast<uint4*>(r + (((2 * (c & 3)) ^ (t & 7)) << 4)) = make_uint4(half2_of<FMT, 0>(w[0]), half2_of<FMT, 1>(w[0]), half2_of<FMT, 0>(w[1]), half2_of<FMT, 1>(w[1]));
-        *reinterpret_cast<uint4*>(r + (((2 * (c & 3) + 1) ^ (t & 7)) << 4)) = make_uint4(half2_of<FMT, 0>(w[2]), half2_of<FMT, 1>(w[2]), half2_of<FMT, 0>(w[3]), half2_of<FMT, 1>(w[3]));
+        const uint32_t w[4] = {ready<FMT>(x.x), ready<FMT>(x.y), ready<FMT>(x.z), ready<FMT>(x.w)};
+        uint8_t* y = to + n * 128;
+        *reinterpret_cast<uint4*>(y + (((2 * (c & 3)) ^ (n & 7)) << 4)) = make_uint4(half2_of<FMT, 0>(w[0]), half2_of<FMT, 1>(w[0]), half2_of<FMT, 0>(w[1]), half2_of<FMT, 1>(w[1]));
+        *reinterpret_cast<uint4*>(y + (((2 * (c & 3) + 1) ^ (n & 7)) << 4)) = make_uint4(half2_of<FMT, 0>(w[2]), half2_of<FMT, 1>(w[2]), half2_of<FMT, 0>(w[3]), half2_of<FMT, 1>(w[3]));
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive((keys ? k_full : v_full) + 8 * st);
-      job = then;
-      load(job);
-      then = next_job();
+      if (lane == 0) { mbar_arrive(c_empty + 8 * slot); mbar_arrive((values ? v_full : k_full) + 8 * st); }
+    }
+  } else if (warp == PRODUCER) {
+    // ---- copies: pages and scales are looked up for eight tiles at a time, a lane for each 16 tokens, and eight tiles ahead ----
+    int g = 0;
+    for (const Part* u; (u = next_part<C>(walk, p)) != nullptr;) {
+      const int n = u->n, h = u->h, pf = u->q.before, pl = pf + u->q.n - 1;
+      auto look_up = [&](int batch) {
+        const int x = 8 * batch + (lane >> 2);
+        if (x >= n) return -1;
+        const int j = (u->tile(x) << SHIFT) + 16 * (lane & 3);
+        if (j > pl || (p.window > 0 && pf - j - 15 >= p.window && j >= p.sinks)) return -1;
+        const int page = p.b.table[u->s * p.b.table_ld + (j >> p.page_shift)];
+        if (page >= 0 && page < p.pages) return page;
+        atomicOr(p.flags, B200_PAGED_BAD_PAGE);
+        return -1;
+      };
+      auto scales_of = [&](int page) { return page < 0 ? make_float2(1.f, 1.f) : make_float2(p.k_scale[(long long)page * p.H + h], p.v_scale[(long long)page * p.H + h]); };
+      int page = -1, page_next = look_up(0);
+      float2 scale = make_float2(1.f, 1.f), scale_next = scales_of(page_next);
+      for (int x = 0; x < n; ++x, ++g) {
+        if ((x & 7) == 0) { page = page_next; scale = scale_next; page_next = look_up((x >> 3) + 1); }
+        if ((x & 7) == 4) scale_next = scales_of(page_next);
+        const int j0 = u->tile(x) << SHIFT, first = 4 * (x & 7);
+        const bool there = (__ballot_sync(0xffffffffu, page >= 0) >> first & 15u) == 15u;
+        TileInfo& t = infos[g % INFOS];
+        if (lane >> 2 == (x & 7)) {
+          const float vs = value_scale(scale.y);
+          t.group[lane & 3] = page >= 0 ? make_float4(scale.x > 0.f ? scale.x : 1.f, __log2f(vs), __frcp_rn(vs), 1.f) : make_float4(1.f, 0.f, 0.f, 0.f);
+        }
+        if (lane == 0) {
+          const bool whole = there && j0 + KEYS <= pf && (p.window <= 0 || pl - j0 < p.window || j0 + KEYS <= p.sinks);
+          const bool seen = there && j0 + KEYS - 1 <= pl && (p.window <= 0 || pf - j0 < p.window || j0 + KEYS <= p.sinks);
+          t.j0 = j0; t.pf = pf; t.pl = pl; t.whole = (whole ? 1 : 0) | (seen ? 2 : 0);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(i_full + 8 * (g % INFOS));
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) {
+          const int j = 4 * g + k, slot = j % SLOTS;
+          warp_wait(c_empty + 8 * slot, ((uint32_t)(j / SLOTS) & 1u) ^ 1u, &quit);
+          const int a = __shfl_sync(0xffffffffu, page, first + 2 * (k & 1)), b = __shfl_sync(0xffffffffu, page, first + 2 * (k & 1) + 1), row = (j0 + 32 * (k & 1)) & (p.P - 1);
+          if (elected()) {
+            const CUtensorMap* map = k & 2 ? &map_v : &map_k;
+            const uint32_t to = base + L::CODES + slot * L::SLOT, full = c_full + 8 * slot;
+            mbar_expect_tx(full, (a >= 0 ? L::SLOT / 2 : 0) + (b >= 0 ? L::SLOT / 2 : 0));
+            if (a >= 0) tma_load_2d(to, map, full, 0, (a * p.H + h) * p.P + row);
+            if (b >= 0) tma_load_2d(to + L::SLOT / 2, map, full, 0, (b * p.H + h) * p.P + ((row + 16) & (p.P - 1)));
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) *(volatile int*)&end = 4 * g;
+    __syncwarp();
+    for (int j = 4 * g; j < 4 * g + CONVERT_WARPS; ++j) {                     // each converter finds that there is no more
+      warp_wait(c_empty + 8 * (j % SLOTS), ((uint32_t)(j / SLOTS) & 1u) ^ 1u, &quit);
+      if (lane == 0) mbar_arrive(c_full + 8 * (j % SLOTS));
     }
   } else {
     // ---- products ----
     constexpr uint32_t id_s = idesc_f16(KEYS, false), id_o = idesc_f16(D, true);
     int g0 = 0, part = 0;                    // tiles and parts in front
-    for (; walk.next(p, u); ++part) {
+    for (const Part* u; (u = next_part<C>(walk, p)) != nullptr; ++part) {
+      const int n = u->n;
       warp_wait(q_full, (uint32_t)part & 1u, &quit);
-      for (int x = 0; x <= u.n; ++x) {
-        if (x < u.n) {
-          const int g = g0 + x, st = g & 1;
-          if (g > 0) warp_wait(s_taken + 8 * (st ^ 1), (uint32_t)((g - 1) >> 1) & 1u, &quit);
-          warp_wait(k_full + 8 * st, (uint32_t)(g >> 1) & 1u, &quit);
+      for (int x = 0; x <= n; ++x) {
+        if (x < n) {
+          const int g = g0 + x, st = g % STAGES, i = g & 1;
+          if (g >= 2) warp_wait(s_taken + 8 * i, (uint32_t)((g - 2) >> 1) & 1u, &quit);
+          warp_wait(k_full + 8 * st, (uint32_t)(g / STAGES) & 1u, &quit);
           tc_fence_after();
-          const uint32_t a = desc_low(base + L::Q), b = desc_low(base + L::K + st * L::TILE);
+          if (elected()) {
 #pragma unroll
-          for (int half = 0; half < D / 64; ++half) umma_block<1>(tmem, a + half * (L::HALF >> 4), b - a, id_s, half > 0 ? 1u : 0u);
-          commit_elected(s_full + 8 * st);
+            for (int k = 0; k < D / 16; ++k) product_tk(tmem + KEYS * i, tmem + Q_AT + 8 * k, base + L::K + st * L::TILE + (k >> 2) * L::HALF + 32 * (k & 3), id_s, k > 0 ? 1u : 0u);
+          }
+          __syncwarp();
+          commit_elected(s_full + 8 * i);
           commit_elected(k_empty + 8 * st);
         }
         if (x > 0) {
-          const int g = g0 + x - 1, st = g & 1;
-          warp_wait(v_full + 8 * st, (uint32_t)(g >> 1) & 1u, &quit);
-          warp_wait(p_full + 8 * st, (uint32_t)(g >> 1) & 1u, &quit);
+          const int g = g0 + x - 1, st = g % STAGES, i = g & 1;
+          warp_wait(v_full + 8 * st, (uint32_t)(g / STAGES) & 1u, &quit);
+          warp_wait(p_full + 8 * i, (uint32_t)(g >> 1) & 1u, &quit);
           tc_fence_after();
           if (elected()) {
 #pragma unroll
             for (int k = 0; k < KEYS / 16; ++k)
-              product_pv(tmem + 256 + 128 * st, tmem + 128 + 64 * st + 8 * k, base + L::V + st * L::TILE + k * 2048, L::HALF, id_o, x > 2 || k > 0 ? 1u : 0u);
+              product_pv(tmem + O_AT + D * i, tmem + P_AT + KEYS / 2 * i + 8 * k, base + L::V + st * L::TILE + k * 2048, L::HALF, id_o, x > 2 || k > 0 ? 1u : 0u);
           }
           __syncwarp();
-          commit_elected(o_done + 8 * st);
+          commit_elected(o_done + 8 * i);
           commit_elected(v_empty + 8 * st);
         }
       }
-      g0 += u.n;
+      g0 += n;
     }
     __syncwarp();
   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(soft_regs<C>()));
-    // ---- weights: a row per thread, which is a column and C of a tile's keys ----
+    // ---- weights: a row per thread, which is a column and HOLD of a tile's keys ----
     const int i = warp >> 2, q4 = warp & 3, in = q4 * 32 + lane, rep = in / C, col = in % C;
-    const uint32_t lanes = (uint32_t)(q4 * 32) << 16, ts = tmem + lanes + rep * C, tp = tmem + lanes + 128 + 64 * i, to = tmem + lanes + 256 + 128 * i;
+    const uint32_t lanes = (uint32_t)(q4 * 32) << 16, ts = tmem + lanes + KEYS * i + rep * HOLD, tp = tmem + lanes + P_AT + KEYS / 2 * i, to = tmem + lanes + O_AT + D * i;
     if constexpr (R > 1) {                   // other copies' keys have no weight here
       const uint32_t zero[16] = {};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) tmem_st16(tp + 16 * k, zero);
+      for (int k = 0; k < KEYS / 32; ++k) tmem_st16(tp + 16 * k, zero);
       tmem_st_wait();
     }
-    int g0 = 0;
-    for (; walk.next(p, u); g0 += u.n) {
-      // queries: f16 after a power of two for each column, as rows and heads of very different size may lie side by side
-      constexpr int PIECES = D / 8, MINE = C * PIECES / (SOFT_WARPS * 32);
-      const int n_cols = u.q.n * p.G - u.ct * C;                              // of this unit, and more
+    // The queries of a part, by the first group of warps: a row per thread, f16 after a power of two, as rows and heads of very different size may lie side by side.
+    auto put_queries = [&](const Part& u) {
+      const int cc = u.ct * C + col, token = cc / p.G;
+      uint4 raw[D / 8];
+      const bf16* const row = p.q + (u.q.r0 + token) * p.q_ld + (long long)(u.h * p.G + cc - token * p.G) * D;
+      const bool has = cc < u.q.n * p.G;
 #pragma unroll
-      for (int k = 0; k < MINE; ++k) {
-        const int x = threadIdx.x + 256 * k, r = x / PIECES, c = x % PIECES, cc = u.ct * C + r, token = cc / p.G;
-        uint4 raw = r < n_cols ? *reinterpret_cast<const uint4*>(p.q + (u.q.r0 + token) * p.q_ld + (long long)(u.h * p.G + cc - token * p.G) * D + 8 * c) : make_uint4(0, 0, 0, 0);
-        const uint32_t v[4] = {raw.x, raw.y, raw.z, raw.w};
-        uint32_t top = 0;                    // magnitudes as numbers, which order like the values
+      for (int k = 0; k < D / 8; ++k) raw[k] = has ? *reinterpret_cast<const uint4*>(row + 8 * k) : make_uint4(0, 0, 0, 0);
+      uint32_t top = 0;                      // magnitudes as numbers, which order like the values
+#pragma unroll
+      for (int k = 0; k < D / 8; ++k) {
+        const uint32_t v[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = max(top, max(v[e] << 16 & 0x7fff0000u, v[e] & 0x7fff0000u));
-#pragma unroll
-        for (int o = PIECES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        // A column that is not finite gets NaN, and no other: it asks as zeros, whose weights say whether it sees anything at all, and its factor tells the end of it.
-        const bool odd = top >= 0x7f800000u;
-        const float power = top && !odd ? power_of_two_in(__uint_as_float(top)) : 1.f, up = 16384.f / power;
-        if (c == 0) factors[r] = odd ? NAN : power * (1.f / 16384.f) * p.scale2;
-        uint32_t o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = odd ? 0u : pack_f16(__uint_as_float(v[e] << 16) * up, __uint_as_float(v[e] & 0xffff0000u) * up);
-#pragma unroll
-        for (int y = r; y < 128; y += C)
-          *reinterpret_cast<uint4*>(smem + L::Q + (c >> 3) * L::HALF + y * 128 + (((c & 7) ^ (y & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      // A column that is not finite gets NaN, and no other: it asks as zeros, whose weights say whether it sees anything at all, and its factor tells the end of it.
+      const bool odd = top >= 0x7f800000u;
+      const float power = top && !odd ? power_of_two_in(__uint_as_float(top)) : 1.f, up = __uint_as_float((268u << 23) - __float_as_uint(power));     // 2^14 / power
+      if (rep == 0) factors[col] = odd ? NAN : power * (1.f / 16384.f) * p.scale2;
+#pragma unroll
+      for (int k = 0; k < D / 8; k += 4) {
+        uint32_t o[16];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t v[4] = {raw[k + e].x, raw[k + e].y, raw[k + e].z, raw[k + e].w};
+#pragma unroll
+          for (int y = 0; y < 4; ++y) o[4 * e + y] = odd ? 0u : pack_f16(__uint_as_float(v[y] << 16) * up, __uint_as_float(v[y] & 0xffff0000u) * up);
+        }
+        tmem_st16(tmem + lanes + Q_AT + 4 * k, o);
+      }
+      tmem_st_wait();
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
-      asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");      // all columns' factors
-      const Tiles<7> tiles(u.q.before, u.q.before + u.q.n - 1, p.window, p.sinks);
-      const int before = u.q.before, last = before + u.q.n - 1, token = (u.ct * C + col) / p.G;
-      const bool has = col < n_cols;
-      const int pos = has ? p.position[u.q.r0 + token] : -1, lo = p.window > 0 ? pos - p.window : -1;         // of what is cached: sees j > lo or j < sinks
-      const uint32_t* const seen_row = p.seen + (long long)(u.q.r0 + token) * p.words;
+    };
+    const Part* next = next_part<C>(walk, p);            // a run has a part at least
+    if (i == 0) put_queries(*next);
+    asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");        // all columns' factors
+    for (int g0 = 0; next != nullptr;) {     // tiles in front
+      const Part& u = *next;
+      const bool alone = u.u0 == 0 && u.u1 == u.n_pos;
+      if (u.u0 == 0 && !alone && threadIdx.x == 0) {
+        const long long runs = run.to - run.from, left = u.n_pos - u.u1;
+        p.split[blockIdx.x] = make_int4(u.s, u.h, u.ct, (int)((left + runs - 1) / runs));
+      }
       const float fac = factors[col];
       float m = -INFINITY, sum = 0.f;
       int done = 0;                          // tiles of this group of warps
@@ -392,24 +462,30 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const TreeP p) {
         warp_wait(i_full + 8 * (g % INFOS), (uint32_t)(g / INFOS) & 1u, &quit);
         warp_wait(s_full + 8 * i, (uint32_t)(g >> 1) & 1u, &quit);
         tc_fence_after();
-        const int j0 = tiles[u.t0 + x] << 7;
-        const float4* ip = info[g % INFOS] + rep * (C / 16);
-        const uint32_t* th = there[g % INFOS];
-        const uint4 t0 = *reinterpret_cast<const uint4*>(th), t1 = *reinterpret_cast<const uint4*>(th + 4);
-        const bool whole = ((t0.x & t0.y & t0.z & t0.w & t1.x & t1.y & t1.z & t1.w) != 0u) & (j0 + KEYS <= before) & ((p.window <= 0) | (last - j0 < p.window) | (j0 + KEYS <= p.sinks));
-        uint32_t r[C];                       // the row's scores: read once, as the registers have room for them
-        float t = -INFINITY, by[C / 16], lv[C / 16];    // score in base 2 = product * by + lv; by > 0, so that the largest score of a page's keys is that of their largest product
+        const TileInfo& info = infos[g % INFOS];
+        const float4* ip = info.group + rep * HOLD / 16;
+        uint32_t r[HOLD];                    // the row's scores
+        float t = -INFINITY, by[HOLD / 16], lv[HOLD / 16];  // score in base 2 = product * by + lv; by > 0, so that the largest score of a page's keys is that of their largest product
+        if constexpr (HOLD == 16) {
+          tmem_ld16(ts, r);
+          tmem_ld_wait16(r);
+        } else {
 #pragma unroll
-        for (int c = 0; c < C / 32; ++c) tmem_ld32(ts + 32 * c, r + 32 * c);
+          for (int c = 0; c < HOLD; c += 32) tmem_ld32(ts + c, r + c);
 #pragma unroll
-        for (int c = 0; c < C / 32; ++c) tmem_ld_wait32(r + 32 * c);
+          for (int c = 0; c < HOLD; c += 32) tmem_ld_wait32(r + c);
+        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_taken + 8 * i);
-        if (!whole) {                        // keys that the row does not see: a bit for each of 32
+        if (!(info.whole & 1)) {             // keys that the row does not see: a bit for each of 32
+          const int before = info.pf, last = info.pl, cc = u.ct * C + col, token = cc / p.G;
+          const bool has = cc < u.q.n * p.G;
+          const int pos = has ? p.position[u.q.r0 + token] : -1, lo = p.window > 0 ? pos - p.window : -1;     // of what is cached: sees j > lo or j < sinks
+          const uint32_t* const seen_row = p.seen + (long long)(u.q.r0 + token) * p.words;
 #pragma unroll
-          for (int c = 0; c < C / 32; ++c) {
-            const int at = j0 + rep * C + 32 * c, off = at - before;
+          for (int c = 0; c < HOLD; c += 32) {
+            const int at = info.j0 + rep * HOLD + c, off = at - before;
             uint32_t seen = has && at < before ? upto(before - 1 - at) & (~upto(lo - at) | upto(p.sinks - 1 - at)) : 0u;
             if (has && at + 31 >= before && at <= last) {                     // the step's own tokens
               const int w = off >> 5, sh = off & 31;
@@ -422,15 +498,15 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const TreeP p) {
                 }
               seen |= own;
             }
-            if (!th[rep * (C / 16) + 2 * c]) seen &= 0xffff0000u;
-            if (!th[rep * (C / 16) + 2 * c + 1]) seen &= 0xffffu;
+            if (ip[c / 16].w == 0.f) seen &= 0xffff0000u;
+            if (HOLD > 16 && ip[HOLD > 16 ? c / 16 + 1 : 0].w == 0.f) seen &= 0xffffu;
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(seen >> e & 1u)) r[32 * c + e] = 0xff800000u;
+            for (int e = 0; e < 32 && e < HOLD; ++e)
+              if (!(seen >> e & 1u)) r[c + e] = 0xff800000u;
           }
         }
 #pragma unroll
-        for (int b = 0; b < C / 16; ++b) {
+        for (int b = 0; b < HOLD / 16; ++b) {
           by[b] = fmaxf(ip[b].x * fac, FLT_MIN);                              // also where fac is NaN
           lv[b] = ip[b].y;
           float mx[2] = {__uint_as_float(r[16 * b]), __uint_as_float(r[16 * b + 1])};
@@ -447,8 +523,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const TreeP p) {
           const float now = t - UNDER, factor = grow ? exp2_fast(m - now) : 1.f;
           if (grow) { m = now; sum *= factor; }
           if (done > 0) {
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {           // seldom: short code
               uint32_t o[16];
               tmem_ld16(to + 16 * c, o);
               tmem_ld_wait16(o);
@@ -462,30 +538,27 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const TreeP p) {
         // log2 s_v - M in one number is off by half a unit of M: only while that is no more than a quarter
         if (__any_sync(0xffffffffu, fabsf(off) > 4194304.f && off < INFINITY)) {
 #pragma unroll
-          for (int e = 0; e < C; ++e) r[e] = __float_as_uint(fmaf(__uint_as_float(r[e]), by[e / 16], lv[e / 16]));
+          for (int e = 0; e < HOLD; ++e) r[e] = __float_as_uint(fmaf(__uint_as_float(r[e]), by[e / 16], lv[e / 16]));
 #pragma unroll
-          for (int b = 0; b < C / 16; ++b) { by[b] = 1.f; lv[b] = 0.f; }
+          for (int b = 0; b < HOLD / 16; ++b) { by[b] = 1.f; lv[b] = 0.f; }
         }
 #pragma unroll
-        for (int c = 0; c < C / 32; ++c) {
-          uint32_t w[16];
+        for (int b = 0; b < HOLD / 16; ++b) {
+          const uint64_t by2 = two(by[b]), add = two(lv[b] - off);
+          uint64_t part = 0;
+          uint32_t w[8];
 #pragma unroll
-          for (int b = 2 * c; b < 2 * c + 2; ++b) {
-            const uint64_t by2 = two(by[b]), add = two(lv[b] - off);
-            uint64_t part = 0;
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              float e0, e1;
-              apart(fma2(together(__uint_as_float(r[16 * b + e]), __uint_as_float(r[16 * b + e + 1])), by2, add), e0, e1);
-              e0 = exp2_fast(e0); e1 = exp2_fast(e1);
-              part = add2(part, together(e0, e1));
-              w[8 * (b & 1) + (e >> 1)] = pack_f16(e0, e1);
-            }
-            float s0, s1;
-            apart(part, s0, s1);
-            sum = fmaf(s0 + s1, ip[b].z, sum);
+          for (int e = 0; e < 16; e += 2) {
+            float e0, e1;
+            apart(fma2(together(__uint_as_float(r[16 * b + e]), __uint_as_float(r[16 * b + e + 1])), by2, add), e0, e1);
+            e0 = exp2_fast(e0); e1 = exp2_fast(e1);
+            part = add2(part, together(e0, e1));
+            w[e >> 1] = pack_f16(e0, e1);
           }
-          tmem_st16(tp + rep * (C / 2) + 16 * c, w);
+          float s0, s1;
+          apart(part, s0, s1);
+          sum = fmaf(s0 + s1, ip[b].z, sum);
+          tmem_st8(tp + rep * (HOLD / 2) + 8 * b, w);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -497,15 +570,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const TreeP p) {
         warp_wait(o_done + 8 * i, (uint32_t)(g >> 1) & 1u, &quit);
         tc_fence_after();
       }
+      next = next_part<C>(walk, p);
       // join the column's 2 R rows
-      const bool alone = u.u0 == 0 && u.u1 == u.n_pos;
-      const int slot = 2 * (int)blockIdx.x + (u.u0 == 0 ? 1 : 0);
-      if (u.u0 == 0 && !alone && threadIdx.x == 0) {
-        const long long runs = run.to - run.from, left = u.n_pos - u.u1;
-        p.split[blockIdx.x] = make_int4(u.s, u.h, u.ct, (int)((left + runs - 1) / runs));
-      }
       ml[128 * i + in] = make_float2(m, sum);
       asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
+      if (i == 0 && next != nullptr) put_queries(*next); // every score has been made: the next part's first ones are beside the joining
       float top = -INFINITY, all = 0.f;
 #pragma unroll
       for (int k = 0; k < 2 * R; ++k) top = fmaxf(top, ml[k * C + col].x);
@@ -515,57 +584,62 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const TreeP p) {
         all = fmaf(y.y, y.x == -INFINITY ? 0.f : exp2_fast(y.x - top), all);
       }
       const float by = m == -INFINITY ? 0.f : exp2_fast(m - top);
-      if (i == 0 && rep == 0) total[col] = make_float2(top, all != 0.f && isnan(fac) ? NAN : all);
-      constexpr int TEAM = 2 * R, PER = 32 / TEAM;                            // threads of a column, dims of each
-      const int c_out = threadIdx.x / TEAM, d_out = (threadIdx.x % TEAM) * PER, cc = u.ct * C + c_out, t_out = cc / p.G;
+      if (i == 1 && rep == 0) total[col] = make_float2(top, all != 0.f && isnan(fac) ? NAN : all);
+      const int r0 = u.q.r0, c0 = u.ct * C, n_cols = u.q.n * p.G - c0, slot = 2 * (int)blockIdx.x + (u.u0 == 0 ? 1 : 0);
+      // in pieces of D / 8 dims, LINE threads a column, whose results lie side by side
+      constexpr int PIECE = D / 8, LINE = PIECE / 4, AT_ONCE = SOFT_WARPS * 32 / LINE;
+      auto place = [](int row, int e) { return row * PIECE * 4 + ((e ^ (D == 128 ? row >> 1 & 3 : row >> 2 & 1)) << 4); };
+      const int d_out = threadIdx.x % LINE, c_first = threadIdx.x / LINE;
       uint8_t* const join = smem + L::JOIN;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
+#pragma unroll 1
+      for (int c = 0; c < 8; ++c) {
+        uint32_t o[PIECE];
         if (done > 0) {
-          tmem_ld32(to + 32 * c, o);
-          tmem_ld_wait32(o);
+          if constexpr (PIECE == 16) { tmem_ld16(to + PIECE * c, o); tmem_ld_wait16(o); }
+          else { tmem_ld8(to + PIECE * c, o); tmem_ld_wait8(o); }
         }
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
+        for (int e = 0; e < LINE; ++e) {
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (done > 0 && by != 0.f) v = make_float4(__uint_as_float(o[e]) * by, __uint_as_float(o[e + 1]) * by, __uint_as_float(o[e + 2]) * by, __uint_as_float(o[e + 3]) * by);
-          *reinterpret_cast<float4*>(join + (128 * i + in) * 128 + (((e >> 2) ^ (in & 7)) << 4)) = v;
+          if (done > 0 && by != 0.f) v = make_float4(__uint_as_float(o[4 * e]) * by, __uint_as_float(o[4 * e + 1]) * by, __uint_as_float(o[4 * e + 2]) * by, __uint_as_float(o[4 * e + 3]) * by);
+          *reinterpret_cast<float4*>(join + place(128 * i + in, e)) = v;
         }
         asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
-        float acc[PER];
 #pragma unroll
-        for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+        for (int c_out = c_first; c_out < C; c_out += AT_ONCE) {
+          if (c_out >= n_cols) break;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < 2 * R; ++k)
-#pragma unroll
-          for (int e = 0; e < PER; e += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(join + (k * C + c_out) * 128 + ((((d_out + e) >> 2) ^ (c_out & 7)) << 4));
-            acc[e] += v.x; acc[e + 1] += v.y; acc[e + 2] += v.z; acc[e + 3] += v.w;
+          for (int k = 0; k < 2 * R; ++k) {
+            const float4 v = *reinterpret_cast<const float4*>(join + place(k * C + c_out, d_out));
+            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
           }
-        if (c_out < n_cols) {
           const float2 tl = total[c_out];
           if (alone) {
+            const int cc = c0 + c_out, t_out = cc / p.G;
             const float inv = tl.y != 0.f ? 1.f / tl.y : 0.f;
-            bf16* out = p.out + (u.q.r0 + t_out) * p.out_ld + (long long)(u.h * p.G + cc - t_out * p.G) * D + 32 * c + d_out;
-#pragma unroll
-            for (int e = 0; e < PER; e += 4) *reinterpret_cast<uint2*>(out + e) = make_uint2(pack_bf16(acc[e] * inv, acc[e + 1] * inv), pack_bf16(acc[e + 2] * inv, acc[e + 3] * inv));
+            bf16* out = p.out + (r0 + t_out) * p.out_ld + (long long)(u.h * p.G + cc - t_out * p.G) * D + PIECE * c + 4 * d_out;
+            *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
           } else {
             const long long at = (long long)slot * C + c_out;
             if (c == 0 && d_out == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = tl;
-#pragma unroll
-            for (int e = 0; e < PER; e += 4) *reinterpret_cast<float4*>(p.part_o + at * D + 32 * c + d_out + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+            *reinterpret_cast<float4*>(p.part_o + at * D + PIECE * c + 4 * d_out) = acc;
           }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
       }
+      g0 += u.n;
       tc_fence_before();
     }
   }
   __syncthreads();
   tc_fence_after();
-  if (warp == SOFT_WARPS + CONVERT_WARPS) tmem_dealloc(tmem, 512);
-  if (threadIdx.x == 0 && quit) atomicOr(p.flags, B200_PAGED_WAIT);
+  if (warp == ISSUER) tmem_dealloc(tmem, 512);
+  if (quit) {                                // let copies in flight land before the block ends
+    if (threadIdx.x == 0) atomicOr(p.flags, B200_PAGED_WAIT);
+    const uint64_t since = global_timer_ns();
+    while (global_timer_ns() - since < 2000000ull) {}
+  }
 }
 
 // Joins the units that are cut: a block for two columns of the one that a CTA has begun, a column's four teams of sixteen threads take its parts in turn.
@@ -646,9 +720,12 @@ template <int D, int FMT, int C>
 int launch(const TreeP& p, int ctas, cudaStream_t st) {
   static std::atomic<uint64_t> limits{0};
   static std::atomic<uint64_t> shares{0};
+  CUtensorMap map_k, map_v;
+  B200_TRY(code_map(&map_k, p.k, (long long)p.pages * p.H * p.P, D));
+  B200_TRY(code_map(&map_v, p.v, (long long)p.pages * p.H * p.P, D));
   B200_TRY(allow_smem(limits, (int)TreeSmem<D>::BYTES, tree_kernel<D, FMT, C>));
   B200_TRY(prefer_smem(shares, 100, tree_kernel<D, FMT, C>, tree_join_kernel<D, C>));
-  B200_TRY(launch_early(tree_kernel<D, FMT, C>, dim3((unsigned)ctas), dim3(THREADS), TreeSmem<D>::BYTES, st, p));
+  B200_TRY(launch_early(tree_kernel<D, FMT, C>, dim3((unsigned)ctas), dim3(THREADS), TreeSmem<D>::BYTES, st, map_k, map_v, p));
   return launch_early(tree_join_kernel<D, C>, dim3((unsigned)(ctas * (C / 2))), dim3(128), 0, st, p);
 }
 template <int D, int FMT>
