@@ -1111,8 +1111,8 @@ int launch_few(const AttnP& p, const FewPlan& f, cudaStream_t st) {
   constexpr int ring = FEW_WARPS * 4 * 32 * D, sums = FEW_WARPS * 8 * (D + 4) * 4, smem = ring + sums + 1024;
   static std::atomic<uint64_t> limits{0};
   CUtensorMap map_k, map_v;
-  B200_TRY(code_map(&map_k, p.k, (long long)p.pages * p.H * p.P, D));
-  B200_TRY(code_map(&map_v, p.v, (long long)p.pages * p.H * p.P, D));
+  B200_TRY(code_map(&map_k, p.k, (long long)p.pages * p.H * p.P, D, 16));
+  B200_TRY(code_map(&map_v, p.v, (long long)p.pages * p.H * p.P, D, 16));
   B200_TRY(allow_smem(limits, smem, few_rows_kernel<D, FMT, NT>));
   // all of an SM's L1 as shared memory, also for what runs in between: left to the driver an SM keeps what the kernel in front left, and then holds one CTA and not two
   static std::atomic<uint64_t> shares{0};
@@ -1151,7 +1151,7 @@ int launch_append(AppendP& p, cudaStream_t st) {
 
 }  // namespace
 
-int code_map(CUtensorMap* m, const void* codes, long long rows, int dim) {
+int code_map(CUtensorMap* m, const void* codes, long long rows, int dim, int box_rows) {
   typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
   static const EncodeFn fn = [] {
@@ -1162,7 +1162,7 @@ int code_map(CUtensorMap* m, const void* codes, long long rows, int dim) {
   }();
   if (!fn) B200_FAIL(B200_ERR_CUDA, "cuTensorMapEncodeTiled not available");
   cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)dim};
-  cuuint32_t box[2] = {(cuuint32_t)dim, 16}, est[2] = {1, 1};
+  cuuint32_t box[2] = {(cuuint32_t)dim, (cuuint32_t)box_rows}, est[2] = {1, 1};
   const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, strides, box, est, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) B200_FAIL(B200_ERR_CUDA, "paged cache: tensor map of %lld rows of %d codes refused (%d)", rows, dim, (int)r);

@@ -158,8 +158,8 @@ __device__ __forceinline__ bool wait_or_quit(uint32_t bar, uint32_t parity, vola
     }
   }
 }
-// paged.cu: a tensor map over a cache's codes, [rows][dim], boxes of 16 whole rows, swizzled by 128 bytes (dim 64: by 64); what a call's host arguments have to be, attention's in its kernels' form
-int code_map(CUtensorMap* m, const void* codes, long long rows, int dim);
+// paged.cu: a tensor map over a cache's codes, [rows][dim], boxes of so many whole rows, swizzled by 128 bytes (dim 64: by 64); what a call's host arguments have to be, attention's in its kernels' form
+int code_map(CUtensorMap* m, const void* codes, long long rows, int dim, int box_rows);
 int checked_cache(const b200_paged_cache* cache, const char* what);
 int checked(const b200_paged_cache* cache, const b200_paged_batch* batch, const char* what);
 int attention_arguments(AttnP* p, const b200_paged_cache* cache, const b200_paged_batch* batch, const void* q_dev, int64_t q_ld, void* out_dev, int64_t out_ld, int q_heads, float scale, int window,

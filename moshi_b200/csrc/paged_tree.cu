@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(128) tree_build_kernel(const BuildP p) {
 // =========================================================================================================================
 // attention
 // =========================================================================================================================
-constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 6, PRODUCER = 14, ISSUER = 15, THREADS = 16 * 32, SHIFT = 6, KEYS = 1 << SHIFT, STAGES = 4, INFOS = 16;
+constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 6, PRODUCER = 14, ISSUER = 15, THREADS = 16 * 32, SHIFT = 6, KEYS = 1 << SHIFT, STAGES = 4, INFOS = 32;
 constexpr int UNIT_COST = 10, MIN_RUN = 10;  // in tiles: what a unit costs beside its own, and the least of a CTA
 
 struct TreeP : AttnP {
@@ -106,8 +106,12 @@ __device__ Run run_of(const AttnP& p) {
   __shared__ long long sums[WARPS];
   __shared__ Run found;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long mine = 0;
-  for (int s = threadIdx.x; s < p.b.S; s += THREADS) mine += work_of<C>(p, s);
+  long long mine = 0, first = 0;
+  for (int s = threadIdx.x; s < p.b.S; s += THREADS) {
+    const long long w = work_of<C>(p, s);
+    if (s == (int)threadIdx.x) first = w;
+    mine += w;
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   if (lane == 0) sums[warp] = mine;
@@ -123,7 +127,7 @@ __device__ Run run_of(const AttnP& p) {
   long long base = 0;
   for (int s0 = 0; s0 < p.b.S; s0 += THREADS) {
     const int s = s0 + (int)threadIdx.x;
-    const long long w = s < p.b.S ? work_of<C>(p, s) : 0;
+    const long long w = s0 == 0 ? first : s < p.b.S ? work_of<C>(p, s) : 0;
     long long in = w;                        // inclusive sums of the warp, then of the block
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -214,6 +218,20 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), R8(r, 0) : "memory");
 }
 #undef R8
+// Both of two neighbouring barriers, asked together.
+__device__ __forceinline__ void wait_two(uint32_t bar, uint32_t parity, volatile int* quit) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%1 + 8], %2;\n\t"
+      "and.pred p, p, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  if (__all_sync(0xffffffffu, done)) return;
+  warp_wait(bar, parity, quit);
+  warp_wait(bar + 8, parity, quit);
+}
 // registers of a weight thread; with those of the others they are what the block was launched with
 template <int C> constexpr int soft_regs() { return C == 128 ? 168 : 144; }
 
@@ -303,60 +321,79 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     }
   } else if (warp == PRODUCER) {
     // ---- copies: pages and scales are looked up for eight tiles at a time, a lane for each 16 tokens, and eight tiles ahead ----
-    int g = 0;
+    const int box = p.P < 32 ? 16 : 32;      // tokens of a copy
+    int g = 0, slot = 0;
+    uint32_t parity = 1;                     // of the slots' turns: 1: they have not been used yet
     for (const Part* u; (u = next_part<C>(walk, p)) != nullptr;) {
       const int n = u->n, h = u->h, pf = u->q.before, pl = pf + u->q.n - 1;
+      const int32_t* const table = p.b.table + u->s * p.b.table_ld;
+      auto first_of = [&](int batch) { return (u->tile(8 * batch + (lane >> 2)) << SHIFT) + 16 * (lane & 3); };        // of the lane's tokens
       auto look_up = [&](int batch) {
-        const int x = 8 * batch + (lane >> 2);
-        if (x >= n) return -1;
-        const int j = (u->tile(x) << SHIFT) + 16 * (lane & 3);
-        if (j > pl || (p.window > 0 && pf - j - 15 >= p.window && j >= p.sinks)) return -1;
-        const int page = p.b.table[u->s * p.b.table_ld + (j >> p.page_shift)];
+        const int j = first_of(batch);
+        if (8 * batch + (lane >> 2) >= n || j > pl || (p.window > 0 && pf - j - 15 >= p.window && j >= p.sinks)) return -1;
+        const int page = table[j >> p.page_shift];
         if (page >= 0 && page < p.pages) return page;
         atomicOr(p.flags, B200_PAGED_BAD_PAGE);
         return -1;
       };
       auto scales_of = [&](int page) { return page < 0 ? make_float2(1.f, 1.f) : make_float2(p.k_scale[(long long)page * p.H + h], p.v_scale[(long long)page * p.H + h]); };
-      int page = -1, page_next = look_up(0);
-      float2 scale = make_float2(1.f, 1.f), scale_next = scales_of(page_next);
+      int page = -1, row = 0, page_next = look_up(0);
+      float2 scale_next = scales_of(page_next);
       for (int x = 0; x < n; ++x, ++g) {
-        if ((x & 7) == 0) { page = page_next; scale = scale_next; page_next = look_up((x >> 3) + 1); }
-        if ((x & 7) == 4) scale_next = scales_of(page_next);
-        const int j0 = u->tile(x) << SHIFT, first = 4 * (x & 7);
-        const bool there = (__ballot_sync(0xffffffffu, page >= 0) >> first & 15u) == 15u;
-        TileInfo& t = infos[g % INFOS];
-        if (lane >> 2 == (x & 7)) {
-          const float vs = value_scale(scale.y);
-          t.group[lane & 3] = page >= 0 ? make_float4(scale.x > 0.f ? scale.x : 1.f, __log2f(vs), __frcp_rn(vs), 1.f) : make_float4(1.f, 0.f, 0.f, 0.f);
-        }
-        if (lane == 0) {
-          const bool whole = there && j0 + KEYS <= pf && (p.window <= 0 || pl - j0 < p.window || j0 + KEYS <= p.sinks);
-          const bool seen = there && j0 + KEYS - 1 <= pl && (p.window <= 0 || pf - j0 < p.window || j0 + KEYS <= p.sinks);
-          t.j0 = j0; t.pf = pf; t.pl = pl; t.whole = (whole ? 1 : 0) | (seen ? 2 : 0);
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(i_full + 8 * (g % INFOS));
-#pragma unroll 1
-        for (int k = 0; k < 4; ++k) {
-          const int j = 4 * g + k, slot = j % SLOTS;
-          warp_wait(c_empty + 8 * slot, ((uint32_t)(j / SLOTS) & 1u) ^ 1u, &quit);
-          const int a = __shfl_sync(0xffffffffu, page, first + 2 * (k & 1)), b = __shfl_sync(0xffffffffu, page, first + 2 * (k & 1) + 1), row = (j0 + 32 * (k & 1)) & (p.P - 1);
-          if (elected()) {
-            const CUtensorMap* map = k & 2 ? &map_v : &map_k;
-            const uint32_t to = base + L::CODES + slot * L::SLOT, full = c_full + 8 * slot;
-            mbar_expect_tx(full, (a >= 0 ? L::SLOT / 2 : 0) + (b >= 0 ? L::SLOT / 2 : 0));
-            if (a >= 0) tma_load_2d(to, map, full, 0, (a * p.H + h) * p.P + row);
-            if (b >= 0) tma_load_2d(to + L::SLOT / 2, map, full, 0, (b * p.H + h) * p.P + ((row + 16) & (p.P - 1)));
+        if ((x & 7) == 0) {                  // what is to be known of the batch
+          page = page_next;
+          const int j = first_of(x >> 3), j0 = j & ~(KEYS - 1), mine = x + (lane >> 2);
+          row = (page * p.H + h) * p.P + (j & (p.P - 1));
+          TileInfo& t = infos[(g + (lane >> 2)) % INFOS];
+          const float vs = value_scale(scale_next.y);
+          const bool there = (__ballot_sync(0xffffffffu, page >= 0) >> (lane & 28) & 15u) == 15u;
+          if (mine < n) {
+            t.group[lane & 3] = page >= 0 ? make_float4(scale_next.x > 0.f ? scale_next.x : 1.f, __log2f(vs), __frcp_rn(vs), 1.f) : make_float4(1.f, 0.f, 0.f, 0.f);
+            if ((lane & 3) == 0) {
+              const bool whole = there && j0 + KEYS <= pf && (p.window <= 0 || pl - j0 < p.window || j0 + KEYS <= p.sinks);
+              const bool seen = there && j0 + KEYS - 1 <= pl && (p.window <= 0 || pf - j0 < p.window || j0 + KEYS <= p.sinks);
+              t.j0 = j0; t.pf = pf; t.pl = pl; t.whole = (whole ? 1 : 0) | (seen ? 2 : 0);
+            }
           }
           __syncwarp();
+          if (mine < n && (lane & 3) == 0) mbar_arrive(i_full + 8 * ((g + (lane >> 2)) % INFOS));
+          page_next = look_up((x >> 3) + 1);
+        }
+        if ((x & 7) == 4) scale_next = scales_of(page_next);
+        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) >> (4 * (x & 7));
+        int rows[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) rows[k] = __shfl_sync(0xffffffffu, row, 4 * (x & 7) + k);
+#pragma unroll
+        for (int values = 0; values < 2; ++values) {
+          wait_two(c_empty + 8 * slot, parity, &quit);
+          if (elected()) {
+            const CUtensorMap* map = values ? &map_v : &map_k;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const uint32_t to = base + L::CODES + (slot + k) * L::SLOT, full = c_full + 8 * (slot + k), two = there >> (2 * k) & 3u;
+              if (box == 32) {               // both halves lie in one page
+                mbar_expect_tx(full, two ? L::SLOT : 0);
+                if (two) tma_load_2d(to, map, full, 0, two & 1u ? rows[2 * k] : rows[2 * k + 1] - 16);
+              } else {
+                mbar_expect_tx(full, (uint32_t)__popc(two) * (L::SLOT / 2));
+                if (two & 1u) tma_load_2d(to, map, full, 0, rows[2 * k]);
+                if (two & 2u) tma_load_2d(to + L::SLOT / 2, map, full, 0, rows[2 * k + 1]);
+              }
+            }
+          }
+          __syncwarp();
+          slot += 2;
+          if (slot == SLOTS) { slot = 0; parity ^= 1u; }
         }
       }
     }
     if (lane == 0) *(volatile int*)&end = 4 * g;
     __syncwarp();
-    for (int j = 4 * g; j < 4 * g + CONVERT_WARPS; ++j) {                     // each converter finds that there is no more
-      warp_wait(c_empty + 8 * (j % SLOTS), ((uint32_t)(j / SLOTS) & 1u) ^ 1u, &quit);
-      if (lane == 0) mbar_arrive(c_full + 8 * (j % SLOTS));
+    for (int k = 0; k < CONVERT_WARPS; ++k) {                                 // each converter finds that there is no more
+      warp_wait(c_empty + 8 * slot, parity, &quit);
+      if (lane == 0) mbar_arrive(c_full + 8 * slot);
+      if (++slot == SLOTS) { slot = 0; parity ^= 1u; }
     }
   } else {
     // ---- products ----
@@ -409,44 +446,61 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
       for (int k = 0; k < KEYS / 32; ++k) tmem_st16(tp + 16 * k, zero);
       tmem_st_wait();
     }
-    // The queries of a part, by the first group of warps: a row per thread, f16 after a power of two, as rows and heads of very different size may lie side by side.
-    auto put_queries = [&](const Part& u) {
-      const int cc = u.ct * C + col, token = cc / p.G;
-      uint4 raw[D / 8];
-      const bf16* const row = p.q + (u.q.r0 + token) * p.q_ld + (long long)(u.h * p.G + cc - token * p.G) * D;
-      const bool has = cc < u.q.n * p.G;
+    // The queries of a part, f16 after a power of two for each column, as rows and heads of very different size may lie side by side.  They come in whole rows, the thread's are piece c of every APART-th column
+    // from r_at on (token and head by counting, not by division), go through the place of the joining, HERE columns at a time, and a row per thread into TMEM.
+    constexpr int PIECES = D / 8, MINE = C * PIECES / (SOFT_WARPS * 32), APART = SOFT_WARPS * 32 / PIECES, HERE = C < 64 ? C : 64;
+    const int c_q = threadIdx.x % PIECES, r_at = threadIdx.x / PIECES;
+    uint8_t* const join = smem + L::JOIN;
+    uint4 raw[MINE];
+    auto load_queries = [&](const Part& u) {
+      const int c0 = u.ct * C, n_cols = u.q.n * p.G - c0, step_t = APART / p.G, step_g = APART - step_t * p.G;
+      int token = (c0 + r_at) / p.G, head = c0 + r_at - token * p.G;
+      const bf16* const q0 = p.q + (long long)u.q.r0 * p.q_ld + (long long)u.h * p.G * D + 8 * c_q;
 #pragma unroll
-      for (int k = 0; k < D / 8; ++k) raw[k] = has ? *reinterpret_cast<const uint4*>(row + 8 * k) : make_uint4(0, 0, 0, 0);
-      uint32_t top = 0;                      // magnitudes as numbers, which order like the values
-#pragma unroll
-      for (int k = 0; k < D / 8; ++k) {
-        const uint32_t v[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top = max(top, max(v[e] << 16 & 0x7fff0000u, v[e] & 0x7fff0000u));
+      for (int k = 0; k < MINE; ++k) {
+        raw[k] = r_at + k * APART < n_cols ? *reinterpret_cast<const uint4*>(q0 + token * p.q_ld + head * D) : make_uint4(0, 0, 0, 0);
+        token += step_t; head += step_g;
+        if (head >= p.G) { head -= p.G; ++token; }
       }
-      // A column that is not finite gets NaN, and no other: it asks as zeros, whose weights say whether it sees anything at all, and its factor tells the end of it.
-      const bool odd = top >= 0x7f800000u;
-      const float power = top && !odd ? power_of_two_in(__uint_as_float(top)) : 1.f, up = __uint_as_float((268u << 23) - __float_as_uint(power));     // 2^14 / power
-      if (rep == 0) factors[col] = odd ? NAN : power * (1.f / 16384.f) * p.scale2;
+    };
+    auto put_queries = [&]() {
 #pragma unroll
-      for (int k = 0; k < D / 8; k += 4) {
-        uint32_t o[16];
+      for (int round = 0; round < C / HERE; ++round) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t v[4] = {raw[k + e].x, raw[k + e].y, raw[k + e].z, raw[k + e].w};
-#pragma unroll
-          for (int y = 0; y < 4; ++y) o[4 * e + y] = odd ? 0u : pack_f16(__uint_as_float(v[y] << 16) * up, __uint_as_float(v[y] & 0xffff0000u) * up);
+        for (int k = round * (MINE * HERE / C); k < (round + 1) * (MINE * HERE / C); ++k) {
+          const int r = r_at + k * APART - round * HERE;
+          *reinterpret_cast<uint4*>(join + r * 2 * D + ((c_q ^ (r & 7)) << 4)) = raw[k];
         }
-        tmem_st16(tmem + lanes + Q_AT + 4 * k, o);
+        asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
+        if (i == 0 && (C / HERE == 1 || warp / (4 / (C / HERE)) == round)) {
+          const int r = col % HERE;
+          uint32_t v[D / 2], top = 0;        // magnitudes as numbers, which order like the values
+#pragma unroll
+          for (int k = 0; k < PIECES; ++k) {
+            const uint4 x = *reinterpret_cast<const uint4*>(join + r * 2 * D + ((k ^ (r & 7)) << 4));
+            v[4 * k] = x.x; v[4 * k + 1] = x.y; v[4 * k + 2] = x.z; v[4 * k + 3] = x.w;
+          }
+#pragma unroll
+          for (int e = 0; e < D / 2; ++e) top = max(top, max(v[e] << 16 & 0x7fff0000u, v[e] & 0x7fff0000u));
+          // A column that is not finite gets NaN, and no other: it asks as zeros, whose weights say whether it sees anything at all, and its factor tells the end of it.
+          const bool odd = top >= 0x7f800000u;
+          const float power = top && !odd ? power_of_two_in(__uint_as_float(top)) : 1.f, up = __uint_as_float((268u << 23) - __float_as_uint(power));     // 2^14 / power
+          if (rep == 0) factors[col] = odd ? NAN : power * (1.f / 16384.f) * p.scale2;
+#pragma unroll
+          for (int e = 0; e < D / 2; ++e) v[e] = odd ? 0u : pack_f16(__uint_as_float(v[e] << 16) * up, __uint_as_float(v[e] & 0xffff0000u) * up);
+#pragma unroll
+          for (int e = 0; e < D / 2; e += 16) tmem_st16(tmem + lanes + Q_AT + e, v + e);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(q_full);
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");    // all columns' factors; the place is free again
       }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
     };
     const Part* next = next_part<C>(walk, p);            // a run has a part at least
-    if (i == 0) put_queries(*next);
-    asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");        // all columns' factors
+    load_queries(*next);
+    put_queries();
     for (int g0 = 0; next != nullptr;) {     // tiles in front
       const Part& u = *next;
       const bool alone = u.u0 == 0 && u.u1 == u.n_pos;
@@ -571,10 +625,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         tc_fence_after();
       }
       next = next_part<C>(walk, p);
+      if (next != nullptr) load_queries(*next);
       // join the column's 2 R rows
       ml[128 * i + in] = make_float2(m, sum);
       asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
-      if (i == 0 && next != nullptr) put_queries(*next); // every score has been made: the next part's first ones are beside the joining
+      if (next != nullptr) put_queries();    // every score has been made: the next part's first ones are beside the joining
       float top = -INFINITY, all = 0.f;
 #pragma unroll
       for (int k = 0; k < 2 * R; ++k) top = fmaxf(top, ml[k * C + col].x);
@@ -590,7 +645,6 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
       constexpr int PIECE = D / 8, LINE = PIECE / 4, AT_ONCE = SOFT_WARPS * 32 / LINE;
       auto place = [](int row, int e) { return row * PIECE * 4 + ((e ^ (D == 128 ? row >> 1 & 3 : row >> 2 & 1)) << 4); };
       const int d_out = threadIdx.x % LINE, c_first = threadIdx.x / LINE;
-      uint8_t* const join = smem + L::JOIN;
 #pragma unroll 1
       for (int c = 0; c < 8; ++c) {
         uint32_t o[PIECE];
@@ -721,8 +775,8 @@ int launch(const TreeP& p, int ctas, cudaStream_t st) {
   static std::atomic<uint64_t> limits{0};
   static std::atomic<uint64_t> shares{0};
   CUtensorMap map_k, map_v;
-  B200_TRY(code_map(&map_k, p.k, (long long)p.pages * p.H * p.P, D));
-  B200_TRY(code_map(&map_v, p.v, (long long)p.pages * p.H * p.P, D));
+  B200_TRY(code_map(&map_k, p.k, (long long)p.pages * p.H * p.P, D, p.P < 32 ? 16 : 32));
+  B200_TRY(code_map(&map_v, p.v, (long long)p.pages * p.H * p.P, D, p.P < 32 ? 16 : 32));
   B200_TRY(allow_smem(limits, (int)TreeSmem<D>::BYTES, tree_kernel<D, FMT, C>));
   B200_TRY(prefer_smem(shares, 100, tree_kernel<D, FMT, C>, tree_join_kernel<D, C>));
   B200_TRY(launch_early(tree_kernel<D, FMT, C>, dim3((unsigned)ctas), dim3(THREADS), TreeSmem<D>::BYTES, st, map_k, map_v, p));
