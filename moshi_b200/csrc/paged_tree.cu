@@ -204,33 +204,51 @@ __device__ __forceinline__ const Part* next_part(Walk& w, const AttnP& p) {
   return more ? &w.part[w.now] : nullptr;
 }
 
-// D[128 rows][n] (+)= A B^T over 16 of k: A in TMEM (8 columns of two f16), B's rows [n][64 of k] in shared memory, swizzled
-__device__ __forceinline__ void product_tk(uint32_t d, uint32_t a, uint32_t b_smem, uint32_t idesc, uint32_t accumulate) {
-  const uint64_t desc = (uint64_t)desc_low(b_smem) | (uint64_t)DESC_HIGH << 32;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a), "l"(desc), "r"(idesc), "r"(accumulate) : "memory");
+// The products of a tile, by one thread of the warp, and a commit behind them; A in TMEM, 8 columns of two f16 for 16 of k.
+// S = Q K^T: K's rows [64 tokens][64 dims], swizzled; the next 16 dims 32 bytes on, the next 64 a half.
+#define MMA(k, acc) "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a" #k "], w" #k ", %3, " acc ";\n\t"
+#define ARG(k, by) "add.u32 a" #k ", %1, 8*" #k ";\n\tadd.u32 x, %2, " by ";\n\tmov.b64 w" #k ", {x, %5};\n\t"
+#define REGS "{\n\t.reg .pred f, t, q;\n\t.reg .b32 x, a0, a1, a2, a3, a4, a5, a6, a7;\n\t.reg .b64 w0, w1, w2, w3, w4, w5, w6, w7;\n\t"
+#define ELECT "setp.ne.b32 t, %5, 0;\n\tsetp.ne.b32 f, %6, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+#define COMMIT "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%4];\n\t}"
+template <int D>
+__device__ __forceinline__ void scores_of_tile(uint32_t s, uint32_t q, uint32_t k_smem, uint32_t idesc, uint32_t bar) {
+  if constexpr (D == 128)
+    asm volatile(REGS ARG(0, "0") ARG(1, "2") ARG(2, "4") ARG(3, "6") ARG(4, "512") ARG(5, "514") ARG(6, "516") ARG(7, "518") ELECT
+                 MMA(0, "f") MMA(1, "t") MMA(2, "t") MMA(3, "t") MMA(4, "t") MMA(5, "t") MMA(6, "t") MMA(7, "t") COMMIT
+                 ::"r"(s), "r"(q), "r"(desc_low(k_smem)), "r"(idesc), "r"(bar), "r"(DESC_HIGH), "r"(0u) : "memory");
+  else
+    asm volatile(REGS ARG(0, "0") ARG(1, "2") ARG(2, "4") ARG(3, "6") ELECT MMA(0, "f") MMA(1, "t") MMA(2, "t") MMA(3, "t") COMMIT
+                 ::"r"(s), "r"(q), "r"(desc_low(k_smem)), "r"(idesc), "r"(bar), "r"(DESC_HIGH), "r"(0u) : "memory");
 }
+// O (+)= P V: V's rows [64 tokens][64 dims], 16 tokens 2048 bytes on, the next 64 dims a half
+__device__ __forceinline__ void sums_of_tile(uint32_t o, uint32_t p, uint32_t v_smem, uint32_t half, uint32_t idesc, uint32_t bar, uint32_t accumulate) {
+  asm volatile(REGS ARG(0, "0") ARG(1, "128") ARG(2, "256") ARG(3, "384") ELECT MMA(0, "f") MMA(1, "t") MMA(2, "t") MMA(3, "t") COMMIT
+               ::"r"(o), "r"(p), "r"(((v_smem & 0x3FFFFu) >> 4) | ((half >> 4) << 16)), "r"(idesc), "r"(bar), "r"(DESC_HIGH), "r"(accumulate) : "memory");
+}
+#undef MMA
+#undef ARG
+#undef REGS
+#undef ELECT
+#undef COMMIT
 #define R8(r, o) "r"((r)[o]), "r"((r)[o + 1]), "r"((r)[o + 2]), "r"((r)[o + 3]), "r"((r)[o + 4]), "r"((r)[o + 5]), "r"((r)[o + 6]), "r"((r)[o + 7])
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), R8(r, 0) : "memory");
 }
 #undef R8
-// Both of two neighbouring barriers, asked together.
-__device__ __forceinline__ void wait_two(uint32_t bar, uint32_t parity, volatile int* quit) {
+// Two barriers, asked together.
+__device__ __forceinline__ void wait_two(uint32_t bar, uint32_t parity, uint32_t bar2, uint32_t parity2, volatile int* quit) {
   uint32_t done;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 q, [%1 + 8], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
       "and.pred p, p, q;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+      : "=r"(done) : "r"(bar), "r"(parity), "r"(bar2), "r"(parity2) : "memory");
   if (__all_sync(0xffffffffu, done)) return;
   warp_wait(bar, parity, quit);
-  warp_wait(bar + 8, parity, quit);
+  warp_wait(bar2, parity2, quit);
 }
 // registers of a weight thread; with those of the others they are what the block was launched with
 template <int C> constexpr int soft_regs() { return C == 128 ? 168 : 144; }
@@ -243,7 +261,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
   constexpr uint32_t P_AT = 2 * KEYS, O_AT = P_AT + KEYS, Q_AT = 512 - D / 2;
   static_assert(O_AT + 2 * D <= Q_AT, "TMEM");
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * SLOTS + 4 * STAGES + 9 + INFOS];
+  __shared__ __align__(8) uint64_t bars[2 * SLOTS + 4 * STAGES + 5 + INFOS];
   __shared__ __align__(16) TileInfo infos[INFOS];
   __shared__ uint32_t tmem_at;
   __shared__ volatile int quit;              // somebody has waited too long: nobody waits any more, and all go through to the end
@@ -254,14 +272,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t bar = smem_u32(bars), c_full = bar, c_empty = c_full + 8 * SLOTS, k_full = c_empty + 8 * SLOTS, k_empty = k_full + 8 * STAGES, v_full = k_empty + 8 * STAGES, v_empty = v_full + 8 * STAGES,
-                 s_full = v_empty + 8 * STAGES, p_full = s_full + 16, o_done = p_full + 16, s_taken = o_done + 16, q_full = s_taken + 16, i_full = q_full + 8;
+  const uint32_t bar = smem_u32(bars), c_full = bar, c_empty = c_full + 8 * SLOTS, k_full = c_empty + 8 * SLOTS, v_full = k_full + 8 * STAGES,
+                 s_done = v_full + 8 * STAGES, o_done = s_done + 8 * STAGES, p_full = o_done + 8 * STAGES, s_taken = p_full + 16, q_full = s_taken + 16, i_full = q_full + 8;
   if (threadIdx.x == 0) {
     quit = 0;
     end = 0x7fffffff;
     for (int i = 0; i < SLOTS; ++i) { mbar_init(c_full + 8 * i, 1); mbar_init(c_empty + 8 * i, 1); }
-    for (int i = 0; i < STAGES; ++i) { mbar_init(k_full + 8 * i, 2); mbar_init(k_empty + 8 * i, 1); mbar_init(v_full + 8 * i, 2); mbar_init(v_empty + 8 * i, 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(s_full + 8 * i, 1); mbar_init(s_taken + 8 * i, 4); mbar_init(p_full + 8 * i, 4); mbar_init(o_done + 8 * i, 1); }
+    for (int i = 0; i < STAGES; ++i) { mbar_init(k_full + 8 * i, 2); mbar_init(v_full + 8 * i, 2); mbar_init(s_done + 8 * i, 1); mbar_init(o_done + 8 * i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(s_taken + 8 * i, 4); mbar_init(p_full + 8 * i, 4); }
     mbar_init(q_full, 4);
     for (int i = 0; i < INFOS; ++i) mbar_init(i_full + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -297,7 +315,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
       const bool values = j & 2;
       warp_wait(c_full + 8 * slot, (uint32_t)(j / SLOTS) & 1u, &quit);
       if (__any_sync(0xffffffffu, quit || j >= *(volatile int*)&end)) break;
-      warp_wait((values ? v_empty : k_empty) + 8 * st, ((uint32_t)(g / STAGES) & 1u) ^ 1u, &quit);
+      warp_wait((values ? o_done : s_done) + 8 * st, ((uint32_t)(g / STAGES) & 1u) ^ 1u, &quit);
       const TileInfo& t = infos[g % INFOS];
       const bool all = !values || (t.whole & 2);         // values that no row sees may be anything; keys are masked
       const uint8_t* from = smem + L::CODES + slot * L::SLOT;
@@ -366,7 +384,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         for (int k = 0; k < 4; ++k) rows[k] = __shfl_sync(0xffffffffu, row, 4 * (x & 7) + k);
 #pragma unroll
         for (int values = 0; values < 2; ++values) {
-          wait_two(c_empty + 8 * slot, parity, &quit);
+          wait_two(c_empty + 8 * slot, parity, c_empty + 8 * slot + 8, parity, &quit);
           if (elected()) {
             const CUtensorMap* map = values ? &map_v : &map_k;
 #pragma unroll
@@ -402,33 +420,21 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     for (const Part* u; (u = next_part<C>(walk, p)) != nullptr; ++part) {
       const int n = u->n;
       warp_wait(q_full, (uint32_t)part & 1u, &quit);
-      for (int x = 0; x <= n; ++x) {
-        if (x < n) {
-          const int g = g0 + x, st = g % STAGES, i = g & 1;
-          if (g >= 2) warp_wait(s_taken + 8 * i, (uint32_t)((g - 2) >> 1) & 1u, &quit);
-          warp_wait(k_full + 8 * st, (uint32_t)(g / STAGES) & 1u, &quit);
+      // scores two tiles in front of the sums: a group of warps finds its next ones when it has made its weights
+#pragma unroll 1
+      for (int x = -2; x < n; ++x) {
+        if (x + 2 < n) {
+          const int g = g0 + x + 2, st = g % STAGES, i = g & 1;
+          if (g >= 2) wait_two(s_taken + 8 * i, (uint32_t)((g - 2) >> 1) & 1u, k_full + 8 * st, (uint32_t)(g / STAGES) & 1u, &quit);
+          else warp_wait(k_full + 8 * st, (uint32_t)(g / STAGES) & 1u, &quit);
           tc_fence_after();
-          if (elected()) {
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) product_tk(tmem + KEYS * i, tmem + Q_AT + 8 * k, base + L::K + st * L::TILE + (k >> 2) * L::HALF + 32 * (k & 3), id_s, k > 0 ? 1u : 0u);
-          }
-          __syncwarp();
-          commit_elected(s_full + 8 * i);
-          commit_elected(k_empty + 8 * st);
+          scores_of_tile<D>(tmem + KEYS * i, tmem + Q_AT, base + L::K + st * L::TILE, id_s, s_done + 8 * st);
         }
-        if (x > 0) {
-          const int g = g0 + x - 1, st = g % STAGES, i = g & 1;
-          warp_wait(v_full + 8 * st, (uint32_t)(g / STAGES) & 1u, &quit);
-          warp_wait(p_full + 8 * i, (uint32_t)(g >> 1) & 1u, &quit);
+        if (x >= 0) {
+          const int g = g0 + x, st = g % STAGES, i = g & 1;
+          wait_two(v_full + 8 * st, (uint32_t)(g / STAGES) & 1u, p_full + 8 * i, (uint32_t)(g >> 1) & 1u, &quit);
           tc_fence_after();
-          if (elected()) {
-#pragma unroll
-            for (int k = 0; k < KEYS / 16; ++k)
-              product_pv(tmem + O_AT + D * i, tmem + P_AT + KEYS / 2 * i + 8 * k, base + L::V + st * L::TILE + k * 2048, L::HALF, id_o, x > 2 || k > 0 ? 1u : 0u);
-          }
-          __syncwarp();
-          commit_elected(o_done + 8 * i);
-          commit_elected(v_empty + 8 * st);
+          sums_of_tile(tmem + O_AT + D * i, tmem + P_AT + KEYS / 2 * i, base + L::V + st * L::TILE, L::HALF, id_o, o_done + 8 * st, x > 1 ? 1u : 0u);
         }
       }
       g0 += n;
@@ -473,23 +479,32 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         }
         asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
         if (i == 0 && (C / HERE == 1 || warp / (4 / (C / HERE)) == round)) {
-          const int r = col % HERE;
-          uint32_t v[D / 2], top = 0;        // magnitudes as numbers, which order like the values
-#pragma unroll
+          const uint8_t* mine = join + col % HERE * 2 * D;
+          const int turn = col & 7;
+          uint32_t top = 0;                  // magnitudes as numbers, which order like the values
+#pragma unroll 2
           for (int k = 0; k < PIECES; ++k) {
-            const uint4 x = *reinterpret_cast<const uint4*>(join + r * 2 * D + ((k ^ (r & 7)) << 4));
-            v[4 * k] = x.x; v[4 * k + 1] = x.y; v[4 * k + 2] = x.z; v[4 * k + 3] = x.w;
-          }
+            const uint4 x = *reinterpret_cast<const uint4*>(mine + ((k ^ turn) << 4));
+            const uint32_t v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-          for (int e = 0; e < D / 2; ++e) top = max(top, max(v[e] << 16 & 0x7fff0000u, v[e] & 0x7fff0000u));
+            for (int e = 0; e < 4; ++e) top = max(top, max(v[e] << 16 & 0x7fff0000u, v[e] & 0x7fff0000u));
+          }
           // A column that is not finite gets NaN, and no other: it asks as zeros, whose weights say whether it sees anything at all, and its factor tells the end of it.
           const bool odd = top >= 0x7f800000u;
           const float power = top && !odd ? power_of_two_in(__uint_as_float(top)) : 1.f, up = __uint_as_float((268u << 23) - __float_as_uint(power));     // 2^14 / power
           if (rep == 0) factors[col] = odd ? NAN : power * (1.f / 16384.f) * p.scale2;
+#pragma unroll 1
+          for (int k = 0; k < PIECES; k += 2) {
+            uint32_t o[8];
 #pragma unroll
-          for (int e = 0; e < D / 2; ++e) v[e] = odd ? 0u : pack_f16(__uint_as_float(v[e] << 16) * up, __uint_as_float(v[e] & 0xffff0000u) * up);
+            for (int e = 0; e < 2; ++e) {
+              const uint4 x = *reinterpret_cast<const uint4*>(mine + (((k + e) ^ turn) << 4));
+              const uint32_t v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-          for (int e = 0; e < D / 2; e += 16) tmem_st16(tmem + lanes + Q_AT + e, v + e);
+              for (int y = 0; y < 4; ++y) o[4 * e + y] = odd ? 0u : pack_f16(__uint_as_float(v[y] << 16) * up, __uint_as_float(v[y] & 0xffff0000u) * up);
+            }
+            tmem_st8(tmem + lanes + Q_AT + 4 * k, o);
+          }
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
@@ -498,23 +513,87 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");    // all columns' factors; the place is free again
       }
     };
-    const Part* next = next_part<C>(walk, p);            // a run has a part at least
-    load_queries(*next);
-    put_queries();
-    for (int g0 = 0; next != nullptr;) {     // tiles in front
+    float fac = 0.f, m = -INFINITY, sum = 0.f;
+    int g0 = 0, done = 0;                    // tiles in front of the part; this group of warps' of the part
+    for (const Part* now = nullptr;;) {
+      // The next part's queries come in beside the end of this one, and its first scores are made while this one's rows are joined.
+      const Part* const next = next_part<C>(walk, p);
+      if (next != nullptr) load_queries(*next);
+      if (now != nullptr) {
+        ml[128 * i + in] = make_float2(m, sum);
+        asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");    // every score has been made
+      }
+      if (next != nullptr) put_queries();
+      if (now != nullptr) {
+        const Part& u = *now;
+        const bool alone = u.u0 == 0 && u.u1 == u.n_pos;
+        float top = -INFINITY, all = 0.f;
+#pragma unroll
+        for (int k = 0; k < 2 * R; ++k) top = fmaxf(top, ml[k * C + col].x);
+#pragma unroll
+        for (int k = 0; k < 2 * R; ++k) {
+          const float2 y = ml[k * C + col];
+          all = fmaf(y.y, y.x == -INFINITY ? 0.f : exp2_fast(y.x - top), all);
+        }
+        const float by = m == -INFINITY ? 0.f : exp2_fast(m - top);
+        if (i == 1 && rep == 0) total[col] = make_float2(top, all != 0.f && isnan(fac) ? NAN : all);
+        const int r0 = u.q.r0, c0 = u.ct * C, n_cols = u.q.n * p.G - c0, slot = 2 * (int)blockIdx.x + (u.u0 == 0 ? 1 : 0);
+        // in pieces of D / 8 dims, LINE threads a column, whose results lie side by side
+        constexpr int PIECE = D / 8, LINE = PIECE / 4, AT_ONCE = SOFT_WARPS * 32 / LINE;
+        auto place = [](int row, int e) { return row * PIECE * 4 + ((e ^ (D == 128 ? row >> 1 & 3 : row >> 2 & 1)) << 4); };
+        const int d_out = threadIdx.x % LINE, c_first = threadIdx.x / LINE;
+#pragma unroll 1
+        for (int c = 0; c < 8; ++c) {
+          uint32_t o[PIECE];
+          if (done > 0) {
+            if constexpr (PIECE == 16) { tmem_ld16(to + PIECE * c, o); tmem_ld_wait16(o); }
+            else { tmem_ld8(to + PIECE * c, o); tmem_ld_wait8(o); }
+          }
+#pragma unroll
+          for (int e = 0; e < LINE; ++e) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (done > 0 && by != 0.f) v = make_float4(__uint_as_float(o[4 * e]) * by, __uint_as_float(o[4 * e + 1]) * by, __uint_as_float(o[4 * e + 2]) * by, __uint_as_float(o[4 * e + 3]) * by);
+            *reinterpret_cast<float4*>(join + place(128 * i + in, e)) = v;
+          }
+          asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
+#pragma unroll
+          for (int c_out = c_first; c_out < C; c_out += AT_ONCE) {
+            if (c_out >= n_cols) break;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 2 * R; ++k) {
+              const float4 v = *reinterpret_cast<const float4*>(join + place(k * C + c_out, d_out));
+              acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+            }
+            const float2 tl = total[c_out];
+            if (alone) {
+              const int cc = c0 + c_out, t_out = cc / p.G;
+              const float inv = tl.y != 0.f ? 1.f / tl.y : 0.f;
+              bf16* out = p.out + (r0 + t_out) * p.out_ld + (long long)(u.h * p.G + cc - t_out * p.G) * D + PIECE * c + 4 * d_out;
+              *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+            } else {
+              const long long at = (long long)slot * C + c_out;
+              if (c == 0 && d_out == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = tl;
+              *reinterpret_cast<float4*>(p.part_o + at * D + PIECE * c + 4 * d_out) = acc;
+            }
+          }
+          asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
+        }
+        g0 += u.n;
+        tc_fence_before();
+      }
+      if (next == nullptr) break;
+      now = next;
       const Part& u = *next;
-      const bool alone = u.u0 == 0 && u.u1 == u.n_pos;
-      if (u.u0 == 0 && !alone && threadIdx.x == 0) {
+      if (u.u0 == 0 && u.u1 < u.n_pos && threadIdx.x == 0) {
         const long long runs = run.to - run.from, left = u.n_pos - u.u1;
         p.split[blockIdx.x] = make_int4(u.s, u.h, u.ct, (int)((left + runs - 1) / runs));
       }
-      const float fac = factors[col];
-      float m = -INFINITY, sum = 0.f;
-      int done = 0;                          // tiles of this group of warps
+      fac = factors[col]; m = -INFINITY; sum = 0.f; done = 0;
       for (int x = (g0 + i) & 1; x < u.n; x += 2, ++done) {
         const int g = g0 + x;
         warp_wait(i_full + 8 * (g % INFOS), (uint32_t)(g / INFOS) & 1u, &quit);
-        warp_wait(s_full + 8 * i, (uint32_t)(g >> 1) & 1u, &quit);
+        warp_wait(s_done + 8 * (g % STAGES), (uint32_t)(g / STAGES) & 1u, &quit);
         tc_fence_after();
         const TileInfo& info = infos[g % INFOS];
         const float4* ip = info.group + rep * HOLD / 16;
@@ -570,7 +649,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         }
         const bool grow = t > __fadd_rd(m, SLACK);     // rounded down: above 2^27 the sum would else round to the score itself, and its weight to infinity
         if (done > 0) {                      // the sum over this group's tile in front has read its weights and settled in O
-          warp_wait(o_done + 8 * i, (uint32_t)((g - 2) >> 1) & 1u, &quit);
+          warp_wait(o_done + 8 * ((g - 2) % STAGES), (uint32_t)((g - 2) / STAGES) & 1u, &quit);
           tc_fence_after();
         }
         if (__any_sync(0xffffffffu, grow)) {
@@ -621,69 +700,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
       }
       if (done > 0) {
         const int g = g0 + ((g0 + i) & 1) + 2 * (done - 1);
-        warp_wait(o_done + 8 * i, (uint32_t)(g >> 1) & 1u, &quit);
+        warp_wait(o_done + 8 * (g % STAGES), (uint32_t)(g / STAGES) & 1u, &quit);
         tc_fence_after();
       }
-      next = next_part<C>(walk, p);
-      if (next != nullptr) load_queries(*next);
-      // join the column's 2 R rows
-      ml[128 * i + in] = make_float2(m, sum);
-      asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
-      if (next != nullptr) put_queries();    // every score has been made: the next part's first ones are beside the joining
-      float top = -INFINITY, all = 0.f;
-#pragma unroll
-      for (int k = 0; k < 2 * R; ++k) top = fmaxf(top, ml[k * C + col].x);
-#pragma unroll
-      for (int k = 0; k < 2 * R; ++k) {
-        const float2 y = ml[k * C + col];
-        all = fmaf(y.y, y.x == -INFINITY ? 0.f : exp2_fast(y.x - top), all);
-      }
-      const float by = m == -INFINITY ? 0.f : exp2_fast(m - top);
-      if (i == 1 && rep == 0) total[col] = make_float2(top, all != 0.f && isnan(fac) ? NAN : all);
-      const int r0 = u.q.r0, c0 = u.ct * C, n_cols = u.q.n * p.G - c0, slot = 2 * (int)blockIdx.x + (u.u0 == 0 ? 1 : 0);
-      // in pieces of D / 8 dims, LINE threads a column, whose results lie side by side
-      constexpr int PIECE = D / 8, LINE = PIECE / 4, AT_ONCE = SOFT_WARPS * 32 / LINE;
-      auto place = [](int row, int e) { return row * PIECE * 4 + ((e ^ (D == 128 ? row >> 1 & 3 : row >> 2 & 1)) << 4); };
-      const int d_out = threadIdx.x % LINE, c_first = threadIdx.x / LINE;
-#pragma unroll 1
-      for (int c = 0; c < 8; ++c) {
-        uint32_t o[PIECE];
-        if (done > 0) {
-          if constexpr (PIECE == 16) { tmem_ld16(to + PIECE * c, o); tmem_ld_wait16(o); }
-          else { tmem_ld8(to + PIECE * c, o); tmem_ld_wait8(o); }
-        }
-#pragma unroll
-        for (int e = 0; e < LINE; ++e) {
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (done > 0 && by != 0.f) v = make_float4(__uint_as_float(o[4 * e]) * by, __uint_as_float(o[4 * e + 1]) * by, __uint_as_float(o[4 * e + 2]) * by, __uint_as_float(o[4 * e + 3]) * by);
-          *reinterpret_cast<float4*>(join + place(128 * i + in, e)) = v;
-        }
-        asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
-#pragma unroll
-        for (int c_out = c_first; c_out < C; c_out += AT_ONCE) {
-          if (c_out >= n_cols) break;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-          for (int k = 0; k < 2 * R; ++k) {
-            const float4 v = *reinterpret_cast<const float4*>(join + place(k * C + c_out, d_out));
-            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-          }
-          const float2 tl = total[c_out];
-          if (alone) {
-            const int cc = c0 + c_out, t_out = cc / p.G;
-            const float inv = tl.y != 0.f ? 1.f / tl.y : 0.f;
-            bf16* out = p.out + (r0 + t_out) * p.out_ld + (long long)(u.h * p.G + cc - t_out * p.G) * D + PIECE * c + 4 * d_out;
-            *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-          } else {
-            const long long at = (long long)slot * C + c_out;
-            if (c == 0 && d_out == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = tl;
-            *reinterpret_cast<float4*>(p.part_o + at * D + PIECE * c + 4 * d_out) = acc;
-          }
-        }
-        asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
-      }
-      g0 += u.n;
-      tc_fence_before();
     }
   }
   __syncthreads();
