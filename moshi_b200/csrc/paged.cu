@@ -565,7 +565,18 @@ __device__ __forceinline__ int piece(int r, int n) { return D == 128 ? r * 128 +
 template <int D>
 __device__ __forceinline__ int token_of(int i) { return (D == 128 ? 0x37156240u : 0x67542310u) >> (4 * i) & 7; }
 
-template <int D, int FMT, int NT>
+// Of a tree's rows, whose own positions the columns have, token j of sequence q for row r: what is cached by the positions, the step's own by the row's mask.
+__device__ __forceinline__ bool sees_in_tree(const AttnP& p, const Seq& q, int r, int pos, int j) {
+  if (pos < 0) return false;
+  const int off = j - q.before;
+  if (off < 0) return p.window <= 0 || pos - j < p.window || j < p.sinks;
+  if (off >= q.n || !(p.seen[(long long)r * p.words + (off >> 5)] >> (off & 31) & 1u)) return false;
+  if (p.window <= 0 || pos - q.before < p.window) return true;
+  const int their = p.position[q.r0 + off];
+  return pos - their < p.window || their < p.sinks;
+}
+
+template <int D, int FMT, int NT, bool TREE>
 __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnP p) {
   constexpr int KS = D / 16, MT = D / 16, COLS = 8 * NT, SIDE = 32 * D;        // bytes of a tile's keys or values
   extern __shared__ uint8_t smem_raw[];
@@ -647,7 +658,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
     const int mine = i + (lane >> 1), j = mine < w.count ? (w.tiles[w.first + mine * FEW_WARPS] << 5) + 16 * (lane & 1) : 0;
     float4 x = make_float4(__int_as_float(HIDDEN), 0.f, -INFINITY, 0.f);
     if (page >= 0) {
-      const bool all = j + 15 <= w.pf && (p.window <= 0 || w.pl - j < p.window || j + 16 <= p.sinks);
+      const bool all = j + 15 <= w.pf - (TREE ? 1 : 0) && (p.window <= 0 || w.pl - j < p.window || j + 16 <= p.sinks);
       x.x = __int_as_float(all ? SEEN : IN_PART);
       x.y = p.k_scale[(long long)page * p.H + w.h];
       const float vs = value_scale(p.v_scale[(long long)page * p.H + w.h]);
@@ -742,7 +753,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
       for (int e = 0; e < 2; ++e) {
         fac[nt][e] = __shfl_sync(0xffffffffu, back, (2 * c + e) * 4) * p.scale2;
         const int cc = nt * 8 + 2 * c + e;
-        pos[nt][e] = cc < n_cols ? q.before + cc / p.G : -1;
+        pos[nt][e] = cc >= n_cols ? -1 : TREE ? (p.window > 0 ? max(p.position[q.r0 + cc / p.G], 0) : q.before) : q.before + cc / p.G;
       }
     }
 
@@ -807,8 +818,13 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (!(has && sees(pos[nt][e & 1], j0 + 16 * half + key_row + 8 * (e >> 1), p.window, p.sinks))) sc[half][nt][e] = -INFINITY;
+            for (int e = 0; e < 4; ++e) {
+              const int j = j0 + 16 * half + key_row + 8 * (e >> 1);
+              bool seen = has;
+              if constexpr (TREE) seen = has && sees_in_tree(p, q, q.r0 + (nt * 8 + 2 * c + (e & 1)) / p.G, pos[nt][e & 1], j);
+              else seen = has && sees(pos[nt][e & 1], j, p.window, p.sinks);
+              if (!seen) sc[half][nt][e] = -INFINITY;
+            }
         }
       }
       float top[NT][2];
@@ -1074,27 +1090,6 @@ int shift_of(int P) { return P == 16 ? 4 : P == 32 ? 5 : P == 64 ? 6 : 7; }
 // there are; the only sequence of a step goes there with all its rows if it may have that many.  (Here / there, 3000 tokens.  32 heads of 128 on 8: 16 requests of 16 columns 39 / 65 us, 64 of them 105 / 233, one 17.5 / 14.8;
 // of 24 columns, as several units a sequence, 87 / 66, of 48 136 / 66.  24 heads of 64 on 4: 16 requests of 18, 24 and 30 columns 26, 26 and 28 / 31, of 24 on 1000 tokens 20 / 19, of 30 on 10000 50 / 81,
 // 64 of 24 61 / 100, one 19 / 13; 32 heads on 8, 32 columns: 16 requests 42 / 53, 4 of them 23 / 21.5.)
-constexpr int few_cols(int dim) { return dim == 64 ? 32 : 16; }
-// CTAs of 8 * nt columns, a wave of them, fewer where the tables allow for less work than that.
-struct FewPlan { int nt, ctas; long long units; bool direct; };
-FewPlan few_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks, int few_rows) {
-  FewPlan f;
-  const long long rows = few_rows <= b->max_rows ? few_rows - 1 : b->max_rows, cols = rows * G;
-  f.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
-  f.units = (long long)b->sequences * c->kv_heads;       // few_cols, and so all rows of a sequence that come here, fit into one
-  long long keys = (long long)b->table_width * c->page_tokens;
-  if (window > 0 && (long long)window + sinks + rows < keys) keys = (long long)window + sinks + rows;
-  const long long tiles = ceil_div64(keys, 32) + 1, runs = ceil_div64(f.units * (tiles + 4), MIN_RUN), wave = 148 * FEW_PER_SM;
-  // A CTA a unit, and nothing to join, where the chip holds all units at once and the longest is not much longer than an equal share: 7 us and 0.25 a tile, against 10.5 and 0.34 for every 296th part of all
-  // tiles and 12 for each unit.  (One token, 32 heads on 8, uncut / cut: 1 request of 1000 tokens 13.4 / 11.3 us, 32 of them 18.2 / 23.7, 8 of 2000 23.3 / 16.7, 32 of them, past the limit, 28.8 / 34.6; 1
-  // session of 374 tokens with 32 heads 8.7 / 11.3.)
-  f.direct = f.units <= wave && tiles <= DIRECT_TILES && 250 * tiles < 3500 + f.units * (tiles + UNIT_COST) * 115 / 100;
-  f.ctas = (int)(f.direct ? f.units : runs < wave ? runs : wave);
-  return f;
-}
-// sums and (maximum, sum of the weights) of two parts per CTA, and where each unit's parts are
-int64_t few_bytes(const FewPlan& f, int D) { return f.direct ? 0 : (int64_t)f.ctas * 2 * 8 * f.nt * (D + 2) * 4 + f.units * 8; }
-
 struct Route { int from_rows; FewPlan few; PromptPlan prompt; int64_t few_bytes, prompt_bytes; };
 Route route(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks) {
   Route r;
@@ -1104,29 +1099,6 @@ Route route(const b200_paged_cache* c, const b200_paged_batch* b, int G, int win
   if (r.from_rows > 1) { r.few = few_plan(c, b, G, window, sinks, r.from_rows); r.few_bytes = (few_bytes(r.few, c->dim) + 15) / 16 * 16; }
   if (many) { r.prompt = prompt_plan(c, b, G, window, sinks); r.prompt_bytes = prompt_bytes(r.prompt, c->dim); }
   return r;
-}
-
-template <int D, int FMT, int NT>
-int launch_few(const AttnP& p, const FewPlan& f, cudaStream_t st) {
-  constexpr int ring = FEW_WARPS * 4 * 32 * D, sums = FEW_WARPS * 8 * (D + 4) * 4, smem = ring + sums + 1024;
-  static std::atomic<uint64_t> limits{0};
-  CUtensorMap map_k, map_v;
-  B200_TRY(code_map(&map_k, p.k, (long long)p.pages * p.H * p.P, D, 16));
-  B200_TRY(code_map(&map_v, p.v, (long long)p.pages * p.H * p.P, D, 16));
-  B200_TRY(allow_smem(limits, smem, few_rows_kernel<D, FMT, NT>));
-  // all of an SM's L1 as shared memory, also for what runs in between: left to the driver an SM keeps what the kernel in front left, and then holds one CTA and not two
-  static std::atomic<uint64_t> shares{0};
-  B200_TRY(prefer_smem(shares, 100, few_rows_kernel<D, FMT, NT>, join_kernel<D, NT>));
-  B200_TRY(launch_early(few_rows_kernel<D, FMT, NT>, dim3((unsigned)f.ctas), dim3(FEW_THREADS), smem, st, map_k, map_v, p));
-  if (f.direct) return B200_OK;
-  const long long most = (long long)p.b.max_rows * p.G < 8 * NT ? (long long)p.b.max_rows * p.G : 8 * NT;
-  return launch_early(join_kernel<D, NT>, dim3((unsigned)(f.units * most)), dim3(128), 0, st, p);
-}
-template <int D, int FMT>
-int launch_few_nt(const AttnP& p, const FewPlan& f, cudaStream_t st) {
-  if constexpr (few_cols(D) > 16)
-    if (f.nt == 4) return launch_few<D, FMT, 4>(p, f, st);
-  return f.nt == 1 ? launch_few<D, FMT, 1>(p, f, st) : launch_few<D, FMT, 2>(p, f, st);
 }
 
 constexpr int WAVE = 148 * 3 / 2;
@@ -1149,7 +1121,63 @@ int launch_append(AppendP& p, cudaStream_t st) {
   return launch_early(append_many_kernel<FMT, D, OWN>, grid, dim3(threads), 0, st, p);
 }
 
+template <int D, int FMT, int NT, bool TREE>
+int launch_few(const AttnP& p, const FewPlan& f, cudaStream_t st) {
+  constexpr int ring = FEW_WARPS * 4 * 32 * D, sums = FEW_WARPS * 8 * (D + 4) * 4, smem = ring + sums + 1024;
+  static std::atomic<uint64_t> limits{0};
+  CUtensorMap map_k, map_v;
+  B200_TRY(code_map(&map_k, p.k, (long long)p.pages * p.H * p.P, D, 16));
+  B200_TRY(code_map(&map_v, p.v, (long long)p.pages * p.H * p.P, D, 16));
+  B200_TRY(allow_smem(limits, smem, few_rows_kernel<D, FMT, NT, TREE>));
+  // all of an SM's L1 as shared memory, also for what runs in between: left to the driver an SM keeps what the kernel in front left, and then holds one CTA and not two
+  static std::atomic<uint64_t> shares{0};
+  B200_TRY(prefer_smem(shares, 100, few_rows_kernel<D, FMT, NT, TREE>, join_kernel<D, NT>));
+  B200_TRY(launch_early(few_rows_kernel<D, FMT, NT, TREE>, dim3((unsigned)f.ctas), dim3(FEW_THREADS), smem, st, map_k, map_v, p));
+  if (f.direct) return B200_OK;
+  const long long most = (long long)p.b.max_rows * p.G < 8 * NT ? (long long)p.b.max_rows * p.G : 8 * NT;
+  return launch_early(join_kernel<D, NT>, dim3((unsigned)(f.units * most)), dim3(128), 0, st, p);
+}
+template <int D, int FMT, bool TREE>
+int launch_few_nt(const AttnP& p, const FewPlan& f, cudaStream_t st) {
+  if constexpr (few_cols(D) > 16)
+    if (f.nt == 4) return launch_few<D, FMT, 4, TREE>(p, f, st);
+  return f.nt == 1 ? launch_few<D, FMT, 1, TREE>(p, f, st) : launch_few<D, FMT, 2, TREE>(p, f, st);
+}
+
 }  // namespace
+
+// CTAs of 8 * nt columns, a wave of them, fewer where the tables allow for less work than that.
+FewPlan few_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks, int few_rows) {
+  FewPlan f;
+  const long long rows = few_rows <= b->max_rows ? few_rows - 1 : b->max_rows, cols = rows * G;
+  f.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
+  f.units = (long long)b->sequences * c->kv_heads;       // few_cols, and so all rows of a sequence that come here, fit into one
+  long long keys = (long long)b->table_width * c->page_tokens;
+  if (window > 0 && (long long)window + sinks + rows < keys) keys = (long long)window + sinks + rows;
+  const long long tiles = ceil_div64(keys, 32) + 1, runs = ceil_div64(f.units * (tiles + 4), MIN_RUN), wave = 148 * FEW_PER_SM;
+  // A CTA a unit, and nothing to join, where the chip holds all units at once and the longest is not much longer than an equal share: 7 us and 0.25 a tile, against 10.5 and 0.34 for every 296th part of all
+  // tiles and 12 for each unit.  (One token, 32 heads on 8, uncut / cut: 1 request of 1000 tokens 13.4 / 11.3 us, 32 of them 18.2 / 23.7, 8 of 2000 23.3 / 16.7, 32 of them, past the limit, 28.8 / 34.6; 1
+  // session of 374 tokens with 32 heads 8.7 / 11.3.)
+  f.direct = f.units <= wave && tiles <= DIRECT_TILES && 250 * tiles < 3500 + f.units * (tiles + UNIT_COST) * 115 / 100;
+  f.ctas = (int)(f.direct ? f.units : runs < wave ? runs : wave);
+  return f;
+}
+// sums and (maximum, sum of the weights) of two parts per CTA, and where each unit's parts are
+int64_t few_bytes(const FewPlan& f, int D) { return f.direct ? 0 : (int64_t)f.ctas * 2 * 8 * f.nt * (D + 2) * 4 + f.units * 8; }
+int few_attention(AttnP p, const FewPlan& f, int fmt, int dim, bool tree, void* work, cudaStream_t st) {
+  p.direct = f.direct;
+  if (!f.direct) {
+    p.part_o = static_cast<float*>(work);
+    p.part_ml = p.part_o + (long long)f.ctas * 2 * 8 * f.nt * dim;
+    p.parts = reinterpret_cast<int2*>(p.part_ml + (long long)f.ctas * 2 * 8 * f.nt * 2);
+  }
+  if (dim == 128) {
+    if (tree) return fmt == INT8 ? launch_few_nt<128, INT8, true>(p, f, st) : launch_few_nt<128, E4M3, true>(p, f, st);
+    return fmt == INT8 ? launch_few_nt<128, INT8, false>(p, f, st) : launch_few_nt<128, E4M3, false>(p, f, st);
+  }
+  if (tree) return fmt == INT8 ? launch_few_nt<64, INT8, true>(p, f, st) : launch_few_nt<64, E4M3, true>(p, f, st);
+  return fmt == INT8 ? launch_few_nt<64, INT8, false>(p, f, st) : launch_few_nt<64, E4M3, false>(p, f, st);
+}
 
 int code_map(CUtensorMap* m, const void* codes, long long rows, int dim, int box_rows) {
   typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -1302,17 +1330,7 @@ int b200_paged_attention(const b200_paged_cache* cache, const b200_paged_batch* 
     }
     B200_TRY(prompt_attention(x, r.prompt, fmt, D, st));
   }
-  if (r.few.units) {
-    const FewPlan& f = r.few;
-    p.direct = f.direct;
-    if (!f.direct) {
-      p.part_o = static_cast<float*>(work_dev);
-      p.part_ml = p.part_o + (long long)f.ctas * 2 * 8 * f.nt * D;
-      p.parts = reinterpret_cast<int2*>(p.part_ml + (long long)f.ctas * 2 * 8 * f.nt * 2);
-    }
-    if (D == 128) B200_TRY((fmt == INT8 ? launch_few_nt<128, INT8>(p, f, st) : launch_few_nt<128, E4M3>(p, f, st)));
-    else B200_TRY((fmt == INT8 ? launch_few_nt<64, INT8>(p, f, st) : launch_few_nt<64, E4M3>(p, f, st)));
-  }
+  if (r.few.units) B200_TRY(few_attention(p, r.few, fmt, D, false, work_dev, st));
   return check_launch("paged_attention");
 }
 

@@ -116,6 +116,10 @@ struct AttnP {
   int pages, P, page_shift, H, G;            // tokens of a page = 1 << page_shift; kv heads; query heads of each
   int window, sinks;
   float scale2;                              // score scale * log2(e)
+  // trees of drafted tokens
+  const uint32_t* seen;                      // [rows][words]: bit i of a row: it sees the sequence's i-th token of the step
+  const int32_t* position;                   // [rows]
+  int words;
   // few rows
   int direct;                                // a CTA per unit
   float *part_o, *part_ml;                   // [CTAs][2][columns][D], [CTAs][2][columns][2]
@@ -164,6 +168,12 @@ int checked_cache(const b200_paged_cache* cache, const char* what);
 int checked(const b200_paged_cache* cache, const b200_paged_batch* batch, const char* what);
 int attention_arguments(AttnP* p, const b200_paged_cache* cache, const b200_paged_batch* batch, const void* q_dev, int64_t q_ld, void* out_dev, int64_t out_ld, int q_heads, float scale, int window,
                         int sinks, const char* what);
+// Attention of few rows: CTAs of 8 * nt columns; tree: the rows are drafted tokens of one.  few_cols: the most columns of a sequence that it takes.
+constexpr int few_cols(int dim) { return dim == 64 ? 32 : 16; }
+struct FewPlan { int nt, ctas; long long units; bool direct; };
+FewPlan few_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks, int few_rows);
+int64_t few_bytes(const FewPlan& f, int D);
+int few_attention(AttnP p, const FewPlan& f, int fmt, int dim, bool tree, void* work, cudaStream_t st);
 // paged_prompt.cu
 struct PromptPlan { int q_tiles, nsplit; long long units; };
 PromptPlan prompt_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks);

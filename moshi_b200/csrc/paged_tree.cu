@@ -71,9 +71,6 @@ constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 6, PRODUCER = 14, ISSUER = 15, THR
 constexpr int UNIT_COST = 10, MIN_RUN = 10;  // in tiles: what a unit costs beside its own, and the least of a CTA
 
 struct TreeP : AttnP {
-  const uint32_t* seen;                      // [rows][words]: bit i of a row: it sees the sequence's i-th token of the step
-  const int32_t* position;                   // [rows]
-  int words;
   int4* split;                               // per CTA: the unit that it begins and does not end (sequence, kv head, columns' number) and how many CTAs behind it have parts of that; 0: there is none
 };
 
@@ -715,70 +712,76 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
   }
 }
 
-// Joins the units that are cut: a block for two columns of the one that a CTA has begun, a column's four teams of sixteen threads take its parts in turn.
+// Joins the units that are cut: a block for 16 columns of the one that a CTA has begun, a warp a column; where there are many parts four warps a column, which take them in turn.
+constexpr int JOIN_COLS = 16, MANY_PARTS = 16;
 template <int D, int C>
-__global__ void __launch_bounds__(128) tree_join_kernel(const TreeP p) {
+__global__ void __launch_bounds__(32 * JOIN_COLS) tree_join_kernel(const TreeP p) {
   pdl_trigger();
   pdl_wait();
-  constexpr int PER = D / 16;
-  __shared__ float o_s[8][D + 4], m_s[8], l_s[8];
-  const int cta = (int)blockIdx.x / (C / 2), col = 2 * ((int)blockIdx.x % (C / 2)) + (threadIdx.x >> 6), team = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * PER;
+  constexpr int PER = D / 32;
+  __shared__ float o_s[JOIN_COLS][D], m_s[JOIN_COLS], l_s[JOIN_COLS];
+  const int cta = (int)blockIdx.x / (C / JOIN_COLS), c0 = (int)blockIdx.x % (C / JOIN_COLS) * JOIN_COLS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 of = p.split[cta];
   if (of.w == 0) return;
   const Seq q = sequence(p.b, of.x, p.P);
-  const int cc = of.z * C + col, token = cc / p.G;
-  const bool has = cc < q.n * p.G;
-  float top = -INFINITY, sum = 0.f, acc[PER];
+  const int n_cols = q.n * p.G - of.z * C, teams = of.w >= MANY_PARTS ? 4 : 1, team = warp & (teams - 1);
+  for (int first = 0; first < JOIN_COLS; first += JOIN_COLS / teams) {
+    const int col = c0 + first + warp / teams;
+    float top = -INFINITY, sum = 0.f, acc[PER];
 #pragma unroll
-  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-  if (has) {
-    // the first part is its run's last, the others are their runs' first
-#pragma unroll 2
-    for (int i = team & 3; i <= of.w; i += 4) {
-      const long long at = (long long)(2 * (cta + i) + (i == 0 ? 1 : 0)) * C + col;
-      const float2 y = reinterpret_cast<const float2*>(p.part_ml)[at];
-      const float now = fmaxf(top, y.x), keep = now == -INFINITY ? 0.f : exp2_fast(top - now), by = now == -INFINITY ? 0.f : exp2_fast(y.x - now);
-      const float4* o = reinterpret_cast<const float4*>(p.part_o + at * D + d0);
-      top = now;
-      sum = fmaf(sum, keep, y.y * by);
+    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+    if (col < n_cols) {
+      // the first part is its run's last, the others are their runs' first
+#pragma unroll 4
+      for (int i = team; i <= of.w; i += teams) {
+        const long long at = (long long)(2 * (cta + i) + (i == 0 ? 1 : 0)) * C + col;
+        const float2 y = reinterpret_cast<const float2*>(p.part_ml)[at];
+        float v[PER];
 #pragma unroll
-      for (int e = 0; e < PER / 4; ++e) {
-        const float4 v = o[e];
-        acc[4 * e] = fmaf(acc[4 * e], keep, v.x * by); acc[4 * e + 1] = fmaf(acc[4 * e + 1], keep, v.y * by);
-        acc[4 * e + 2] = fmaf(acc[4 * e + 2], keep, v.z * by); acc[4 * e + 3] = fmaf(acc[4 * e + 3], keep, v.w * by);
+        for (int e = 0; e < PER; ++e) v[e] = p.part_o[at * D + 32 * e + lane];
+        const float now = fmaxf(top, y.x), keep = now == -INFINITY ? 0.f : exp2_fast(top - now), by = now == -INFINITY ? 0.f : exp2_fast(y.x - now);
+        top = now;
+        sum = fmaf(sum, keep, y.y * by);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] = fmaf(acc[e], keep, v[e] * by);
       }
     }
+    if (teams > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < PER; ++e) o_s[warp][32 * e + lane] = acc[e];
+      if (lane == 0) { m_s[warp] = top; l_s[warp] = sum; }
+      __syncthreads();
+      if (team) continue;
+      for (int i = 1; i < teams; ++i) {
+        const float now = fmaxf(top, m_s[warp + i]), keep = now == -INFINITY ? 0.f : exp2_fast(top - now), by = now == -INFINITY ? 0.f : exp2_fast(m_s[warp + i] - now);
+        top = now;
+        sum = fmaf(sum, keep, l_s[warp + i] * by);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] = fmaf(acc[e], keep, o_s[warp + i][32 * e + lane] * by);
+      }
+    }
+    if (col >= n_cols) continue;
+    const int cc = of.z * C + col, token = cc / p.G;
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+    bf16* out = p.out + (q.r0 + token) * p.out_ld + (long long)(of.y * p.G + cc - token * p.G) * D + lane;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) out[32 * e] = __float2bfloat16_rn(acc[e] * inv);
   }
-#pragma unroll
-  for (int e = 0; e < PER; ++e) o_s[team][d0 + e] = acc[e];
-  if ((threadIdx.x & 15) == 0) { m_s[team] = top; l_s[team] = sum; }
-  __syncthreads();
-  if ((team & 3) || !has) return;
-  top = -INFINITY; sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top = fmaxf(top, m_s[team + i]);
-#pragma unroll
-  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float by = m_s[team + i] == -INFINITY ? 0.f : exp2_fast(m_s[team + i] - top);
-    sum = fmaf(l_s[team + i], by, sum);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] = fmaf(o_s[team + i][d0 + e], by, acc[e]);
-  }
-  const float inv = sum != 0.f ? 1.f / sum : 0.f;
-  bf16* out = p.out + (q.r0 + token) * p.out_ld + (long long)(of.y * p.G + cc - token * p.G) * D + d0;
-#pragma unroll
-  for (int e = 0; e < PER; e += 4) *reinterpret_cast<uint2*>(out + e) = make_uint2(pack_bf16(acc[e] * inv, acc[e + 1] * inv), pack_bf16(acc[e + 2] * inv, acc[e + 3] * inv));
 }
 
 // =========================================================================================================================
 // host
 // =========================================================================================================================
-struct TreePlan { int cols, ctas; };
+struct TreePlan { int cols, ctas; FewPlan few; };      // few.units: the columns of a sequence are few enough for the kernel of few rows
 TreePlan tree_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks) {
   TreePlan f;
+  memset(&f, 0, sizeof(f));
   const long long cols = (long long)b->max_rows * G;
+  if (cols <= few_cols(c->dim)) {
+    f.few = few_plan(c, b, G, window, sinks, 0x7fffffff);
+    return f;
+  }
   f.cols = cols <= 32 ? 32 : cols <= 64 ? 64 : 128;
   long long keys = (long long)b->table_width * c->page_tokens;
   if (window > 0 && (long long)window + sinks + b->max_rows < keys) keys = (long long)window + sinks + b->max_rows;
@@ -787,7 +790,7 @@ TreePlan tree_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, 
   return f;
 }
 // sums and (maximum, sum of the weights) of two parts per CTA, and the units that are cut
-int64_t tree_bytes(const TreePlan& f, int D) { return (int64_t)f.ctas * (2 * f.cols * (D + 2) * 4 + 16); }
+int64_t tree_bytes(const TreePlan& f, int D) { return f.few.units ? few_bytes(f.few, D) : (int64_t)f.ctas * (2 * f.cols * (D + 2) * 4 + 16); }
 
 template <int D, int FMT, int C>
 int launch(const TreeP& p, int ctas, cudaStream_t st) {
@@ -799,7 +802,7 @@ int launch(const TreeP& p, int ctas, cudaStream_t st) {
   B200_TRY(allow_smem(limits, (int)TreeSmem<D>::BYTES, tree_kernel<D, FMT, C>));
   B200_TRY(prefer_smem(shares, 100, tree_kernel<D, FMT, C>, tree_join_kernel<D, C>));
   B200_TRY(launch_early(tree_kernel<D, FMT, C>, dim3((unsigned)ctas), dim3(THREADS), TreeSmem<D>::BYTES, st, map_k, map_v, p));
-  return launch_early(tree_join_kernel<D, C>, dim3((unsigned)(ctas * (C / 2))), dim3(128), 0, st, p);
+  return launch_early(tree_join_kernel<D, C>, dim3((unsigned)(ctas * (C / JOIN_COLS))), dim3(32 * JOIN_COLS), 0, st, p);
 }
 template <int D, int FMT>
 int launch_cols(const TreeP& p, const TreePlan& f, cudaStream_t st) {
@@ -846,15 +849,21 @@ int b200_paged_tree_attention(const b200_paged_cache* cache, const b200_paged_ba
   if (batch->total_rows == 0 || batch->max_rows == 0) return B200_OK;
   const TreePlan f = tree_plan(cache, batch, p.G, window, sinks);
   const int64_t need = tree_bytes(f, cache->dim);
-  if (!work_dev || work_bytes < need || (reinterpret_cast<uintptr_t>(work_dev) & 15))
+  if (f.few.units > 0x7fffffffll / 64) B200_FAIL(B200_ERR_SHAPE, "paged_tree_attention: %d sequences with %d heads in one call", batch->sequences, q_heads);
+  if (need > 0 && (!work_dev || work_bytes < need || (reinterpret_cast<uintptr_t>(work_dev) & 15)))
     B200_FAIL(B200_ERR_INVALID, "paged_tree_attention: a workspace of %lld bytes; b200_paged_tree_attention_bytes asks for %lld, on a 16-byte border", (long long)work_bytes, (long long)need);
   DeviceGuard guard(cache->device);
   p.seen = tree->seen_dev; p.position = tree->position_dev; p.words = tree->words;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool i8 = cache->kv_dtype == B200_KV_INT8;
+  if (f.few.units) {
+    p.from_rows = 0x7fffffff;
+    B200_TRY(few_attention(p, f.few, i8 ? INT8 : E4M3, cache->dim, true, work_dev, st));
+    return check_launch("paged_tree_attention");
+  }
   p.part_o = static_cast<float*>(work_dev);
   p.part_ml = p.part_o + (long long)f.ctas * 2 * f.cols * cache->dim;
   p.split = reinterpret_cast<int4*>(p.part_ml + (long long)f.ctas * 2 * f.cols * 2);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool i8 = cache->kv_dtype == B200_KV_INT8;
   if (cache->dim == 128) B200_TRY((i8 ? launch_cols<128, INT8>(p, f, st) : launch_cols<128, E4M3>(p, f, st)));
   else B200_TRY((i8 ? launch_cols<64, INT8>(p, f, st) : launch_cols<64, E4M3>(p, f, st)));
   return check_launch("paged_tree_attention");
