@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(128) tree_build_kernel(const BuildP p) {
 // attention
 // =========================================================================================================================
 constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 6, PRODUCER = 14, ISSUER = 15, THREADS = 16 * 32, SHIFT = 6, KEYS = 1 << SHIFT, STAGES = 4, INFOS = 32;
-constexpr int UNIT_COST = 10, MIN_RUN = 10;  // in tiles: what a unit costs beside its own, and the least of a CTA
+constexpr int UNIT_COST = 12, MIN_RUN = 12;  // in tiles: what a unit costs beside its own, and the least of a CTA
 
 struct TreeP : AttnP {
   int4* split;                               // per CTA: the unit that it begins and does not end (sequence, kv head, columns' number) and how many CTAs behind it have parts of that; 0: there is none
@@ -589,8 +589,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
       fac = factors[col]; m = -INFINITY; sum = 0.f; done = 0;
       for (int x = (g0 + i) & 1; x < u.n; x += 2, ++done) {
         const int g = g0 + x;
-        warp_wait(i_full + 8 * (g % INFOS), (uint32_t)(g / INFOS) & 1u, &quit);
-        warp_wait(s_done + 8 * (g % STAGES), (uint32_t)(g / STAGES) & 1u, &quit);
+        wait_two(i_full + 8 * (g % INFOS), (uint32_t)(g / INFOS) & 1u, s_done + 8 * (g % STAGES), (uint32_t)(g / STAGES) & 1u, &quit);
         tc_fence_after();
         const TileInfo& info = infos[g % INFOS];
         const float4* ip = info.group + rep * HOLD / 16;
