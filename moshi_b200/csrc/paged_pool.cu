@@ -309,7 +309,8 @@ __global__ void __launch_bounds__(ONE) reserve_kernel(const ReserveP p) {
     int need = 0, copy = 0;
     if (s < S) {
       const int held = p.o.held[s], page = begun[s];
-      need = max(want(s, held) - held, 0);
+      const int pages = want(s, held);
+      need = pages < 0 ? 0 : pages - held;
       if (page >= 0) {
         int rank = 0;
         for (int i = 0; i < s; ++i) rank += begun[i] == page;

@@ -842,10 +842,11 @@ int b200_paged_tree_attention(const b200_paged_cache* cache, const b200_paged_ba
   using namespace b200::paged;
   TreeP p;
   B200_TRY(attention_arguments(&p, cache, batch, q_dev, q_ld, out_dev, out_ld, q_heads, scale, window, sinks, "paged_tree_attention"));
-  if (!tree || !tree->seen_dev || !tree->position_dev) B200_FAIL(B200_ERR_INVALID, "paged_tree_attention: null pointer in the tree");
+  const bool empty = batch->total_rows == 0 || batch->max_rows == 0;
+  if (!tree || (!empty && (!tree->seen_dev || !tree->position_dev))) B200_FAIL(B200_ERR_INVALID, "paged_tree_attention: null pointer in the tree");
   if (batch->max_rows > MAX_NODES || tree->words < 1 || (long long)tree->words * 32 < batch->max_rows || tree->words > MAX_NODES / 32)
     B200_FAIL(B200_ERR_SHAPE, "paged_tree_attention: trees of up to %d tokens (at most %d), masks of %d words", batch->max_rows, MAX_NODES, tree->words);
-  if (batch->total_rows == 0 || batch->max_rows == 0) return B200_OK;
+  if (empty) return B200_OK;
   const TreePlan f = tree_plan(cache, batch, p.G, window, sinks);
   const int64_t need = tree_bytes(f, cache->dim);
   if (f.few.units > 0x7fffffffll / 64) B200_FAIL(B200_ERR_SHAPE, "paged_tree_attention: %d sequences with %d heads in one call", batch->sequences, q_heads);
