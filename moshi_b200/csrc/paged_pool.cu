@@ -29,12 +29,12 @@ constexpr int KEEP_THREADS = 256;
 
 // The least number of doublings with which a page's largest code reaches `top`.  Both sides are products of a code and a scale, so that equal scales never double.
 template <int FMT>
-__device__ __forceinline__ int doublings_for(float top, float s_old) {
-  const float limit = s_old * code_max<FMT>();
+__device__ __forceinline__ int doublings_for(double top, float s_old) {
+  const double limit = (double)s_old * (double)code_max<FMT>();
   if (!(top > limit)) return 0;
   int power;
-  const float part = frexpf(top / limit, &power);
-  return part == 0.5f ? power - 1 : power;
+  const double part = frexp(top / limit, &power);
+  return part == 0.5 ? power - 1 : power;
 }
 template <int FMT>
 __device__ __forceinline__ float largest_code(const uint4& x) {
@@ -61,6 +61,27 @@ __device__ __forceinline__ uint4 converted(const uint4& x, float s, float by) {
   for (int i = 0; i < 4; ++i) {
     const float2 a = float2_of<FMT, 0>(w[i]), b = float2_of<FMT, 1>(w[i]);
     o[i] = codes4<FMT>(one(a.x), one(a.y), one(b.x), one(b.y));
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+// The same in 64 bits.  Where rows give a page its scale, quotients of their codes are ratios of whole numbers, and halves among them are common: in 32 bits it would be chance which way those go.
+template <int FMT>
+__device__ __forceinline__ uint4 converted_far(const uint4& x, double s, double by) {
+  const double inv = 1.0 / by;
+  auto one = [&](float c) {
+    const double v = (double)c * s, q = v * inv;
+    return fma(fma(-q, by, v), inv, q);
+  };
+  const uint32_t w[4] = {ready<FMT>(x.x), ready<FMT>(x.y), ready<FMT>(x.z), ready<FMT>(x.w)};
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 a = float2_of<FMT, 0>(w[i]), b = float2_of<FMT, 1>(w[i]);
+    double q[4] = {one(a.x), one(a.y), one(b.x), one(b.y)};
+    if constexpr (FMT == INT8)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[e] = rint(q[e]);
+    o[i] = codes4<FMT>((float)q[0], (float)q[1], (float)q[2], (float)q[3]);
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
@@ -127,7 +148,7 @@ __global__ void __launch_bounds__(KEEP_THREADS) keep_kernel(const __grid_constan
     if (page < 0) continue;                              // its rows are left out
     const int first = block * p.P, i0 = max(first - q.before, 0), i1 = (int)min((long long)first + p.P - q.before, (long long)count), older = max(q.before - first, 0);
     // the largest value that comes from another page
-    float top = 0.f;
+    double top = 0.0;
     bool far = false, near = false;
     for (int i = i0 + row0; i - row0 < i1; i += RPS) {
       if (i >= i1) continue;
@@ -136,20 +157,23 @@ __global__ void __launch_bounds__(KEEP_THREADS) keep_kernel(const __grid_constan
       const int source = table[b];
       far = true;
       if (source < 0 || source >= p.pages) { atomicOr(p.flags, B200_PAGED_BAD_PAGE); continue; }
-      top = fmaxf(top, largest_code<FMT>(*reinterpret_cast<const uint4*>(at(source, from - b * p.P))) * scales[(long long)source * p.H + h]);
+      top = fmax(top, (double)largest_code<FMT>(*reinterpret_cast<const uint4*>(at(source, from - b * p.P))) * (double)scales[(long long)source * p.H + h]);
     }
-    top = warp_max(top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
     far = __any_sync(0xffffffffu, far);
     const bool resident = older > 0 || __any_sync(0xffffffffu, near);
     const float s_old = scales[(long long)page * p.H + h];
     float sc = s_old;
+    double own = 0.0;                                    // the scale that the rows themselves give the page
     int doublings = 0;
     if (far) {
       if (resident && s_old > 0.f) {
         doublings = doublings_for<FMT>(top, s_old);
         sc = ldexpf(s_old, doublings);
       } else {
-        sc = top > 0.f ? fmaxf(top / code_max<FMT>(), SCALE_MIN) : 0.f;
+        own = top > 0.0 ? fmax(top / (double)code_max<FMT>(), (double)SCALE_MIN) : 0.0;
+        sc = (float)own;
         doublings = -1;
       }
     }
@@ -171,7 +195,11 @@ __global__ void __launch_bounds__(KEEP_THREADS) keep_kernel(const __grid_constan
         } else {
           const int source = table[b];
           put = source >= 0 && source < p.pages;
-          if (put) x = converted<FMT>(*reinterpret_cast<const uint4*>(at(source, from - b * p.P)), scales[(long long)source * p.H + h], sc);
+          if (put) {
+            const uint4 was = *reinterpret_cast<const uint4*>(at(source, from - b * p.P));
+            const float s_from = scales[(long long)source * p.H + h];
+            x = own > 0.0 ? converted_far<FMT>(was, (double)s_from, own) : converted<FMT>(was, s_from, sc);
+          }
         }
       }
       __syncwarp();                                      // rows of a sweep are read before one is written
