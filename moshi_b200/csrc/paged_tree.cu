@@ -264,8 +264,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
   __shared__ volatile int quit;              // somebody has waited too long: nobody waits any more, and all go through to the end
   __shared__ int end;                        // number of the converters' jobs, once it is known
   __shared__ float factors[C];               // of a column: what turns a product of codes into a score in base 2, but for the keys' scale
-  __shared__ float2 ml[256], total[C];
-  __shared__ Walk walks[THREADS / 32];
+  __shared__ float2 ml[256], total[2][C];
+  __shared__ Walk walks[SOFT_WARPS + 2];     // of the weights' warps, the producer and the issuer
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_at;
-  Walk& walk = walks[warp];
+  Walk& walk = walks[warp < SOFT_WARPS ? warp : warp == PRODUCER ? SOFT_WARPS : SOFT_WARPS + 1];
   if (lane == 0 && (warp < SOFT_WARPS || warp >= PRODUCER)) {
     walk.f = run.from; walk.to = run.to; walk.base = run.base; walk.now = 0;
     walk_to<C>(walk, p, run.s);
@@ -468,53 +468,53 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     };
     auto put_queries = [&]() {
 #pragma unroll
+      for (int k = 0; k < MINE; ++k) {
+        uint32_t v[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w}, top = 0;    // magnitudes as numbers, which order like the values
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, max(v[e] << 16 & 0x7fff0000u, v[e] & 0x7fff0000u));
+#pragma unroll
+        for (int o = PIECES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // A column that is not finite gets NaN, and no other: it asks as zeros, whose weights say whether it sees anything at all, and its factor tells the end of it.
+        const bool odd = top >= 0x7f800000u;
+        const float power = top && !odd ? power_of_two_in(__uint_as_float(top)) : 1.f, up = __uint_as_float((268u << 23) - __float_as_uint(power));     // 2^14 / power
+        if (c_q == 0) factors[r_at + k * APART] = odd ? NAN : power * (1.f / 16384.f) * p.scale2;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = odd ? 0u : pack_f16(__uint_as_float(v[e] << 16) * up, __uint_as_float(v[e] & 0xffff0000u) * up);
+        raw[k] = make_uint4(v[0], v[1], v[2], v[3]);
+      }
+#pragma unroll
       for (int round = 0; round < C / HERE; ++round) {
 #pragma unroll
         for (int k = round * (MINE * HERE / C); k < (round + 1) * (MINE * HERE / C); ++k) {
           const int r = r_at + k * APART - round * HERE;
           *reinterpret_cast<uint4*>(join + r * 2 * D + ((c_q ^ (r & 7)) << 4)) = raw[k];
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");    // all columns' factors, too
         if (i == 0 && (C / HERE == 1 || warp / (4 / (C / HERE)) == round)) {
           const uint8_t* mine = join + col % HERE * 2 * D;
-          const int turn = col & 7;
-          uint32_t top = 0;                  // magnitudes as numbers, which order like the values
 #pragma unroll 2
-          for (int k = 0; k < PIECES; ++k) {
-            const uint4 x = *reinterpret_cast<const uint4*>(mine + ((k ^ turn) << 4));
-            const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+          for (int k = 0; k < PIECES; k += 4) {
+            uint32_t v[16];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = max(top, max(v[e] << 16 & 0x7fff0000u, v[e] & 0x7fff0000u));
-          }
-          // A column that is not finite gets NaN, and no other: it asks as zeros, whose weights say whether it sees anything at all, and its factor tells the end of it.
-          const bool odd = top >= 0x7f800000u;
-          const float power = top && !odd ? power_of_two_in(__uint_as_float(top)) : 1.f, up = __uint_as_float((268u << 23) - __float_as_uint(power));     // 2^14 / power
-          if (rep == 0) factors[col] = odd ? NAN : power * (1.f / 16384.f) * p.scale2;
-#pragma unroll 1
-          for (int k = 0; k < PIECES; k += 2) {
-            uint32_t o[8];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint4 x = *reinterpret_cast<const uint4*>(mine + (((k + e) ^ turn) << 4));
-              const uint32_t v[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-              for (int y = 0; y < 4; ++y) o[4 * e + y] = odd ? 0u : pack_f16(__uint_as_float(v[y] << 16) * up, __uint_as_float(v[y] & 0xffff0000u) * up);
+            for (int e = 0; e < 4; ++e) {
+              const uint4 x = *reinterpret_cast<const uint4*>(mine + (((k + e) ^ (col & 7)) << 4));
+              v[4 * e] = x.x; v[4 * e + 1] = x.y; v[4 * e + 2] = x.z; v[4 * e + 3] = x.w;
             }
-            tmem_st8(tmem + lanes + Q_AT + 4 * k, o);
+            tmem_st16(tmem + lanes + Q_AT + 4 * k, v);
           }
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(q_full);
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");    // all columns' factors; the place is free again
+        asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");    // the place is free again
       }
     };
     float fac = 0.f, m = -INFINITY, sum = 0.f;
     int g0 = 0, done = 0;                    // tiles in front of the part; this group of warps' of the part
+    const Part* next = next_part<C>(walk, p);            // a run has a part at least
     for (const Part* now = nullptr;;) {
       // The next part's queries come in beside the end of this one, and its first scores are made while this one's rows are joined.
-      const Part* const next = next_part<C>(walk, p);
       if (next != nullptr) load_queries(*next);
       if (now != nullptr) {
         ml[128 * i + in] = make_float2(m, sum);
@@ -524,6 +524,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
       if (now != nullptr) {
         const Part& u = *now;
         const bool alone = u.u0 == 0 && u.u1 == u.n_pos;
+        tc_fence_after();
+        // Join the column's 2 R rows.  Both groups' sums of a row lie in the row's lane: the first group of warps has half of the dims of both, the second the rest; the R copies go through shared memory.
         float top = -INFINITY, all = 0.f;
 #pragma unroll
         for (int k = 0; k < 2 * R; ++k) top = fmaxf(top, ml[k * C + col].x);
@@ -532,52 +534,64 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
           const float2 y = ml[k * C + col];
           all = fmaf(y.y, y.x == -INFINITY ? 0.f : exp2_fast(y.x - top), all);
         }
-        const float by = m == -INFINITY ? 0.f : exp2_fast(m - top);
-        if (i == 1 && rep == 0) total[col] = make_float2(top, all != 0.f && isnan(fac) ? NAN : all);
+        float by[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) by[k] = ml[128 * k + in].x == -INFINITY ? 0.f : exp2_fast(ml[128 * k + in].x - top);
+        if (rep == 0) total[i][col] = make_float2(top, all != 0.f && isnan(fac) ? NAN : all);
         const int r0 = u.q.r0, c0 = u.ct * C, n_cols = u.q.n * p.G - c0, slot = 2 * (int)blockIdx.x + (u.u0 == 0 ? 1 : 0);
         // in pieces of D / 8 dims, LINE threads a column, whose results lie side by side
-        constexpr int PIECE = D / 8, LINE = PIECE / 4, AT_ONCE = SOFT_WARPS * 32 / LINE;
+        constexpr int PIECE = D / 8, LINE = PIECE / 4, AT_ONCE = 128 / LINE;
         auto place = [](int row, int e) { return row * PIECE * 4 + ((e ^ (D == 128 ? row >> 1 & 3 : row >> 2 & 1)) << 4); };
-        const int d_out = threadIdx.x % LINE, c_first = threadIdx.x / LINE;
+        const int d_out = in % LINE, c_first = in / LINE;
+        uint8_t* const mine = join + i * (128 * PIECE * 4);
 #pragma unroll 1
-        for (int c = 0; c < 8; ++c) {
-          uint32_t o[PIECE];
-          if (done > 0) {
-            if constexpr (PIECE == 16) { tmem_ld16(to + PIECE * c, o); tmem_ld_wait16(o); }
-            else { tmem_ld8(to + PIECE * c, o); tmem_ld_wait8(o); }
+        for (int c = 0; c < 4; ++c) {
+          const int d0 = (4 * i + c) * PIECE;
+          uint32_t o[2][PIECE];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t at = tmem + lanes + O_AT + D * k + d0;
+            if constexpr (PIECE == 16) tmem_ld16(at, o[k]); else tmem_ld8(at, o[k]);
           }
 #pragma unroll
+          for (int k = 0; k < 2; ++k) { if constexpr (PIECE == 16) tmem_ld_wait16(o[k]); else tmem_ld_wait8(o[k]); }
+#pragma unroll
           for (int e = 0; e < LINE; ++e) {
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (done > 0 && by != 0.f) v = make_float4(__uint_as_float(o[4 * e]) * by, __uint_as_float(o[4 * e + 1]) * by, __uint_as_float(o[4 * e + 2]) * by, __uint_as_float(o[4 * e + 3]) * by);
-            *reinterpret_cast<float4*>(join + place(128 * i + in, e)) = v;
+            float v[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {    // a group that has seen nothing may have anything there
+              v[y] = by[0] != 0.f ? __uint_as_float(o[0][4 * e + y]) * by[0] : 0.f;
+              if (by[1] != 0.f) v[y] = fmaf(__uint_as_float(o[1][4 * e + y]), by[1], v[y]);
+            }
+            *reinterpret_cast<float4*>(mine + place(in, e)) = make_float4(v[0], v[1], v[2], v[3]);
           }
-          asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
+          asm volatile("bar.sync %0, 128;" ::"r"(2 + i) : "memory");
 #pragma unroll
           for (int c_out = c_first; c_out < C; c_out += AT_ONCE) {
             if (c_out >= n_cols) break;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int k = 0; k < 2 * R; ++k) {
-              const float4 v = *reinterpret_cast<const float4*>(join + place(k * C + c_out, d_out));
+            for (int k = 0; k < R; ++k) {
+              const float4 v = *reinterpret_cast<const float4*>(mine + place(k * C + c_out, d_out));
               acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
             }
-            const float2 tl = total[c_out];
+            const float2 tl = total[i][c_out];
             if (alone) {
               const int cc = c0 + c_out, t_out = cc / p.G;
               const float inv = tl.y != 0.f ? 1.f / tl.y : 0.f;
-              bf16* out = p.out + (r0 + t_out) * p.out_ld + (long long)(u.h * p.G + cc - t_out * p.G) * D + PIECE * c + 4 * d_out;
+              bf16* out = p.out + (r0 + t_out) * p.out_ld + (long long)(u.h * p.G + cc - t_out * p.G) * D + d0 + 4 * d_out;
               *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
             } else {
               const long long at = (long long)slot * C + c_out;
-              if (c == 0 && d_out == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = tl;
-              *reinterpret_cast<float4*>(p.part_o + at * D + PIECE * c + 4 * d_out) = acc;
+              if (i == 0 && c == 0 && d_out == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = tl;
+              *reinterpret_cast<float4*>(p.part_o + at * D + d0 + 4 * d_out) = acc;
             }
           }
-          asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");
+          asm volatile("bar.sync %0, 128;" ::"r"(2 + i) : "memory");
         }
         g0 += u.n;
         tc_fence_before();
+        asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");    // both groups have read both sums
       }
       if (next == nullptr) break;
       now = next;
@@ -587,6 +601,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         p.split[blockIdx.x] = make_int4(u.s, u.h, u.ct, (int)((left + runs - 1) / runs));
       }
       fac = factors[col]; m = -INFINITY; sum = 0.f; done = 0;
+      next = next_part<C>(walk, p);
+      if (next != nullptr) {                 // its queries into L2
+        const int cc = next->ct * C + (int)threadIdx.x % C, token = cc / p.G;
+        const bf16* row = p.q + (next->q.r0 + token) * p.q_ld + (long long)(next->h * p.G + cc - token * p.G) * D;
+        if (cc < next->q.n * p.G && (int)threadIdx.x < C * (D / 64)) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + (int)threadIdx.x / C * 64));
+      }
       for (int x = (g0 + i) & 1; x < u.n; x += 2, ++done) {
         const int g = g0 + x;
         wait_two(i_full + 8 * (g % INFOS), (uint32_t)(g / INFOS) & 1u, s_done + 8 * (g % STAGES), (uint32_t)(g / STAGES) & 1u, &quit);
