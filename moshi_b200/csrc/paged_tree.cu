@@ -76,7 +76,7 @@ struct TreeP : AttnP {
 
 template <int D>
 struct TreeSmem {
-  static constexpr int SLOTS = CONVERT_WARPS * (D == 128 ? 3 : 6);            // places of 32 tokens' codes; a place is always the same warp's
+  static constexpr int SLOTS = CONVERT_WARPS * (D == 128 ? 3 : 6), PAIRS = SLOTS / 2;         // places of 32 tokens' codes; a place is always the same warp's; two of them side by side have a tile's keys or values
   static constexpr uint32_t HALF = KEYS * 128, TILE = HALF * (D / 64);        // a tile's f16 rows, in halves of 64 dims
   static constexpr uint32_t SLOT = 32 * D, K = 0, V = K + STAGES * TILE, CODES = V + STAGES * TILE, JOIN = CODES + SLOTS * SLOT, BYTES = JOIN + 256 * D / 2 + 1024;
 };
@@ -253,12 +253,12 @@ template <int C> constexpr int soft_regs() { return C == 128 ? 168 : 144; }
 template <int D, int FMT, int C>
 __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TreeP p) {
   typedef TreeSmem<D> L;
-  constexpr int R = 128 / C, HOLD = KEYS / R, SLOTS = L::SLOTS;               // HOLD: scores of a weight thread
+  constexpr int R = 128 / C, HOLD = KEYS / R, SLOTS = L::SLOTS, PAIRS = L::PAIRS;        // HOLD: scores of a weight thread
   // TMEM: scores and weights of the two groups of warps, their sums, the queries
   constexpr uint32_t P_AT = 2 * KEYS, O_AT = P_AT + KEYS, Q_AT = 512 - D / 2;
   static_assert(O_AT + 2 * D <= Q_AT, "TMEM");
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * SLOTS + 4 * STAGES + 5 + INFOS];
+  __shared__ __align__(8) uint64_t bars[2 * PAIRS + 4 * STAGES + 5 + INFOS];
   __shared__ __align__(16) TileInfo infos[INFOS];
   __shared__ uint32_t tmem_at;
   __shared__ volatile int quit;              // somebody has waited too long: nobody waits any more, and all go through to the end
@@ -269,12 +269,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t bar = smem_u32(bars), c_full = bar, c_empty = c_full + 8 * SLOTS, k_full = c_empty + 8 * SLOTS, v_full = k_full + 8 * STAGES,
+  const uint32_t bar = smem_u32(bars), c_full = bar, c_empty = c_full + 8 * PAIRS, k_full = c_empty + 8 * PAIRS, v_full = k_full + 8 * STAGES,
                  s_done = v_full + 8 * STAGES, o_done = s_done + 8 * STAGES, p_full = o_done + 8 * STAGES, s_taken = p_full + 16, q_full = s_taken + 16, i_full = q_full + 8;
   if (threadIdx.x == 0) {
     quit = 0;
     end = 0x7fffffff;
-    for (int i = 0; i < SLOTS; ++i) { mbar_init(c_full + 8 * i, 1); mbar_init(c_empty + 8 * i, 1); }
+    for (int i = 0; i < PAIRS; ++i) { mbar_init(c_full + 8 * i, 1); mbar_init(c_empty + 8 * i, 2); }
     for (int i = 0; i < STAGES; ++i) { mbar_init(k_full + 8 * i, 2); mbar_init(v_full + 8 * i, 2); mbar_init(s_done + 8 * i, 1); mbar_init(o_done + 8 * i, 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(s_taken + 8 * i, 4); mbar_init(p_full + 8 * i, 4); }
     mbar_init(q_full, 4);
@@ -308,9 +308,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     // lanes of a row's second 64 dims take the neighbouring row, so that eight lanes' pieces of the f16 tile lie in different banks
     const int r_in = lane / LANES ^ (D == 128 ? c >> 2 : 0);
     for (int j = warp - SOFT_WARPS;; j += CONVERT_WARPS) {
-      const int slot = j % SLOTS, g = j >> 2, st = g % STAGES, half = j & 1;
+      const int slot = j % SLOTS, pair = slot >> 1, g = j >> 2, st = g % STAGES, half = j & 1;
       const bool values = j & 2;
-      warp_wait(c_full + 8 * slot, (uint32_t)(j / SLOTS) & 1u, &quit);
+      warp_wait(c_full + 8 * pair, (uint32_t)(j / SLOTS) & 1u, &quit);
       if (__any_sync(0xffffffffu, quit || j >= *(volatile int*)&end)) break;
       warp_wait((values ? o_done : s_done) + 8 * st, ((uint32_t)(g / STAGES) & 1u) ^ 1u, &quit);
       const TileInfo& t = infos[g % INFOS];
@@ -332,13 +332,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) { mbar_arrive(c_empty + 8 * slot); mbar_arrive((values ? v_full : k_full) + 8 * st); }
+      if (lane == 0) { mbar_arrive(c_empty + 8 * pair); mbar_arrive((values ? v_full : k_full) + 8 * st); }
     }
   } else if (warp == PRODUCER) {
     // ---- copies: pages and scales are looked up for eight tiles at a time, a lane for each 16 tokens, and eight tiles ahead ----
-    const int box = p.P < 32 ? 16 : 32;      // tokens of a copy
-    int g = 0, slot = 0;
-    uint32_t parity = 1;                     // of the slots' turns: 1: they have not been used yet
+    const int groups = min(p.P, KEYS) / 16;  // of 16 tokens, that a copy has
+    int g = 0, pair = 0;
+    uint32_t parity = 1;                     // of the places' turns: 1: they have not been used yet
     for (const Part* u; (u = next_part<C>(walk, p)) != nullptr;) {
       const int n = u->n, h = u->h, pf = u->q.before, pl = pf + u->q.n - 1;
       const int32_t* const table = p.b.table + u->s * p.b.table_ld;
@@ -375,40 +375,36 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
           page_next = look_up((x >> 3) + 1);
         }
         if ((x & 7) == 4) scale_next = scales_of(page_next);
-        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) >> (4 * (x & 7));
-        int rows[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) rows[k] = __shfl_sync(0xffffffffu, row, 4 * (x & 7) + k);
-#pragma unroll
-        for (int values = 0; values < 2; ++values) {
-          wait_two(c_empty + 8 * slot, parity, c_empty + 8 * slot + 8, parity, &quit);
-          if (elected()) {
-            const CUtensorMap* map = values ? &map_v : &map_k;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const uint32_t to = base + L::CODES + (slot + k) * L::SLOT, full = c_full + 8 * (slot + k), two = there >> (2 * k) & 3u;
-              if (box == 32) {               // both halves lie in one page
-                mbar_expect_tx(full, two ? L::SLOT : 0);
-                if (two) tma_load_2d(to, map, full, 0, two & 1u ? rows[2 * k] : rows[2 * k + 1] - 16);
-              } else {
-                mbar_expect_tx(full, (uint32_t)__popc(two) * (L::SLOT / 2));
-                if (two & 1u) tma_load_2d(to, map, full, 0, rows[2 * k]);
-                if (two & 2u) tma_load_2d(to + L::SLOT / 2, map, full, 0, rows[2 * k + 1]);
-              }
-            }
-          }
-          __syncwarp();
-          slot += 2;
-          if (slot == SLOTS) { slot = 0; parity ^= 1u; }
+        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) >> (4 * (x & 7)) & 15u;
+        const int pair_v = pair + 1 == PAIRS ? 0 : pair + 1;
+        const uint32_t parity_v = pair + 1 == PAIRS ? parity ^ 1u : parity;
+        wait_two(c_empty + 8 * pair, parity, c_empty + 8 * pair_v, parity_v, &quit);
+        uint32_t copies = 0;                 // a bit each: a group of their tokens is there
+        for (int b = 0; b < 4; b += groups) copies |= (there >> b & ((1u << groups) - 1u)) ? 1u << b : 0u;
+        const uint32_t bytes = (uint32_t)(__popc(copies) * groups * 16 * D);
+        if (elected()) {
+          mbar_expect_tx(c_full + 8 * pair, bytes);
+          mbar_expect_tx(c_full + 8 * pair_v, bytes);
         }
+        for (uint32_t left = copies; left; left &= left - 1) {
+          const int b = __ffs(left) - 1, f = __ffs(there >> b) - 1;           // the copy's first group, and the first of them that is there: all lie in one page
+          const int from = __shfl_sync(0xffffffffu, row, 4 * (x & 7) + b + f) - 16 * f;
+          if (elected()) {
+            tma_load_2d(base + L::CODES + 2 * pair * L::SLOT + b * 16 * D, &map_k, c_full + 8 * pair, 0, from);
+            tma_load_2d(base + L::CODES + 2 * pair_v * L::SLOT + b * 16 * D, &map_v, c_full + 8 * pair_v, 0, from);
+          }
+        }
+        __syncwarp();
+        pair += 2;
+        if (pair >= PAIRS) { pair -= PAIRS; parity ^= 1u; }
       }
     }
     if (lane == 0) *(volatile int*)&end = 4 * g;
     __syncwarp();
-    for (int k = 0; k < CONVERT_WARPS; ++k) {                                 // each converter finds that there is no more
-      warp_wait(c_empty + 8 * slot, parity, &quit);
-      if (lane == 0) mbar_arrive(c_full + 8 * slot);
-      if (++slot == SLOTS) { slot = 0; parity ^= 1u; }
+    for (int k = 0; k < CONVERT_WARPS / 2; ++k) {                             // each converter finds that there is no more
+      warp_wait(c_empty + 8 * pair, parity, &quit);
+      if (lane == 0) mbar_arrive(c_full + 8 * pair);
+      if (++pair == PAIRS) { pair = 0; parity ^= 1u; }
     }
   } else {
     // ---- products ----
@@ -816,8 +812,8 @@ int launch(const TreeP& p, int ctas, cudaStream_t st) {
   static std::atomic<uint64_t> limits{0};
   static std::atomic<uint64_t> shares{0};
   CUtensorMap map_k, map_v;
-  B200_TRY(code_map(&map_k, p.k, (long long)p.pages * p.H * p.P, D, p.P < 32 ? 16 : 32));
-  B200_TRY(code_map(&map_v, p.v, (long long)p.pages * p.H * p.P, D, p.P < 32 ? 16 : 32));
+  B200_TRY(code_map(&map_k, p.k, (long long)p.pages * p.H * p.P, D, p.P < KEYS ? p.P : KEYS));
+  B200_TRY(code_map(&map_v, p.v, (long long)p.pages * p.H * p.P, D, p.P < KEYS ? p.P : KEYS));
   B200_TRY(allow_smem(limits, (int)TreeSmem<D>::BYTES, tree_kernel<D, FMT, C>));
   B200_TRY(prefer_smem(shares, 100, tree_kernel<D, FMT, C>, tree_join_kernel<D, C>));
   B200_TRY(launch_early(tree_kernel<D, FMT, C>, dim3((unsigned)ctas), dim3(THREADS), TreeSmem<D>::BYTES, st, map_k, map_v, p));
