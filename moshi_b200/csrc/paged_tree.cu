@@ -310,25 +310,33 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     for (int j = warp - SOFT_WARPS;; j += CONVERT_WARPS) {
       const int slot = j % SLOTS, pair = slot >> 1, g = j >> 2, st = g % STAGES, half = j & 1;
       const bool values = j & 2;
-      warp_wait(c_full + 8 * pair, (uint32_t)(j / SLOTS) & 1u, &quit);
+      // the codes, and the f16 tile's place: where there are no more jobs, it is free as well
+      wait_two(c_full + 8 * pair, (uint32_t)(j / SLOTS) & 1u, (values ? o_done : s_done) + 8 * st, ((uint32_t)(g / STAGES) & 1u) ^ 1u, &quit);
       if (__any_sync(0xffffffffu, quit || j >= *(volatile int*)&end)) break;
-      warp_wait((values ? o_done : s_done) + 8 * st, ((uint32_t)(g / STAGES) & 1u) ^ 1u, &quit);
-      const TileInfo& t = infos[g % INFOS];
-      const bool all = !values || (t.whole & 2);         // values that no row sees may be anything; keys are masked
       const uint8_t* from = smem + L::CODES + slot * L::SLOT;
       uint8_t* const to = smem + (values ? L::V : L::K) + st * L::TILE + (c >> 2) * L::HALF;
-#pragma unroll 4
-      for (int i = 0; i < 32 / STEP; ++i) {
-        const int r = i * STEP + r_in, n = 32 * half + r;
-        uint4 x = *reinterpret_cast<const uint4*>(from + (D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ (r >> 1 & 3)) << 4)));
-        if (!all) {
-          const int token = t.j0 + n;
-          if (!(t.group[n >> 4].w != 0.f && token <= t.pl && (p.window <= 0 || t.pf - token < p.window || token < p.sinks))) x = make_uint4(0, 0, 0, 0);
-        }
+      auto fetch = [&](int r) { return *reinterpret_cast<const uint4*>(from + (D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ (r >> 1 & 3)) << 4))); };
+      auto put = [&](int r, const uint4& x) {
+        const int n = 32 * half + r;
         const uint32_t w[4] = {ready<FMT>(x.x), ready<FMT>(x.y), ready<FMT>(x.z), ready<FMT>(x.w)};
         uint8_t* y = to + n * 128;
         *reinterpret_cast<uint4*>(y + (((2 * (c & 3)) ^ (n & 7)) << 4)) = make_uint4(half2_of<FMT, 0>(w[0]), half2_of<FMT, 1>(w[0]), half2_of<FMT, 0>(w[1]), half2_of<FMT, 1>(w[1]));
         *reinterpret_cast<uint4*>(y + (((2 * (c & 3) + 1) ^ (n & 7)) << 4)) = make_uint4(half2_of<FMT, 0>(w[2]), half2_of<FMT, 1>(w[2]), half2_of<FMT, 0>(w[3]), half2_of<FMT, 1>(w[3]));
+      };
+      const TileInfo& t = infos[g % INFOS];
+      if (!values || (t.whole & 2)) {
+        uint4 x[32 / STEP];
+#pragma unroll
+        for (int i = 0; i < 32 / STEP; ++i) x[i] = fetch(i * STEP + r_in);
+#pragma unroll
+        for (int i = 0; i < 32 / STEP; ++i) put(i * STEP + r_in, x[i]);
+      } else {                               // values that no row sees may be anything; keys are masked
+#pragma unroll 1
+        for (int i = 0; i < 32 / STEP; ++i) {
+          const int r = i * STEP + r_in, token = t.j0 + 32 * half + r;
+          const bool seen = t.group[2 * half + (r >> 4)].w != 0.f && token <= t.pl && (p.window <= 0 || t.pf - token < p.window || token < p.sinks);
+          put(r, seen ? fetch(r) : make_uint4(0, 0, 0, 0));
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
