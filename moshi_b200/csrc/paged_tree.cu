@@ -89,47 +89,64 @@ template <int C>
 __device__ __forceinline__ int units_of(const AttnP& p, const Seq& q) { return !q.ok || q.n == 0 ? 0 : p.H * ((q.n * p.G + C - 1) / C); }
 // all units of a sequence take its whole range, from the first row's window on
 __device__ __forceinline__ int places_of(const AttnP& p, const Seq& q) { return Tiles<SHIFT>(q.before, q.before + q.n - 1, p.window, p.sinks).n + UNIT_COST; }
+// A sequence's units and the places of each.
+struct Share {
+  Seq q;
+  int units, places;
+  __device__ __forceinline__ long long work() const { return (long long)units * places; }
+};
 template <int C>
-__device__ __forceinline__ long long work_of(const AttnP& p, int s) {
-  const Seq q = sequence(p.b, s, p.P);
-  const int u = units_of<C>(p, q);
-  return u ? (long long)u * places_of(p, q) : 0;
+__device__ __forceinline__ Share share_of(const AttnP& p, int s) {
+  Share x;
+  x.q = sequence(p.b, s, p.P);
+  x.units = units_of<C>(p, x.q);
+  x.places = x.units ? places_of(p, x.q) : 1;
+  return x;
 }
-struct Run { long long from, to, base; int s; };      // this CTA's places; the sequence that it begins in and the places in front of that
-// by all threads of the block
+struct Run { long long from, to, base; int s; Share share; };        // this CTA's places; the sequence that it begins in (-1: there is none for it), and the places in front of that
+// By all threads of the block.  Where there is a CTA for every unit, and the longest is not much longer than an equal share, each has one whole: a unit that is cut costs a second start and the join.  (16 requests of
+// 3000 tokens, 80 columns of 8 heads: 50 us as equal runs, 44 us whole.)
+constexpr int CUT_COST = 20;
 template <int C>
-__device__ Run run_of(const AttnP& p) {
+__device__ __forceinline__ void run_of(const AttnP& p, Run& found) {
   constexpr int WARPS = THREADS / 32;
-  __shared__ long long sums[WARPS];
-  __shared__ Run found;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long mine = 0, first = 0;
-  for (int s = threadIdx.x; s < p.b.S; s += THREADS) {
-    const long long w = work_of<C>(p, s);
-    if (s == (int)threadIdx.x) first = w;
-    mine += w;
+  __shared__ long long sums[WARPS], unit_sums[WARPS];
+  __shared__ int tops[WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, S = p.b.S;
+  const Share mine = share_of<C>(p, min((int)threadIdx.x, S - 1));
+  long long total = 0, units = 0;
+  int longest = 0;
+  for (int s = threadIdx.x; s < S; s += THREADS) {
+    const Share x = s == (int)threadIdx.x ? mine : share_of<C>(p, s);
+    total += x.work(); units += x.units;
+    longest = max(longest, x.units ? x.places : 0);
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) sums[warp] = mine;
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    units += __shfl_xor_sync(0xffffffffu, units, o);
+    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+  }
+  if (lane == 0) { sums[warp] = total; unit_sums[warp] = units; tops[warp] = longest; }
   if (threadIdx.x == 0) found.s = -1;
   __syncthreads();
-  long long total = 0;
+  total = units = longest = 0;
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) total += sums[w];
+  for (int w = 0; w < WARPS; ++w) { total += sums[w]; units += unit_sums[w]; longest = max(longest, tops[w]); }
   const long long run = max((total + gridDim.x - 1) / gridDim.x, (long long)MIN_RUN);
-  Run r;
-  r.from = run * blockIdx.x; r.to = min(r.from + run, total); r.s = -1; r.base = 0;
-  if (r.from >= total) return r;
-  long long base = 0;
-  for (int s0 = 0; s0 < p.b.S; s0 += THREADS) {
+  const bool whole = units <= (long long)gridDim.x && longest <= run + CUT_COST;
+  const long long from = whole ? blockIdx.x : run * blockIdx.x;               // units or places
+  if (from >= (whole ? units : total)) return;
+  long long base = 0;                        // in front of the round
+  for (int s0 = 0; s0 < S; s0 += THREADS) {
     const int s = s0 + (int)threadIdx.x;
-    const long long w = s0 == 0 ? first : s < p.b.S ? work_of<C>(p, s) : 0;
+    const Share x = s0 == 0 ? mine : share_of<C>(p, min(s, S - 1));
+    const long long w = s < S ? (whole ? x.units : x.work()) : 0;
     long long in = w;                        // inclusive sums of the warp, then of the block
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, in, o);
-      if (lane >= o) in += x;
+      const long long y = __shfl_up_sync(0xffffffffu, in, o);
+      if (lane >= o) in += y;
     }
     __syncthreads();
     if (lane == 31) sums[warp] = in;
@@ -140,13 +157,20 @@ __device__ Run run_of(const AttnP& p) {
       if (i < warp) in += sums[i];
       all += sums[i];
     }
-    if (base + in - w <= r.from && r.from < base + in) { found.s = s; found.base = base + in - w; }
+    if (base + in - w <= from && from < base + in) {
+      found.s = s; found.share = x;
+      if (whole) {                           // places are counted from this sequence on
+        found.base = 0;
+        found.from = (from - (base + in - w)) * x.places; found.to = found.from + x.places;
+      } else {
+        found.base = base + in - w;
+        found.from = from; found.to = min(from + run, total);
+      }
+    }
     __syncthreads();
     if (found.s >= 0) break;
     base += all;
   }
-  r.s = found.s; r.base = found.base;
-  return r;
 }
 // A part of a unit: places u0 .. u1 - 1 of n_pos, of which the first UNIT_COST are no tiles; tiles t0 .. t0 + n - 1 of the sequence's.
 struct Part {
@@ -158,36 +182,36 @@ struct Part {
 // A warp's way through its CTA's parts.  It lies in shared memory, as every warp's roles have other uses for 20 registers.
 struct Walk {
   long long f, to, base;
-  int s, units, places;
-  Seq q;
-  Part part[2];                              // the last one at `now`, the one in front of it beside it
-  int now;
+  int s, now;                                // part[now]: the last one; the one in front of it lies beside it
+  Share share;
+  Part part[2];
 };
-template <int C>
-__device__ __forceinline__ void walk_to(Walk& w, const AttnP& p, int s) {
-  w.s = s;
-  w.q = sequence(p.b, s, p.P);
-  w.units = units_of<C>(p, w.q);
-  w.places = w.units ? places_of(p, w.q) : 1;
-}
 // by one lane
 template <int C>
 __device__ __forceinline__ bool walk_on(Walk& w, const AttnP& p) {
-  if (w.f >= w.to) return false;
-  while (w.f >= w.base + (long long)w.units * w.places && w.s + 1 < p.b.S) {  // the next sequence that has work
-    w.base += (long long)w.units * w.places;
-    walk_to<C>(w, p, w.s + 1);
+  long long f = w.f, base = w.base;
+  const long long to = w.to;
+  int s = w.s;
+  Share x = w.share;
+  if (f >= to) return false;
+  if (f >= base + x.work()) {                // the next sequence that has work
+    do {
+      base += x.work();
+      x = share_of<C>(p, ++s);
+    } while (f >= base + x.work() && s + 1 < p.b.S);
+    w.base = base; w.s = s; w.share = x;
   }
+  const Tiles<SHIFT> tiles(x.q.before, x.q.before + x.q.n - 1, p.window, p.sinks);
+  const long long o = f - base;
+  const int u = o < 0x7fffffffll ? (int)((uint32_t)o / (uint32_t)x.places) : (int)(o / x.places), cts = x.units / p.H;
+  Part y;
+  y.q = x.q; y.s = s; y.h = u / cts; y.ct = u - y.h * cts; y.n_pos = x.places;
+  y.u0 = (int)(o - (long long)u * x.places); y.u1 = (int)min((long long)x.places, y.u0 + (to - f));
+  y.t0 = max(y.u0 - UNIT_COST, 0); y.n = max(y.u1 - UNIT_COST, 0) - y.t0;
+  y.first = tiles.first; y.from = tiles.from;
+  w.f = f + y.u1 - y.u0;
   w.now ^= 1;
-  Part& x = w.part[w.now];
-  const long long o = w.f - w.base;
-  const int u = o < 0x7fffffffll ? (int)((uint32_t)o / (uint32_t)w.places) : (int)(o / w.places), cts = w.units / p.H;
-  x.q = w.q; x.s = w.s; x.h = u / cts; x.ct = u - x.h * cts; x.n_pos = w.places;
-  x.u0 = (int)(o - (long long)u * w.places); x.u1 = (int)min((long long)w.places, x.u0 + (w.to - w.f));
-  w.f += x.u1 - x.u0;
-  const Tiles<SHIFT> tiles(w.q.before, w.q.before + w.q.n - 1, p.window, p.sinks);
-  x.first = tiles.first; x.from = tiles.from;
-  x.t0 = max(x.u0 - UNIT_COST, 0); x.n = max(x.u1 - UNIT_COST, 0) - x.t0;
+  w.part[w.now] = y;
   return true;
 }
 // by the whole warp: the next part, null behind the last
@@ -285,7 +309,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
   pdl_wait();
   if (blockIdx.x == 0) record_sequences(p.b, p.P, p.flags, THREADS);
   if (threadIdx.x == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
-  const Run run = run_of<C>(p);
+  __shared__ Run run;
+  run_of<C>(p, run);
   if (run.s < 0) return;                     // the whole block
   if (warp == ISSUER) tmem_alloc(smem_u32(&tmem_at), 512);
   tc_fence_before();
@@ -294,8 +319,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
   const uint32_t tmem = tmem_at;
   Walk& walk = walks[warp < SOFT_WARPS ? warp : warp == PRODUCER ? SOFT_WARPS : SOFT_WARPS + 1];
   if (lane == 0 && (warp < SOFT_WARPS || warp >= PRODUCER)) {
-    walk.f = run.from; walk.to = run.to; walk.base = run.base; walk.now = 0;
-    walk_to<C>(walk, p, run.s);
+    walk.f = run.from; walk.to = run.to; walk.base = run.base; walk.s = run.s; walk.share = run.share; walk.now = 0;
   }
 
   // Tiles are numbered through all parts, g = 0, 1, ..: tile g has the places g % STAGES of keys and values, and the weight warps g & 1; its codes are the jobs 4 g .. 4 g + 3, 32 tokens of keys or values each.
