@@ -78,7 +78,7 @@ class Call:
         return lib.b200_page_pool_compact(self.ref("no_pool", self.p), self.ref("no_cache", self.c), self.args["n_caches"], self.args["work"], self.args["work_bytes"], None)
 
 
-NAMES = ("tree_join", "tree_kernel", "tree_build", "few_rows", "join_kernel", "append_few", "append_many", "keep_kernel", "rearrange_count", "rearrange_take", "reserve_kernel", "compact_kernel", "renumber", "copy_kernel")
+NAMES = ("tree_join", "tree_kernel", "tree_build", "few_rows", "join_kernel", "append_few", "append_many", "keep_kernel", "rearrange_small", "rearrange_count", "rearrange_take", "reserve_kernel", "compact_kernel", "renumber", "copy_kernel")
 
 
 def kernels(fake, call, what):
@@ -108,10 +108,12 @@ def test_which_kernels_the_others_launch(fake):
     assert kernels(fake, Call(axes=1, pair_axis=None), "append") == [(0, "append_many")]
     assert kernels(fake, Call(), "keep") == [(0, "keep_kernel")] and kernels(fake, Call(n_caches=64), "keep") == [(0, "keep_kernel")] and kernels(fake, Call(n_caches=65), "keep") == 2 * [(0, "keep_kernel")]
     assert kernels(fake, Call(total_rows=0), "keep") == []
-    assert kernels(fake, Call(), "rearrange") == [(0, "rearrange_count"), (0, "rearrange_take")]
+    assert kernels(fake, Call(), "rearrange") == [(0, "rearrange_small")] and kernels(fake, Call(p_sequences=1025, p_width=4), "rearrange") == [(0, "rearrange_count"), (0, "rearrange_take")]
+    assert kernels(fake, Call(p_sequences=129), "rearrange") == [(0, "rearrange_count"), (0, "rearrange_take")]
     assert kernels(fake, Call(), "reserve") == [(0, "reserve_kernel"), (0, "copy_kernel")] and kernels(fake, Call(n_caches=130), "reserve") == [(0, "reserve_kernel")] + 3 * [(0, "copy_kernel")]
     assert kernels(fake, Call(n_caches=0, no_cache=1), "reserve") == [(0, "reserve_kernel")]
-    assert kernels(fake, Call(), "compact") == [(0, "compact_kernel"), (0, "renumber"), (0, "copy_kernel")]
+    assert kernels(fake, Call(), "compact") == [(0, "compact_kernel"), (0, "copy_kernel")]
+    assert kernels(fake, Call(p_sequences=129), "compact") == [(0, "compact_kernel"), (0, "renumber"), (0, "copy_kernel")]
 
 
 def test_every_page_size_and_head_size(fake):
