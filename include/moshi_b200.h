@@ -645,7 +645,7 @@ typedef struct {
   int32_t *refs_dev;                  /* [pages] */
   int32_t *flags_dev;                 /* one word */
   int64_t table_ld;
-  int32_t sequences, table_width;     /* at most 4096 sequences */
+  int32_t sequences, table_width;     /* at most 4096 sequences; their product below 2^31 - 2^16 */
   int32_t pages, page_tokens;
   int32_t device;
 } b200_page_pool;

@@ -570,7 +570,7 @@ Layers layers_of(const b200_paged_cache* caches, int n) {
 }
 int check_pool(const b200_page_pool* o, const char* what) {
   if (!o || !o->table_dev || !o->lengths_dev || !o->held_dev || !o->refs_dev || !o->flags_dev) B200_FAIL(B200_ERR_INVALID, "%s: null pointer in the pool", what);
-  if (o->sequences < 1 || o->sequences > MAX_SEQUENCES || o->table_width < 1 || o->table_ld < o->table_width || o->pages < 1 || o->pages > 0x7fff0000 ||
+  if (o->sequences < 1 || o->sequences > MAX_SEQUENCES || o->table_width < 1 || o->table_ld < o->table_width || o->pages < 1 || o->pages > 0x7fff0000 || (long long)o->sequences * o->table_width > 0x7fff0000 ||
       (o->page_tokens != 16 && o->page_tokens != 32 && o->page_tokens != 64 && o->page_tokens != 128) || (long long)o->table_width * o->page_tokens > 0x7fffff00ll)
     B200_FAIL(B200_ERR_SHAPE, "%s: %d sequences (at most %d) with tables of %d pages, %d pages of %d tokens", what, o->sequences, MAX_SEQUENCES, o->table_width, o->pages, o->page_tokens);
   return B200_OK;

@@ -193,7 +193,8 @@ def test_keeps_that_are_refused(fake, changed):
 
 
 @pytest.mark.parametrize("changed", [dict(no_pool=1), *({n: None} for n in ("p_table", "lengths", "held", "refs", "p_flags")), dict(p_sequences=0), dict(p_sequences=4097), dict(p_width=0), dict(p_ld=63), dict(p_pages=0),
-                                     dict(p_page_tokens=20), dict(p_width=1 << 26, p_ld=1 << 26)], ids=str)
+                                     dict(p_page_tokens=20), dict(p_width=1 << 26, p_ld=1 << 26),
+                                     dict(p_sequences=4096, p_width=1 << 19, p_ld=1 << 19, p_page_tokens=16)], ids=str)
 def test_pools_that_are_refused(fake, changed):
     for what in ("rearrange", "reserve", "compact"):
         refused(fake, Call(**changed), what)
