@@ -631,7 +631,7 @@ int b200_paged_tree_build(const b200_paged_batch* batch, const b200_paged_tree* 
 int64_t b200_paged_tree_attention_bytes(const b200_paged_cache* cache, const b200_paged_batch* batch, int q_heads, int window, int sinks);
 int b200_paged_tree_attention(const b200_paged_cache* cache, const b200_paged_batch* batch, const b200_paged_tree* tree, const void* q_dev, int64_t q_ld, void* out_dev, int64_t out_ld, int q_heads,
                               float scale, int window, int sinks, void* work_dev, int64_t work_bytes, void* stream);
-/* The rows of a step that are kept move to the front, in n_caches caches that are alike (one per layer): sequence s keeps its rows kept[rows[s] + i], i < counts[s], which rise (else it is left out), and
+/* The rows of a step that are kept move to the front, in n_caches caches that are alike, with memory of their own (one per layer): sequence s keeps its rows kept[rows[s] + i], i < counts[s], which rise (else it is left out), and
  * row i of them lies in place before[s] + i afterwards; what lies behind is of no use any more.  Within a page codes move as they are.  A row that comes from another page is rounded once more, to the scale of
  * the page that it moves to, which is doubled until the row fits, or is the rows' own where nothing else of use is left there.  The first cache's flags are used. */
 int b200_paged_keep(const b200_paged_cache* caches, int n_caches, const b200_paged_batch* batch, const int32_t* kept_dev, const int32_t* counts_dev, void* stream);

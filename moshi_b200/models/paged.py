@@ -334,6 +334,8 @@ class PagePool:
         caches = list(caches)
         if not caches or any((c.device, c.pages, c._shape, c.dtype) != (caches[0].device, caches[0].pages, caches[0]._shape, caches[0].dtype) for c in caches):
             raise ValueError("a pool's caches are alike: device, pages, sizes and type")
+        if len({c.k.data_ptr() for c in caches}) < len(caches):
+            raise ValueError("a pool's caches have memory of their own: what moves in one would move twice")
         if not 1 <= sequences <= 4096 or width < 1:
             raise ValueError(f"{sequences} sequences (1 .. 4096) of {width} pages")
         self.caches, self.device, self.sequences, self.width, self.pages = caches, caches[0].device, int(sequences), int(width), caches[0].pages

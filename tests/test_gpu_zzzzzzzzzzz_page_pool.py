@@ -265,3 +265,9 @@ def test_forked_requests_read_what_they_share_and_write_on_their_own():
         want, _ = alone.read(PagedBatch(i32([[0, 1]]), i32([0]), i32([0, 21]), 21, 21))
         assert torch.equal(k[21 * s:21 * s + 21], want)
     assert pool.error_flags() == 0 and cache.error_flags() == 0
+
+
+def test_a_cache_is_in_a_pool_once():
+    cache = PagedKVCache(8, 2, 64, 16, "int8")
+    with pytest.raises(ValueError, match="memory of their own"):
+        PagePool([cache, PagedKVCache(8, 2, 64, 16, "int8"), cache], 2, 2)
