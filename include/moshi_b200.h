@@ -654,7 +654,8 @@ int64_t b200_page_pool_bytes(const b200_page_pool* pool);
  * that were held in reserve are given back too.  A source that is no sequence leaves the sequence what it is. */
 int b200_page_pool_rearrange(const b200_page_pool* pool, const int32_t* source_dev, void* work_dev, int64_t work_bytes, void* stream);
 /* Sequence s gets pages for add[s] >= 0 tokens behind its lengths[s].  Where the page of the first of them is partly filled and shared it gets a copy of its own, in all caches; of the sequences that share one in
- * this call, the last keeps it if nobody else holds it.  Free pages go out by rising numbers, to sequences by rising numbers, a copy before the sequence's other pages.  If there are too few nobody gets any. */
+ * this call, the last keeps it if nobody else holds it.  Free pages go out by rising numbers, to sequences by rising numbers, a copy before the sequence's other pages.  If there are too few nobody gets any.  A sequence whose
+ * pages behind its tokens are shared (it was made shorter, and not rearranged since) is left out. */
 int b200_page_pool_reserve(const b200_page_pool* pool, const b200_paged_cache* caches, int n_caches, const int32_t* add_dev, void* work_dev, int64_t work_bytes, void* stream);
 /* Pages in use move to the lowest numbers, in all caches: those at or above the number of pages in use go, by rising numbers, into the free ones below it. */
 int b200_page_pool_compact(const b200_page_pool* pool, const b200_paged_cache* caches, int n_caches, void* work_dev, int64_t work_bytes, void* stream);

@@ -355,6 +355,7 @@ struct ReserveP {
 __global__ void __launch_bounds__(ONE) reserve_kernel(const ReserveP p) {
   pdl_trigger();
   pdl_wait();
+  constexpr int COPIED = -2, LEFT_OUT = -3;
   __shared__ int begun[MAX_SEQUENCES], from[MAX_SEQUENCES + 1];      // the shared page that a sequence goes on in, -1: none; its first place among all pages that are needed
   const int tid = threadIdx.x, S = p.o.S, P = p.o.P;
   auto want = [&](int s, int held) {                     // pages that the sequence is to hold; -1: left out
@@ -366,15 +367,22 @@ __global__ void __launch_bounds__(ONE) reserve_kernel(const ReserveP p) {
 #pragma unroll
   for (int k = 0; k < 4; ++k) refs[k] = 4 * tid + k < p.o.pages ? p.o.refs[4 * tid + k] : 1;
   for (int s = tid; s < S; s += ONE) {
-    const int held = p.o.held[s], n = p.o.lengths[s];
+    const int held = p.o.held[s], n = p.o.lengths[s], next = pages_of(p.o, s, held);      // next: its first page without tokens
     int page = -1;
-    if (want(s, held) < 0) atomicOr(p.o.flags, B200_PAGED_BAD_BATCH);
-    else if (p.add[s] > 0 && n % P) {
-      page = p.o.table[s * p.o.table_ld + n / P];
-      if (page < 0 || page >= p.o.pages) { atomicOr(p.o.flags, B200_PAGED_BAD_PAGE); page = -1; }
-      else if (p.o.refs[page] <= 1) page = -1;
+    bool out = want(s, held) < 0;
+    if (!out && p.add[s] > 0) {
+      const int32_t* table = p.o.table + s * p.o.table_ld;
+      const int spare = next < held ? table[next] : -1;
+      if (n % P) {
+        page = table[n / P];
+        if (page < 0 || page >= p.o.pages) { atomicOr(p.o.flags, B200_PAGED_BAD_PAGE); page = -1; }
+        else if (p.o.refs[page] <= 1) page = -1;
+      }
+      // a page that others have tokens in: the sequence was made shorter and not rearranged
+      out = spare >= 0 && spare < p.o.pages && p.o.refs[spare] > 1;
     }
-    begun[s] = page;
+    if (out) atomicOr(p.o.flags, B200_PAGED_BAD_BATCH);
+    begun[s] = out ? LEFT_OUT : page;
   }
   __syncthreads();
   int needed = 0, copied = 0;
@@ -383,8 +391,7 @@ __global__ void __launch_bounds__(ONE) reserve_kernel(const ReserveP p) {
     int need = 0, copy = 0;
     if (s < S) {
       const int held = p.o.held[s], page = begun[s];
-      const int pages = want(s, held);
-      need = pages < 0 ? 0 : pages - held;
+      need = page == LEFT_OUT ? 0 : want(s, held) - held;
       if (page >= 0) {
         int rank = 0;
         for (int i = 0; i < s; ++i) rank += begun[i] == page;
@@ -426,7 +433,7 @@ __global__ void __launch_bounds__(ONE) reserve_kernel(const ReserveP p) {
     p.o.refs[to] = 1;
     atomicSub(p.o.refs + x.x, 1);
     p.moves[i] = make_int2(x.x, to);
-    begun[x.y] = -2;
+    begun[x.y] = COPIED;
   }
   __syncthreads();
   for (int i = tid; i < needed; i += ONE) {
@@ -435,14 +442,14 @@ __global__ void __launch_bounds__(ONE) reserve_kernel(const ReserveP p) {
       const int mid = (lo + hi) / 2;
       if (from[mid] <= i) lo = mid; else hi = mid;
     }
-    const int b = i - from[lo] - (begun[lo] == -2);
+    const int b = i - from[lo] - (begun[lo] == COPIED);
     if (b < 0) continue;
     const int page = p.free_pages[i];
     p.o.table[lo * p.o.table_ld + p.o.held[lo] + b] = page;
     p.o.refs[page] = 1;
   }
   __syncthreads();
-  for (int s = tid; s < S; s += ONE) p.o.held[s] += from[s + 1] - from[s] - (begun[s] == -2);
+  for (int s = tid; s < S; s += ONE) p.o.held[s] += from[s + 1] - from[s] - (begun[s] == COPIED);
 }
 
 // ---- what is in use to the front ----

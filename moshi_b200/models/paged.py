@@ -327,7 +327,7 @@ def _keep(caches: tp.Sequence[PagedKVCache], ref, n: int, batch: PagedBatch, kep
 
 class PagePool:
     """Who holds which pages, on the device, for sequences whose tokens lie in ``caches`` (one per layer, alike).  ``table`` i32 [sequences, width], -1 behind what a sequence holds; ``lengths`` i32 [sequences]: tokens that
-    it has (the caller's to raise, by what a step has left); ``held``: pages that it holds, enough for them; ``refs`` i32 [pages]: sequences that hold a page.  A pool begins empty.  ``table`` and
+    it has (the caller's to raise, by what a step has left, or to lower, before a ``rearrange`` that gives back what lies behind); ``held``: pages that it holds, enough for them; ``refs`` i32 [pages]: sequences that hold a page.  A pool begins empty.  ``table`` and
     ``lengths`` are what a ``PagedBatch`` takes.  The calls may be captured; none waits."""
 
     def __init__(self, caches: tp.Sequence[PagedKVCache], sequences: int, width: int):
@@ -367,7 +367,8 @@ class PagePool:
 
     def reserve(self, add: torch.Tensor) -> None:
         """Pages for add[s] tokens (i32 [sequences]) behind the lengths[s] that sequence s has: by rising numbers, to sequences by rising numbers.  Where the next token goes to a partly filled page that others hold too, the
-        sequence gets a copy of it first, in all caches (of those in this call that share it, the last keeps it if nobody else holds it).  With too few free pages nobody gets any, and NO_PAGES is recorded."""
+        sequence gets a copy of it first, in all caches (of those in this call that share it, the last keeps it if nobody else holds it).  A sequence whose pages behind its tokens are shared (it was made shorter without a ``rearrange``)
+        is left out, and BAD_BATCH is recorded.  With too few free pages nobody gets any, and NO_PAGES is recorded: what the step would write to may be shared still."""
         at, work = self._of_sequences("add", add), self._work()
         rc = self._reserve(self._ref, self._caches, len(self.caches), at, work.data_ptr(), self._bytes, _stream(self._index))
         if rc:

@@ -124,6 +124,8 @@ class Pool:
             if a <= 0 or n + a > self.width * self.page_tokens:
                 continue
             block = n // self.page_tokens
+            if self._blocks(n) < len(table[s]) and self.refs[table[s][self._blocks(n)]] > 1:      # shorter than it was, and not rearranged since: left out
+                continue
             if n % self.page_tokens and refs[table[s][block]] > 1:
                 if not free:
                     return None

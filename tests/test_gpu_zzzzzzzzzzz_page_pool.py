@@ -271,3 +271,19 @@ def test_a_cache_is_in_a_pool_once():
     cache = PagedKVCache(8, 2, 64, 16, "int8")
     with pytest.raises(ValueError, match="memory of their own"):
         PagePool([cache, PagedKVCache(8, 2, 64, 16, "int8"), cache], 2, 2)
+
+
+@pytest.mark.parametrize("shorter", [3, 16, 20, 32])
+def test_a_sequence_that_was_made_shorter(shorter):
+    """What lies behind its tokens may be another's: it gets pages once it has been rearranged, and none before."""
+    b = Both(32, 16, 3, 6)
+    b.reserve([70, 5, 0])
+    b.rearrange([0, 1, 0])
+    for x in (b.want.lengths, b.pool.lengths):
+        x[0] = shorter
+    assert b.reserve([1, 3, 0], grow=False) == []
+    b.check(paged.BAD_BATCH)
+    b.rearrange([0, 1, 2])
+    b.check()
+    assert len(b.reserve([1, 3, 1])) == (shorter % 16 > 0)      # the third's last page is its own now
+    b.check()

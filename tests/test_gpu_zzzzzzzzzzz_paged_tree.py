@@ -109,6 +109,13 @@ def test_larger_trees(form, heads, sizes):
     check([0, 37, 100, 5, 64][:len(sizes)], [some_tree(n, 3 * n) for n in sizes], heads, form)
 
 
+@pytest.mark.parametrize("size", [2, 5, 18])
+def test_many_sequences(size):
+    """More than a block looks at in one go, most of them short, some empty."""
+    r = random.Random(size)
+    check([r.choice([0, 1, 17, 40]) for _ in range(1500)], [some_tree(r.randint(0, size), i) for i in range(1500)], (8, 1), ("int8", 64, 16))
+
+
 @pytest.mark.parametrize("kind", ["chain", "star", "roots"])
 @pytest.mark.parametrize("size", [5, 40])
 def test_kinds_of_trees(kind, size):
@@ -494,6 +501,40 @@ def test_more_caches_than_a_launch_takes():
     pool.rearrange(i32([0, 0]))
     pool.reserve(i32([1, 0]))
     assert pool.table[:, 0].tolist() == [0, 1] and all(torch.equal(c.k[0], c.k[1]) for c in caches)
+
+
+@pytest.mark.parametrize("seed", range(3))
+def test_captured_keeps_follow_their_tensors(seed):
+    """Two caches' keeps in graphs that are replayed side by side, with other paths each time."""
+    graphs, cases = [], []
+    for i in range(2):
+        c = Content([70, 25, 90], 2, 64, 32, "int8", seed=seed + i)
+        cache, kept, counts = c.cache(), i32([0] * 90), i32([0] * 3)
+        batch = batch_of(c.table, [30, 5, 60], [40, 20, 30])
+        cache.keep(batch, kept, counts)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            cache.keep(batch, kept, counts)
+        graphs.append(graph), cases.append((c, cache, kept, counts, batch, torch.cuda.Stream()))
+    r = random.Random(seed)
+    for _ in range(4):
+        alone = []
+        for c, cache, kept, counts, batch, _ in cases:
+            paths = [sorted(r.sample(range(n), r.randint(0, n))) for n in (40, 20, 30)]
+            kept.copy_(i32([x for p, n in zip(paths, (40, 20, 30)) for x in p + [0] * (n - len(p))])), counts.copy_(i32([len(p) for p in paths]))
+            other = PagedKVCache(c.pages, 2, 64, 32, "int8")
+            for a, b in ((other.k, cache.k), (other.v, cache.v), (other.k_scale, cache.k_scale), (other.v_scale, cache.v_scale)):
+                a.copy_(b)
+            other.keep(batch, kept, counts)
+            alone.append(other)
+        torch.cuda.synchronize()
+        for graph, case in zip(graphs, cases):
+            with torch.cuda.stream(case[-1]):
+                graph.replay()
+        torch.cuda.synchronize()
+        for other, (_, cache, *_) in zip(alone, cases):
+            assert all(torch.equal(getattr(other, n).nan_to_num(-1) if "scale" in n else getattr(other, n), getattr(cache, n).nan_to_num(-1) if "scale" in n else getattr(cache, n)) for n in ("k", "v", "k_scale", "v_scale"))
+            assert cache.error_flags() == 0
 
 
 # ---- refusals ----
