@@ -103,75 +103,6 @@ __device__ __forceinline__ Share share_of(const AttnP& p, int s) {
   x.places = x.units ? places_of(p, x.q) : 1;
   return x;
 }
-struct Run { long long from, to, base; int s; Share share; };        // this CTA's places; the sequence that it begins in (-1: there is none for it), and the places in front of that
-// By all threads of the block.  Where there is a CTA for every unit, and the longest is not much longer than an equal share, each has one whole: a unit that is cut costs a second start and the join.  (16 requests of
-// 3000 tokens, 80 columns of 8 heads: 50 us as equal runs, 44 us whole.)
-constexpr int CUT_COST = 20;
-template <int C>
-__device__ __forceinline__ void run_of(const AttnP& p, Run& found) {
-  constexpr int WARPS = THREADS / 32;
-  __shared__ long long sums[WARPS], unit_sums[WARPS];
-  __shared__ int tops[WARPS];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, S = p.b.S;
-  const Share mine = share_of<C>(p, min((int)threadIdx.x, S - 1));
-  long long total = 0, units = 0;
-  int longest = 0;
-  for (int s = threadIdx.x; s < S; s += THREADS) {
-    const Share x = s == (int)threadIdx.x ? mine : share_of<C>(p, s);
-    total += x.work(); units += x.units;
-    longest = max(longest, x.units ? x.places : 0);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-    units += __shfl_xor_sync(0xffffffffu, units, o);
-    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-  }
-  if (lane == 0) { sums[warp] = total; unit_sums[warp] = units; tops[warp] = longest; }
-  if (threadIdx.x == 0) found.s = -1;
-  __syncthreads();
-  total = units = longest = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) { total += sums[w]; units += unit_sums[w]; longest = max(longest, tops[w]); }
-  const long long run = max((total + gridDim.x - 1) / gridDim.x, (long long)MIN_RUN);
-  const bool whole = units <= (long long)gridDim.x && longest <= run + CUT_COST;
-  const long long from = whole ? blockIdx.x : run * blockIdx.x;               // units or places
-  if (from >= (whole ? units : total)) return;
-  long long base = 0;                        // in front of the round
-  for (int s0 = 0; s0 < S; s0 += THREADS) {
-    const int s = s0 + (int)threadIdx.x;
-    const Share x = s0 == 0 ? mine : share_of<C>(p, min(s, S - 1));
-    const long long w = s < S ? (whole ? x.units : x.work()) : 0;
-    long long in = w;                        // inclusive sums of the warp, then of the block
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, in, o);
-      if (lane >= o) in += y;
-    }
-    __syncthreads();
-    if (lane == 31) sums[warp] = in;
-    __syncthreads();
-    long long all = 0;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) {
-      if (i < warp) in += sums[i];
-      all += sums[i];
-    }
-    if (base + in - w <= from && from < base + in) {
-      found.s = s; found.share = x;
-      if (whole) {                           // places are counted from this sequence on
-        found.base = 0;
-        found.from = (from - (base + in - w)) * x.places; found.to = found.from + x.places;
-      } else {
-        found.base = base + in - w;
-        found.from = from; found.to = min(from + run, total);
-      }
-    }
-    __syncthreads();
-    if (found.s >= 0) break;
-    base += all;
-  }
-}
 // A part of a unit: places u0 .. u1 - 1 of n_pos, of which the first UNIT_COST are no tiles; tiles t0 .. t0 + n - 1 of the sequence's.
 struct Part {
   Seq q;
@@ -181,11 +112,113 @@ struct Part {
 };
 // A warp's way through its CTA's parts.  It lies in shared memory, as every warp's roles have other uses for 20 registers.
 struct Walk {
-  long long f, to, base;
+  long long f, to, base, run;                // places; run: the CTAs' equal share
   int s, now;                                // part[now]: the last one; the one in front of it lies beside it
   Share share;
   Part part[2];
 };
+// Where a CTA's walk begins, `run`: places of an equal share.  Where there is a CTA for every unit, and the longest is not much longer than a share, each has one whole: a unit that is cut costs a second start and the
+// join.  (16 requests of 3000 tokens, 80 columns of 8 heads: 50 us as equal runs, 44 us whole.)
+constexpr int CUT_COST = 20, UNITS_MOST = 1 << 20;       // more units are as many as that: it is many either way
+struct Shares {
+  long long run, from;                       // from: the CTA's first place or, where it has one whole, its unit
+  bool whole;
+  __device__ __forceinline__ Shares(long long total, int units, int longest) {
+    const long long up = total + gridDim.x - 1;
+    run = max(up >> 32 ? up / gridDim.x : (long long)((uint32_t)up / gridDim.x), (long long)MIN_RUN);
+    whole = units <= (int)gridDim.x && longest <= run + CUT_COST;
+    from = whole ? blockIdx.x : run * blockIdx.x;
+  }
+};
+// Sequence s, whose work (units, where CTAs have them whole) ends at `end` of all sequences', is the one that the CTA begins in.
+__device__ __forceinline__ void begin_in(Walk& w, const Shares& x, int s, const Share& share, long long end, long long size, long long total) {
+  w.now = 0; w.s = s; w.share = share; w.run = x.run;
+  if (x.whole) {                             // places are counted from this sequence on
+    w.base = 0;
+    w.f = (x.from - (end - size)) * share.places; w.to = w.f + share.places;
+  } else {
+    w.base = end - size;
+    w.f = x.from; w.to = min(x.from + x.run, total);
+  }
+}
+// By a warp, for up to 32 sequences.
+template <int C>
+__device__ __forceinline__ void start_alone(const AttnP& p, Walk& w) {
+  const int lane = threadIdx.x & 31;
+  const Share x = share_of<C>(p, min(lane, p.b.S - 1));
+  const bool is = lane < p.b.S;
+  const long long work = is ? x.work() : 0;
+  const int units = is ? min(x.units, UNITS_MOST) : 0, longest = __reduce_max_sync(0xffffffffu, units ? x.places : 0);
+  long long in = work;                       // inclusive sums
+  int units_in = units;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, in, o);
+    const int z = __shfl_up_sync(0xffffffffu, units_in, o);
+    if (lane >= o) { in += y; units_in += z; }
+  }
+  const long long total = __shfl_sync(0xffffffffu, in, 31);
+  const Shares shares(total, __shfl_sync(0xffffffffu, units_in, 31), longest);
+  const long long size = shares.whole ? units : work, end = shares.whole ? units_in : in;
+  const bool here = end - size <= shares.from && shares.from < end;
+  if (here) begin_in(w, shares, lane, x, end, size, total);
+  if (!__any_sync(0xffffffffu, here) && lane == 0) w.f = w.to = 0;            // there is no work for this CTA
+  __syncwarp();
+}
+// By all threads of the block, for any number.
+template <int C>
+__device__ __forceinline__ void start_together(const AttnP& p, Walk& found) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ long long sums[WARPS];
+  __shared__ int unit_sums[WARPS], tops[WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, S = p.b.S;
+  const Share mine = share_of<C>(p, min((int)threadIdx.x, S - 1));
+  long long total = 0;
+  int units = 0, longest = 0;
+  for (int s = threadIdx.x; s < S; s += THREADS) {
+    const Share x = s == (int)threadIdx.x ? mine : share_of<C>(p, s);
+    total += x.work(); units = min(units + min(x.units, UNITS_MOST), UNITS_MOST);
+    longest = max(longest, x.units ? x.places : 0);
+  }
+  units = min(__reduce_add_sync(0xffffffffu, units), UNITS_MOST);
+  longest = __reduce_max_sync(0xffffffffu, longest);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) { sums[warp] = total; unit_sums[warp] = units; tops[warp] = longest; }
+  if (threadIdx.x == 0) found.s = -1;
+  __syncthreads();
+  total = lane < WARPS ? sums[lane] : 0;
+  units = __reduce_add_sync(0xffffffffu, lane < WARPS ? unit_sums[lane] : 0);
+  longest = __reduce_max_sync(0xffffffffu, lane < WARPS ? tops[lane] : 0);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  const Shares shares(total, units, longest);
+  long long base = 0;                        // in front of the round
+  for (int s0 = 0; s0 < S; s0 += THREADS) {
+    const int s = s0 + (int)threadIdx.x;
+    const Share x = s0 == 0 ? mine : share_of<C>(p, min(s, S - 1));
+    const long long size = s < S ? (shares.whole ? x.units : x.work()) : 0;
+    long long in = size;                     // inclusive sums of the warp, then of the block
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, in, o);
+      if (lane >= o) in += y;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = in;
+    __syncthreads();
+    long long all = lane < WARPS ? sums[lane] : 0, front = lane < warp ? all : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { all += __shfl_xor_sync(0xffffffffu, all, o); front += __shfl_xor_sync(0xffffffffu, front, o); }
+    const long long end = base + front + in;
+    if (end - size <= shares.from && shares.from < end) begin_in(found, shares, s, x, end, size, total);
+    __syncthreads();
+    if (found.s >= 0) break;
+    base += all;
+  }
+  if (threadIdx.x == 0 && found.s < 0) found.f = found.to = 0;                // there is no work for this CTA
+  __syncthreads();
+}
 // by one lane
 template <int C>
 __device__ __forceinline__ bool walk_on(Walk& w, const AttnP& p) {
@@ -305,28 +338,34 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     for (int i = 0; i < INFOS; ++i) mbar_init(i_full + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  __syncthreads();                           // the barriers have begun
   pdl_trigger();
   pdl_wait();
-  if (blockIdx.x == 0) record_sequences(p.b, p.P, p.flags, THREADS);
-  if (threadIdx.x == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
-  __shared__ Run run;
-  run_of<C>(p, run);
-  if (run.s < 0) return;                     // the whole block
   if (warp == ISSUER) tmem_alloc(smem_u32(&tmem_at), 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = tmem_at;
   Walk& walk = walks[warp < SOFT_WARPS ? warp : warp == PRODUCER ? SOFT_WARPS : SOFT_WARPS + 1];
-  if (lane == 0 && (warp < SOFT_WARPS || warp >= PRODUCER)) {
-    walk.f = run.from; walk.to = run.to; walk.base = run.base; walk.s = run.s; walk.share = run.share; walk.now = 0;
+  const bool walks_on = warp < SOFT_WARPS || warp >= PRODUCER;
+  if (p.b.S <= 32) {                         // a warp finds its way without the others
+    if (walks_on) start_alone<C>(p, walk);
+  } else {
+    __shared__ Walk start;
+    start_together<C>(p, start);
+    if (walks_on && lane == 0) walk = start;
   }
+  auto tmem_ready = [&]() {                  // by the issuer and the weights' warps
+    tc_fence_before();
+    asm volatile("bar.sync 4, %0;" ::"n"((SOFT_WARPS + 1) * 32) : "memory");
+    tc_fence_after();
+    return tmem_at;
+  };
 
   // Tiles are numbered through all parts, g = 0, 1, ..: tile g has the places g % STAGES of keys and values, and the weight warps g & 1; its codes are the jobs 4 g .. 4 g + 3, 32 tokens of keys or values each.
   if (warp >= SOFT_WARPS) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(256 - soft_regs<C>()));
   if (warp < PRODUCER) {
     // ---- codes into f16 tiles ----
+    if (blockIdx.x == 0)                     // until the first come: what every call looks at
+      for (int s = (int)threadIdx.x - SOFT_WARPS * 32; s < p.b.S; s += CONVERT_WARPS * 32)
+        if (!sequence(p.b, s, p.P).ok) atomicOr(p.flags, B200_PAGED_BAD_BATCH);
     constexpr int LANES = D / 16, STEP = 32 / LANES;     // lanes a row, rows at a time
     const int c = lane % LANES;
     // lanes of a row's second 64 dims take the neighbouring row, so that eight lanes' pieces of the f16 tile lie in different banks
@@ -385,20 +424,39 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
       };
       auto scales_of = [&](int page) { return page < 0 ? make_float2(1.f, 1.f) : make_float2(p.k_scale[(long long)page * p.H + h], p.v_scale[(long long)page * p.H + h]); };
       int page = -1, row = 0, page_next = look_up(0);
+      uint32_t there = 0, copies = 0;        // of the batch's groups: those that are there, and those of them that begin a copy
       float2 scale_next = scales_of(page_next);
       for (int x = 0; x < n; ++x, ++g) {
-        if ((x & 7) == 0) {                  // what is to be known of the batch
+        const int tile = x & 7;
+        if (tile == 0) {                     // a batch: a copy is made by the lane of its first group that is there; all of its groups lie in one page
           page = page_next;
+          row = (page * p.H + h) * p.P + (first_of(x >> 3) & (p.P - 1) & -16 * groups);
+          there = __ballot_sync(0xffffffffu, page >= 0);
+          copies = __ballot_sync(0xffffffffu, page >= 0 && !(there & ((1u << lane) - (1u << (lane & -groups)))));
+        }
+        if (tile == 4) scale_next = scales_of(page_next);
+        const int pair_v = pair + 1 == PAIRS ? 0 : pair + 1;
+        const uint32_t parity_v = pair + 1 == PAIRS ? parity ^ 1u : parity;
+        wait_two(c_empty + 8 * pair, parity, c_empty + 8 * pair_v, parity_v, &quit);
+        if (elected()) {
+          const uint32_t bytes = (uint32_t)(__popc(copies >> 4 * tile & 15u) * groups * 16 * D);
+          mbar_expect_tx(c_full + 8 * pair, bytes);
+          mbar_expect_tx(c_full + 8 * pair_v, bytes);
+        }
+        __syncwarp();
+        const bool makes = (lane >> 2) == tile && (copies >> lane & 1u);
+        const uint32_t to = base + L::CODES + (lane & 3 & -groups) * 16 * D;
+        if (makes) tma_load_2d(to + 2 * pair * L::SLOT, &map_k, c_full + 8 * pair, 0, row);
+        if (tile == 0) {                     // what is to be known of the batch: behind its first keys, which do not wait for scales
           const int j = first_of(x >> 3), j0 = j & ~(KEYS - 1), mine = x + (lane >> 2);
-          row = (page * p.H + h) * p.P + (j & (p.P - 1));
           TileInfo& t = infos[(g + (lane >> 2)) % INFOS];
           const float vs = value_scale(scale_next.y);
-          const bool there = (__ballot_sync(0xffffffffu, page >= 0) >> (lane & 28) & 15u) == 15u;
+          const bool all = (there >> (lane & 28) & 15u) == 15u;
           if (mine < n) {
             t.group[lane & 3] = page >= 0 ? make_float4(scale_next.x > 0.f ? scale_next.x : 1.f, __log2f(vs), __frcp_rn(vs), 1.f) : make_float4(1.f, 0.f, 0.f, 0.f);
             if ((lane & 3) == 0) {
-              const bool whole = there && j0 + KEYS <= pf && (p.window <= 0 || pl - j0 < p.window || j0 + KEYS <= p.sinks);
-              const bool seen = there && j0 + KEYS - 1 <= pl && (p.window <= 0 || pf - j0 < p.window || j0 + KEYS <= p.sinks);
+              const bool whole = all && j0 + KEYS <= pf && (p.window <= 0 || pl - j0 < p.window || j0 + KEYS <= p.sinks);
+              const bool seen = all && j0 + KEYS - 1 <= pl && (p.window <= 0 || pf - j0 < p.window || j0 + KEYS <= p.sinks);
               t.j0 = j0; t.pf = pf; t.pl = pl; t.whole = (whole ? 1 : 0) | (seen ? 2 : 0);
             }
           }
@@ -406,26 +464,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
           if (mine < n && (lane & 3) == 0) mbar_arrive(i_full + 8 * ((g + (lane >> 2)) % INFOS));
           page_next = look_up((x >> 3) + 1);
         }
-        if ((x & 7) == 4) scale_next = scales_of(page_next);
-        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) >> (4 * (x & 7)) & 15u;
-        const int pair_v = pair + 1 == PAIRS ? 0 : pair + 1;
-        const uint32_t parity_v = pair + 1 == PAIRS ? parity ^ 1u : parity;
-        wait_two(c_empty + 8 * pair, parity, c_empty + 8 * pair_v, parity_v, &quit);
-        uint32_t copies = 0;                 // a bit each: a group of their tokens is there
-        for (int b = 0; b < 4; b += groups) copies |= (there >> b & ((1u << groups) - 1u)) ? 1u << b : 0u;
-        const uint32_t bytes = (uint32_t)(__popc(copies) * groups * 16 * D);
-        if (elected()) {
-          mbar_expect_tx(c_full + 8 * pair, bytes);
-          mbar_expect_tx(c_full + 8 * pair_v, bytes);
-        }
-        for (uint32_t left = copies; left; left &= left - 1) {
-          const int b = __ffs(left) - 1, f = __ffs(there >> b) - 1;           // the copy's first group, and the first of them that is there: all lie in one page
-          const int from = __shfl_sync(0xffffffffu, row, 4 * (x & 7) + b + f) - 16 * f;
-          if (elected()) {
-            tma_load_2d(base + L::CODES + 2 * pair * L::SLOT + b * 16 * D, &map_k, c_full + 8 * pair, 0, from);
-            tma_load_2d(base + L::CODES + 2 * pair_v * L::SLOT + b * 16 * D, &map_v, c_full + 8 * pair_v, 0, from);
-          }
-        }
+        if (makes) tma_load_2d(to + 2 * pair_v * L::SLOT, &map_v, c_full + 8 * pair_v, 0, row);
         __syncwarp();
         pair += 2;
         if (pair >= PAIRS) { pair -= PAIRS; parity ^= 1u; }
@@ -441,6 +480,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
   } else {
     // ---- products ----
     constexpr uint32_t id_s = idesc_f16(KEYS, false), id_o = idesc_f16(D, true);
+    const uint32_t tmem = tmem_ready();
     int g0 = 0, part = 0;                    // tiles and parts in front
     for (const Part* u; (u = next_part<C>(walk, p)) != nullptr; ++part) {
       const int n = u->n;
@@ -469,6 +509,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(soft_regs<C>()));
     // ---- weights: a row per thread, which is a column and HOLD of a tile's keys ----
+    if (threadIdx.x == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+    const uint32_t tmem = tmem_ready();
     const int i = warp >> 2, q4 = warp & 3, in = q4 * 32 + lane, rep = in / C, col = in % C;
     const uint32_t lanes = (uint32_t)(q4 * 32) << 16, ts = tmem + lanes + KEYS * i + rep * HOLD, tp = tmem + lanes + P_AT + KEYS / 2 * i, to = tmem + lanes + O_AT + D * i;
     if constexpr (R > 1) {                   // other copies' keys have no weight here
@@ -625,7 +667,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
       now = next;
       const Part& u = *next;
       if (u.u0 == 0 && u.u1 < u.n_pos && threadIdx.x == 0) {
-        const long long runs = run.to - run.from, left = u.n_pos - u.u1;
+        const long long runs = walk.run, left = u.n_pos - u.u1;
         p.split[blockIdx.x] = make_int4(u.s, u.h, u.ct, (int)((left + runs - 1) / runs));
       }
       fac = factors[col]; m = -INFINITY; sum = 0.f; done = 0;
@@ -751,7 +793,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
   }
   __syncthreads();
   tc_fence_after();
-  if (warp == ISSUER) tmem_dealloc(tmem, 512);
+  if (warp == ISSUER) tmem_dealloc(tmem_at, 512);
   if (quit) {                                // let copies in flight land before the block ends
     if (threadIdx.x == 0) atomicOr(p.flags, B200_PAGED_WAIT);
     const uint64_t since = global_timer_ns();
