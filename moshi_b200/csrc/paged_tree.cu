@@ -594,6 +594,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
       if (now != nullptr) {
         const Part& u = *now;
         const bool alone = u.u0 == 0 && u.u1 == u.n_pos;
+        if (u.n > 0) {                       // the last tile's sum, and with it all in front
+          const int g = g0 + u.n - 1;
+          warp_wait(o_done + 8 * (g % STAGES), (uint32_t)(g / STAGES) & 1u, &quit);
+        }
         tc_fence_after();
         // Join the column's 2 R rows.  Both groups' sums of a row lie in the row's lane: the first group of warps has half of the dims of both, the second the rest; the R copies go through shared memory.
         float top = -INFINITY, all = 0.f;
@@ -607,57 +611,89 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         float by[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) by[k] = ml[128 * k + in].x == -INFINITY ? 0.f : exp2_fast(ml[128 * k + in].x - top);
-        if (rep == 0) total[i][col] = make_float2(top, all != 0.f && isnan(fac) ? NAN : all);
+        if (all != 0.f && isnan(fac)) all = NAN;
         const int r0 = u.q.r0, c0 = u.ct * C, n_cols = u.q.n * p.G - c0, slot = 2 * (int)blockIdx.x + (u.u0 == 0 ? 1 : 0);
-        // in pieces of D / 8 dims, LINE threads a column, whose results lie side by side
-        constexpr int PIECE = D / 8, LINE = PIECE / 4, AT_ONCE = 128 / LINE;
-        auto place = [](int row, int e) { return row * PIECE * 4 + ((e ^ (D == 128 ? row >> 1 & 3 : row >> 2 & 1)) << 4); };
-        const int d_out = in % LINE, c_first = in / LINE;
-        uint8_t* const mine = join + i * (128 * PIECE * 4);
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          const int d0 = (4 * i + c) * PIECE;
-          uint32_t o[2][PIECE];
+        constexpr int PIECE = D / 8;         // dims at a time
+        uint32_t o[2][PIECE];
+        auto fetch_sums = [&](int d0) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const uint32_t at = tmem + lanes + O_AT + D * k + d0;
             if constexpr (PIECE == 16) tmem_ld16(at, o[k]); else tmem_ld8(at, o[k]);
           }
+        };
+        auto both_sums = [&](float* v) {     // a group that has seen nothing may have anything there
 #pragma unroll
           for (int k = 0; k < 2; ++k) { if constexpr (PIECE == 16) tmem_ld_wait16(o[k]); else tmem_ld_wait8(o[k]); }
 #pragma unroll
-          for (int e = 0; e < LINE; ++e) {
-            float v[4];
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {    // a group that has seen nothing may have anything there
-              v[y] = by[0] != 0.f ? __uint_as_float(o[0][4 * e + y]) * by[0] : 0.f;
-              if (by[1] != 0.f) v[y] = fmaf(__uint_as_float(o[1][4 * e + y]), by[1], v[y]);
-            }
-            *reinterpret_cast<float4*>(mine + place(in, e)) = make_float4(v[0], v[1], v[2], v[3]);
+          for (int e = 0; e < PIECE; ++e) {
+            v[e] = by[0] != 0.f ? __uint_as_float(o[0][e]) * by[0] : 0.f;
+            if (by[1] != 0.f) v[e] = fmaf(__uint_as_float(o[1][e]), by[1], v[e]);
           }
-          asm volatile("bar.sync %0, 128;" ::"r"(2 + i) : "memory");
+        };
+        if constexpr (R == 1) {              // a thread has its column alone
+          const int cc = c0 + col, t_out = cc / p.G;
+          const float inv = all != 0.f ? 1.f / all : 0.f;
+          bf16* const out = p.out + (r0 + t_out) * p.out_ld + (long long)(u.h * p.G + cc - t_out * p.G) * D;
+          const long long at = (long long)slot * C + col;
+          if (!alone && i == 0 && col < n_cols) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(top, all);
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            const int d0 = (4 * i + c) * PIECE;
+            float v[PIECE];
+            fetch_sums(d0);
+            both_sums(v);
+            if (col >= n_cols) continue;
 #pragma unroll
-          for (int c_out = c_first; c_out < C; c_out += AT_ONCE) {
-            if (c_out >= n_cols) break;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int k = 0; k < R; ++k) {
-              const float4 v = *reinterpret_cast<const float4*>(mine + place(k * C + c_out, d_out));
-              acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-            }
-            const float2 tl = total[i][c_out];
-            if (alone) {
-              const int cc = c0 + c_out, t_out = cc / p.G;
-              const float inv = tl.y != 0.f ? 1.f / tl.y : 0.f;
-              bf16* out = p.out + (r0 + t_out) * p.out_ld + (long long)(u.h * p.G + cc - t_out * p.G) * D + d0 + 4 * d_out;
-              *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-            } else {
-              const long long at = (long long)slot * C + c_out;
-              if (i == 0 && c == 0 && d_out == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = tl;
-              *reinterpret_cast<float4*>(p.part_o + at * D + d0 + 4 * d_out) = acc;
+            for (int e = 0; e < PIECE; e += 8) {
+              if (alone) {
+                *reinterpret_cast<uint4*>(out + d0 + e) = make_uint4(pack_bf16(v[e] * inv, v[e + 1] * inv), pack_bf16(v[e + 2] * inv, v[e + 3] * inv), pack_bf16(v[e + 4] * inv, v[e + 5] * inv), pack_bf16(v[e + 6] * inv, v[e + 7] * inv));
+              } else {
+                *reinterpret_cast<float4*>(p.part_o + at * D + d0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                *reinterpret_cast<float4*>(p.part_o + at * D + d0 + e + 4) = make_float4(v[e + 4], v[e + 5], v[e + 6], v[e + 7]);
+              }
             }
           }
-          asm volatile("bar.sync %0, 128;" ::"r"(2 + i) : "memory");
+        } else {
+          if (rep == 0) total[i][col] = make_float2(top, all);
+          // LINE threads a column, whose results lie side by side
+          constexpr int LINE = PIECE / 4, AT_ONCE = 128 / LINE;
+          auto place = [](int row, int e) { return row * PIECE * 4 + ((e ^ (D == 128 ? row >> 1 & 3 : row >> 2 & 1)) << 4); };
+          const int d_out = in % LINE, c_first = in / LINE;
+          uint8_t* const mine = join + i * (128 * PIECE * 4);
+          fetch_sums(4 * i * PIECE);
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            const int d0 = (4 * i + c) * PIECE;
+            float v[PIECE];
+            both_sums(v);
+#pragma unroll
+            for (int e = 0; e < LINE; ++e) *reinterpret_cast<float4*>(mine + place(in, e)) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+            if (c < 3) fetch_sums(d0 + PIECE);           // on their way beside this piece
+            asm volatile("bar.sync %0, 128;" ::"r"(2 + i) : "memory");
+#pragma unroll
+            for (int c_out = c_first; c_out < C; c_out += AT_ONCE) {
+              if (c_out >= n_cols) break;
+              float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+              for (int k = 0; k < R; ++k) {
+                const float4 y = *reinterpret_cast<const float4*>(mine + place(k * C + c_out, d_out));
+                acc.x += y.x; acc.y += y.y; acc.z += y.z; acc.w += y.w;
+              }
+              const float2 tl = total[i][c_out];
+              if (alone) {
+                const int cc = c0 + c_out, t_out = cc / p.G;
+                const float inv = tl.y != 0.f ? 1.f / tl.y : 0.f;
+                bf16* out = p.out + (r0 + t_out) * p.out_ld + (long long)(u.h * p.G + cc - t_out * p.G) * D + d0 + 4 * d_out;
+                *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+              } else {
+                const long long at = (long long)slot * C + c_out;
+                if (i == 0 && c == 0 && d_out == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = tl;
+                *reinterpret_cast<float4*>(p.part_o + at * D + d0 + 4 * d_out) = acc;
+              }
+            }
+            asm volatile("bar.sync %0, 128;" ::"r"(2 + i) : "memory");
+          }
         }
         g0 += u.n;
         tc_fence_before();
@@ -783,11 +819,6 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + 8 * i);
-      }
-      if (done > 0) {
-        const int g = g0 + ((g0 + i) & 1) + 2 * (done - 1);
-        warp_wait(o_done + 8 * (g % STAGES), (uint32_t)(g / STAGES) & 1u, &quit);
-        tc_fence_after();
       }
     }
   }
