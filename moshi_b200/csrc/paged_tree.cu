@@ -71,7 +71,8 @@ constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 6, PRODUCER = 14, ISSUER = 15, THR
 constexpr int UNIT_COST = 12, MIN_RUN = 12;  // in tiles: what a unit costs beside its own, and the least of a CTA
 
 struct TreeP : AttnP {
-  int4* split;                               // per CTA: the unit that it begins and does not end (sequence, kv head, columns' number) and how many CTAs behind it have parts of that; 0: there is none
+  int4* split;                               // per CTA: the unit that it begins and does not end, or has a middle of (sequence, kv head, columns' number); how many CTAs behind the first have parts of that, 0: there is
+                                             // no such unit; and in the upper half how many CTAs back it begins
 };
 
 template <int D>
@@ -631,6 +632,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
             if (by[1] != 0.f) v[e] = fmaf(__uint_as_float(o[1][e]), by[1], v[e]);
           }
         };
+        float4* const parts = reinterpret_cast<float4*>(p.part_o) + (long long)slot * (D / 4) * C;           // [D / 4][C]
         if constexpr (R == 1) {              // a thread has its column alone
           const int cc = c0 + col, t_out = cc / p.G;
           const float inv = all != 0.f ? 1.f / all : 0.f;
@@ -649,8 +651,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
               if (alone) {
                 *reinterpret_cast<uint4*>(out + d0 + e) = make_uint4(pack_bf16(v[e] * inv, v[e + 1] * inv), pack_bf16(v[e + 2] * inv, v[e + 3] * inv), pack_bf16(v[e + 4] * inv, v[e + 5] * inv), pack_bf16(v[e + 6] * inv, v[e + 7] * inv));
               } else {
-                *reinterpret_cast<float4*>(p.part_o + at * D + d0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                *reinterpret_cast<float4*>(p.part_o + at * D + d0 + e + 4) = make_float4(v[e + 4], v[e + 5], v[e + 6], v[e + 7]);
+                parts[(d0 + e) / 4 * C + col] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                parts[(d0 + e + 4) / 4 * C + col] = make_float4(v[e + 4], v[e + 5], v[e + 6], v[e + 7]);
               }
             }
           }
@@ -689,7 +691,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
               } else {
                 const long long at = (long long)slot * C + c_out;
                 if (i == 0 && c == 0 && d_out == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = tl;
-                *reinterpret_cast<float4*>(p.part_o + at * D + d0 + 4 * d_out) = acc;
+                parts[(d0 / 4 + d_out) * C + c_out] = acc;
               }
             }
             asm volatile("bar.sync %0, 128;" ::"r"(2 + i) : "memory");
@@ -702,9 +704,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
       if (next == nullptr) break;
       now = next;
       const Part& u = *next;
-      if (u.u0 == 0 && u.u1 < u.n_pos && threadIdx.x == 0) {
-        const long long runs = walk.run, left = u.n_pos - u.u1;
-        p.split[blockIdx.x] = make_int4(u.s, u.h, u.ct, (int)((left + runs - 1) / runs));
+      if (u.u1 < u.n_pos && threadIdx.x == 0) {
+        const int runs = (int)min(walk.run, 1ll << 30), back = (u.u0 + runs - 1) / runs;
+        p.split[blockIdx.x] = make_int4(u.s, u.h, u.ct, (back + (u.n_pos - u.u1 + runs - 1) / runs) | back << 16);
       }
       fac = factors[col]; m = -INFINITY; sum = 0.f; done = 0;
       next = next_part<C>(walk, p);
@@ -832,62 +834,52 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
   }
 }
 
-// Joins the units that are cut: a block for 16 columns of the one that a CTA has begun, a warp a column; where there are many parts four warps a column, which take them in turn.
-constexpr int JOIN_COLS = 16, MANY_PARTS = 16;
+// Joins the units that are cut, four dims of a column a thread (parts are [D / 4][C] of those; a warp has 4 columns and 8 such pieces, so that reads and writes are whole sectors).  A block has 16 columns of the unit that
+// its CTA has begun; where there are many parts it has four, two or one of them, 4, 8 or 16 threads to a piece that take the parts in turn, and the blocks of the CTAs that have middles of the unit have the others.
+constexpr int JOIN_COLS = 16, MANY_PARTS = 4;
 template <int D, int C>
-__global__ void __launch_bounds__(32 * JOIN_COLS) tree_join_kernel(const TreeP p) {
+__global__ void __launch_bounds__(JOIN_COLS * D / 4) tree_join_kernel(const TreeP p) {
   pdl_trigger();
   pdl_wait();
-  constexpr int PER = D / 32;
-  __shared__ float o_s[JOIN_COLS][D], m_s[JOIN_COLS], l_s[JOIN_COLS];
-  const int cta = (int)blockIdx.x / (C / JOIN_COLS), c0 = (int)blockIdx.x % (C / JOIN_COLS) * JOIN_COLS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int4 of = p.split[cta];
-  if (of.w == 0) return;
+  constexpr int QUADS = D / 4, BLOCKS = C / JOIN_COLS;   // pieces of a column; blocks of a CTA
+  __shared__ float4 o_s[JOIN_COLS * QUADS];
+  __shared__ float2 ml_s[JOIN_COLS * QUADS];
+  const int4 of = p.split[blockIdx.x / BLOCKS];
+  const int parts = of.w & 0xffff, back = of.w >> 16, block = (int)blockIdx.x % BLOCKS, cta = (int)blockIdx.x / BLOCKS - back;
+  const bool many = parts >= MANY_PARTS;
+  const int cols = parts >= 16 ? 1 : parts >= 8 ? 2 : 4, threads = QUADS * cols, teams = many ? JOIN_COLS / cols : 1;
+  if (parts == 0 || (many ? (back * BLOCKS + block) * cols >= C : back > 0)) return;        // parts * BLOCKS * cols >= C
   const Seq q = sequence(p.b, of.x, p.P);
-  const int n_cols = q.n * p.G - of.z * C, teams = of.w >= MANY_PARTS ? 4 : 1, team = warp & (teams - 1);
-  for (int first = 0; first < JOIN_COLS; first += JOIN_COLS / teams) {
-    const int col = c0 + first + warp / teams;
-    float top = -INFINITY, sum = 0.f, acc[PER];
-#pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-    if (col < n_cols) {
-      // the first part is its run's last, the others are their runs' first
-#pragma unroll 4
-      for (int i = team; i <= of.w; i += teams) {
-        const long long at = (long long)(2 * (cta + i) + (i == 0 ? 1 : 0)) * C + col;
-        const float2 y = reinterpret_cast<const float2*>(p.part_ml)[at];
-        float v[PER];
-#pragma unroll
-        for (int e = 0; e < PER; ++e) v[e] = p.part_o[at * D + 32 * e + lane];
-        const float now = fmaxf(top, y.x), keep = now == -INFINITY ? 0.f : exp2_fast(top - now), by = now == -INFINITY ? 0.f : exp2_fast(y.x - now);
-        top = now;
-        sum = fmaf(sum, keep, y.y * by);
-#pragma unroll
-        for (int e = 0; e < PER; ++e) acc[e] = fmaf(acc[e], keep, v[e] * by);
-      }
+  const int n_cols = q.n * p.G - of.z * C, team = (int)threadIdx.x / threads, in = (int)threadIdx.x % threads, quad = in / cols;
+  const int col = cols * (many ? back * BLOCKS + block : 4 * block + team) + in % cols;
+  float top = -INFINITY, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float y_top, float y_sum, const float4& v) {
+    const float now = fmaxf(top, y_top), keep = now == -INFINITY ? 0.f : exp2_fast(top - now), by = now == -INFINITY ? 0.f : exp2_fast(y_top - now);
+    top = now;
+    sum = fmaf(sum, keep, y_sum * by);
+    acc.x = fmaf(acc.x, keep, v.x * by); acc.y = fmaf(acc.y, keep, v.y * by); acc.z = fmaf(acc.z, keep, v.z * by); acc.w = fmaf(acc.w, keep, v.w * by);
+  };
+  if (col < n_cols) {
+    // the first part is its run's last, the others are their runs' first
+#pragma unroll 2
+    for (int i = many ? team : 0; i <= parts; i += teams) {
+      const long long slot = 2 * (cta + i) + (i == 0 ? 1 : 0);
+      const float2 y = reinterpret_cast<const float2*>(p.part_ml)[slot * C + col];
+      add(y.x, y.y, reinterpret_cast<const float4*>(p.part_o)[(slot * QUADS + quad) * C + col]);
     }
-    if (teams > 1) {
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < PER; ++e) o_s[warp][32 * e + lane] = acc[e];
-      if (lane == 0) { m_s[warp] = top; l_s[warp] = sum; }
-      __syncthreads();
-      if (team) continue;
-      for (int i = 1; i < teams; ++i) {
-        const float now = fmaxf(top, m_s[warp + i]), keep = now == -INFINITY ? 0.f : exp2_fast(top - now), by = now == -INFINITY ? 0.f : exp2_fast(m_s[warp + i] - now);
-        top = now;
-        sum = fmaf(sum, keep, l_s[warp + i] * by);
-#pragma unroll
-        for (int e = 0; e < PER; ++e) acc[e] = fmaf(acc[e], keep, o_s[warp + i][32 * e + lane] * by);
-      }
-    }
-    if (col >= n_cols) continue;
-    const int cc = of.z * C + col, token = cc / p.G;
-    const float inv = sum != 0.f ? 1.f / sum : 0.f;
-    bf16* out = p.out + (q.r0 + token) * p.out_ld + (long long)(of.y * p.G + cc - token * p.G) * D + lane;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) out[32 * e] = __float2bfloat16_rn(acc[e] * inv);
   }
+  if (many) {
+    o_s[threadIdx.x] = acc; ml_s[threadIdx.x] = make_float2(top, sum);
+    __syncthreads();
+    if (team) return;
+    for (int k = in + threads; k < JOIN_COLS * QUADS; k += threads) add(ml_s[k].x, ml_s[k].y, o_s[k]);
+  }
+  if (col >= n_cols) return;
+  const int cc = of.z * C + col, token = cc / p.G;
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  bf16* out = p.out + (q.r0 + token) * p.out_ld + (long long)(of.y * p.G + cc - token * p.G) * D + 4 * quad;
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
 }
 
 // =========================================================================================================================
@@ -922,7 +914,7 @@ int launch(const TreeP& p, int ctas, cudaStream_t st) {
   B200_TRY(allow_smem(limits, (int)TreeSmem<D>::BYTES, tree_kernel<D, FMT, C>));
   B200_TRY(prefer_smem(shares, 100, tree_kernel<D, FMT, C>, tree_join_kernel<D, C>));
   B200_TRY(launch_early(tree_kernel<D, FMT, C>, dim3((unsigned)ctas), dim3(THREADS), TreeSmem<D>::BYTES, st, map_k, map_v, p));
-  return launch_early(tree_join_kernel<D, C>, dim3((unsigned)(ctas * (C / JOIN_COLS))), dim3(32 * JOIN_COLS), 0, st, p);
+  return launch_early(tree_join_kernel<D, C>, dim3((unsigned)(ctas * (C / JOIN_COLS))), dim3(JOIN_COLS * D / 4), 0, st, p);
 }
 template <int D, int FMT>
 int launch_cols(const TreeP& p, const TreePlan& f, cudaStream_t st) {
