@@ -4,10 +4,14 @@
 // and a tree has 20 to 100 columns as often as not: the rows are R = 128 / C copies of the columns, of which each weighs 64 / R of a tile's keys.  So all threads of the weights have work whatever C is, with a
 // running maximum of their own; the products of a copy's rows with the other copies' keys are thrown away (scores) or made of zeros (P is block-diagonal, and the zeros are written once).  Tiles go to
 // two groups of weight warps in turn, with a sum O of each, so that the scores of one tile, the weights of another and the sum over a third are made at the same time.  At a unit's end its 2 R sums
-// are joined through shared memory.
+// are joined, both groups' where they lie in TMEM, the copies' through shared memory.
 //
 // Codes come as swizzled tensor copies (a producer warp, 72 KB on their way); six warps turn them into f16 tiles; one issues the products: S = Q K^T with Q in TMEM, O += P V with P there.  Units lie
-// one behind the other and are cut into equal runs, one per CTA, as in paged.cu.  Codes, scales, f16 tiles and the lazy maximum are those of paged_prompt.cu.
+// one behind the other and are cut into equal runs, one per CTA, as in paged.cu; a CTA finds its own at its start.  Codes, scales, f16 tiles and the lazy maximum are those of paged_prompt.cu.
+//
+// Bound: the chain of a tile, scores - weights - sum, beside the instructions around it: 950 clocks with 32 columns (products 512, three quarters of them thrown away or with zeros), 1350 with 128 (exponentials 512); and
+// 7000 to 9000 clocks a unit, 7000 to a CTA's first scores, as its code is cold and the reads depend on one another (lengths, page, codes).  64 requests of 3000 tokens, 32 heads on 8: 32 columns 109 us (HBM: 62), 64 columns 120, 128
+// columns 151.  Fewer than 17 columns (33 at head size 64) are better off with paged.cu's kernel of few rows, in warps of their own: 48 sessions of 12 rows, a head of the cache each, 200 us, as 32 columns here 263.
 #include "paged_tc.cuh"
 
 #include <cfloat>
