@@ -10,7 +10,7 @@
 // one behind the other and are cut into equal runs, one per CTA, as in paged.cu; a CTA finds its own at its start.  Codes, scales, f16 tiles and the lazy maximum are those of paged_prompt.cu.
 //
 // Bound: the chain of a tile, scores - weights - sum, beside the instructions around it: 950 clocks with 32 columns (products 512, three quarters of them thrown away or with zeros), 1350 with 128 (exponentials 512); and
-// 7000 to 9000 clocks a unit, 7000 to a CTA's first scores, as its code is cold and the reads depend on one another (lengths, page, codes).  64 requests of 3000 tokens, 32 heads on 8: 32 columns 109 us (HBM: 62), 64 columns 120, 128
+// 7000 to 9000 clocks a unit, 7000 to a CTA's first scores, as its code is cold and the reads depend on one another (lengths, page, codes).  64 requests of 3000 tokens, 32 heads on 8: 32 columns 108 us (HBM: 62), 64 columns 119, 128
 // columns 151.  Fewer than 17 columns (33 at head size 64) are better off with paged.cu's kernel of few rows, in warps of their own: 48 sessions of 12 rows, a head of the cache each, 200 us, as 32 columns here 263.
 #include "paged_tc.cuh"
 
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(128) tree_build_kernel(const BuildP p) {
 // attention
 // =========================================================================================================================
 constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 6, PRODUCER = 14, ISSUER = 15, THREADS = 16 * 32, SHIFT = 6, KEYS = 1 << SHIFT, STAGES = 4, INFOS = 32;
-constexpr int UNIT_COST = 12, MIN_RUN = 12;  // in tiles: what a unit costs beside its own, and the least of a CTA
+constexpr int UNIT_COST = 8, MIN_RUN = 12;   // in tiles: what a unit costs beside its own (16 requests with 6, 8, 12, 16: 48.1, 48.0, 48.4, 50.6 us; 32 with 20 columns 46.4, 45.2, 45.9, 48.0), and the least of a CTA
 
 struct TreeP : AttnP {
   int4* split;                               // per CTA: the unit that it begins and does not end, or has a middle of (sequence, kv head, columns' number); how many CTAs behind the first have parts of that, 0: there is
