@@ -109,6 +109,23 @@ def test_larger_trees(form, heads, sizes):
     check([0, 37, 100, 5, 64][:len(sizes)], [some_tree(n, 3 * n) for n in sizes], heads, form)
 
 
+@pytest.mark.parametrize("size", [10, 14, 25])
+@pytest.mark.parametrize("dim,page", [(128, 64), (64, 128)])
+def test_one_unit_for_all_ctas(size, dim, page):
+    """One head of the cache: 4, 12 and over 50 parts of a unit, of 32 to 128 columns."""
+    for length in (3000, 9500, 40000):
+        check([length], [some_tree(size, length)], (4, 1), ("int8", dim, page))
+    check([14000, 20000], [some_tree(size, 1), some_tree(size - 1, 2)], (4, 1), ("fp8_e4m3", dim, page), window=12800, sinks=100)
+
+
+@pytest.mark.parametrize("n", [1, 31, 32, 33, 512, 513])
+def test_numbers_of_sequences(n):
+    """A warp looks at 32 sequences, a block at 512."""
+    r = random.Random(n)
+    check([r.choice([0, 5, 30, 64]) for _ in range(n)], [some_tree(r.randint(0, 9) if i + 1 < n else 9, i) for i in range(n)], (8, 1), ("int8", 64, 32))
+    check([r.choice([0, 300, 500]) for _ in range(n)], [some_tree(r.choice([0, 0, 0, 5]) if i + 1 < n else 5, i) for i in range(n)], (8, 1), ("int8", 128, 32))
+
+
 @pytest.mark.parametrize("size", [2, 5, 18])
 def test_many_sequences(size):
     """More than a block looks at in one go, most of them short, some empty."""
