@@ -443,11 +443,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         const int pair_v = pair + 1 == PAIRS ? 0 : pair + 1;
         const uint32_t parity_v = pair + 1 == PAIRS ? parity ^ 1u : parity;
         wait_two(c_empty + 8 * pair, parity, c_empty + 8 * pair_v, parity_v, &quit);
-        if (elected()) {
-          const uint32_t bytes = (uint32_t)(__popc(copies >> 4 * tile & 15u) * groups * 16 * D);
-          mbar_expect_tx(c_full + 8 * pair, bytes);
-          mbar_expect_tx(c_full + 8 * pair_v, bytes);
-        }
+        const uint32_t bytes = (uint32_t)(__popc(copies >> 4 * tile & 15u) * groups * 16 * D);
+        if (elected()) mbar_expect_tx(c_full + 8 * pair, bytes);
         __syncwarp();
         const bool makes = (lane >> 2) == tile && (copies >> lane & 1u);
         const uint32_t to = base + L::CODES + (lane & 3 & -groups) * 16 * D;
@@ -468,7 +465,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
           __syncwarp();
           if (mine < n && (lane & 3) == 0) mbar_arrive(i_full + 8 * ((g + (lane >> 2)) % INFOS));
           page_next = look_up((x >> 3) + 1);
+          __syncwarp();
         }
+        // The values' only arrival, behind the infos: their converters read those, and a tile without pages has no copy that would hold the phase open.
+        if (elected()) mbar_expect_tx(c_full + 8 * pair_v, bytes);
+        __syncwarp();
         if (makes) tma_load_2d(to + 2 * pair_v * L::SLOT, &map_v, c_full + 8 * pair_v, 0, row);
         __syncwarp();
         pair += 2;

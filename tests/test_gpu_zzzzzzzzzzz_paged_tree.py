@@ -659,3 +659,36 @@ def test_drafting_step_by_step(dtype, dim, page, window, sinks):
                 # a step from appending (half, and halves of it for each doubling) and half a step from the one move; e4m3: half steps of the value, twice, and of the subnormals
                 tol = 1.5 * step_of if dtype == "int8" else 2 * 2.0 ** -4 * want.abs() * (1 + 2.0 ** -4) + 3 * 2.0 ** -10 * step_of
                 assert want.shape == got.shape and bool(((got - want).abs() <= tol * (1 + 2.0 ** -9)).all())
+
+
+# ---- pages that are missing ----
+@pytest.mark.parametrize("dim,page", [(128, 64), (128, 128), (64, 64), (64, 128)])
+@pytest.mark.parametrize("size", [1, 5, 10, 25])
+def test_tiles_without_a_page_count_for_nothing(size, dim, page):
+    """4, 20, 40 and 100 columns over tables that lack whole tiles: the first ones, single ones and runs of them, at the beginnings of cut units too.  What lay in shared memory, here bytes that are NaN in e4m3, must not be taken for their values."""
+    r = random.Random(size + dim + page)
+    for lengths, heads in (([700, 9000], (4, 1)), ([300, 0, 2000, 1100], (16, 4))):
+        trees = [some_tree(size, 10 + s) for s in range(len(lengths))]
+        c = Content([n + size for n in lengths], heads[1], dim, page, "fp8_e4m3", seed=size)
+        q = torch.randn(size * len(lengths), heads[0], dim, generator=torch.Generator().manual_seed(size)).bfloat16().cuda()
+        parents, batch = i32([x for t in trees for x in t]), batch_of(c.table, lengths, [size] * len(lengths))
+        tree = PagedTree(batch, parents)
+        odd = PagedKVCache(c.pages, heads[1], dim, page, "int8")
+        odd.k.fill_(127), odd.v.fill_(-1), odd.k_scale.fill_(0.01), odd.v_scale.fill_(1.0)
+        cache, table, seen = c.cache(), c.table.clone(), []
+        for s, n in enumerate(lengths):
+            missing = {b for b in range((n + size) // page) if b in (0, 8, 9) or b % 16 == 15 or r.random() < 0.15} - {(n + size - 1) // page}
+            mask = drafts.visible(trees[s], n)
+            for b in missing:
+                table[s, b] = -1
+                mask[:, b * page:(b + 1) * page] = False
+            seen.append(mask)
+        for _ in range(3):
+            odd.attend(batch, q, tree=tree)
+            batch.table.copy_(table)
+            out = cache.attend(batch, q, tree=tree).double().cpu()
+            batch.table.copy_(c.table)
+            for s in range(len(lengths)):
+                want, tol = drafts.attend(q[size * s:size * (s + 1)].double().cpu(), *c.kvt(s), seen[s], dim ** -0.5)
+                assert bool(((out[size * s:size * (s + 1)] - want).abs() <= tol).all()), (lengths, s)
+        assert cache.error_flags() == paged.BAD_PAGE and odd.error_flags() == 0
