@@ -309,6 +309,16 @@ __device__ __forceinline__ void wait_two(uint32_t bar, uint32_t parity, uint32_t
   warp_wait(bar, parity, quit);
   warp_wait(bar2, parity2, quit);
 }
+// A barrier of some of the block's warps, by whole warps: it asks for all lanes of a warp together, which stores and loops of single lanes in front of it may have parted.
+__device__ __forceinline__ void meet(int id, int threads) {
+  __syncwarp();
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+template <int ID, int N>
+__device__ __forceinline__ void meet() {
+  __syncwarp();
+  asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
+}
 // registers of a weight thread; with those of the others they are what the block was launched with
 template <int C> constexpr int soft_regs() { return C == 128 ? 168 : 144; }
 
@@ -356,9 +366,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
     start_together<C>(p, start);
     if (walks_on && lane == 0) walk = start;
   }
+  __syncwarp();                              // registers are taken and given by whole warps
   auto tmem_ready = [&]() {                  // by the issuer and the weights' warps
     tc_fence_before();
-    asm volatile("bar.sync 4, %0;" ::"n"((SOFT_WARPS + 1) * 32) : "memory");
+    meet<4, (SOFT_WARPS + 1) * 32>();
     tc_fence_after();
     return tmem_at;
   };
@@ -565,7 +576,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
           const int r = r_at + k * APART - round * HERE;
           *reinterpret_cast<uint4*>(join + r * 2 * D + ((c_q ^ (r & 7)) << 4)) = raw[k];
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");    // all columns' factors, too
+        meet<1, SOFT_WARPS * 32>();    // all columns' factors, too
         if (i == 0 && (C / HERE == 1 || warp / (4 / (C / HERE)) == round)) {
           const uint8_t* mine = join + col % HERE * 2 * D;
 #pragma unroll 2
@@ -583,7 +594,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
           __syncwarp();
           if (lane == 0) mbar_arrive(q_full);
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");    // the place is free again
+        meet<1, SOFT_WARPS * 32>();    // the place is free again
       }
     };
     float fac = 0.f, m = -INFINITY, sum = 0.f;
@@ -594,7 +605,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
       if (next != nullptr) load_queries(*next);
       if (now != nullptr) {
         ml[128 * i + in] = make_float2(m, sum);
-        asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");    // every score has been made
+        meet<1, SOFT_WARPS * 32>();    // every score has been made
       }
       if (next != nullptr) put_queries();
       if (now != nullptr) {
@@ -648,21 +659,24 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
           for (int c = 0; c < 4; ++c) {
             const int d0 = (4 * i + c) * PIECE;
             float v[PIECE];
+            __syncwarp();                    // sums are read by whole warps, and some lanes may have had a column in front of this
             fetch_sums(d0);
             both_sums(v);
-            if (col >= n_cols) continue;
+            if (col < n_cols) {
 #pragma unroll
-            for (int e = 0; e < PIECE; e += 8) {
-              if (alone) {
-                *reinterpret_cast<uint4*>(out + d0 + e) = make_uint4(pack_bf16(v[e] * inv, v[e + 1] * inv), pack_bf16(v[e + 2] * inv, v[e + 3] * inv), pack_bf16(v[e + 4] * inv, v[e + 5] * inv), pack_bf16(v[e + 6] * inv, v[e + 7] * inv));
-              } else {
-                parts[(d0 + e) / 4 * C + col] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                parts[(d0 + e + 4) / 4 * C + col] = make_float4(v[e + 4], v[e + 5], v[e + 6], v[e + 7]);
+              for (int e = 0; e < PIECE; e += 8) {
+                if (alone) {
+                  *reinterpret_cast<uint4*>(out + d0 + e) = make_uint4(pack_bf16(v[e] * inv, v[e + 1] * inv), pack_bf16(v[e + 2] * inv, v[e + 3] * inv), pack_bf16(v[e + 4] * inv, v[e + 5] * inv), pack_bf16(v[e + 6] * inv, v[e + 7] * inv));
+                } else {
+                  parts[(d0 + e) / 4 * C + col] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                  parts[(d0 + e + 4) / 4 * C + col] = make_float4(v[e + 4], v[e + 5], v[e + 6], v[e + 7]);
+                }
               }
             }
           }
         } else {
           if (rep == 0) total[i][col] = make_float2(top, all);
+          __syncwarp();
           // LINE threads a column, whose results lie side by side
           constexpr int LINE = PIECE / 4, AT_ONCE = 128 / LINE;
           auto place = [](int row, int e) { return row * PIECE * 4 + ((e ^ (D == 128 ? row >> 1 & 3 : row >> 2 & 1)) << 4); };
@@ -677,7 +691,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
 #pragma unroll
             for (int e = 0; e < LINE; ++e) *reinterpret_cast<float4*>(mine + place(in, e)) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
             if (c < 3) fetch_sums(d0 + PIECE);           // on their way beside this piece
-            asm volatile("bar.sync %0, 128;" ::"r"(2 + i) : "memory");
+            meet(2 + i, 128);
 #pragma unroll
             for (int c_out = c_first; c_out < C; c_out += AT_ONCE) {
               if (c_out >= n_cols) break;
@@ -699,12 +713,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
                 parts[(d0 / 4 + d_out) * C + c_out] = acc;
               }
             }
-            asm volatile("bar.sync %0, 128;" ::"r"(2 + i) : "memory");
+            meet(2 + i, 128);
           }
         }
         g0 += u.n;
         tc_fence_before();
-        asm volatile("bar.sync 1, %0;" ::"n"(SOFT_WARPS * 32) : "memory");    // both groups have read both sums
+        meet<1, SOFT_WARPS * 32>();    // both groups have read both sums
       }
       if (next == nullptr) break;
       now = next;
@@ -784,6 +798,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
         if (__any_sync(0xffffffffu, grow)) {
           const float now = t - UNDER, factor = grow ? exp2_fast(m - now) : 1.f;
           if (grow) { m = now; sum *= factor; }
+          __syncwarp();
           if (done > 0) {
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {           // seldom: short code

@@ -692,3 +692,14 @@ def test_tiles_without_a_page_count_for_nothing(size, dim, page):
                 want, tol = drafts.attend(q[size * s:size * (s + 1)].double().cpu(), *c.kvt(s), seen[s], dim ** -0.5)
                 assert bool(((out[size * s:size * (s + 1)] - want).abs() <= tol).all()), (lengths, s)
         assert cache.error_flags() == paged.BAD_PAGE and odd.error_flags() == 0
+
+
+# ---- columns that end inside a warp ----
+@pytest.mark.parametrize("dim,page", [(128, 64), (64, 32)])
+@pytest.mark.parametrize("size", [17, 31, 33, 47, 65, 95, 97, 100, 127, 129, 161, 193])
+def test_units_whose_last_warp_is_partly_filled(size, dim, page):
+    """One head: as many columns as rows.  Units that a CTA has whole, cut ones, and the same again with another sequence's columns beside them."""
+    check([100, 30], [some_tree(size, 1), some_tree(size - 9, 2)], (1, 1), ("int8", dim, page))
+    first = check([7000], [some_tree(size, 3)], (1, 1), ("fp8_e4m3", dim, page))
+    assert all(torch.equal(first, check([7000], [some_tree(size, 3)], (1, 1), ("fp8_e4m3", dim, page))) for _ in range(3))
+    check([700, 50, 3000], [some_tree(size, 4), some_tree(1, 5), some_tree(size // 2, 6)], (3, 3), ("int8", dim, page), window=500, sinks=5)
