@@ -881,6 +881,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_PER_SM) few_rows_kernel(const
           else *reinterpret_cast<uint2*>(v + piece<D>(r, g >> 1) + 8 * (g & 1)) = make_uint2(0, 0);
         }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");            // the next copy into this place comes behind these writes
+      __syncwarp();                          // lanes with and without such tokens together again: the products ask for whole warps
     };
     auto add_values = [&](int i) {
 #pragma unroll

@@ -288,3 +288,17 @@ def test_a_step_in_two_batches_over_the_same_tensors(dtype, dim, page):
     # the same rows cut into other ranges: 32-bit sums in another order, weights in f16, and half a step of bf16 each
     want = one.attend(batch, want_q).float()
     assert bool(((out.float() - want).abs() <= 2.0 ** -7 * torch.maximum(out.float().abs(), want.abs()) + 2.0 ** -9 * 3).all())
+
+
+@pytest.mark.parametrize("dim,page", [(128, 16), (64, 64)])
+def test_last_tiles_in_which_only_some_lanes_hide_tokens(dim, page):
+    """Every number of tokens in the last tile; what lies behind them is NaN.  The same call gives the same bits."""
+    lengths = list(range(1, 34)) + [95, 96, 97]
+    c = Content(lengths, 2, dim, page, "fp8_e4m3")
+    cache, q = c.cache(), torch.randn(len(lengths), 8, dim, generator=torch.Generator().manual_seed(4)).bfloat16().cuda()
+    batch = batch_of(c.table, [n - 1 for n in lengths], [1] * len(lengths))
+    out = [cache.attend(batch, q) for _ in range(5)]
+    assert all(torch.equal(x, out[0]) for x in out) and cache.error_flags() == 0
+    for s, n in enumerate(lengths):
+        want, tol = oracle.attend(q[s:s + 1].double().cpu(), *c.kvt(s), n - 1, dim ** -0.5)
+        assert bool(((out[0][s:s + 1].double().cpu() - want).abs() <= tol).all()), n
