@@ -62,15 +62,27 @@ def _entry(name: str):
     return fn
 
 
+class _Fixed:
+    """Attributes whose addresses the library has: once set, they take nothing but the same tensor back, as ``pool.lengths += counts`` gives it.  Another tensor would not be looked at, and the first one's memory
+    would be somebody else's."""
+    _fixed: tp.ClassVar[frozenset[str]] = frozenset()
+
+    def __setattr__(self, name: str, value: tp.Any) -> None:
+        if name in self._fixed and self.__dict__.get(name, value) is not value:
+            raise AttributeError(f"{type(self).__name__}.{name} stays the tensor that it is: write into it (copy_, +=)")
+        object.__setattr__(self, name, value)
+
+
 def turns_of(freqs: tp.Iterable[float]) -> list[int]:
     """Turns per position, of frequencies in radians, as fractions of 2^64: the product with a position drops whole turns and nothing else."""
     return [((num * _TURN // den + (1 << 127)) >> 128) % (1 << 64) for num, den in (f.as_integer_ratio() for f in freqs)]
 
 
-class RotaryTable:
+class RotaryTable(_Fixed):
     """Frequencies of a position rotation: ``base ** (-2 j / rot_dims)`` radians per position for the pair j, or ``freqs`` (rot_dims / 2 numbers).  ``pairing``: "adjacent" turns
     dimensions (2j, 2j + 1), "halves" (j, j + rot_dims / 2); dimensions from ``rot_dims`` on stay as they are.  ``axes``: for each pair the axis (0 .. 3) whose position turns it, where rows have positions of
     several (time, height, width); those are given to every ``append``."""
+    _fixed = frozenset(("turns", "pair_axis"))
 
     def __init__(self, rot_dims: int, base: float = 10000.0, pairing: str = "adjacent", freqs: tp.Sequence[float] | None = None, device: torch.device | str = "cuda",
                  axes: tp.Sequence[int] | None = None):
@@ -94,11 +106,12 @@ class RotaryTable:
         self.pair_axis = torch.tensor(axes, dtype=torch.uint8, device=self.device) if self.axes > 1 else None
 
 
-class PagedBatch:
+class PagedBatch(_Fixed):
     """One step.  ``table`` i32 [sequences, pages]: where a sequence's tokens lie; ``before`` i32 [sequences]: tokens that it has cached in front of the step; ``rows`` i32
     [sequences + 1]: sequence s adds rows[s] .. rows[s + 1] - 1 (none, one or many) of the step's ``total_rows``.  ``max_rows``: the most that any of them adds.  The work is laid
     out by it, and a sequence with more is left out; without it (``total_rows``) a step of many sequences takes longer than it has to (48 of one row each: attention 1.4 times, append 2.5 to 3.7
     times as long).  The tensors stay where they are and may be refilled between steps of a captured graph."""
+    _fixed = frozenset(("table", "before", "rows"))
 
     def __init__(self, table: torch.Tensor, before: torch.Tensor, rows: torch.Tensor, total_rows: int, max_rows: int | None = None):
         for name, t, dims in (("table", table, 2), ("before", before, 1), ("rows", rows, 1)):
@@ -120,15 +133,14 @@ class PagedBatch:
         self._ref = C.addressof(self._c)
 
 
-class PagedTree:
+class PagedTree(_Fixed):
     """The rows of a batch as trees of drafted tokens.  ``parents`` i32 [total_rows]: row i of a sequence comes behind its row parents[rows[s] + i], which has a lower number, or, -1, behind the last cached token; a
     parent that is neither counts as -1 and is recorded.  At most 1024 rows of a sequence.  A row's position is before + depth (``positions`` i32 [total_rows], for ``append``); it sees what
     is cached, itself and those that it comes behind (``seen`` i32 [total_rows, words], bit i for the sequence's row i).  All layers of a step share a tree; once ``parents`` or the batch's tensors have been refilled,
     ``update`` fills it anew on the current stream."""
+    _fixed = frozenset(("batch", "seen", "positions", "flags"))
 
     def __init__(self, batch: PagedBatch, parents: torch.Tensor):
-        if parents.dtype != torch.int32 or parents.shape != (batch.total_rows,) or parents.device != batch.device or (parents.numel() > 1 and parents.stride(0) != 1):
-            raise ValueError(f"parents: i32 [{batch.total_rows}], dense, on {batch.device}; got {parents.dtype}, {tuple(parents.shape)}, {parents.device}")
         if batch.max_rows > MAX_NODES:
             raise ValueError(f"trees of up to {batch.max_rows} rows: {MAX_NODES} at most")
         words = max(1, -(-batch.max_rows // 32))
@@ -140,6 +152,17 @@ class PagedTree:
         self._ref = C.addressof(self._c)
         self._build = _entry("b200_paged_tree_build")
         self.update()
+
+    @property
+    def parents(self) -> torch.Tensor:
+        return self._parents
+
+    @parents.setter
+    def parents(self, t: torch.Tensor) -> None:
+        rows, device = self.batch.total_rows, self.batch.device
+        if t.dtype != torch.int32 or t.shape != (rows,) or t.device != device or (t.numel() > 1 and t.stride(0) != 1):
+            raise ValueError(f"parents: i32 [{rows}], dense, on {device}; got {t.dtype}, {tuple(t.shape)}, {t.device}")
+        self._parents = t
 
     def update(self) -> None:
         rc = self._build(self.batch._ref, self._ref, self.parents.data_ptr(), self.flags.data_ptr(), self.batch._index, _stream(self.batch._index)) if self.batch.total_rows else 0
@@ -156,9 +179,10 @@ class PagedTree:
         self.flags.zero_()
 
 
-class PagedKVCache:
+class PagedKVCache(_Fixed):
     """The pages of one layer: ``k``, ``v`` [pages, kv_heads, page_tokens, head_dim] int8 or float8_e4m3fn, with ``k_scale``, ``v_scale`` f32 [pages, kv_heads]; a code stands for
     code * scale.  A new cache's content is arbitrary: what no append has written is never looked at."""
+    _fixed = frozenset(("k", "v", "k_scale", "v_scale", "flags"))
 
     def __init__(self, pages: int, kv_heads: int, head_dim: int, page_tokens: int = 64, dtype: str = "int8", device: torch.device | str = "cuda"):
         if dtype not in _KV:
@@ -325,13 +349,14 @@ def _keep(caches: tp.Sequence[PagedKVCache], ref, n: int, batch: PagedBatch, kep
         _lib.check(rc)
 
 
-class PagePool:
+class PagePool(_Fixed):
     """Who holds which pages, on the device, for sequences whose tokens lie in ``caches`` (one per layer, alike).  ``table`` i32 [sequences, width], -1 behind what a sequence holds; ``lengths`` i32 [sequences]: tokens that
     it has (the caller's to raise, by what a step has left, or to lower, before a ``rearrange`` that gives back what lies behind); ``held``: pages that it holds, enough for them; ``refs`` i32 [pages]: sequences that hold a page.  A pool begins empty.  ``table`` and
     ``lengths`` are what a ``PagedBatch`` takes.  The calls may be captured; none waits."""
+    _fixed = frozenset(("table", "lengths", "held", "refs", "flags", "caches"))
 
     def __init__(self, caches: tp.Sequence[PagedKVCache], sequences: int, width: int):
-        caches = list(caches)
+        caches = tuple(caches)
         if not caches or any((c.device, c.pages, c._shape, c.dtype) != (caches[0].device, caches[0].pages, caches[0]._shape, caches[0].dtype) for c in caches):
             raise ValueError("a pool's caches are alike: device, pages, sizes and type")
         if len({c.k.data_ptr() for c in caches}) < len(caches):

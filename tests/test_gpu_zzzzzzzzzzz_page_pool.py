@@ -287,3 +287,17 @@ def test_a_sequence_that_was_made_shorter(shorter):
     b.check()
     assert len(b.reserve([1, 3, 1])) == (shorter % 16 > 0)      # the third's last page is its own now
     b.check()
+
+
+def test_a_pool_s_tensors_stay():
+    """The library has their addresses: another tensor in their place is refused, and the calls go on with the ones that there are."""
+    b = Both(32, 16, 3, 6)
+    b.reserve([20, 5, 0], grow=False)
+    for name in ("table", "lengths", "held", "refs", "flags"):
+        with pytest.raises(AttributeError, match=name):
+            setattr(b.pool, name, getattr(b.pool, name) + 0)
+    b.pool.lengths += i32([20, 5, 0])
+    b.want.lengths = [20, 5, 0]
+    b.rearrange([0, 0, 1])
+    b.reserve([1, 1, 30])
+    b.check()

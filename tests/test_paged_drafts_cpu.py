@@ -2,11 +2,13 @@
 import ctypes as C
 import math
 import random
+import types
 
 import pytest
 import torch
 
 from moshi_b200 import _lib
+from moshi_b200.models import paged
 from oracle import drafts, paged as oracle
 
 from . import fake_cuda
@@ -206,6 +208,49 @@ def test_pools_and_caches_that_do_not_fit_together(fake):
         refused(fake, Call(**changed), "compact")
     refused(fake, Call(source=None), "rearrange")
     refused(fake, Call(add=None), "reserve")
+
+
+# ---- attributes that the library has the addresses of ----
+@pytest.mark.parametrize("kind,names", [(paged.RotaryTable, ("turns", "pair_axis")), (paged.PagedBatch, ("table", "before", "rows")), (paged.PagedTree, ("seen", "positions", "flags")),
+                                        (paged.PagedKVCache, ("k", "v", "k_scale", "v_scale", "flags")), (paged.PagePool, ("table", "lengths", "held", "refs", "flags"))])
+def test_tensors_are_written_into_and_not_replaced(kind, names):
+    x = kind.__new__(kind)
+    for name in names:
+        t = torch.zeros(4, dtype=torch.int32)
+        setattr(x, name, t)
+        with pytest.raises(AttributeError, match=f"{name} stays"):
+            setattr(x, name, t + 1)
+        with pytest.raises(AttributeError, match=f"{name} stays"):
+            setattr(x, name, t[:])
+        setattr(x, name, t)
+        assert getattr(x, name) is t
+    x.other = 1
+    x.other = 2
+
+
+def test_lengths_are_raised_in_place():
+    pool = paged.PagePool.__new__(paged.PagePool)
+    pool.lengths = torch.zeros(3, dtype=torch.int32)
+    at = pool.lengths.data_ptr()
+    pool.lengths += torch.tensor([1, 2, 3], dtype=torch.int32)
+    assert pool.lengths.tolist() == [1, 2, 3] and pool.lengths.data_ptr() == at
+    with pytest.raises(AttributeError, match="PagePool.lengths stays"):
+        pool.lengths = pool.lengths + 1
+    assert pool.lengths.tolist() == [1, 2, 3]
+
+
+def test_a_tree_s_parents_may_be_others_of_its_rows():
+    tree = paged.PagedTree.__new__(paged.PagedTree)
+    tree.batch = types.SimpleNamespace(total_rows=3, device=torch.device("cpu"))
+    for good in (torch.zeros(3, dtype=torch.int32), torch.zeros(9, dtype=torch.int32)[3:6]):
+        tree.parents = good
+        assert tree.parents is good
+    for bad in (torch.zeros(3), torch.zeros(4, dtype=torch.int32), torch.zeros(6, dtype=torch.int32)[::2], torch.zeros(3, 1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32, device="meta")):
+        with pytest.raises(ValueError, match="parents"):
+            tree.parents = bad
+    assert tree.parents is good
+    with pytest.raises(AttributeError):
+        tree.batch = types.SimpleNamespace(total_rows=9, device=torch.device("cpu"))
 
 
 # ---- the oracle's own properties ----
