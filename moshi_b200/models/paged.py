@@ -42,6 +42,7 @@ _TURN = (1 << 192) * 10 ** 60 // (2 * 314159265358979323846264338327950288419716
 BAD_BATCH, BAD_PAGE, NOT_FINITE, WAIT, BAD_TREE, NO_PAGES = 1, 2, 4, 8, 16, 32
 MAX_NODES = 1024                                # of a tree
 MAX_AXES = 4
+_OVER = "the cache's keys, values and scales lie over one another: what is written to one would change another"
 
 
 def _cuda(device: torch.device | str) -> torch.device:
@@ -60,6 +61,12 @@ def _entry(name: str):
     if fn is None:
         raise RuntimeError(f"this build of the library has no {name}; build all of it with `python -m moshi_b200.build`")
     return fn
+
+
+def _apart(tensors: tp.Iterable[torch.Tensor]) -> bool:
+    """Whether no byte belongs to two of these contiguous tensors."""
+    ranges = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors)
+    return all(a[1] <= b[0] for a, b in zip(ranges, ranges[1:]))
 
 
 class _Fixed:
@@ -196,7 +203,8 @@ class PagedKVCache(_Fixed):
 
     @classmethod
     def from_tensors(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> "PagedKVCache":
-        """A cache in the caller's memory.  Scales of pages in use lie within 2^-60 .. 2^58; where one is 0, all codes of that page and head are 0."""
+        """A cache in the caller's memory.  Scales of pages in use lie within 2^-60 .. 2^58; where one is 0, all codes of that page and head are 0.  Tensors that lie over one another can be read, and not written
+        to (``append``, ``keep``, a pool)."""
         self = cls.__new__(cls)
         self._take(k, v, k_scale, v_scale)
         return self
@@ -214,11 +222,15 @@ class PagedKVCache(_Fixed):
         self.pages, self.kv_heads, self.page_tokens, self.head_dim = k.shape
         self.dtype = _NAMES[k.dtype]
         self._index, self._shape = self.device.index, (self.page_tokens, self.kv_heads, self.head_dim)
+        self._own = _apart(self._tensors())
         self.flags = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._c = _lib.PagedCacheC(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.flags.data_ptr(), self.pages, self.page_tokens, self.kv_heads, self.head_dim, _KV[self.dtype][1], self.device.index)
         self._ref = C.addressof(self._c)
         self._append, self._attend, self._bytes, self._read = (_entry(f"b200_paged_{n}") for n in ("append", "attention", "attention_bytes", "read"))
         self._append_at, self._attend_tree, self._tree_bytes, self._keep = (_entry(f"b200_paged_{n}") for n in ("append_at", "tree_attention", "tree_attention_bytes", "keep"))
+
+    def _tensors(self) -> tuple[torch.Tensor, ...]:
+        return self.k, self.v, self.k_scale, self.v_scale
 
     def _rows(self, name: str, t: torch.Tensor, batch: PagedBatch, heads: int) -> int:
         """Checks a step's tensor [total_rows, heads, head_dim]; its elements from row to row."""
@@ -244,6 +256,8 @@ class PagedKVCache(_Fixed):
         """Stores the step's keys and values, bf16 [total_rows, kv_heads, head_dim] (rows may lie apart, as in a projection of all three), keys rotated by their positions.  Returns
         the queries ``q`` [total_rows, q_heads, head_dim] rotated likewise, in ``q_out`` (which may be ``q``) or a new tensor.  ``positions`` i32 [total_rows] or [axes, total_rows]: positions of the rows' own
         for the rotation, as a tree's tokens have (``PagedTree.positions``) or an image's patches; where a row is stored does not go by them."""
+        if not self._own:
+            raise ValueError(_OVER)
         k_ld, v_ld = self._rows("k", k, batch, self.kv_heads), self._rows("v", v, batch, self.kv_heads)
         if rotary is not None and (rotary.device != self.device or rotary.rot_dims > self.head_dim):
             raise ValueError(f"{rotary.rot_dims} rotated dimensions on {rotary.device} for heads of {self.head_dim} on {self.device}")
@@ -325,6 +339,8 @@ class PagedKVCache(_Fixed):
     def keep(self, batch: PagedBatch, kept: torch.Tensor, counts: torch.Tensor) -> None:
         """Of the step's rows sequence s keeps counts[s] (i32 [sequences]), those of the numbers kept[rows[s]], kept[rows[s] + 1], .. (i32 [total_rows]) among its own, which rise: the accepted path of a
         tree.  They move to the places from before[s] on, and what lies behind them is of no use any more.  Codes move as they are within a page; to another page's scale they are rounded once more."""
+        if not self._own:
+            raise ValueError(_OVER)
         _keep([self], self._ref, 1, batch, kept, counts)
 
     def error_flags(self) -> int:
@@ -359,7 +375,7 @@ class PagePool(_Fixed):
         caches = tuple(caches)
         if not caches or any((c.device, c.pages, c._shape, c.dtype) != (caches[0].device, caches[0].pages, caches[0]._shape, caches[0].dtype) for c in caches):
             raise ValueError("a pool's caches are alike: device, pages, sizes and type")
-        if len({c.k.data_ptr() for c in caches}) < len(caches):
+        if not _apart(t for c in caches for t in c._tensors()):
             raise ValueError("a pool's caches have memory of their own: what moves in one would move twice")
         if not 1 <= sequences <= 4096 or width < 1:
             raise ValueError(f"{sequences} sequences (1 .. 4096) of {width} pages")

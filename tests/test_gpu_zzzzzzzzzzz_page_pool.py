@@ -301,3 +301,24 @@ def test_a_pool_s_tensors_stay():
     b.rearrange([0, 0, 1])
     b.reserve([1, 1, 30])
     b.check()
+
+
+def test_caches_that_share_memory_are_read_only():
+    """Two layers with one tensor of values, or of scales, or keys a page apart in one allocation; keys that are the values too."""
+    def cache(k, v, k_scale, v_scale):
+        return PagedKVCache.from_tensors(k, v, k_scale, v_scale)
+    k, v = (torch.zeros(17, 2, 16, 64, dtype=torch.int8, device="cuda") for _ in range(2))
+    scales = [torch.ones(8, 2, device="cuda") for _ in range(4)]
+    others = [torch.zeros(8, 2, 16, 64, dtype=torch.int8, device="cuda") for _ in range(3)]
+    first = cache(k[:8], v[:8], *scales[:2])
+    for second in (cache(others[0], v[:8], *scales[2:]), cache(others[0], others[1], scales[0], scales[3]), cache(others[0], others[1], scales[2], scales[1]), cache(k[7:15], others[1], *scales[2:]),
+                   cache(others[0], k[1:9], *scales[2:]), cache(others[0], others[0], *scales[2:])):
+        with pytest.raises(ValueError, match="memory of their own"):
+            PagePool([first, second], 2, 2)
+    PagePool([first, cache(k[8:16], v[8:16], *scales[2:])], 2, 2)            # side by side in one allocation
+    both = cache(others[0], others[0], *scales[2:])
+    batch, x = PagedBatch(i32([[0, 1]]), i32([0]), i32([0, 3]), 3, 3), torch.zeros(3, 2, 64, dtype=torch.bfloat16, device="cuda")
+    for call in (lambda: both.append(batch, x, x), lambda: both.keep(batch, i32([1, 2, 0]), i32([2]))):
+        with pytest.raises(ValueError, match="over one another"):
+            call()
+    assert bool((both.attend(batch, x) == 0).all()) and both.error_flags() == 0

@@ -253,6 +253,13 @@ def test_a_tree_s_parents_may_be_others_of_its_rows():
         tree.batch = types.SimpleNamespace(total_rows=9, device=torch.device("cpu"))
 
 
+def test_memory_that_lies_over_itself_is_found():
+    a, b, c = torch.zeros(100, dtype=torch.int8), torch.zeros(64), torch.zeros(10, dtype=torch.float64)
+    assert paged._apart([a, b, c]) and paged._apart([a[:50], a[50:], b[10:20], b[:10], b[20:]]) and paged._apart([]) and paged._apart([b])
+    for over in ([a, b, a], [a, c, a[99:]], [a[:51], b, a[50:]], [b[:11], b[10:].view(torch.int32)], [c, c[3:4], b]):
+        assert not paged._apart(over)
+
+
 # ---- the oracle's own properties ----
 def test_lines_and_depths():
     parents = [-1, 0, 0, 2, -1, 4, 3, 9, -5]
