@@ -651,7 +651,8 @@ typedef struct {
 } b200_page_pool;
 int64_t b200_page_pool_bytes(const b200_page_pool* pool);
 /* All at once, sequence i becomes what sequence source[i] was: its tokens' pages are held by one more; -1: it becomes empty.  So requests are forked, beams change places, and pages are given back.  Pages
- * that were held in reserve are given back too.  A source that is no sequence leaves the sequence what it is. */
+ * that were held in reserve are given back too.  A source that is no sequence leaves the sequence what it is.  A sequence whose length is negative or more than its pages take (lengths raised behind a reserve that
+ * recorded B200_PAGED_NO_PAGES) counts as empty: so is what it becomes, all of its pages are given back, and B200_PAGED_BAD_BATCH is recorded. */
 int b200_page_pool_rearrange(const b200_page_pool* pool, const int32_t* source_dev, void* work_dev, int64_t work_bytes, void* stream);
 /* Sequence s gets pages for add[s] >= 0 tokens behind its lengths[s].  Where the page of the first of them is partly filled and shared it gets a copy of its own, in all caches; of the sequences that share one in
  * this call, the last keeps it if nobody else holds it.  Free pages go out by rising numbers, to sequences by rising numbers, a copy before the sequence's other pages.  If there are too few nobody gets any.  A sequence whose

@@ -261,7 +261,8 @@ __device__ __forceinline__ int source_of(const RearrangeP& p, int i) {
   const int s = p.source[i];
   return s >= -1 && s < p.o.S ? s : i;
 }
-// A block per sequence as it was: its pages get as many references as there are sequences that it becomes, and what it holds behind its tokens is given back.
+// A block per sequence as it was: its pages get as many references as there are sequences that it becomes, and what it holds behind its tokens is given back; all of it, where its length is not one that its pages
+// can have, as nobody could give them back later.
 __global__ void __launch_bounds__(256) rearrange_count_kernel(const RearrangeP p) {
   pdl_trigger();
   pdl_wait();
@@ -276,14 +277,11 @@ __global__ void __launch_bounds__(256) rearrange_count_kernel(const RearrangeP p
   }
   if (mine) atomicAdd(&becomes, mine);
   __syncthreads();
-  const int held = p.o.held[s];
-  int n = pages_of(p.o, s, held);
-  if (n < 0) {                                           // it is left out: nobody gets its pages, and they stay as they are
-    n = 0;
-    if (threadIdx.x == 0) { atomicOr(p.o.flags, B200_PAGED_BAD_BATCH); p.old_pages[s] = 0; p.old_lengths[s] = 0; }
-    return;
+  const int held = min(p.o.held[s], p.o.W), fits = pages_of(p.o, s, p.o.held[s]), n = max(fits, 0);       // one whose length and pages do not fit together counts as empty
+  if (threadIdx.x == 0) {
+    if (fits < 0) atomicOr(p.o.flags, B200_PAGED_BAD_BATCH);
+    p.old_pages[s] = n; p.old_lengths[s] = fits < 0 ? 0 : p.o.lengths[s];
   }
-  if (threadIdx.x == 0) { p.old_pages[s] = n; p.old_lengths[s] = p.o.lengths[s]; }
   for (int b = threadIdx.x; b < held; b += blockDim.x) {
     const int page = p.o.table[s * p.o.table_ld + b];
     if (b < n) p.old_table[(long long)s * p.o.W + b] = page;
@@ -318,12 +316,12 @@ __global__ void __launch_bounds__(ONE) rearrange_small_kernel(const RearrangeP p
     if (p.source[s] < -1 || p.source[s] >= S || n < 0) atomicOr(p.o.flags, B200_PAGED_BAD_BATCH);
     if (from >= 0) atomicAdd(becomes + from, 1);
     tokens[s] = n < 0 ? 0 : p.o.lengths[s];
-    n_pages[s] = n;                                      // -1: left out, and its pages stay as they are
+    n_pages[s] = max(n, 0);                              // one whose length and pages do not fit together counts as empty
   }
   __syncthreads();
   for (int i = threadIdx.x; i < S * W; i += ONE) {
     const int x = i / W, b = i - x * W, n = n_pages[x];
-    if (n < 0 || b >= p.o.held[x]) continue;
+    if (b >= p.o.held[x]) continue;
     const int page = p.o.table[x * p.o.table_ld + b];
     old[i] = page;
     if (page < 0 || page >= p.o.pages) { atomicOr(p.o.flags, B200_PAGED_BAD_PAGE); continue; }
@@ -332,7 +330,7 @@ __global__ void __launch_bounds__(ONE) rearrange_small_kernel(const RearrangeP p
   }
   __syncthreads();
   if (s < S) {
-    p.o.held[s] = from < 0 ? 0 : max(n_pages[from], 0);
+    p.o.held[s] = from < 0 ? 0 : n_pages[from];
     p.o.lengths[s] = from < 0 ? 0 : tokens[from];
     becomes[s] = from;
   }

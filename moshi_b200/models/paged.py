@@ -400,7 +400,8 @@ class PagePool(_Fixed):
         return t.data_ptr()
 
     def rearrange(self, source: torch.Tensor) -> None:
-        """All at once, sequence i becomes what sequence source[i] was (i32 [sequences]), -1: empty.  Forks requests (their pages are shared), moves beams, gives pages back; so are pages that were held in reserve."""
+        """All at once, sequence i becomes what sequence source[i] was (i32 [sequences]), -1: empty.  Forks requests (their pages are shared), moves beams, gives pages back; so are pages that were held in reserve.
+        A sequence whose length is negative or more than its pages take counts as empty: it gives all of its pages back, and BAD_BATCH is recorded."""
         at, work = self._of_sequences("source", source), self._work()
         rc = self._rearrange(self._ref, at, work.data_ptr(), self._bytes, _stream(self._index))
         if rc:

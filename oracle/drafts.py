@@ -107,7 +107,8 @@ class Pool:
     def rearrange(self, source: list[int]) -> None:
         n = len(source)
         source = [s if -1 <= s < n else i for i, s in enumerate(source)]
-        table, lengths = self.table, self.lengths
+        # one whose length is not one that its pages can have counts as empty
+        table, lengths = self.table, [x if 0 <= x <= len(t) * self.page_tokens else 0 for x, t in zip(self.lengths, self.table)]
         self.table = [list(table[s][:self._blocks(lengths[s])]) if s >= 0 else [] for s in source]
         self.lengths = [lengths[s] if s >= 0 else 0 for s in source]
         self.refs = [0] * len(self.refs)

@@ -322,3 +322,41 @@ def test_caches_that_share_memory_are_read_only():
         with pytest.raises(ValueError, match="over one another"):
             call()
     assert bool((both.attend(batch, x) == 0).all()) and both.error_flags() == 0
+
+
+@pytest.mark.parametrize("sequences,width", [(6, 8), (1100, 8)])
+@pytest.mark.parametrize("source", ["itself", "others", "nobody"])
+@pytest.mark.parametrize("wrong", [-1, -2 ** 31, 33, 2 ** 31 - 1])
+def test_a_length_that_the_pages_do_not_take_loses_no_pages(sequences, width, source, wrong):
+    """By the kernel of small tables and by that of large ones: the sequence becomes empty and its pages are free again."""
+    b = Both(40, 16, sequences, width)
+    rest = [0] * (sequences - 4)
+    b.reserve([20, 32, 0, 5] + rest)
+    b.rearrange([0, 1, 1, 3] + [-1] * (sequences - 4))
+    b.reserve([1, 0, 1, 0] + rest)                       # the third goes on behind two shared pages
+    b.check()
+    for x in (b.want.lengths, b.pool.lengths):
+        x[1] = wrong
+    b.rearrange({"itself": [0, 1, 2, 3], "others": [1, 1, 2, 1], "nobody": [0, -1, 2, 3]}[source] + [-1] * (sequences - 4))
+    b.check(paged.BAD_BATCH)
+    assert b.pool.refs.sum() == b.pool.held.sum() and b.pool.held[1] == 0
+    b.rearrange([-1] * sequences)
+    b.check()
+    assert bool((b.pool.refs == 0).all())
+    assert b.reserve([7 * 16, 8 * 16, 8 * 16, 8 * 16] + [16] * min(9, sequences - 4) + [0] * (sequences - 4 - min(9, sequences - 4))) is not None
+    b.check()
+
+
+def test_lengths_raised_without_pages():
+    """A step that got none, and whose lengths were raised all the same: what the sequence held goes back, the others are as they were."""
+    b = Both(6, 16, 3, 6)
+    b.reserve([40, 16, 0])
+    assert b.reserve([20, 20, 20], grow=False) is None
+    for s, n in enumerate((60, 36, 0)):
+        b.want.lengths[s] = n
+    b.pool.lengths += i32([20, 20, 0])
+    b.check(paged.NO_PAGES)
+    b.rearrange([0, 1, 2])
+    b.check(paged.BAD_BATCH)
+    assert b.reserve([96, 0, 0]) is not None
+    b.check()
