@@ -938,7 +938,9 @@ int launch(const TreeP& p, int ctas, cudaStream_t st) {
 }
 template <int D, int FMT>
 int launch_cols(const TreeP& p, const TreePlan& f, cudaStream_t st) {
-  return f.cols == 32 ? launch<D, FMT, 32>(p, f.ctas, st) : f.cols == 64 ? launch<D, FMT, 64>(p, f.ctas, st) : launch<D, FMT, 128>(p, f.ctas, st);
+  if constexpr (few_cols(D) < 32)            // at head size 64 so few columns go to the kernel of few rows
+    if (f.cols == 32) return launch<D, FMT, 32>(p, f.ctas, st);
+  return f.cols == 64 ? launch<D, FMT, 64>(p, f.ctas, st) : launch<D, FMT, 128>(p, f.ctas, st);
 }
 
 }  // namespace
