@@ -11,7 +11,7 @@
 //
 // Bound: the chain of a tile, scores - weights - sum, beside the instructions around it: 950 clocks with 32 columns (products 512, three quarters of them thrown away or with zeros), 1350 with 128 (exponentials 512); and
 // 7000 to 9000 clocks a unit, 7000 to a CTA's first scores, as its code is cold and the reads depend on one another (lengths, page, codes).  64 requests of 3000 tokens, 32 heads on 8: 32 columns 108 us (HBM: 62), 64 columns 119, 128
-// columns 151.  Fewer than 17 columns (33 at head size 64) are better off with paged.cu's kernel of few rows, in warps of their own: 48 sessions of 12 rows, a head of the cache each, 200 us, as 32 columns here 263.
+// columns 151.  Few columns go to paged.cu's kernel of few rows, in warps of their own (tree_plan).
 #include "paged_tc.cuh"
 
 #include <cfloat>
@@ -72,7 +72,9 @@ __global__ void __launch_bounds__(128) tree_build_kernel(const BuildP p) {
 // attention
 // =========================================================================================================================
 constexpr int SOFT_WARPS = 8, CONVERT_WARPS = 6, PRODUCER = 14, ISSUER = 15, THREADS = 16 * 32, SHIFT = 6, KEYS = 1 << SHIFT, STAGES = 4, INFOS = 32;
-constexpr int UNIT_COST = 8, MIN_RUN = 12;   // in tiles: what a unit costs beside its own (16 requests with 6, 8, 12, 16: 48.1, 48.0, 48.4, 50.6 us; 32 with 20 columns 46.4, 45.2, 45.9, 48.0), and the least of a CTA
+// In tiles: what a unit costs beside its own (16 requests with 6, 8, 12, 16: 48.1, 48.0, 48.4, 50.6 us; 32 with 20 columns 46.4, 45.2, 45.9, 48.0), and the least of a CTA (9, 12, 16, 24: 40 columns on 3000 tokens, 8 heads 17.1,
+// 16.9, 18.0, 21.4 us, one head 13.6, 14.9, 16.7, 20.3; 4 requests of 100 columns on 1000 tokens 20.1, 19.9, 19.9, 19.0).
+constexpr int UNIT_COST = 8, MIN_RUN = 12;
 
 struct TreeP : AttnP {
   int4* split;                               // per CTA: the unit that it begins and does not end, or has a middle of (sequence, kv head, columns' number); how many CTAs behind the first have parts of that, 0: there is
@@ -123,7 +125,7 @@ struct Walk {
   Part part[2];
 };
 // Where a CTA's walk begins, `run`: places of an equal share.  Where there is a CTA for every unit, and the longest is not much longer than a share, each has one whole: a unit that is cut costs a second start and the
-// join.  (16 requests of 3000 tokens, 80 columns of 8 heads: 50 us as equal runs, 44 us whole.)
+// join.  (CUT_COST 0, 20, 60, on 80 columns of 8 heads: 16 requests of 3000 tokens 44.1, 39.9, 40.1 us, of 400 tokens 23.2, 15.9, 15.9, 8 of 3000 tokens 31.9, 31.9, 38.8; narrow heads under a window 24.6, 19.9, 19.9.)
 constexpr int CUT_COST = 20, UNITS_MOST = 1 << 20;       // more units are as many as that: it is many either way
 struct Shares {
   long long run, from;                       // from: the CTA's first place or, where it has one whole, its unit
@@ -855,7 +857,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_kernel(const __grid_constant_
 }
 
 // Joins the units that are cut, four dims of a column a thread (parts are [D / 4][C] of those; a warp has 4 columns and 8 such pieces, so that reads and writes are whole sectors).  A block has 16 columns of the unit that
-// its CTA has begun; where there are many parts it has four, two or one of them, 4, 8 or 16 threads to a piece that take the parts in turn, and the blocks of the CTAs that have middles of the unit have the others.
+// its CTA has begun; where there are many parts it has four, two or one of them, 4, 8 or 16 threads to a piece that take the parts in turn, and the blocks of the CTAs that have middles of the unit have the others.  (Many: four at least, as the blocks of
+// fewer could not cover 16 columns each, four at a time.  With 4, 8, 16: 100 columns of one head on 3000 tokens 16.0, 16.7, 16.8 us, on 9500 16.8, 16.7, 19.6, on 131000 39.8, 39.6, 45.3; with none 97.)
 constexpr int JOIN_COLS = 16, MANY_PARTS = 4;
 template <int D, int C>
 __global__ void __launch_bounds__(JOIN_COLS * D / 4) tree_join_kernel(const TreeP p) {
@@ -906,6 +909,9 @@ __global__ void __launch_bounds__(JOIN_COLS * D / 4) tree_join_kernel(const Tree
 // host
 // =========================================================================================================================
 struct TreePlan { int cols, ctas; FewPlan few; };      // few.units: the columns of a sequence are few enough for the kernel of few rows
+// Up to few_cols columns go to the kernel of few rows, the border that steps without a tree have.  Both sides (there / as 32 columns here, us; int8, 3000 tokens, 32 heads on 8; 1, 16, 64 requests).  Head size 128: 8 columns
+// 13.7, 29, 80 / 16, 34, 104; 16 columns 18.9, 42, 110 / 16.2, 34, 107; 48 sessions of 12 rows, 32 heads of their own, 200 / 189.  Head size 64: 8 columns 11.9, 23, 63 / 14.2, 28, 84; 16 columns 16.1, 30, 82 / 14.4, 28, 85;
+// 32 columns 25, 47, 128 / 14.4, 29, 87.  For trees the border is thus too high: from 9 columns on (17 at head size 64) this side is the quicker one.
 TreePlan tree_plan(const b200_paged_cache* c, const b200_paged_batch* b, int G, int window, int sinks) {
   TreePlan f;
   memset(&f, 0, sizeof(f));
