@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       if (!sequence(p.b, i, p.P).ok) atomicOr(p.flags, B200_PAGED_BAD_BATCH);
   Unit u;
   if (!unit_of(p, u)) return;
+  __syncwarp();                              // lanes that looked at different sequences together again: TMEM is asked for by a whole warp
   if (warp == SOFT_WARPS + CONVERT_WARPS) tmem_alloc(smem_u32(&tmem_at), 512);
   const int tiles_q = u.rows > 128 ? 2 : 1;
   const Tiles<7> tiles(u.pf, u.pl, p.window, p.sinks);
@@ -345,6 +346,7 @@ __global__ void __launch_bounds__(THREADS, 1) prompt_kernel(const AttnP p) {
       if (__any_sync(0xffffffffu, grow)) {
         const float now = t - UNDER, factor = grow ? exp2_fast(m - now) : 1.f;
         if (grow) { m = now; sum *= factor; }
+        __syncwarp();
         if (x > 0) {
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {

@@ -367,7 +367,7 @@ def _keep(caches: tp.Sequence[PagedKVCache], ref, n: int, batch: PagedBatch, kep
 
 class PagePool(_Fixed):
     """Who holds which pages, on the device, for sequences whose tokens lie in ``caches`` (one per layer, alike).  ``table`` i32 [sequences, width], -1 behind what a sequence holds; ``lengths`` i32 [sequences]: tokens that
-    it has (the caller's to raise, by what a step has left, or to lower, before a ``rearrange`` that gives back what lies behind); ``held``: pages that it holds, enough for them; ``refs`` i32 [pages]: sequences that hold a page.  A pool begins empty.  ``table`` and
+    it has (the caller's to raise in place, by what a step has left, or to lower, before a ``rearrange`` that gives back what lies behind); ``held``: pages that it holds, enough for them; ``refs`` i32 [pages]: sequences that hold a page.  A pool begins empty.  ``table`` and
     ``lengths`` are what a ``PagedBatch`` takes.  The calls may be captured; none waits."""
     _fixed = frozenset(("table", "lengths", "held", "refs", "flags", "caches"))
 

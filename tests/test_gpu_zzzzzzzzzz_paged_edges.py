@@ -302,3 +302,18 @@ def test_last_tiles_in_which_only_some_lanes_hide_tokens(dim, page):
     for s, n in enumerate(lengths):
         want, tol = oracle.attend(q[s:s + 1].double().cpu(), *c.kvt(s), n - 1, dim ** -0.5)
         assert bool(((out[0][s:s + 1].double().cpu() - want).abs() <= tol).all()), n
+
+
+@pytest.mark.parametrize("sequences", [1, 33, 500, 700])
+def test_prompts_among_any_number_of_sequences(sequences):
+    """The first block looks at all of them, 512 at a time: whole warps, parts of one, several turns."""
+    lengths, new = [40] * sequences, [0] * sequences
+    new[0] = new[-1] = 40
+    c = Content(lengths, 1, 64, 64, "int8")
+    cache, q = c.cache(), torch.randn(sum(new), 8, 64, generator=torch.Generator().manual_seed(4)).bfloat16().cuda()
+    batch = batch_of(c.table, [n - m for n, m in zip(lengths, new)], new)
+    out = [cache.attend(batch, q) for _ in range(3)]
+    assert all(torch.equal(x, out[0]) for x in out) and cache.error_flags() == 0
+    for at, s in enumerate(sorted({0, sequences - 1})):
+        want, tol = oracle.attend(q[40 * at:40 * at + 40].double().cpu(), *c.kvt(s), 0, 64 ** -0.5)
+        assert bool(((out[0][40 * at:40 * at + 40].double().cpu() - want).abs() <= tol).all()), s
